@@ -181,12 +181,12 @@ def _mulhilo(a, m):
 
 
 def _philox(n, seed):
-    """n 32-bit words of Philox4x32-10 (Salmon et al., Parallel random numbers: as easy as 1, 2, 3; 2011): the words of the
+    """n 32-bit words of Philox4x32-7 (Salmon et al., Parallel random numbers: as easy as 1, 2, 3; 2011): the words of the
     counters 0, 1, 2, ... under the key `seed`."""
     i = torch.arange((n + 3) // 4, device="cuda", dtype=torch.int64)
     c0, c1, c2, c3 = i & 0xFFFFFFFF, i >> 32, torch.zeros_like(i), torch.zeros_like(i)
     k0, k1 = seed & 0xFFFFFFFF, seed >> 32 & 0xFFFFFFFF
-    for r in range(10):
+    for r in range(7):
         h0, l0 = _mulhilo(c0, 0xD2511F53)
         h1, l1 = _mulhilo(c2, 0xCD9E8D57)
         c0, c1, c2, c3 = h1 ^ c1 ^ k0, l1, h0 ^ c3 ^ k1, l0
@@ -312,7 +312,7 @@ def _words(n, seed):
     c[0] = np.arange(c.shape[1], dtype=np.uint64)
     c[1], c[0] = c[0] >> sh, c[0] & low
     key = [seed % 2 ** 32, seed // 2 ** 32 % 2 ** 32]
-    for _ in range(10):
+    for _ in range(7):
         a, b = c[0] * np.uint64(0xD2511F53), c[2] * np.uint64(0xCD9E8D57)
         c = np.stack([(b >> sh) ^ c[1] ^ np.uint64(key[0]), b & low, (a >> sh) ^ c[3] ^ np.uint64(key[1]), a & low])
         key = [(key[0] + 0x9E3779B9) % 2 ** 32, (key[1] + 0xBB67AE85) % 2 ** 32]
