@@ -91,6 +91,11 @@ typedef struct {
     const int32_t* fsa_num_states;    /* host, [G]                                             */
 } wf_graph_host;
 
+/* element types of the output head's entry points */
+#define WF_F32 0
+#define WF_BF16 1
+#define WF_F16 2
+
 int wf_version(void);
 const char* wf_last_error(void);
 
@@ -422,6 +427,28 @@ int wf_label_grad_sums(const float* grad, int64_t strideB, int64_t strideT, int3
  * Used by bench.py for the per-kernel roofline numbers.                                          */
 int wf_timing_enable(int on);
 int wf_timing_read(float* ms);
+
+/* ---- the output head: what stands between an encoder and the losses (rnnp.py:116-122) -----------------------------------
+ * Rows of D elements, unit stride inside a row, `ldx` elements from one row to the next (0: the same row); outputs are
+ * contiguous.  `type`: WF_F32 / WF_BF16 / WF_F16.  Sums and statistics are fp32 whatever the type; results are rounded once.
+ *
+ * wf_layer_norm: y = (x - mean) * rstd * weight + bias per row, rstd = 1 / sqrt(var + eps).  weight / bias: [D] of
+ *   `param_type`, either may be NULL.  stats (fp32 [N][2] = mean, rstd) is what wf_layer_norm_backward takes; may be NULL.
+ *   D <= 32768 (WF_EUNSUPPORTED beyond).
+ * wf_layer_norm_backward: dx [N][D] of `type`; dweight / dbias [D] of `param_type`, either may be NULL (then no workspace is
+ *   needed when both are).  Sums over the rows run in a fixed order: the same inputs give the same bits.                  */
+int wf_layer_norm(const void* x, int64_t ldx, int64_t N, int32_t D, int32_t type, const void* weight, const void* bias,
+                  int32_t param_type, float eps, void* y, float* stats, void* stream);
+int wf_layer_norm_backward_workspace_bytes(int64_t N, int32_t D, int32_t type, size_t* bytes);
+int wf_layer_norm_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t N, int32_t D, int32_t type,
+                           const void* weight, int32_t param_type, const float* stats, void* dx, void* dweight, void* dbias,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* wf_dropout: y[i] = x[i] / (1 - p) where word i % 4 of Philox4x32-7(counter i / 4, key seed) >= floor(p 2^32), else 0 (also
+ *   for an x[i] that is not finite); 0 <= p <= 1.  x, y: contiguous, n elements; in place is allowed.  The backward pass is
+ *   the same call on the incoming gradient.  seed_dev != NULL: the key is read from device memory when the kernel runs (a
+ *   captured graph then takes another mask on every replay that finds another seed there).                               */
+int wf_dropout(const void* x, int64_t n, int32_t type, double p, uint64_t seed, const uint64_t* seed_dev, void* y, void* stream);
 
 #ifdef __cplusplus
 }

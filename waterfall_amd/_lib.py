@@ -17,6 +17,10 @@ WF_PREZERO = 16
 WF_ACCUMULATE = 32
 WF_TOT_F64 = 64
 
+WF_F32 = 0
+WF_BF16 = 1
+WF_F16 = 2
+
 
 class WfError(RuntimeError):
     pass
@@ -38,6 +42,8 @@ _i32 = C.c_int32
 _i64 = C.c_int64
 _u32 = C.c_uint32
 _sz = C.c_size_t
+_f32 = C.c_float
+_u64 = C.c_uint64
 
 _SIGS = {
     "wf_version": (C.c_int, []),
@@ -92,6 +98,10 @@ _SIGS = {
                                           _i32, _u32, _p, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _p]),
     "wf_search_lattice": (C.c_int, [_p, _p, _p, _p, _i64, _i64, _i32, _i32, _p, _i32, _i32, C.c_float, C.c_float, _i32, _i32,
                                     _u32, _p, _p, _p, _p, _p, _p, _sz, _p]),
+    "wf_layer_norm": (C.c_int, [_p, _i64, _i64, _i32, _i32, _p, _p, _i32, _f32, _p, _p, _p]),
+    "wf_layer_norm_backward_workspace_bytes": (C.c_int, [_i64, _i32, _i32, C.POINTER(_sz)]),
+    "wf_layer_norm_backward": (C.c_int, [_p, _i64, _p, _i64, _i64, _i32, _i32, _p, _i32, _p, _p, _p, _p, _p, _sz, _p]),
+    "wf_dropout": (C.c_int, [_p, _i64, _i32, C.c_double, _u64, _p, _p, _p]),
 }
 
 
