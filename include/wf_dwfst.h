@@ -450,6 +450,42 @@ int wf_layer_norm_backward(const void* dy, int64_t lddy, const void* x, int64_t 
  *   captured graph then takes another mask on every replay that finds another seed there).                               */
 int wf_dropout(const void* x, int64_t n, int32_t type, double p, uint64_t seed, const uint64_t* seed_dev, void* y, void* stream);
 
+/* The projection z = x W^T + b (x [N][D], W [V][D], both of `type`; bias [V] of `bias_type` or NULL) and what ends it.  fp32
+ * operands are multiplied in three exact bf16 parts (errors of fp32's own size), 16-bit ones as they are, sums in fp32.
+ * An output whose bias is -inf is masked: probability 0.  A row whose every output is masked has log-probabilities of -inf
+ * (and no gradient), as an infeasible utterance has.  What is not finite in a row of x stays in that row's results.
+ *
+ * wf_linear_workspace_bytes: what = 0 wf_linear_log_softmax, 1 its backward, 2 wf_linear_cross_entropy, 3 its backward.
+ *   Sizes beyond N 2^30, D 2^20, V 2^24: WF_EUNSUPPORTED.
+ * wf_linear_log_softmax: log_probs fp32 [N][V] = z - logsumexp(z): what wf_fb_logsum takes.
+ * wf_linear_log_softmax_backward: grad fp32 [N][V], `ldg` elements between rows.  Rows whose gradient is all zero (the frames
+ *   behind an utterance's end) take no part: their x may hold anything.
+ * wf_linear_cross_entropy: loss [N] = logsumexp(z) - (1 - smoothing) z[target] - smoothing mean(z); targets int32
+ *   (targets_wide 0) or int64.  Rows whose target is `ignore_index` take no part: loss 0, their x may hold anything.  Any
+ *   other target outside [0, V): loss NaN, no gradient.  lse [N] is what the backward call takes.  total (may be NULL): the
+ *   sum of the losses, divided by the number of rows that take part where `mean` (0 rows: 0).  The logits are not kept.
+ * wf_linear_cross_entropy_backward: grad: device, [N] (grad_rows) or one value for every row; `mean` as in the forward call.
+ *   The gradients of the logits exist for pieces of the outputs, 256 MB at a time.
+ * Both backward calls: dx [N][D], dweight [V][D] of `type`, dbias [V] of `bias_type`, each may be NULL.  16-bit types: the
+ * gradient of a logit is rounded to `type` before the products (fp16: relative to the largest incoming gradient).  Sums run
+ * in a fixed order: the same inputs give the same bits.                                                                  */
+int wf_linear_workspace_bytes(int32_t what, int64_t N, int32_t D, int32_t V, int32_t type, size_t* bytes);
+int wf_linear_log_softmax(const void* x, int64_t ldx, int64_t N, int32_t D, const void* weight, int64_t ldw, int32_t V, int32_t type,
+                          const void* bias, int32_t bias_type, float* log_probs, void* workspace, size_t workspace_bytes,
+                          void* stream);
+int wf_linear_log_softmax_backward(const float* log_probs, const float* grad, int64_t ldg, const void* x, int64_t ldx, int64_t N,
+                                   int32_t D, const void* weight, int64_t ldw, int32_t V, int32_t type, int32_t bias_type,
+                                   void* dx, void* dweight, void* dbias, void* workspace, size_t workspace_bytes, void* stream);
+int wf_linear_cross_entropy(const void* x, int64_t ldx, int64_t N, int32_t D, const void* weight, int64_t ldw, int32_t V,
+                            int32_t type, const void* bias, int32_t bias_type, const void* targets, int32_t targets_wide,
+                            int64_t ignore_index, float smoothing, float* loss, float* lse, float* total, int32_t mean,
+                            void* workspace, size_t workspace_bytes, void* stream);
+int wf_linear_cross_entropy_backward(const float* grad, int32_t grad_rows, int32_t mean, const float* lse, const void* x, int64_t ldx,
+                                     int64_t N, int32_t D, const void* weight, int64_t ldw, int32_t V, int32_t type,
+                                     const void* bias, int32_t bias_type, const void* targets, int32_t targets_wide,
+                                     int64_t ignore_index, float smoothing, void* dx, void* dweight, void* dbias,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

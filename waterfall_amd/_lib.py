@@ -102,6 +102,14 @@ _SIGS = {
     "wf_layer_norm_backward_workspace_bytes": (C.c_int, [_i64, _i32, _i32, C.POINTER(_sz)]),
     "wf_layer_norm_backward": (C.c_int, [_p, _i64, _p, _i64, _i64, _i32, _i32, _p, _i32, _p, _p, _p, _p, _p, _sz, _p]),
     "wf_dropout": (C.c_int, [_p, _i64, _i32, C.c_double, _u64, _p, _p, _p]),
+    "wf_linear_workspace_bytes": (C.c_int, [_i32, _i64, _i32, _i32, _i32, C.POINTER(_sz)]),
+    "wf_linear_log_softmax": (C.c_int, [_p, _i64, _i64, _i32, _p, _i64, _i32, _i32, _p, _i32, _p, _p, _sz, _p]),
+    "wf_linear_log_softmax_backward": (C.c_int, [_p, _p, _i64, _p, _i64, _i64, _i32, _p, _i64, _i32, _i32, _i32, _p, _p, _p,
+                                                 _p, _sz, _p]),
+    "wf_linear_cross_entropy": (C.c_int, [_p, _i64, _i64, _i32, _p, _i64, _i32, _i32, _p, _i32, _p, _i32, _i64, _f32, _p, _p,
+                                          _p, _i32, _p, _sz, _p]),
+    "wf_linear_cross_entropy_backward": (C.c_int, [_p, _i32, _i32, _p, _p, _i64, _i64, _i32, _p, _i64, _i32, _i32, _p, _i32, _p,
+                                                   _i32, _i64, _f32, _p, _p, _p, _p, _sz, _p]),
 }
 
 

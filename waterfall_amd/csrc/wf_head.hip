@@ -451,3 +451,1133 @@ extern "C" int wf_dropout(const void* x, int64_t n, int32_t type, double p, uint
     HIP_TRY(hipGetLastError());
     return WF_OK;
 }
+
+// =====================================================================================================================
+// the projection z = x W^T + b and what follows it
+//
+// Forward of both losses, and every product of their gradients, is one tiled matrix product on the matrix cores with its own
+// epilogue.  Operands are 16-bit.  fp32 operands are split exactly into three bf16 parts by truncation (8 + 8 + 8 bits of the
+// 24) and the six products of parts down to 2^-16 of the leading one are summed in the same fp32 accumulators: the three
+// that are left out are below 2^-23 of |a||b|, the size of fp32's own rounding.  (At 1/6 of the 16-bit rate that is still 2.6
+// times what the fp32 matrix instructions could give.)
+//
+// A tile is staged by direct global -> LDS loads, double buffered, one barrier per 64 of K.  An operand is stored either
+// with K contiguous (rows of 64 K values are staged, fragments are plain 16-byte LDS reads) or with K as its row index (64
+// rows are staged, fragments come from the transposing LDS reads).  So W serves z = x W^T and dx = dz W, and x serves z
+// and dW = dz^T x, from one copy each.  16-byte chunks are permuted within their row so that both kinds of reads spread over
+// the banks: the permutation is applied to the global address, since the direct load writes LDS in lane order.
+
+struct Operand {
+    const void* p;           // 16-bit elements
+    int64_t ld;              // elements between rows
+    int32_t rows;            // rows that exist (loads beyond are clamped to the last one)
+    int32_t cols;            // K as row index: columns that exist, a multiple of 8
+};
+struct Product {
+    Operand a, b;            // C[m][n] = sum_k A[m][k] B[n][k]
+    int32_t mtiles, ntiles;
+    int32_t ktiles;          // 64-wide K tiles of one part
+    int32_t parts;           // 1, or 6 products of bf16 parts
+    int32_t aoff[6], boff[6];    // element offsets of the parts
+    const int32_t* live;     // NULL, or the number of rows (device): what is behind is skipped
+    int32_t live_is_k;       // ... counts K (else n)
+    int32_t splits;          // K is cut into this many runs
+};
+
+template <class T> struct Mfma;
+template <> struct Mfma<bf16> {
+    typedef bf16 v8 __attribute__((ext_vector_type(8)));
+    static __device__ inline v16f mul(v8 a, v8 b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mfma<f16> {
+    typedef f16 v8 __attribute__((ext_vector_type(8)));
+    static __device__ inline v16f mul(v8 a, v8 b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s lds_v4s;
+
+// One operand of a workgroup's tile: R rows of the product by kBK of K.
+template <int R, int WAVES, bool KROW> struct Stage {
+    static constexpr int kBytes = R * kBK * 2;
+    static constexpr int kChunks = KROW ? R / 8 : kBK / 8;       // 16-byte chunks of a staged row
+    static constexpr int kPer = 64 / kChunks;                    // staged rows that one load of a wave covers
+    static constexpr int kLoads = (KROW ? kBK : R) / kPer / WAVES;
+    static_assert(!KROW || WAVES % 2 == 0, "the row permutation of a lane is the same for all its loads");
+    const char* base;        // uniform: start of the tile's rows
+    uint32_t off[kLoads];    // this lane's byte offsets
+    int64_t kstep;           // bytes from one K tile to the next
+    uint32_t pitch;          // KROW: bytes of a row
+    int32_t lrow[KROW ? kLoads : 1];
+    int32_t rows;
+    uint32_t col;
+
+    __device__ inline void init(const Operand& o, int first, int wave, int lane) {
+        const int r = lane / kChunks, c = lane % kChunks;
+        if constexpr (!KROW) {
+            base = (const char*)o.p + (int64_t)first * o.ld * 2;
+            kstep = kBK * 2;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int row = (i * WAVES + wave) * kPer + r;
+                off[i] = (uint32_t)min(row, o.rows - 1 - first) * (uint32_t)(o.ld * 2) + (uint32_t)((c ^ (row & 7)) * 16);
+            }
+        } else {
+            base = (const char*)o.p;
+            kstep = (int64_t)kBK * o.ld * 2;
+            pitch = (uint32_t)(o.ld * 2);
+            rows = o.rows;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                lrow[i] = (i * WAVES + wave) * kPer + r;
+                col = (uint32_t)min(first + (c ^ ((lrow[i] & 3) << 1)) * 8, o.cols - 8) * 2;
+                off[i] = (uint32_t)lrow[i] * pitch + col;
+            }
+        }
+    }
+    // K tile `kt` at element offset `part` of the operand into LDS
+    __device__ inline void load(char* lds, int kt, int part, int wave) const {
+        const char* b = base + (int64_t)part * 2 + kt * kstep;
+        char* dst = lds + wave * 1024;
+        if constexpr (KROW) {
+            const int left = rows - kt * kBK;        // rows of this tile that exist
+            if (left < kBK) {
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i)
+                    __builtin_amdgcn_global_load_lds((glb_void*)(b + (int64_t)min(lrow[i], left - 1) * pitch + col), (lds_void*)(dst + i * WAVES * 1024), 16, 0, 0);
+                return;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+            __builtin_amdgcn_global_load_lds((glb_void*)(b + off[i]), (lds_void*)(dst + i * WAVES * 1024), 16, 0, 0);
+    }
+    // 8 values of K (16 ks + 8 (lane / 32) ..) of row `first` + lane % 32
+    template <class T> static __device__ inline typename Mfma<T>::v8 frag(const char* lds, int first, int ks, int lane) {
+        typename Mfma<T>::v8 v;
+        if constexpr (!KROW) {
+            const int r = first + (lane & 31), c = (ks * 2 + (lane >> 5)) ^ (r & 7);
+            v = *(const typename Mfma<T>::v8*)(lds + r * (kBK * 2) + c * 16);
+        } else {
+            // 16 lanes read 4 rows of K by 16 columns; lane i gets column i of the four rows
+            const int i = lane & 15, k = ks * 16 + (lane >> 5) * 8 + (i >> 2), c = first + (lane & 16) + (i & 3) * 4;
+            const int chunk = (c >> 3) ^ ((i >> 2) << 1);
+            const char* q = lds + k * (R * 2) + chunk * 16 + (c & 7) * 2;
+            union { v4s h[2]; typename Mfma<T>::v8 v; } u;
+            u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)q);
+            u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(q + 4 * R * 2));
+            v = u.v;
+        }
+        return v;
+    }
+};
+
+// The workgroup's accumulators: tile (tm, tn), K run `split`.  false: nothing to do (all of the tile's rows are dead).
+template <class T, int BM, int BN, int WM, int WN, bool AK, bool BK, bool COLSUM = false> struct Tile {
+    static constexpr int kWaves = WM * WN, kThreads = kWaves * 64;
+    static constexpr int MI = BM / WM / 32, NI = BN / WN / 32;
+    using SA = Stage<BM, kWaves, AK>;
+    using SB = Stage<BN, kWaves, BK>;
+    static constexpr int kLds = 2 * (SA::kBytes + SB::kBytes);
+    v16f acc[MI][NI];
+    v16f colsum[COLSUM ? NI : 1];    // every row: sum_k B[n][k]
+    int tm, tn, split, wm, wn, lane, live;
+
+    __device__ inline bool place(const Product& p) {
+        // a chip's 8 dies take workgroups in turn: each die gets a run of neighbouring tiles, so that its L2 sees the same rows
+        // again.  Within a run the n tiles move slowest: the A tiles of one B tile follow each other.
+        const int tiles = p.mtiles * p.ntiles, all = tiles * p.splits, per = (all + 7) / 8;
+        const int id = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+        if ((int)(blockIdx.x >> 3) >= per || id >= all) return false;
+        split = id / tiles;
+        tm = id % tiles % p.mtiles;
+        tn = id % tiles / p.mtiles;
+        lane = threadIdx.x & 63;
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        wm = wave % WM;
+        wn = wave / WM;
+        live = p.live ? __builtin_amdgcn_readfirstlane(*p.live) : 0x7fffffff;
+        return p.live_is_k || tn * BN < live;
+    }
+    __device__ inline void run(const Product& p, char* lds) {
+        const int wave = wm + wn * WM;
+        SA sa;
+        SB sb;
+        sa.init(p.a, tm * BM, wave, lane);
+        sb.init(p.b, tn * BN, wave, lane);
+        int ktiles = p.ktiles;
+        if (p.live_is_k) ktiles = min(ktiles, (live + kBK - 1) / kBK);
+        const int its = ktiles * p.parts;
+        const int from = (int)((int64_t)its * split / p.splits), to = (int)((int64_t)its * (split + 1) / p.splits);
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) acc[i][j] = v16f{};
+        if constexpr (COLSUM)
+            for (int j = 0; j < NI; ++j) colsum[j] = v16f{};
+        if (from >= to) return;
+        int part = from / ktiles, kt = from % ktiles;
+        auto stage = [&](int buf) {
+            char* s = lds + buf * (SA::kBytes + SB::kBytes);
+            sa.load(s, kt, p.aoff[part], wave);
+            sb.load(s + SA::kBytes, kt, p.boff[part], wave);
+            if (++kt == ktiles) { kt = 0; ++part; }
+        };
+        stage(0);
+        typename Mfma<T>::v8 ones;
+        for (int i = 0; i < 8; ++i) ones[i] = (T)1.f;
+        // (of fp32 parts: once per part of B, beside the leading part of A)
+        const int sums = COLSUM && tm == 0 && wm == 0 ? (p.parts == 1 ? its : 3 * ktiles) : 0;
+        for (int it = from; it < to; ++it) {
+            const int buf = (it - from) & 1;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // this wave's loads of tile `it` have landed ...
+            __builtin_amdgcn_s_barrier();                        // ... and everybody's; nobody reads the other buffer any more
+            asm volatile("" ::: "memory");
+            if (it + 1 < to) stage(buf ^ 1);
+            const char* s = lds + buf * (SA::kBytes + SB::kBytes);
+            typename Mfma<T>::v8 a[2][MI], b[2][NI];
+            auto frags = [&](int ks) {
+#pragma unroll
+                for (int i = 0; i < MI; ++i) a[ks & 1][i] = SA::template frag<T>(s, wm * (BM / WM) + i * 32, ks, lane);
+#pragma unroll
+                for (int j = 0; j < NI; ++j) b[ks & 1][j] = SB::template frag<T>(s + SA::kBytes, wn * (BN / WN) + j * 32, ks, lane);
+            };
+            frags(0);
+#pragma unroll
+            for (int ks = 0; ks < kBK / 16; ++ks) {
+                if (ks + 1 < kBK / 16) frags(ks + 1);
+#pragma unroll
+                for (int j = 0; j < NI; ++j)
+#pragma unroll
+                    for (int i = 0; i < MI; ++i) acc[i][j] = Mfma<T>::mul(a[ks & 1][i], b[ks & 1][j], acc[i][j]);
+                if constexpr (COLSUM)
+                    if (it < sums)
+#pragma unroll
+                        for (int j = 0; j < NI; ++j) colsum[j] = Mfma<T>::mul(ones, b[ks & 1][j], colsum[j]);
+            }
+        }
+    }
+    // accumulator element e of tile (i, j): row m(i, e), column n(j) of the product
+    __device__ inline int m(int i, int e) const { return tm * BM + wm * (BM / WM) + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3); }
+    __device__ inline int n(int j) const { return tn * BN + wn * (BN / WN) + j * 32 + (lane & 31); }
+};
+
+template <bool BIG> struct Shape {         // 256 x 256 by 8 waves, or 128 x 128 by 4
+    static constexpr int BM = BIG ? 256 : 128, BN = BM, WM = 2, WN = BIG ? 4 : 2, kThreads = WM * WN * 64;
+};
+template <class T> constexpr int parts_of() { return sizeof(T) == 4 ? 3 : 1; }      // 16-bit planes of an operand
+template <class T> struct Half { typedef T type; };
+template <> struct Half<float> { typedef bf16 type; };
+
+// v in three bf16 parts of 8 significand bits each, by truncation; the parts below a value that is not finite are 0
+struct Split3 { uint16_t h[3]; };
+__device__ inline Split3 split3(float v) {
+    Split3 s;
+    const uint32_t a = __float_as_uint(v) & 0xffff0000u;
+    s.h[0] = (uint16_t)(a >> 16);
+    if ((a & 0x7f800000u) == 0x7f800000u) {          // keeps a NaN a NaN when its upper significand bits are 0
+        if (v != v) s.h[0] |= 0x40;
+        s.h[1] = s.h[2] = 0;
+        return s;
+    }
+    const float r = v - __uint_as_float(a);
+    const uint32_t b = __float_as_uint(r) & 0xffff0000u;
+    s.h[1] = (uint16_t)(b >> 16);
+    s.h[2] = (uint16_t)(__float_as_uint(r - __uint_as_float(b)) >> 16);
+    return s;
+}
+template <class T> __device__ inline uint16_t bits16(float v) {
+    const T h = (T)v;
+    uint16_t u;
+    __builtin_memcpy(&u, &h, 2);
+    return u;
+}
+
+// Rows of D elements into packed operand rows: planes of Dp (a multiple of 64, zeros behind D).  pos == NULL: row n goes to
+// row n.  Else row n goes to row pos[n]; pos[n] < 0: the row is dead -- it is left out, and its row of `clear` (the gradient
+// of x) becomes 0.  256 rows more of the grid clear the packed rows from the last live one to the next multiple of 256.
+struct PackArgs {
+    const void* src;
+    int64_t ld, N;
+    int D, Dp;
+    const int32_t *pos, *live;
+    uint16_t* dst;
+    void* clear;
+    int tail;                // the grid has the 256 rows more
+};
+template <class T> __global__ void __launch_bounds__(256) pack_kernel(PackArgs a) {
+    constexpr int P = parts_of<T>(), VEC = 8;
+    const int lane = threadIdx.x & 63;
+    const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    int64_t c = n;
+    int D = a.D;
+    if (n >= a.N) {
+        if (!a.tail) return;
+        const int live = a.live ? *a.live : (int)a.N;
+        c = live + (n - a.N);
+        if (c >= (live + kRowPad - 1) / kRowPad * kRowPad) return;
+        D = 0;
+    } else if (a.pos) {
+        c = a.pos[n];
+        if (c < 0) {
+            if (a.clear)
+                for (int d = lane; d < a.D; d += 64) ((T*)a.clear)[n * a.D + d] = (T)0.f;
+            return;
+        }
+    }
+    const T* x = (const T*)a.src + n * a.ld;
+    uint16_t* y = a.dst + c * (int64_t)P * a.Dp;
+    for (int d = lane * VEC; d < a.Dp; d += 64 * VEC) {
+        Pack<T, VEC> v;
+        if (D > d) v = load_n<T, VEC>(x + d, D - d);
+        else
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v.v[i] = (T)0.f;
+        if constexpr (P == 1) {
+            __builtin_memcpy(y + d, &v, sizeof(v));
+        } else {
+            Pack<uint16_t, VEC> h[3];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const Split3 s = split3(v.v[i]);
+#pragma unroll
+                for (int p = 0; p < 3; ++p) h[p].v[i] = s.h[p];
+            }
+#pragma unroll
+            for (int p = 0; p < 3; ++p) __builtin_memcpy(y + (size_t)p * a.Dp + d, &h[p], sizeof(h[p]));
+        }
+    }
+}
+
+// ---- the rows that take part ----------------------------------------------------------------------------------------
+// A padded batch holds rows that no loss reads: frames without a target, frames whose incoming gradient is all zero.  They are
+// left out of every product (their features may hold anything, NaN included): live rows are packed in their order.
+struct Rows {                // in the workspace
+    int32_t* live;           // [1] number of live rows
+    float* scale;            // [1] what the gradients of logits are relative to when they are rounded to 16 bits
+    int32_t* pos;            // [N] packed row of row n, -1: dead
+    int32_t* idx;            // [Npad] row of packed row c
+    int32_t* target;         // [Npad] its target, -1: none that is in range
+    float* g;                // [Npad] its incoming gradient relative to the largest
+    float* lse;              // [Npad]
+};
+struct RowsArgs {
+    Rows r;
+    int64_t N;
+    int V;
+    const void* targets;     // cross entropy: row n is live iff targets[n] != ignore
+    int target_wide;
+    int64_t ignore;
+    const float* peak;       // log-softmax backward: row n is live iff peak[n] (largest |gradient|) is not 0
+    float *loss, *lse;       // cross entropy forward: dead rows' outputs (0)
+    const float* gout;       // backward: incoming gradient, one for all rows or per row
+    int gout_rows, mean;
+    const float* lse_in;
+    float hit;               // backward: 1 - smoothing, or 1 where that is 0
+};
+__device__ inline int64_t target_of(const RowsArgs& a, int64_t n) {
+    return a.target_wide ? ((const int64_t*)a.targets)[n] : (int64_t)((const int32_t*)a.targets)[n];
+}
+// one workgroup: every thread owns a run of rows, counts its live ones, and writes them behind those of the threads before it
+__global__ void __launch_bounds__(1024) rows_kernel(RowsArgs a) {
+    __shared__ int cnt[1024];
+    __shared__ float top[16];
+    const int t = threadIdx.x;
+    const int64_t per = (a.N + 1023) / 1024, from = min(a.N, t * per), to = min(a.N, from + per);
+    auto alive = [&](int64_t n) { return a.targets ? target_of(a, n) != a.ignore : a.peak[n] != 0.f; };
+    int c = 0;
+    float peak = 0.f;
+    for (int64_t n = from; n < to; ++n)
+        if (alive(n)) {
+            ++c;
+            if (a.peak || a.gout) peak = fmaxf(peak, a.peak ? a.peak[n] : fabsf(a.gout[a.gout_rows ? n : 0]));
+        }
+    cnt[t] = c;
+    peak = wave_max(peak);
+    if ((t & 63) == 0) top[t >> 6] = peak;
+    __syncthreads();
+    for (int o = 1; o < 1024; o <<= 1) {
+        const int v = t >= o ? cnt[t - o] : 0;
+        __syncthreads();
+        cnt[t] += v;
+        __syncthreads();
+    }
+    const int live = cnt[1023];
+    int at = cnt[t] - c;
+    // What a 16-bit gradient of a logit is relative to.  Cross entropy: the largest incoming gradient, times the target's own
+    // share 1 - smoothing: where all rows weigh the same, the entry of a target is then -1 + p / (1 - smoothing) and not some
+    // number whose rounding is the same in every row and adds up over them.  Log-probabilities: a power of two near the largest
+    // incoming gradient.  fp16 needs either to stay inside its range: what then falls below its 2^-24 is below that of a row's.
+    float scale = 0.f;
+    for (int i = 0; i < 16; ++i) scale = fmaxf(scale, top[i]);
+    if (!(scale > 0.f && scale < INFINITY)) scale = 1.f;
+    else if (a.peak) {
+        int e = 0;
+        (void)frexpf(scale, &e);
+        scale = ldexpf(1.f, max(-100, min(100, e)));
+    }
+    const float by = scale;
+    if (a.mean && live > 0) scale /= (float)live;
+    scale *= a.hit;
+    for (int64_t n = from; n < to; ++n) {
+        if (!alive(n)) {
+            a.r.pos[n] = -1;
+            if (a.loss) a.loss[n] = 0.f;
+            if (a.lse) a.lse[n] = 0.f;
+            continue;
+        }
+        a.r.pos[n] = at;
+        a.r.idx[at] = (int32_t)n;
+        if (a.targets) {
+            const int64_t v = target_of(a, n);
+            a.r.target[at] = v >= 0 && v < a.V ? (int32_t)v : -1;
+        }
+        if (a.gout) {
+            a.r.g[at] = a.r.target[at] < 0 ? 0.f : a.gout[a.gout_rows ? n : 0] / by;
+            a.r.lse[at] = a.lse_in[n];
+        }
+        ++at;
+    }
+    if (t == 0) { *a.r.live = live; *a.r.scale = scale; }
+    // packed rows up to the end of the last tile: no gradient
+    if (a.gout)
+        for (int i = live + t; i < (live + kRowPad - 1) / kRowPad * kRowPad; i += 1024) { a.r.g[i] = 0.f; a.r.lse[i] = 0.f; a.r.target[i] = -1; }
+}
+
+// ---- epilogues ------------------------------------------------------------------------------------------------------
+struct Logits {              // what every product z = x W^T needs behind the accumulators
+    const void* bias;        // [V] or NULL
+    int32_t btype, v0, V;    // the product's W rows are outputs v0 .., V is the number of outputs that exist
+};
+// bias of the tile's outputs in LDS; outputs that do not exist get -inf, so that they take no part in any softmax
+__device__ inline void stage_bias(const Logits& l, int first, int count, float* dst) {
+    for (int i = threadIdx.x; i < count; i += blockDim.x) {
+        const int v = l.v0 + first + i;
+        dst[i] = v < l.V ? (l.bias ? load_any(l.bias, l.btype, v) : 0.f) : -INFINITY;
+    }
+}
+
+struct StatsArgs {
+    Product p;
+    Logits l;
+    float *top, *sum, *all;  // [mtiles * WM][pitch]: largest logit, sum of exp(z - largest), sum of z (label smoothing, or NULL)
+    int64_t pitch;
+    const int32_t* target;   // packed row -> target, or NULL
+    float* zt;               // its logit
+};
+// Row statistics of z, tile by tile: A = W (a lane's registers run along the outputs), B = x (a lane is one row): the softmax
+// sums are register loops and one exchange between the lane halves.
+template <class T, bool BIG> __global__ void __launch_bounds__(Shape<BIG>::kThreads, BIG ? 2 : 2) stats_kernel(StatsArgs a) {
+    using S = Shape<BIG>;
+    using Tl = Tile<T, S::BM, S::BN, S::WM, S::WN, false, false>;
+    __shared__ __align__(16) char lds[Tl::kLds];
+    __shared__ float bias[S::BM];
+    Tl t;
+    if (!t.place(a.p)) return;
+    stage_bias(a.l, t.tm * S::BM, S::BM, bias);
+    t.run(a.p, lds);
+    __syncthreads();
+    const int64_t at = (int64_t)(t.tm * S::WM + t.wm) * a.pitch;
+#pragma unroll
+    for (int j = 0; j < Tl::NI; ++j) {
+        const int c = t.n(j), want = a.target && c < t.live ? a.target[c] - a.l.v0 : -1;
+        float top = -INFINITY, all = 0.f, zt = 0.f;
+        bool here = false;
+#pragma unroll
+        for (int i = 0; i < Tl::MI; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int m = t.m(i, e);
+                const float z = t.acc[i][j][e] + bias[m - t.tm * S::BM];
+                t.acc[i][j][e] = z;
+                top = fmaxf(top, z);
+                if (a.all) all += a.l.v0 + m < a.l.V ? z : 0.f;
+                if (m == want) { zt = z; here = true; }
+            }
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float ref = top == -INFINITY ? 0.f : top;          // a row of -inf: its exponentials are 0, not NaN
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < Tl::MI; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sum += __expf(t.acc[i][j][e] - ref);
+        sum += __shfl_xor(sum, 32);
+        if (a.all) all += __shfl_xor(all, 32);
+        if (here) a.zt[c] = zt;
+        if (t.lane < 32 && c < a.pitch) {
+            a.top[at + c] = top;
+            a.sum[at + c] = sum;
+            if (a.all) a.all[at + c] = all;
+        }
+    }
+}
+
+// The tiles' statistics of a row joined: lse, and the loss of the row where there are targets.
+struct JoinArgs {
+    const float *top, *sum, *all, *zt;
+    int64_t pitch, N;
+    int tiles, V;
+    const int32_t *live, *idx, *target;
+    float smoothing;
+    float *lse, *loss;
+};
+__global__ void __launch_bounds__(256) join_kernel(JoinArgs a) {
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (c >= (a.live ? (int64_t)*a.live : a.N)) return;
+    float top = -INFINITY;
+    for (int q = 0; q < a.tiles; ++q) top = fmaxf(top, a.top[q * a.pitch + c]);
+    float sum = 0.f, all = 0.f;
+    for (int q = 0; q < a.tiles; ++q) {
+        const float m = a.top[q * a.pitch + c];
+        sum += a.sum[q * a.pitch + c] * (m == -INFINITY ? 1.f : __expf(m - top));     // (-inf: its sum is 0, or NaN)
+        if (a.all) all += a.all[q * a.pitch + c];
+    }
+    const float lse = (top == -INFINITY ? 0.f : top) + logf(sum);
+    const int64_t n = a.idx ? a.idx[c] : c;
+    a.lse[n] = lse;
+    if (a.loss) {
+        const int t = a.target[c];
+        float loss = NAN;                                     // a target that is no output: loud, and no read out of range
+        if (t >= 0) {
+            loss = lse;
+            if (a.smoothing != 1.f) loss -= (1.f - a.smoothing) * a.zt[c];
+            if (a.smoothing != 0.f) loss -= a.smoothing * (all / (float)a.V);
+            if (lse == -INFINITY) loss = INFINITY;            // every output is masked: as unlikely as a target can be
+        }
+        a.loss[n] = loss;
+    }
+}
+__global__ void __launch_bounds__(1024) total_kernel(const float* loss, int64_t N, const int32_t* live, int mean, float* out) {
+    __shared__ float s[16];
+    float v = 0.f;
+    for (int64_t n = threadIdx.x; n < N; n += 1024) v += loss[n];
+    v = wave_sum(v);
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        v = 0.f;
+        for (int i = 0; i < 16; ++i) v += s[i];
+        if (mean && live) v /= (float)max(1, *live);
+        *out = v;
+    }
+}
+
+struct LogProbArgs {
+    Product p;               // A = x, B = W: a lane is one output, 32 of them make 128 bytes of a row
+    Logits l;
+    const float* lse;
+    float* out;
+    int64_t N;
+};
+template <class T, bool BIG> __global__ void __launch_bounds__(Shape<BIG>::kThreads, 2) log_prob_kernel(LogProbArgs a) {
+    using S = Shape<BIG>;
+    using Tl = Tile<T, S::BM, S::BN, S::WM, S::WN, false, false>;
+    __shared__ __align__(16) char lds[Tl::kLds];
+    __shared__ float bias[S::BN], lse[S::BM];
+    Tl t;
+    if (!t.place(a.p)) return;
+    stage_bias(a.l, t.tn * S::BN, S::BN, bias);
+    for (int i = threadIdx.x; i < S::BM; i += S::kThreads) {
+        const int64_t n = (int64_t)t.tm * S::BM + i;
+        const float v = n < a.N ? a.lse[n] : 0.f;
+        lse[i] = v == -INFINITY ? 0.f : v;                   // a row of -inf stays one
+    }
+    t.run(a.p, lds);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < Tl::MI; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int64_t n = t.m(i, e);
+            if (n >= a.N) continue;
+            const float l = lse[n - (int64_t)t.tm * S::BM];
+#pragma unroll
+            for (int j = 0; j < Tl::NI; ++j) {
+                const int v = t.n(j);
+                if (v < a.l.V) a.out[n * a.l.V + v] = t.acc[i][j][e] + bias[v - t.tn * S::BN] - l;
+            }
+        }
+}
+
+struct DzArgs {
+    Product p;               // A = W's piece, B = the live rows of x
+    Logits l;
+    const int32_t* target;
+    const float *g, *lse;
+    float smoothing;
+    int32_t outputs;         // all of them, not the piece's
+    uint16_t* dz;            // [Npad][planes][pitch]
+    int64_t pitch;
+};
+// 16-bit planes of four neighbouring values
+template <class T> __device__ inline void store_dz4(uint16_t* row, int64_t pitch, int v, const float (&d)[4]) {
+    if constexpr (parts_of<T>() == 1) {
+        Pack<uint16_t, 4> h;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h.v[i] = bits16<T>(d[i]);
+        __builtin_memcpy(row + v, &h, 8);
+    } else {
+        Pack<uint16_t, 4> h[3];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const Split3 s = split3(d[i]);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) h[p].v[i] = s.h[p];
+        }
+#pragma unroll
+        for (int p = 0; p < 3; ++p) __builtin_memcpy(row + p * pitch + v, &h[p], 8);
+    }
+}
+// d loss / d z of a piece of the outputs from logits that are computed again: g (p - (1 - e) [v = target] - e / V), rounded to
+// the type of x for the products that follow (fp32: exact parts), as a 16-bit training step's stored gradients are.
+template <class X, bool BIG> __global__ void __launch_bounds__(Shape<BIG>::kThreads, 2) dz_kernel(DzArgs a) {
+    using T = typename Half<X>::type;
+    using S = Shape<BIG>;
+    using Tl = Tile<T, S::BM, S::BN, S::WM, S::WN, false, false>;
+    __shared__ __align__(16) char lds[Tl::kLds];
+    __shared__ __align__(16) float bias[S::BM];
+    Tl t;
+    if (!t.place(a.p)) return;
+    stage_bias(a.l, t.tm * S::BM, S::BM, bias);
+    t.run(a.p, lds);
+    __syncthreads();
+    // relative to g_max (1 - e): (p - e / V) / (1 - e) - [v = target]
+    const float even = a.smoothing / (float)a.outputs, share = a.smoothing < 1.f ? 1.f / (1.f - a.smoothing) : 1.f;
+    const float hit = a.smoothing < 1.f ? 1.f : 0.f;
+#pragma unroll
+    for (int j = 0; j < Tl::NI; ++j) {
+        const int c = t.n(j);
+        const bool in = c < t.live;
+        const float g = in ? a.g[c] : 0.f, lse = in ? a.lse[c] : 0.f, ref = lse == -INFINITY ? 0.f : lse;
+        const int want = in ? a.target[c] - a.l.v0 : -1;
+        const bool dead = g == 0.f || lse == -INFINITY;
+        uint16_t* row = a.dz + (int64_t)c * parts_of<X>() * a.pitch;
+#pragma unroll
+        for (int i = 0; i < Tl::MI; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int m = t.m(i, q * 4);
+                float d[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float z = t.acc[i][j][q * 4 + e] + bias[m - t.tm * S::BM + e];
+                    d[e] = g * ((__expf(z - ref) - even) * share - (m + e == want ? hit : 0.f));
+                    if (dead || a.l.v0 + m + e >= a.l.V) d[e] = 0.f;
+                }
+                if (m < a.pitch) store_dz4<X>(row, a.pitch, m, d);
+            }
+    }
+}
+
+struct GradArgs {
+    Product p;
+    int32_t M;               // columns (features) that exist
+    int64_t N;               // rows that exist
+    float* part;             // [splits][N][M] sums, or NULL: straight to out
+    int32_t add;             // ... added to what is there
+    float* colpart;          // [splits][N] sums of B's rows (the bias' gradient), or NULL
+    const float* scale;
+    void* out;               // [.][M]
+    int32_t otype;
+    const int32_t* idx;      // row of out, or NULL
+    void* colout;
+    int32_t ctype;
+};
+// C[n][m] for a gradient: m runs along features (registers: 4 neighbours), n along rows of x or of W.
+template <class T, bool BIG, bool BK, bool COLSUM> __global__ void __launch_bounds__(Shape<BIG>::kThreads, 2) grad_kernel(GradArgs a) {
+    using S = Shape<BIG>;
+    using Tl = Tile<T, S::BM, S::BN, S::WM, S::WN, true, BK, COLSUM>;
+    __shared__ __align__(16) char lds[Tl::kLds];
+    Tl t;
+    if (!t.place(a.p)) return;
+    t.run(a.p, lds);
+    const float scale = a.part ? 1.f : *a.scale;
+    const int64_t N = a.p.live && !a.p.live_is_k ? min(a.N, (int64_t)t.live) : a.N;
+#pragma unroll
+    for (int j = 0; j < Tl::NI; ++j) {
+        const int n = t.n(j);
+        if (n >= N) continue;
+        if constexpr (COLSUM)
+            if ((a.colpart || a.colout) && t.tm == 0 && t.wm == 0 && t.lane < 32) {
+                if (a.part) a.colpart[(int64_t)t.split * a.N + n] = t.colsum[j][0];
+                else store_any(a.colout, a.ctype, n, t.colsum[j][0] * *a.scale);
+            }
+#pragma unroll
+        for (int i = 0; i < Tl::MI; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int m = t.m(i, q * 4);
+                if (m >= a.M) continue;
+                const int left = a.M - m;
+                if (a.part) {
+                    float* at = a.part + ((int64_t)t.split * a.N + n) * a.M + m;
+                    Pack<float, 4> v;
+                    if (a.add) v = load_n<float, 4>(at, left);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v.v[e] = (a.add ? v.v[e] : 0.f) + t.acc[i][j][q * 4 + e];
+                    store_n<float, 4>(at, v, left);
+                } else {
+                    const int64_t r = (a.idx ? a.idx[n] : n) * (int64_t)a.M + m;
+                    if (a.otype == WF_F32) {
+                        Pack<float, 4> v;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v.v[e] = t.acc[i][j][q * 4 + e] * scale;
+                        store_n<float, 4>((float*)a.out + r, v, left);
+                    } else {
+                        Pack<T, 4> v;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v.v[e] = (T)(t.acc[i][j][q * 4 + e] * scale);
+                        store_n<T, 4>((T*)a.out + r, v, left);
+                    }
+                }
+            }
+    }
+}
+
+// out[row(n)][m] = scale * sum over splits of part[s][n][m], and the same for the column sums
+struct FoldArgs {
+    const float *part, *colpart, *scale;
+    int32_t splits, M;
+    int64_t N;
+    const int32_t *live, *idx;
+    void *out, *colout;
+    int32_t otype, ctype;
+};
+__global__ void __launch_bounds__(256) fold_kernel(FoldArgs a) {
+    const int64_t N = a.live ? min(a.N, (int64_t)*a.live) : a.N;
+    const float scale = *a.scale;
+    const int64_t all = N * a.M, stride = a.N * a.M;
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < all; i += (int64_t)gridDim.x * 1024) {
+        const int left = (int)min((int64_t)4, all - i);
+        Pack<float, 4> v = load_n<float, 4>(a.part + i, left);
+        for (int s = 1; s < a.splits; ++s) {
+            const auto w = load_n<float, 4>(a.part + s * stride + i, left);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v.v[e] += w.v[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (e >= left) break;
+            const int64_t k = i + e;
+            store_any(a.out, a.otype, a.idx ? a.idx[k / a.M] * (int64_t)a.M + k % a.M : k, v.v[e] * scale);
+        }
+    }
+    if (a.colout)
+        for (int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x; n < N; n += (int64_t)gridDim.x * 256) {
+            float v = a.colpart[n];
+            for (int s = 1; s < a.splits; ++s) v += a.colpart[s * a.N + n];
+            store_any(a.colout, a.ctype, n, v * scale);
+        }
+}
+
+// ---- the gradient that comes into log-probabilities -----------------------------------------------------------------
+// sum and largest magnitude of every row of G; a workgroup a row
+__global__ void __launch_bounds__(256) grad_rows_kernel(const float* G, int64_t ldg, int V, float* sum, float* peak) {
+    __shared__ float s[4], p[4];
+    const float* g = G + blockIdx.x * ldg;
+    float v = 0.f, m = 0.f;
+    for (int i = threadIdx.x * 4; i < V; i += 1024) {
+        const auto q = load_n<float, 4>(g + i, V - i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { v += q.v[e]; m = fmaxf(m, q.v[e] != q.v[e] ? INFINITY : fabsf(q.v[e])); }
+    }
+    v = wave_sum(v);
+    m = wave_max(m);
+    if ((threadIdx.x & 63) == 0) { s[threadIdx.x >> 6] = v; p[threadIdx.x >> 6] = m; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        sum[blockIdx.x] = (s[0] + s[1]) + (s[2] + s[3]);
+        peak[blockIdx.x] = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
+    }
+}
+// dz = G - exp(lp) sum(G) of the live rows and the outputs [v0, v0 + width), packed; a workgroup a packed row
+struct LogDzArgs {
+    const float *G, *lp, *sum, *scale;
+    int64_t ldg;
+    const int32_t *live, *idx;
+    int32_t V, v0, width;
+    uint16_t* dz;
+    int64_t pitch;
+};
+template <class X> __global__ void __launch_bounds__(256) log_dz_kernel(LogDzArgs a) {
+    const int64_t c = blockIdx.x;
+    const int live = *a.live;
+    if (c >= (int64_t)(live + kRowPad - 1) / kRowPad * kRowPad) return;
+    uint16_t* row = a.dz + c * parts_of<X>() * a.pitch;
+    const bool in = c < live;
+    const int64_t n = in ? a.idx[c] : 0;
+    const float* g = a.G + n * a.ldg + a.v0;
+    const float* lp = a.lp + n * a.V + a.v0;
+    const float s = in ? a.sum[n] : 0.f, inv = 1.f / *a.scale;
+    const int width = in ? a.width : 0;
+    for (int v = threadIdx.x * 4; v < a.pitch; v += 1024) {
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
+        if (v < width) {
+            const auto q = load_n<float, 4>(g + v, width - v);
+            const auto l = load_n<float, 4>(lp + v, width - v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[e] = v + e < width ? (q.v[e] - __expf(l.v[e]) * s) * inv : 0.f;
+        }
+        store_dz4<X>(row, a.pitch, v, d);
+    }
+}
+
+// ---- host side --------------------------------------------------------------------------------------------------------
+namespace {
+constexpr size_t kPieceBytes = (size_t)256 << 20;      // gradients of logits in hand at a time: what the last-level cache holds
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+
+// Tile shape and K splits of a product of m x n over `its` K tiles.  256 x 256 tiles run one per CU at 1.15 times the rate of
+// 128 x 128 tiles, which run two per CU (measured at 5120 x 16384 x 512: 926 against 837 TFLOP/s; 4096^3: 1172 / 983); the
+// cheaper of both by rounds of the chip is taken.  A product that does not fill the chip is split over K while a split
+// keeps 8 K tiles; a split costs about 6 K tiles (its prologue and the partial sums).
+struct Grid { bool big; int mt, nt, splits; };
+Grid plan_grid(int64_t m, int64_t n, int64_t its, bool may_split) {
+    Grid best = {};
+    double least = 0;
+    for (int big = 0; big < 2; ++big) {
+        const int64_t b = big ? 256 : 128, mt = ceil_div(m, b), nt = ceil_div(n, b);
+        const int64_t slots = big ? kCUs : 2 * kCUs;
+        for (int64_t s = 1; s == 1 || (may_split && s <= 32 && its / s >= 8); ++s) {
+            const double cost = (double)ceil_div(mt * nt * s, slots) * (big ? 4.0 : 2 * 1.15) * (double)(ceil_div(its, s) + 6);
+            if (least == 0 || cost < least) { least = cost; best = {big != 0, (int)mt, (int)nt, (int)s}; }
+        }
+    }
+    return best;
+}
+
+struct Arena {               // carves the workspace; with base == NULL it only counts
+    char* base;
+    size_t used = 0;
+    template <class T> T* take(size_t n) {
+        T* p = base ? (T*)(base + used) : nullptr;
+        used = (used + n * sizeof(T) + 255) & ~(size_t)255;
+        return p;
+    }
+};
+
+enum { kLogFwd = 0, kLogBwd = 1, kCeFwd = 2, kCeBwd = 3 };
+struct LinearPlan {
+    int what, D, V, type, parts, Dp;
+    int64_t N, Npad, pitch, width;      // width: outputs of a piece, pitch: its padded row
+    int pieces;
+    Grid fwd, logp, dz, dx, dw;
+    Rows rows;
+    uint16_t *xp, *wp, *dzp;
+    float *top, *sum, *all, *zt, *gsum, *gpeak, *part_x, *part_w, *part_c;
+    size_t bytes;
+};
+int make_linear_plan(int what, int64_t N, int32_t D, int32_t V, int32_t type, void* ws, LinearPlan* out) {
+    if (!known_type(type)) return wf_fail(WF_EINVAL, "wf_linear: unknown element type");
+    if (N < 0 || D < 1 || V < 1) return wf_fail(WF_EINVAL, "wf_linear: bad size (N %lld, D %d, V %d)", (long long)N, D, V);
+    if (N > (1 << 30) || D > (1 << 20) || V > (1 << 24) || ceil_div(N, 128) * ceil_div(V, 128) > (1 << 29))
+        return wf_fail(WF_EUNSUPPORTED, "wf_linear: N %lld, D %d, V %d is beyond what one call takes", (long long)N, D, V);
+    LinearPlan p = {};
+    p.what = what; p.N = N; p.D = D; p.V = V; p.type = type;
+    p.parts = type == WF_F32 ? 3 : 1;
+    const int products = type == WF_F32 ? 6 : 1;
+    p.Dp = (int)round_up(D, kBK);
+    p.Npad = std::max<int64_t>(kRowPad, round_up(N, kRowPad));
+    const bool bwd = what == kLogBwd || what == kCeBwd;
+    Arena a = {(char*)ws};
+    p.rows.live = a.take<int32_t>(1);
+    p.rows.scale = a.take<float>(1);
+    p.rows.pos = a.take<int32_t>(N);
+    p.rows.idx = a.take<int32_t>(p.Npad);
+    p.rows.target = a.take<int32_t>(p.Npad);
+    p.rows.g = a.take<float>(p.Npad);
+    p.rows.lse = a.take<float>(p.Npad);
+    p.xp = a.take<uint16_t>((size_t)p.Npad * p.parts * p.Dp);
+    p.wp = a.take<uint16_t>((size_t)V * p.parts * p.Dp);
+    const int64_t dits = (int64_t)products * p.Dp / kBK;
+    if (!bwd) {
+        p.fwd = plan_grid(V, N, dits, false);
+        p.logp = plan_grid(N, V, dits, false);
+        const size_t q = (size_t)p.fwd.mt * 2 * p.Npad;
+        p.top = a.take<float>(q);
+        p.sum = a.take<float>(q);
+        if (what == kCeFwd) { p.all = a.take<float>(q); p.zt = a.take<float>(p.Npad); }
+        else p.zt = a.take<float>(p.Npad);            // lse
+    } else {
+        const int64_t fit = std::max<int64_t>(kRowPad, (int64_t)(kPieceBytes / ((size_t)p.Npad * p.parts * 2)) / kRowPad * kRowPad);
+        p.pieces = (int)ceil_div(V, fit);
+        p.width = p.pitch = round_up(ceil_div(V, p.pieces), kRowPad);
+        p.pieces = (int)ceil_div(V, p.width);
+        p.dzp = a.take<uint16_t>((size_t)p.Npad * p.parts * p.pitch);
+        p.dz = plan_grid(p.width, N, dits, false);
+        p.dx = plan_grid(D, N, products * p.pitch / kBK, true);
+        p.dw = plan_grid(D, p.width, products * ceil_div(N, kBK), true);
+        if (p.dx.splits > 1 || p.pieces > 1) p.part_x = a.take<float>((size_t)p.dx.splits * N * D);
+        if (p.dw.splits > 1) p.part_w = a.take<float>((size_t)p.dw.splits * p.width * D);
+        p.part_c = a.take<float>((size_t)p.dw.splits * p.width);
+        if (what == kLogBwd) { p.gsum = a.take<float>(N); p.gpeak = a.take<float>(N); }
+    }
+    p.bytes = a.used + 256;
+    *out = p;
+    return WF_OK;
+}
+int linear_plan_in(int what, int64_t N, int32_t D, int32_t V, int32_t type, void* ws, size_t bytes, LinearPlan* out) {
+    char* at = (char*)(((uintptr_t)ws + 255) & ~(uintptr_t)255);
+    int rc = make_linear_plan(what, N, D, V, type, at, out);
+    if (rc) return rc;
+    if (!ws || bytes < out->bytes) return wf_fail(WF_ENOSPC, "wf_linear: workspace too small (%zu B given, %zu B needed)", bytes, out->bytes);
+    return WF_OK;
+}
+
+void set_parts(Product* p, int type, int64_t aplane, int64_t bplane) {
+    static const int part_a[6] = {0, 0, 0, 1, 1, 2}, part_b[6] = {0, 1, 2, 0, 1, 0};
+    p->parts = type == WF_F32 ? 6 : 1;
+    for (int i = 0; i < 6; ++i) {
+        p->aoff[i] = (int32_t)(type == WF_F32 ? part_a[i] * aplane : 0);
+        p->boff[i] = (int32_t)(type == WF_F32 ? part_b[i] * bplane : 0);
+    }
+}
+unsigned grid_of(const Product& p) { return (unsigned)(ceil_div((int64_t)p.mtiles * p.ntiles * p.splits, 8) * 8); }
+template <class F> void with_half(int type, F&& f) { if (type == WF_F16) f(f16()); else f(bf16()); }
+template <class F> void with_big(bool big, F&& f) { if (big) f(std::true_type()); else f(std::false_type()); }
+
+bool direct_rows(const void* p, int64_t ld, int64_t D, int type) {   // usable as an operand where it lies
+    return type != WF_F32 && D % kBK == 0 && ld % 8 == 0 && (uintptr_t)p % 16 == 0;
+}
+int pack_rows(const PackArgs& a, int type, hipStream_t st) {
+    with_type(type, [&](auto t) { pack_kernel<decltype(t)><<<(unsigned)ceil_div(a.N + kRowPad, 4), 256, 0, st>>>(a); });
+    HIP_TRY(hipGetLastError());
+    return WF_OK;
+}
+// W as an operand: where it lies, or packed
+int weight_operand(const LinearPlan& p, const void* w, int64_t ldw, hipStream_t st, Operand* o) {
+    if (direct_rows(w, ldw, p.D, p.type)) { *o = {w, ldw, p.V, p.Dp}; return WF_OK; }
+    *o = {p.wp, (int64_t)p.parts * p.Dp, p.V, p.Dp};
+    PackArgs a = {w, ldw, p.V, p.D, p.Dp, nullptr, nullptr, p.wp, nullptr, 0};
+    with_type(p.type, [&](auto t) { pack_kernel<decltype(t)><<<(unsigned)ceil_div(p.V, 4), 256, 0, st>>>(a); });   // (no rows behind W)
+    HIP_TRY(hipGetLastError());
+    return WF_OK;
+}
+Operand packed_x(const LinearPlan& p) { return {p.xp, (int64_t)p.parts * p.Dp, (int32_t)p.Npad, p.Dp}; }
+
+int linear_check(const char* who, const void* x, int64_t ldx, int64_t N, const void* w, int64_t ldw, const void* bias, int32_t btype) {
+    if (!w || (N > 0 && !x)) return wf_fail(WF_EINVAL, "%s: null pointer", who);
+    if (ldx < 0 || ldw < 0) return wf_fail(WF_EINVAL, "%s: negative row stride", who);
+    if (bias && !known_type(btype)) return wf_fail(WF_EINVAL, "%s: unknown element type", who);
+    return WF_OK;
+}
+
+int run_stats(const LinearPlan& p, const Operand& w, const Operand& x, const void* bias, int btype, const int32_t* live,
+              const int32_t* target, bool all, hipStream_t st) {
+    StatsArgs s = {};
+    s.p = {w, x, p.fwd.mt, p.fwd.nt, p.Dp / kBK, 1, {}, {}, live, 0, 1};
+    set_parts(&s.p, p.type, p.Dp, p.Dp);
+    s.l = {bias, btype, 0, p.V};
+    s.top = p.top; s.sum = p.sum; s.all = all ? p.all : nullptr; s.pitch = p.Npad; s.target = target; s.zt = p.zt;
+    with_half(p.type, [&](auto t) {
+        with_big(p.fwd.big, [&](auto b) {
+            stats_kernel<decltype(t), decltype(b)::value><<<grid_of(s.p), Shape<decltype(b)::value>::kThreads, 0, st>>>(s);
+        });
+    });
+    HIP_TRY(hipGetLastError());
+    return WF_OK;
+}
+
+// dx, dW, db from a piece's dz, then the next piece: dx is summed over the pieces, dW and db are final per piece
+struct GradOut { void *dx, *dw, *db; int btype; };
+int run_grads(const LinearPlan& p, const Operand& w, int piece, const GradOut& o, hipStream_t st) {
+    const int64_t v0 = piece * p.width, width = std::min<int64_t>(p.width, p.V - v0);
+    const Operand x = packed_x(p);
+    const int64_t zld = p.parts * p.pitch;
+    if (o.dx) {
+        GradArgs g = {};
+        Operand wv = {(const uint16_t*)w.p + v0 * w.ld, w.ld, (int32_t)width, w.cols};
+        Operand z = {p.dzp, zld, (int32_t)p.Npad, (int32_t)p.pitch};
+        g.p = {wv, z, p.dx.mt, p.dx.nt, (int32_t)ceil_div(width, kBK), 1, {}, {}, p.rows.live, 0, p.dx.splits};
+        set_parts(&g.p, p.type, p.Dp, p.pitch);
+        g.M = p.D; g.N = p.N; g.part = p.part_x; g.add = piece > 0; g.scale = p.rows.scale; g.out = o.dx; g.otype = p.type; g.idx = p.rows.idx;
+        with_half(p.type, [&](auto t) {
+            with_big(p.dx.big, [&](auto b) {
+                grad_kernel<decltype(t), decltype(b)::value, false, false><<<grid_of(g.p), Shape<decltype(b)::value>::kThreads, 0, st>>>(g);
+            });
+        });
+        HIP_TRY(hipGetLastError());
+        if (p.part_x && piece == p.pieces - 1) {
+            FoldArgs f = {p.part_x, nullptr, p.rows.scale, p.dx.splits, p.D, p.N, p.rows.live, p.rows.idx, o.dx, nullptr, p.type, 0};
+            fold_kernel<<<(unsigned)std::min<int64_t>(ceil_div(p.N * p.D, 1024), 2048), 256, 0, st>>>(f);
+            HIP_TRY(hipGetLastError());
+        }
+    }
+    if (o.dw || o.db) {
+        const size_t es = p.type == WF_F32 ? 4 : 2, bs = o.btype == WF_F32 ? 4 : 2;
+        GradArgs g = {};
+        Operand z = {p.dzp, zld, (int32_t)p.Npad, (int32_t)p.pitch};
+        g.p = {x, z, p.dw.mt, (int32_t)ceil_div(width, p.dw.big ? 256 : 128), (int32_t)ceil_div(p.N, kBK), 1, {}, {}, p.rows.live, 1, p.dw.splits};
+        set_parts(&g.p, p.type, p.Dp, p.pitch);
+        g.M = o.dw ? p.D : 0; g.N = width; g.part = p.part_w; g.colpart = o.db ? p.part_c : nullptr; g.scale = p.rows.scale;
+        g.out = o.dw ? (char*)o.dw + (size_t)v0 * p.D * es : nullptr;
+        g.otype = p.type;
+        g.colout = o.db ? (char*)o.db + v0 * bs : nullptr;
+        g.ctype = o.btype;
+        if (!o.dw) g.p.mtiles = 1;
+        with_half(p.type, [&](auto t) {
+            with_big(p.dw.big, [&](auto b) {
+                grad_kernel<decltype(t), decltype(b)::value, true, true><<<grid_of(g.p), Shape<decltype(b)::value>::kThreads, 0, st>>>(g);
+            });
+        });
+        HIP_TRY(hipGetLastError());
+        if (p.part_w) {
+            FoldArgs f = {p.part_w, g.colpart, p.rows.scale, p.dw.splits, g.M, width, nullptr, nullptr, g.out, g.colout, p.type, o.btype};
+            fold_kernel<<<(unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(width * p.D, 1024), 2048)), 256, 0, st>>>(f);
+            HIP_TRY(hipGetLastError());
+        }
+    }
+    return WF_OK;
+}
+__global__ void __launch_bounds__(256) zero_rows_kernel(uint16_t* p, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0;
+}
+int zero_fill(void* p, int64_t elements, int type, hipStream_t st) {
+    const int64_t n = elements * (type == WF_F32 ? 2 : 1);
+    if (!p || n == 0) return WF_OK;
+    zero_rows_kernel<<<(unsigned)std::min<int64_t>(ceil_div(n, 256), 2048), 256, 0, st>>>((uint16_t*)p, n);
+    HIP_TRY(hipGetLastError());
+    return WF_OK;
+}
+}  // namespace
+
+extern "C" int wf_linear_workspace_bytes(int32_t what, int64_t N, int32_t D, int32_t V, int32_t type, size_t* bytes) {
+    if (!bytes) return wf_fail(WF_EINVAL, "null bytes");
+    if (what < 0 || what > 3) return wf_fail(WF_EINVAL, "wf_linear_workspace_bytes: unknown call %d", what);
+    LinearPlan p;
+    int rc = make_linear_plan(what, N, D, V, type, nullptr, &p);
+    if (rc) return rc;
+    *bytes = p.bytes;
+    return WF_OK;
+}
+
+extern "C" int wf_linear_log_softmax(const void* x, int64_t ldx, int64_t N, int32_t D, const void* weight, int64_t ldw, int32_t V,
+                                     int32_t type, const void* bias, int32_t bias_type, float* log_probs, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+    int rc = linear_check("wf_linear_log_softmax", x, ldx, N, weight, ldw, bias, bias_type);
+    if (rc) return rc;
+    LinearPlan p;
+    if ((rc = linear_plan_in(kLogFwd, N, D, V, type, workspace, workspace_bytes, &p))) return rc;
+    if (N == 0) return WF_OK;
+    if (!log_probs) return wf_fail(WF_EINVAL, "wf_linear_log_softmax: null pointer");
+    hipStream_t st = (hipStream_t)stream;
+    Operand w, xo = {x, ldx, (int32_t)N, p.Dp};
+    if ((rc = weight_operand(p, weight, ldw, st, &w))) return rc;
+    if (!direct_rows(x, ldx, D, type)) {
+        xo = packed_x(p);
+        if ((rc = pack_rows({x, ldx, N, D, p.Dp, nullptr, nullptr, p.xp, nullptr, 1}, type, st))) return rc;
+    }
+    if ((rc = run_stats(p, w, xo, bias, bias_type, nullptr, nullptr, false, st))) return rc;
+    JoinArgs j = {p.top, p.sum, nullptr, nullptr, p.Npad, N, p.fwd.mt * 2, V, nullptr, nullptr, nullptr, 0.f, p.zt, nullptr};
+    join_kernel<<<(unsigned)ceil_div(N, 256), 256, 0, st>>>(j);
+    LogProbArgs l = {};
+    l.p = {xo, w, p.logp.mt, p.logp.nt, p.Dp / kBK, 1, {}, {}, nullptr, 0, 1};
+    set_parts(&l.p, type, p.Dp, p.Dp);
+    l.l = {bias, bias_type, 0, V};
+    l.lse = p.zt; l.out = log_probs; l.N = N;
+    with_half(type, [&](auto t) {
+        with_big(p.logp.big, [&](auto b) {
+            log_prob_kernel<decltype(t), decltype(b)::value><<<grid_of(l.p), Shape<decltype(b)::value>::kThreads, 0, st>>>(l);
+        });
+    });
+    HIP_TRY(hipGetLastError());
+    return WF_OK;
+}
+
+extern "C" int wf_linear_log_softmax_backward(const float* log_probs, const float* grad, int64_t ldg, const void* x, int64_t ldx,
+                                              int64_t N, int32_t D, const void* weight, int64_t ldw, int32_t V, int32_t type,
+                                              int32_t bias_type, void* dx, void* dweight, void* dbias, void* workspace,
+                                              size_t workspace_bytes, void* stream) {
+    int rc = linear_check("wf_linear_log_softmax_backward", x, ldx, N, weight, ldw, dbias, bias_type);
+    if (rc) return rc;
+    LinearPlan p;
+    if ((rc = linear_plan_in(kLogBwd, N, D, V, type, workspace, workspace_bytes, &p))) return rc;
+    hipStream_t st = (hipStream_t)stream;
+    if (N == 0) return (rc = zero_fill(dweight, (int64_t)V * D, type, st)) ? rc : zero_fill(dbias, V, bias_type, st);
+    if (!log_probs || !grad || ldg < 0) return wf_fail(WF_EINVAL, "wf_linear_log_softmax_backward: null pointer");
+    Operand w;
+    if ((rc = weight_operand(p, weight, ldw, st, &w))) return rc;
+    grad_rows_kernel<<<(unsigned)N, 256, 0, st>>>(grad, ldg, V, p.gsum, p.gpeak);
+    RowsArgs r = {};
+    r.r = p.rows; r.N = N; r.V = V; r.peak = p.gpeak; r.hit = 1.f;
+    rows_kernel<<<1, 1024, 0, st>>>(r);
+    if ((rc = pack_rows({x, ldx, N, D, p.Dp, p.rows.pos, p.rows.live, p.xp, dx, 1}, type, st))) return rc;
+    for (int piece = 0; piece < p.pieces; ++piece) {
+        const int64_t v0 = piece * p.width;
+        LogDzArgs z = {grad, log_probs, p.gsum, p.rows.scale, ldg, p.rows.live, p.rows.idx, V, (int32_t)v0,
+                       (int32_t)std::min<int64_t>(p.width, V - v0), p.dzp, p.pitch};
+        with_type(type, [&](auto t) { log_dz_kernel<decltype(t)><<<(unsigned)p.Npad, 256, 0, st>>>(z); });
+        HIP_TRY(hipGetLastError());
+        if ((rc = run_grads(p, w, piece, {dx, dweight, dbias, bias_type}, st))) return rc;
+    }
+    return WF_OK;
+}
+
+extern "C" int wf_linear_cross_entropy(const void* x, int64_t ldx, int64_t N, int32_t D, const void* weight, int64_t ldw, int32_t V,
+                                       int32_t type, const void* bias, int32_t bias_type, const void* targets, int32_t targets_wide,
+                                       int64_t ignore_index, float smoothing, float* loss, float* lse, float* total,
+                                       int32_t mean, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = linear_check("wf_linear_cross_entropy", x, ldx, N, weight, ldw, bias, bias_type);
+    if (rc) return rc;
+    if (!(smoothing >= 0.f && smoothing <= 1.f)) return wf_fail(WF_EINVAL, "wf_linear_cross_entropy: label smoothing %g", smoothing);
+    LinearPlan p;
+    if ((rc = linear_plan_in(kCeFwd, N, D, V, type, workspace, workspace_bytes, &p))) return rc;
+    hipStream_t st = (hipStream_t)stream;
+    if (N == 0) return zero_fill(total, 1, WF_F32, st);
+    if (!targets || !loss || !lse) return wf_fail(WF_EINVAL, "wf_linear_cross_entropy: null pointer");
+    Operand w;
+    if ((rc = weight_operand(p, weight, ldw, st, &w))) return rc;
+    RowsArgs r = {};
+    r.r = p.rows; r.N = N; r.V = V; r.targets = targets; r.target_wide = targets_wide; r.ignore = ignore_index; r.loss = loss; r.lse = lse;
+    rows_kernel<<<1, 1024, 0, st>>>(r);
+    if ((rc = pack_rows({x, ldx, N, D, p.Dp, p.rows.pos, p.rows.live, p.xp, nullptr, 1}, type, st))) return rc;
+    if ((rc = run_stats(p, w, packed_x(p), bias, bias_type, p.rows.live, p.rows.target, smoothing != 0.f, st))) return rc;
+    JoinArgs j = {p.top, p.sum, smoothing != 0.f ? p.all : nullptr, p.zt, p.Npad, N, p.fwd.mt * 2, V, p.rows.live, p.rows.idx,
+                  p.rows.target, smoothing, lse, loss};
+    join_kernel<<<(unsigned)ceil_div(N, 256), 256, 0, st>>>(j);
+    if (total) total_kernel<<<1, 1024, 0, st>>>(loss, N, p.rows.live, mean, total);
+    HIP_TRY(hipGetLastError());
+    return WF_OK;
+}
+
+extern "C" int wf_linear_cross_entropy_backward(const float* grad, int32_t grad_rows, int32_t mean, const float* lse, const void* x,
+                                                int64_t ldx, int64_t N, int32_t D, const void* weight, int64_t ldw, int32_t V,
+                                                int32_t type, const void* bias, int32_t bias_type, const void* targets,
+                                                int32_t targets_wide, int64_t ignore_index, float smoothing, void* dx,
+                                                void* dweight, void* dbias, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = linear_check("wf_linear_cross_entropy_backward", x, ldx, N, weight, ldw, bias, bias_type);
+    if (rc) return rc;
+    if (dbias && !known_type(bias_type)) return wf_fail(WF_EINVAL, "wf_linear_cross_entropy_backward: unknown element type");
+    if (!(smoothing >= 0.f && smoothing <= 1.f)) return wf_fail(WF_EINVAL, "wf_linear_cross_entropy_backward: label smoothing %g", smoothing);
+    LinearPlan p;
+    if ((rc = linear_plan_in(kCeBwd, N, D, V, type, workspace, workspace_bytes, &p))) return rc;
+    hipStream_t st = (hipStream_t)stream;
+    if (N == 0) return (rc = zero_fill(dweight, (int64_t)V * D, type, st)) ? rc : zero_fill(dbias, V, bias_type, st);
+    if (!targets || !grad || !lse) return wf_fail(WF_EINVAL, "wf_linear_cross_entropy_backward: null pointer");
+    Operand w;
+    if ((rc = weight_operand(p, weight, ldw, st, &w))) return rc;
+    RowsArgs r = {};
+    r.r = p.rows; r.N = N; r.V = V; r.targets = targets; r.target_wide = targets_wide; r.ignore = ignore_index;
+    r.gout = grad; r.gout_rows = grad_rows; r.mean = mean; r.lse_in = lse; r.hit = smoothing < 1.f ? 1.f - smoothing : 1.f;
+    rows_kernel<<<1, 1024, 0, st>>>(r);
+    if ((rc = pack_rows({x, ldx, N, D, p.Dp, p.rows.pos, p.rows.live, p.xp, dx, 1}, type, st))) return rc;
+    for (int piece = 0; piece < p.pieces; ++piece) {
+        const int64_t v0 = piece * p.width, width = std::min<int64_t>(p.width, V - v0);
+        DzArgs z = {};
+        Operand wv = {(const uint16_t*)w.p + v0 * w.ld, w.ld, (int32_t)width, w.cols};
+        z.p = {wv, packed_x(p), (int32_t)ceil_div(width, p.dz.big ? 256 : 128), p.dz.nt, p.Dp / kBK, 1, {}, {}, p.rows.live, 0, 1};
+        set_parts(&z.p, type, p.Dp, p.Dp);
+        z.l = {bias, bias_type, (int32_t)v0, (int32_t)(v0 + width)};
+        z.target = p.rows.target; z.g = p.rows.g; z.lse = p.rows.lse; z.smoothing = smoothing; z.outputs = V; z.dz = p.dzp; z.pitch = p.pitch;
+        with_type(type, [&](auto t) {
+            with_big(p.dz.big, [&](auto b) {
+                dz_kernel<decltype(t), decltype(b)::value><<<grid_of(z.p), Shape<decltype(b)::value>::kThreads, 0, st>>>(z);
+            });
+        });
+        HIP_TRY(hipGetLastError());
+        if ((rc = run_grads(p, w, piece, {dx, dweight, dbias, bias_type}, st))) return rc;
+    }
+    return WF_OK;
+}

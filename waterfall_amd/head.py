@@ -18,7 +18,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 from .graph import _on, _ptr, _stream
 
-__all__ = ["layer_norm", "dropout"]
+__all__ = ["layer_norm", "dropout", "linear_log_softmax", "linear_cross_entropy", "OutputHead"]
 
 _TYPES = {torch.float32: _lib.WF_F32, torch.bfloat16: _lib.WF_BF16, torch.float16: _lib.WF_F16}
 
@@ -159,3 +159,184 @@ def dropout(x, p, seed):
     else:
         seed = int(seed) & 0xFFFFFFFFFFFFFFFF
     return _Dropout.apply(x, p, seed)
+
+
+# ---- the projection ---------------------------------------------------------------------------------------------------
+
+_LOG_FWD, _LOG_BWD, _CE_FWD, _CE_BWD = range(4)
+
+
+def _linear_ws(what, N, D, V, x):
+    n = C.c_size_t(0)
+    _lib.check(_lib.lib().wf_linear_workspace_bytes(what, N, D, V, _TYPES[x.dtype], C.byref(n)))
+    return torch.empty(n.value, dtype=torch.uint8, device=x.device), n.value
+
+
+def _check_linear(who, x, weight, bias):
+    _check(x, "x")
+    _check(weight, "weight", like=x, dtype=x.dtype)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"{who}: x needs a last dimension of at least one element")
+    if weight.dim() != 2 or weight.shape[1] != x.shape[-1] or weight.shape[0] < 1:
+        raise ValueError(f"{who}: weight has shape {tuple(weight.shape)}, expected [V, {x.shape[-1]}]")
+    if bias is not None:
+        _check(bias, "bias", like=x)
+        if bias.shape != weight.shape[:1]:
+            raise ValueError(f"{who}: bias has shape {tuple(bias.shape)}, expected [{weight.shape[0]}]")
+
+
+def _linear_args(x, weight, bias):
+    """(what keeps the tensors alive, the arguments x .. type)"""
+    v, ldx = _rows(x)
+    w, ldw = _rows(weight)
+    N, D = v.shape
+    return (v, w), (_ptr(v), ldx, N, D, _ptr(w), ldw, w.shape[0], _TYPES[x.dtype])
+
+
+class _LinearLogSoftmax(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        dev = x.device
+        keep, a = _linear_args(x, weight, bias)
+        N, D, V = a[2], a[3], a[6]
+        bt = _TYPES[bias.dtype] if bias is not None else 0
+        lp = torch.empty(x.shape[:-1] + (V,), dtype=torch.float32, device=dev)
+        with _on(dev):
+            ws, n = _linear_ws(_LOG_FWD, N, D, V, x)
+            _lib.check(_lib.lib().wf_linear_log_softmax(*a, _ptr(bias), bt, _ptr(lp), _ptr(ws), n, _stream(dev)))
+        ctx.save_for_backward(x, weight, bias, lp)
+        return lp
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        x, weight, bias, lp = ctx.saved_tensors
+        dev = x.device
+        keep, a = _linear_args(x, weight, bias)
+        N, D, V = a[2], a[3], a[6]
+        g, ldg = _rows(grad)
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if ctx.needs_input_grad[0] else None
+        dw = torch.empty(weight.shape, dtype=x.dtype, device=dev) if ctx.needs_input_grad[1] else None
+        db = torch.empty(V, dtype=bias.dtype, device=dev) if ctx.needs_input_grad[2] else None
+        with _on(dev):
+            ws, n = _linear_ws(_LOG_BWD, N, D, V, x)
+            _lib.check(_lib.lib().wf_linear_log_softmax_backward(
+                _ptr(lp), _ptr(g), ldg, *a, _TYPES[bias.dtype] if bias is not None else 0, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), n,
+                _stream(dev)))
+        return dx, dw, db
+
+
+def linear_log_softmax(x, weight, bias=None):
+    """log_softmax(x weight^T + bias) as float32 [..., V]: the log-probabilities that ``DenseFsaVec`` takes.
+
+    x [..., D], weight [V, D]: float32, bfloat16 or float16, both of one type; bias [V] or None, any of the three.  float32 is
+    computed to float32's accuracy (no reduced-precision product).  A bias of -inf masks an output; a row whose every output
+    is masked is all -inf and has no gradient.  In the backward pass rows whose incoming gradient is all zero (frames behind an
+    utterance's end) are left out whatever they hold; 16-bit types round the gradient of a logit to x's type before it enters
+    the products."""
+    _check_linear("linear_log_softmax", x, weight, bias)
+    return _LinearLogSoftmax.apply(x, weight, None if bias is None else bias.contiguous())
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, targets, bias, ignore_index, smoothing, reduction):
+        dev = x.device
+        keep, a = _linear_args(x, weight, bias)
+        N, D, V = a[2], a[3], a[6]
+        ctx.rest = (_TYPES[bias.dtype] if bias is not None else 0, 1 if targets.dtype == torch.int64 else 0, ignore_index, smoothing)
+        ctx.reduction = reduction
+        bt, wide = ctx.rest[:2]
+        loss = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+        lse = torch.empty(N, dtype=torch.float32, device=dev)
+        total = torch.empty((), dtype=torch.float32, device=dev) if reduction != "none" else None
+        with _on(dev):
+            ws, n = _linear_ws(_CE_FWD, N, D, V, x)
+            _lib.check(_lib.lib().wf_linear_cross_entropy(*a, _ptr(bias), bt, _ptr(targets), wide, ignore_index, smoothing, _ptr(loss),
+                                                          _ptr(lse), _ptr(total), 1 if reduction == "mean" else 0, _ptr(ws), n,
+                                                          _stream(dev)))
+        ctx.save_for_backward(x, weight, targets, bias, lse)
+        return loss if total is None else total
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        x, weight, targets, bias, lse = ctx.saved_tensors
+        dev = x.device
+        keep, a = _linear_args(x, weight, bias)
+        N, D, V = a[2], a[3], a[6]
+        bt, wide, ignore_index, smoothing = ctx.rest
+        g = grad.contiguous()
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if ctx.needs_input_grad[0] else None
+        dw = torch.empty(weight.shape, dtype=x.dtype, device=dev) if ctx.needs_input_grad[1] else None
+        db = torch.empty(V, dtype=bias.dtype, device=dev) if ctx.needs_input_grad[3] else None
+        with _on(dev):
+            ws, n = _linear_ws(_CE_BWD, N, D, V, x)
+            _lib.check(_lib.lib().wf_linear_cross_entropy_backward(
+                _ptr(g), 1 if ctx.reduction == "none" else 0, 1 if ctx.reduction == "mean" else 0, _ptr(lse), *a, _ptr(bias), bt,
+                _ptr(targets), wide, ignore_index, smoothing, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), n, _stream(dev)))
+        return dx, dw, None, db, None, None, None
+
+
+def linear_cross_entropy(x, weight, targets, bias=None, ignore_index=-1, label_smoothing=0.0, reduction="mean"):
+    """Softmax cross entropy of x weight^T + bias against ``targets``, without keeping the logits: forward leaves one number per
+    row, backward computes the logits again piece by piece.
+
+    x [..., D], weight [V, D], bias as for ``linear_log_softmax``; targets [...]: int32 or int64.  Rows whose target is
+    ``ignore_index`` (by default -1, the label of the arcs that take no frame) have no loss, no gradient and may hold anything.
+    A target that is neither it nor an output makes its row's loss NaN (nothing is read out of range) and has no gradient.
+
+    reduction: 'none' (float32 [...]), 'sum', or 'mean' over the rows that take part (0 where there are none)."""
+    _check_linear("linear_cross_entropy", x, weight, bias)
+    if not isinstance(targets, torch.Tensor) or targets.dtype not in (torch.int32, torch.int64):
+        raise TypeError("linear_cross_entropy: targets must be an int32 or int64 tensor")
+    if targets.device != x.device:
+        raise ValueError(f"linear_cross_entropy: targets are on {targets.device}, x is on {x.device}")
+    if targets.shape != x.shape[:-1]:
+        raise ValueError(f"linear_cross_entropy: targets have shape {tuple(targets.shape)}, expected {tuple(x.shape[:-1])}")
+    if not 0.0 <= float(label_smoothing) <= 1.0:
+        raise ValueError(f"linear_cross_entropy: label_smoothing must be in [0, 1], got {label_smoothing}")
+    if reduction not in ("none", "sum", "mean"):
+        raise ValueError(f"linear_cross_entropy: unknown reduction {reduction!r}")
+    return _LinearCrossEntropy.apply(x, weight, targets.contiguous(), None if bias is None else bias.contiguous(), int(ignore_index),
+                                     float(label_smoothing), reduction)
+
+
+class OutputHead(nn.Module):
+    """Encoder output [..., D] -> log-probabilities [..., V] for ``DenseFsaVec`` / ``graphloss``: layer norm, dropout (in
+    training), projection with log-softmax (the tail of the reference's models, ``rnnp.py:116-122``).
+
+        head = wf.OutputHead(encoder_dim, lang.num_nn_output, dropout=0.1)
+        loss = wf.graphloss(decoding_graph=graphs, dense_fsa_vec=wf.DenseFsaVec(head(enc), segments), ...)
+        loss = loss + 0.1 * head.cross_entropy(enc, frame_targets)         # on the same projection
+
+    Parameters may be float32 beside 16-bit activations: the projection's are cast to the activations' type.  Dropout takes
+    its seed from torch's generator of the device (``torch.manual_seed``), on the device: it can be captured in a graph."""
+
+    def __init__(self, idim, num_outputs, dropout=0.0, norm=True, bias=True, eps=1e-5, device=None, dtype=None):
+        super().__init__()
+        if not 0.0 <= dropout <= 1.0:
+            raise ValueError(f"OutputHead: dropout must be in [0, 1], got {dropout}")
+        kw = dict(device=device, dtype=dtype)
+        self.dropout, self.eps = float(dropout), float(eps)
+        self.norm_weight = nn.Parameter(torch.ones(idim, **kw)) if norm else None
+        self.norm_bias = nn.Parameter(torch.zeros(idim, **kw)) if norm else None
+        self.weight = nn.Parameter(torch.empty(num_outputs, idim, **kw))
+        self.bias = nn.Parameter(torch.zeros(num_outputs, **kw)) if bias else None
+        nn.init.normal_(self.weight, std=idim ** -0.5)
+
+    def features(self, x):
+        if self.norm_weight is not None:
+            x = layer_norm(x, self.norm_weight, self.norm_bias, self.eps)
+        if self.training and self.dropout > 0.0:
+            seed = torch.empty(1, dtype=torch.int64, device=x.device).random_()
+            x = dropout(x, self.dropout, seed)
+        return x
+
+    def forward(self, x):
+        x = self.features(x)
+        return linear_log_softmax(x, self.weight.to(x.dtype), self.bias)
+
+    def cross_entropy(self, x, targets, ignore_index=-1, label_smoothing=0.0, reduction="mean"):
+        x = self.features(x)
+        return linear_cross_entropy(x, self.weight.to(x.dtype), targets, self.bias, ignore_index, label_smoothing, reduction)
