@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 
@@ -464,8 +465,10 @@ extern "C" int wf_dropout(const void* x, int64_t n, int32_t type, double p, uint
 // A tile is staged by direct global -> LDS loads, double buffered, one barrier per 64 of K.  An operand is stored either
 // with K contiguous (rows of 64 K values are staged, fragments are plain 16-byte LDS reads) or with K as its row index (64
 // rows are staged, fragments come from the transposing LDS reads).  So W serves z = x W^T and dx = dz W, and x serves z
-// and dW = dz^T x, from one copy each.  16-byte chunks are permuted within their row so that both kinds of reads spread over
-// the banks: the permutation is applied to the global address, since the direct load writes LDS in lane order.
+// and dW = dz^T x, from one copy each.  16-byte chunks are permuted within their row so that 256 bytes read in a clock fall into
+// 64 different banks: chunk c of row r sits at c ^ (r / 2) % 8 (16 rows of 128 bytes at the same c), and at c ^ 4 (r % 4) where
+// K is the row (4 rows by 64 bytes).  The permutation is applied to the global address, since the direct load writes LDS in
+// lane order.  (Permutations that spread only 128 bytes, r % 8 and 2 (r % 4), had half of all LDS cycles lost to conflicts.)
 
 struct Operand {
     const void* p;           // 16-bit elements
@@ -505,7 +508,7 @@ template <int R, int WAVES, bool KROW> struct Stage {
     static constexpr int kLoads = (KROW ? kBK : R) / kPer / WAVES;
     static_assert(!KROW || WAVES % 2 == 0, "the row permutation of a lane is the same for all its loads");
     const char* base;        // uniform: start of the tile's rows
-    uint32_t off[kLoads];    // this lane's byte offsets
+    uint32_t off[KROW ? 1 : kLoads];   // this lane's byte offsets
     int64_t kstep;           // bytes from one K tile to the next
     uint32_t pitch;          // KROW: bytes of a row
     int32_t lrow[KROW ? kLoads : 1];
@@ -520,7 +523,7 @@ template <int R, int WAVES, bool KROW> struct Stage {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
                 const int row = (i * WAVES + wave) * kPer + r;
-                off[i] = (uint32_t)min(row, o.rows - 1 - first) * (uint32_t)(o.ld * 2) + (uint32_t)((c ^ (row & 7)) * 16);
+                off[i] = (uint32_t)min(row, o.rows - 1 - first) * (uint32_t)(o.ld * 2) + (uint32_t)((c ^ (row >> 1 & 7)) * 16);
             }
         } else {
             base = (const char*)o.p;
@@ -530,51 +533,93 @@ template <int R, int WAVES, bool KROW> struct Stage {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
                 lrow[i] = (i * WAVES + wave) * kPer + r;
-                col = (uint32_t)min(first + (c ^ ((lrow[i] & 3) << 1)) * 8, o.cols - 8) * 2;
-                off[i] = (uint32_t)lrow[i] * pitch + col;
+                col = (uint32_t)min(first + (c ^ ((lrow[i] & 3) << 2)) * 8, o.cols - 8) * 2;
             }
         }
     }
-    // K tile `kt` at element offset `part` of the operand into LDS
-    __device__ inline void load(char* lds, int kt, int part, int wave) const {
-        const char* b = base + (int64_t)part * 2 + kt * kstep;
-        char* dst = lds + wave * 1024;
-        if constexpr (KROW) {
-            const int left = rows - kt * kBK;        // rows of this tile that exist
-            if (left < kBK) {
-#pragma unroll
-                for (int i = 0; i < kLoads; ++i)
-                    __builtin_amdgcn_global_load_lds((glb_void*)(b + (int64_t)min(lrow[i], left - 1) * pitch + col), (lds_void*)(dst + i * WAVES * 1024), 16, 0, 0);
-                return;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i)
-            __builtin_amdgcn_global_load_lds((glb_void*)(b + off[i]), (lds_void*)(dst + i * WAVES * 1024), 16, 0, 0);
+    // Where K tile `kt` at element offset `part` of the operand starts
+    __device__ inline const char* tile(int kt, int part) const { return base + (int64_t)part * 2 + kt * kstep; }
+    // load i of that tile into LDS; `left`: rows of K that exist from there on
+    __device__ inline void load(char* lds, const char* from, int left, int i, int wave) const {
+        uint32_t o;
+        if constexpr (KROW) o = (uint32_t)min(lrow[i], left - 1) * pitch + col;
+        else o = off[i];
+        __builtin_amdgcn_global_load_lds((glb_void*)(from + o), (lds_void*)(lds + (i * WAVES + wave) * 1024), 16, 0, 0);
     }
-    // 8 values of K (16 ks + 8 (lane / 32) ..) of row `first` + lane % 32
-    template <class T> static __device__ inline typename Mfma<T>::v8 frag(const char* lds, int first, int ks, int lane) {
-        typename Mfma<T>::v8 v;
-        if constexpr (!KROW) {
-            const int r = first + (lane & 31), c = (ks * 2 + (lane >> 5)) ^ (r & 7);
-            v = *(const typename Mfma<T>::v8*)(lds + r * (kBK * 2) + c * 16);
-        } else {
-            // 16 lanes read 4 rows of K by 16 columns; lane i gets column i of the four rows
-            const int i = lane & 15, k = ks * 16 + (lane >> 5) * 8 + (i >> 2), c = first + (lane & 16) + (i & 3) * 4;
-            const int chunk = (c >> 3) ^ ((i >> 2) << 1);
-            const char* q = lds + k * (R * 2) + chunk * 16 + (c & 7) * 2;
-            union { v4s h[2]; typename Mfma<T>::v8 v; } u;
-            u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)q);
-            u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(q + 4 * R * 2));
-            v = u.v;
+    // 8 values of K (16 ks + 8 (lane / 32) ..) of rows `first` + 32 f + lane % 32, fragment f of F.  K contiguous: 16-byte reads.
+    template <class T, int F> static __device__ inline void frags(typename Mfma<T>::v8 (&v)[F], const char* lds, int first, int ks, int lane) {
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+            const int r = first + f * 32 + (lane & 31), c = (ks * 2 + (lane >> 5)) ^ (r >> 1 & 7);
+            v[f] = *(const typename Mfma<T>::v8*)(lds + r * (kBK * 2) + c * 16);
         }
-        return v;
+    }
+    // K as row index: 16 lanes read 4 rows of K by 16 columns and lane i gets column i of the four rows.  Where this lane reads
+    // fragment f of the first step (`first` is a multiple of 128 or of 64, and so is every 32 of it a step of the permutation).
+    static __device__ inline uint32_t address(int f, int first, int lane) {
+        const int i = lane & 15, k = (lane >> 5) * 8 + (i >> 2), c = first + f * 32 + (lane & 16) + (i & 3) * 4;
+        return (uint32_t)(k * (R * 2) + ((c >> 3) ^ ((i >> 2) << 2)) * 16 + (c & 7) * 2);
     }
 };
 
+// The transposing reads of a step's fragments, with their wait: the compiler's own form of them waits for every direct load in
+// flight.  OFF: bytes from the first step's rows, 4 ROW the second four rows of K.
+template <int OFF, int ROW, class V> __device__ inline void read_tr(V (&v)[2], const uint32_t (&p)[2]) {
+    typedef int v2i __attribute__((ext_vector_type(2)));
+    v2i r[4];
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
+        "ds_read_b64_tr_b16 %2, %5 offset:%6\n\tds_read_b64_tr_b16 %3, %5 offset:%7\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
+        : "v"(p[0]), "v"(p[1]), "n"(OFF), "n"(OFF + 4 * ROW) : "memory");
+    __builtin_memcpy(&v, &r, sizeof(r));
+}
+template <int OFF, int ROW, class V> __device__ inline void read_tr(V (&v)[4], const uint32_t (&p)[4]) {
+    typedef int v2i __attribute__((ext_vector_type(2)));
+    v2i r[8];
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+        : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "n"(OFF), "n"(OFF + 4 * ROW) : "memory");
+    __builtin_memcpy(&v, &r, sizeof(r));
+}
+template <int AOFF, int BOFF, int ROW, class V> __device__ inline void read_tr(V (&a)[2], const uint32_t (&p)[2], V (&b)[2], const uint32_t (&q)[2]) {
+    typedef int v2i __attribute__((ext_vector_type(2)));
+    v2i r[4], t[4];
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %4, %10 offset:%14\n\tds_read_b64_tr_b16 %5, %10 offset:%15\n\t"
+        "ds_read_b64_tr_b16 %6, %11 offset:%14\n\tds_read_b64_tr_b16 %7, %11 offset:%15\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(t[0]), "=&v"(t[1]), "=&v"(t[2]), "=&v"(t[3])
+        : "v"(p[0]), "v"(p[1]), "v"(q[0]), "v"(q[1]), "n"(AOFF), "n"(AOFF + 4 * ROW), "n"(BOFF), "n"(BOFF + 4 * ROW) : "memory");
+    __builtin_memcpy(&a, &r, sizeof(r));
+    __builtin_memcpy(&b, &t, sizeof(t));
+}
+template <int AOFF, int BOFF, int ROW, class V> __device__ inline void read_tr(V (&a)[4], const uint32_t (&p)[4], V (&b)[2], const uint32_t (&q)[2]) {
+    typedef int v2i __attribute__((ext_vector_type(2)));
+    v2i r[8], t[4];
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %12 offset:%18\n\tds_read_b64_tr_b16 %1, %12 offset:%19\n\t"
+        "ds_read_b64_tr_b16 %2, %13 offset:%18\n\tds_read_b64_tr_b16 %3, %13 offset:%19\n\t"
+        "ds_read_b64_tr_b16 %4, %14 offset:%18\n\tds_read_b64_tr_b16 %5, %14 offset:%19\n\t"
+        "ds_read_b64_tr_b16 %6, %15 offset:%18\n\tds_read_b64_tr_b16 %7, %15 offset:%19\n\t"
+        "ds_read_b64_tr_b16 %8, %16 offset:%20\n\tds_read_b64_tr_b16 %9, %16 offset:%21\n\t"
+        "ds_read_b64_tr_b16 %10, %17 offset:%20\n\tds_read_b64_tr_b16 %11, %17 offset:%21\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7]), "=&v"(t[0]),
+          "=&v"(t[1]), "=&v"(t[2]), "=&v"(t[3])
+        : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(q[0]), "v"(q[1]), "n"(AOFF), "n"(AOFF + 4 * ROW), "n"(BOFF), "n"(BOFF + 4 * ROW)
+        : "memory");
+    __builtin_memcpy(&a, &r, sizeof(r));
+    __builtin_memcpy(&b, &t, sizeof(t));
+}
+
 // The workgroup's accumulators: tile (tm, tn), K run `split`.  false: nothing to do (all of the tile's rows are dead).
 template <class T, int BM, int BN, int WM, int WN, bool AK, bool BK, bool COLSUM = false> struct Tile {
-    static constexpr int kWaves = WM * WN, kThreads = kWaves * 64;
+    static constexpr int kWaves = WM * WN, kThreads = kWaves * 64, kBand = 8;
     static constexpr int MI = BM / WM / 32, NI = BN / WN / 32;
     using SA = Stage<BM, kWaves, AK>;
     using SB = Stage<BN, kWaves, BK>;
@@ -584,14 +629,15 @@ template <class T, int BM, int BN, int WM, int WN, bool AK, bool BK, bool COLSUM
     int tm, tn, split, wm, wn, lane, live;
 
     __device__ inline bool place(const Product& p) {
-        // a chip's 8 dies take workgroups in turn: each die gets a run of neighbouring tiles, so that its L2 sees the same rows
-        // again.  Within a run the n tiles move slowest: the A tiles of one B tile follow each other.
+        // a chip's 8 dies take workgroups in turn: each die gets a run of neighbouring tiles, in bands of kBand m tiles, so that
+        // the 32 or 64 tiles that its CUs work on at a time share their rows in its L2
         const int tiles = p.mtiles * p.ntiles, all = tiles * p.splits, per = (all + 7) / 8;
         const int id = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
         if ((int)(blockIdx.x >> 3) >= per || id >= all) return false;
         split = id / tiles;
-        tm = id % tiles % p.mtiles;
-        tn = id % tiles / p.mtiles;
+        const int r = id % tiles, band = r / (kBand * p.ntiles), high = min(kBand, p.mtiles - band * kBand);
+        tm = band * kBand + (r - band * kBand * p.ntiles) % high;
+        tn = (r - band * kBand * p.ntiles) / high;
         lane = threadIdx.x & 63;
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         wm = wave % WM;
@@ -599,7 +645,8 @@ template <class T, int BM, int BN, int WM, int WN, bool AK, bool BK, bool COLSUM
         live = p.live ? __builtin_amdgcn_readfirstlane(*p.live) : 0x7fffffff;
         return p.live_is_k || tn * BN < live;
     }
-    __device__ inline void run(const Product& p, char* lds) {
+    // bias: NULL, or what the accumulators start from, by the tile's rows
+    __device__ inline void run(const Product& p, char* lds, const float* bias = nullptr) {
         const int wave = wm + wn * WM;
         SA sa;
         SB sb;
@@ -609,43 +656,114 @@ template <class T, int BM, int BN, int WM, int WN, bool AK, bool BK, bool COLSUM
         if (p.live_is_k) ktiles = min(ktiles, (live + kBK - 1) / kBK);
         const int its = ktiles * p.parts;
         const int from = (int)((int64_t)its * split / p.splits), to = (int)((int64_t)its * (split + 1) / p.splits);
+        constexpr int kSteps = kBK / 16, kLoads = SA::kLoads + SB::kLoads;
+        int part = 0, kt = 0;
+        if (from < to) { part = from / ktiles; kt = from % ktiles; }
+        const char *ta = nullptr, *tb = nullptr;
+        int la = 0, lb = 0;
+        auto next = [&]() {
+            ta = sa.tile(kt, p.aoff[part]);
+            tb = sb.tile(kt, p.boff[part]);
+            if constexpr (AK) la = sa.rows - kt * kBK;
+            if constexpr (BK) lb = sb.rows - kt * kBK;
+            if (++kt == ktiles) { kt = 0; ++part; }
+        };
+        auto load = [&](char* s, int i) {
+            if (i < SA::kLoads) sa.load(s, ta, la, i, wave);
+            else if (i < kLoads) sb.load(s + SA::kBytes, tb, lb, i - SA::kLoads, wave);
+        };
+        if (from < to) {
+            next();
 #pragma unroll
-        for (int i = 0; i < MI; ++i)
+            for (int i = 0; i < kLoads; ++i) load(lds, i);
+        }
+        if (bias) {
+            __syncthreads();
 #pragma unroll
-            for (int j = 0; j < NI; ++j) acc[i][j] = v16f{};
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const v4f v = *(const v4f*)(bias + wm * (BM / WM) + i * 32 + 8 * q + 4 * (lane >> 5));
+#pragma unroll
+                    for (int j = 0; j < NI; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[i][j][q * 4 + e] = v[e];
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j) acc[i][j] = v16f{};
+        }
         if constexpr (COLSUM)
             for (int j = 0; j < NI; ++j) colsum[j] = v16f{};
         if (from >= to) return;
-        int part = from / ktiles, kt = from % ktiles;
-        auto stage = [&](int buf) {
-            char* s = lds + buf * (SA::kBytes + SB::kBytes);
-            sa.load(s, kt, p.aoff[part], wave);
-            sb.load(s + SA::kBytes, kt, p.boff[part], wave);
-            if (++kt == ktiles) { kt = 0; ++part; }
-        };
-        stage(0);
         typename Mfma<T>::v8 ones;
         for (int i = 0; i < 8; ++i) ones[i] = (T)1.f;
         // (of fp32 parts: once per part of B, beside the leading part of A)
         const int sums = COLSUM && tm == 0 && wm == 0 ? (p.parts == 1 ? its : 3 * ktiles) : 0;
-        for (int it = from; it < to; ++it) {
-            const int buf = (it - from) & 1;
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // this wave's loads of tile `it` have landed ...
-            __builtin_amdgcn_s_barrier();                        // ... and everybody's; nobody reads the other buffer any more
+        // Fragments run one step of 16 K ahead of the matrix instructions, across tiles too: the barrier of a tile stands before
+        // its last step, when the last fragments are in registers.  From there on the tile's buffer is free: half of the loads
+        // of the tile after next go out there, the other half a step later, and all have two steps before they are waited
+        // for.  (With the barrier between tiles and the loads over all four steps: 4096^3 the same 1280 TFLOP/s, 512 x 32768 x
+        // 5120, whose operand comes from HBM, 984 against 1121.)
+        typename Mfma<T>::v8 a[2][MI], b[2][NI];
+        uint32_t pa[AK ? MI : 1], pb[BK ? NI : 1];       // LDS addresses of the transposing reads in the first buffer
+        if constexpr (AK)
+#pragma unroll
+            for (int i = 0; i < MI; ++i) pa[i] = (uint32_t)(uintptr_t)(lds_void*)lds + SA::address(i, wm * (BM / WM), lane);
+        if constexpr (BK)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) pb[j] = (uint32_t)(uintptr_t)(lds_void*)lds + SA::kBytes + SB::address(j, wn * (BN / WN), lane);
+        auto frags = [&](uint32_t buf, auto step) {      // buf: byte offset of the tile's buffer
+            constexpr int ks = decltype(step)::value, w = ks & 1;
+            uint32_t qa[AK ? MI : 1], qb[BK ? NI : 1];
+            if constexpr (AK)
+#pragma unroll
+                for (int i = 0; i < MI; ++i) qa[i] = pa[i] + buf;
+            if constexpr (BK)
+#pragma unroll
+                for (int j = 0; j < NI; ++j) qb[j] = pb[j] + buf;
+            if constexpr (AK && BK) {
+                static_assert(BM == BN, "one row length");
+                read_tr<ks * 16 * BM * 2, ks * 16 * BN * 2, BM * 2>(a[w], qa, b[w], qb);
+            } else {
+                if constexpr (!BK) SB::template frags<T>(b[w], lds + buf + SA::kBytes, wn * (BN / WN), ks, lane);
+                if constexpr (AK) read_tr<ks * 16 * BM * 2, BM * 2>(a[w], qa);
+                else SA::template frags<T>(a[w], lds + buf, wm * (BM / WM), ks, lane);
+            }
+        };
+        auto land = [&]() {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // this wave's loads have landed, its LDS reads are done ...
+            __builtin_amdgcn_s_barrier();                                // ... and everybody's
             asm volatile("" ::: "memory");
-            if (it + 1 < to) stage(buf ^ 1);
-            const char* s = lds + buf * (SA::kBytes + SB::kBytes);
-            typename Mfma<T>::v8 a[2][MI], b[2][NI];
-            auto frags = [&](int ks) {
+        };
+        constexpr int kTile = SA::kBytes + SB::kBytes;
+        land();
+        if (from + 1 < to) {
+            next();
 #pragma unroll
-                for (int i = 0; i < MI; ++i) a[ks & 1][i] = SA::template frag<T>(s, wm * (BM / WM) + i * 32, ks, lane);
+            for (int i = 0; i < kLoads / 2; ++i) load(lds + kTile, i);
+        }
+        frags(0, std::integral_constant<int, 0>());
+        for (int it = from; it < to; ++it) {
+            const uint32_t buf = (uint32_t)((it - from) & 1) * kTile, other = (uint32_t)kTile - buf;
+            auto step = [&](auto k) {
+                constexpr int ks = decltype(k)::value;
+                if (ks == 0 && it + 1 < to)
 #pragma unroll
-                for (int j = 0; j < NI; ++j) b[ks & 1][j] = SB::template frag<T>(s + SA::kBytes, wn * (BN / WN) + j * 32, ks, lane);
-            };
-            frags(0);
+                    for (int i = kLoads / 2; i < kLoads; ++i) load(lds + other, i);
+                if constexpr (ks + 1 < kSteps) {
+                    frags(buf, std::integral_constant<int, ks + 1>());
+                } else if (it + 1 < to) {
+                    land();
+                    if (it + 2 < to) {
+                        next();
 #pragma unroll
-            for (int ks = 0; ks < kBK / 16; ++ks) {
-                if (ks + 1 < kBK / 16) frags(ks + 1);
+                        for (int i = 0; i < kLoads / 2; ++i) load(lds + buf, i);
+                    }
+                    frags(other, std::integral_constant<int, 0>());
+                }
 #pragma unroll
                 for (int j = 0; j < NI; ++j)
 #pragma unroll
@@ -654,7 +772,12 @@ template <class T, int BM, int BN, int WM, int WN, bool AK, bool BK, bool COLSUM
                     if (it < sums)
 #pragma unroll
                         for (int j = 0; j < NI; ++j) colsum[j] = Mfma<T>::mul(ones, b[ks & 1][j], colsum[j]);
-            }
+            };
+            static_assert(kSteps == 4, "written out below");
+            step(std::integral_constant<int, 0>());
+            step(std::integral_constant<int, 1>());
+            step(std::integral_constant<int, 2>());
+            step(std::integral_constant<int, 3>());
         }
     }
     // accumulator element e of tile (i, j): row m(i, e), column n(j) of the product
@@ -662,8 +785,13 @@ template <class T, int BM, int BN, int WM, int WN, bool AK, bool BK, bool COLSUM
     __device__ inline int n(int j) const { return tn * BN + wn * (BN / WN) + j * 32 + (lane & 31); }
 };
 
+// The tiles' LDS is the launch's dynamic part: with a static array the compiler knows that a direct load may write what an LDS
+// read reads, and waits for all direct loads before every read (1.3 times the time of the whole product).
+extern __shared__ __align__(16) char tile_lds[];
+
 template <bool BIG> struct Shape {         // 256 x 256 by 8 waves, or 128 x 128 by 4
     static constexpr int BM = BIG ? 256 : 128, BN = BM, WM = 2, WN = BIG ? 4 : 2, kThreads = WM * WN * 64;
+    static constexpr int kLds = 2 * (BM + BN) * kBK * 2;
 };
 template <class T> constexpr int parts_of() { return sizeof(T) == 4 ? 3 : 1; }      // 16-bit planes of an operand
 template <class T> struct Half { typedef T type; };
@@ -778,38 +906,31 @@ struct RowsArgs {
 __device__ inline int64_t target_of(const RowsArgs& a, int64_t n) {
     return a.target_wide ? ((const int64_t*)a.targets)[n] : (int64_t)((const int32_t*)a.targets)[n];
 }
-// one workgroup: every thread owns a run of rows, counts its live ones, and writes them behind those of the threads before it
+// One workgroup walks the rows 16 x 1024 at a time: row n = i 1024 + thread of a chunk, all 16 flags of a thread loaded at
+// once, counted by wave votes; a prefix over the (i, wave) counts gives every live row its place.
+constexpr int kRowsPer = 16;
 __global__ void __launch_bounds__(1024) rows_kernel(RowsArgs a) {
-    __shared__ int cnt[1024];
+    __shared__ int cnt[kRowsPer * 16];
     __shared__ float top[16];
-    const int t = threadIdx.x;
-    const int64_t per = (a.N + 1023) / 1024, from = min(a.N, t * per), to = min(a.N, from + per);
+    __shared__ int base;
+    const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
     auto alive = [&](int64_t n) { return a.targets ? target_of(a, n) != a.ignore : a.peak[n] != 0.f; };
-    int c = 0;
-    float peak = 0.f;
-    for (int64_t n = from; n < to; ++n)
-        if (alive(n)) {
-            ++c;
-            if (a.peak || a.gout) peak = fmaxf(peak, a.peak ? a.peak[n] : fabsf(a.gout[a.gout_rows ? n : 0]));
-        }
-    cnt[t] = c;
-    peak = wave_max(peak);
-    if ((t & 63) == 0) top[t >> 6] = peak;
-    __syncthreads();
-    for (int o = 1; o < 1024; o <<= 1) {
-        const int v = t >= o ? cnt[t - o] : 0;
-        __syncthreads();
-        cnt[t] += v;
-        __syncthreads();
-    }
-    const int live = cnt[1023];
-    int at = cnt[t] - c;
     // What a 16-bit gradient of a logit is relative to.  Cross entropy: the largest incoming gradient, times the target's own
     // share 1 - smoothing: where all rows weigh the same, the entry of a target is then -1 + p / (1 - smoothing) and not some
     // number whose rounding is the same in every row and adds up over them.  Log-probabilities: a power of two near the largest
     // incoming gradient.  fp16 needs either to stay inside its range: what then falls below its 2^-24 is below that of a row's.
     float scale = 0.f;
-    for (int i = 0; i < 16; ++i) scale = fmaxf(scale, top[i]);
+    if (a.peak || a.gout) {
+        float peak = 0.f;
+        if (a.gout && !a.gout_rows) peak = fabsf(a.gout[0]);
+        else
+            for (int64_t n = t; n < a.N; n += 1024)
+                if (a.peak || alive(n)) peak = fmaxf(peak, a.peak ? a.peak[n] : fabsf(a.gout[n]));
+        peak = wave_max(peak);
+        if (lane == 0) top[wave] = peak;
+        __syncthreads();
+        for (int i = 0; i < 16; ++i) scale = fmaxf(scale, top[i]);
+    }
     if (!(scale > 0.f && scale < INFINITY)) scale = 1.f;
     else if (a.peak) {
         int e = 0;
@@ -817,34 +938,79 @@ __global__ void __launch_bounds__(1024) rows_kernel(RowsArgs a) {
         scale = ldexpf(1.f, max(-100, min(100, e)));
     }
     const float by = scale;
-    if (a.mean && live > 0) scale /= (float)live;
-    scale *= a.hit;
-    for (int64_t n = from; n < to; ++n) {
-        if (!alive(n)) {
-            a.r.pos[n] = -1;
-            if (a.loss) a.loss[n] = 0.f;
-            if (a.lse) a.lse[n] = 0.f;
-            continue;
+    if (t == 0) base = 0;
+    for (int64_t n0 = 0; n0 < a.N; n0 += kRowsPer * 1024) {
+        uint64_t vote[kRowsPer];
+        bool is[kRowsPer];
+#pragma unroll
+        for (int i = 0; i < kRowsPer; ++i) {
+            const int64_t n = n0 + i * 1024 + t;
+            is[i] = n < a.N && alive(n);
         }
-        a.r.pos[n] = at;
-        a.r.idx[at] = (int32_t)n;
-        if (a.targets) {
-            const int64_t v = target_of(a, n);
-            a.r.target[at] = v >= 0 && v < a.V ? (int32_t)v : -1;
+        __syncthreads();                   // (base is written; the counts' last readers are done)
+#pragma unroll
+        for (int i = 0; i < kRowsPer; ++i) {
+            vote[i] = __ballot(is[i]);
+            if (lane == 0) cnt[i * 16 + wave] = __popcll(vote[i]);
         }
-        if (a.gout) {
-            a.r.g[at] = a.r.target[at] < 0 ? 0.f : a.gout[a.gout_rows ? n : 0] / by;
-            a.r.lse[at] = a.lse_in[n];
+        __syncthreads();
+        if (wave == 0) {                   // inclusive prefix of 256 counts, four to a lane
+            int v[4], s = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { s += cnt[lane * 4 + j]; v[j] = s; }
+            int before = s;
+            for (int o = 1; o < 64; o <<= 1) { const int u = __shfl_up(before, o); if (lane >= o) before += u; }
+            before -= s;
+            const int b = base;
+            int all = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { const int c = cnt[lane * 4 + j]; cnt[lane * 4 + j] = b + before + v[j] - c; all = b + before + v[j]; }
+            if (lane == 63) base = all;
         }
-        ++at;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kRowsPer; ++i) {
+            const int64_t n = n0 + i * 1024 + t;
+            if (n >= a.N) break;
+            if (!is[i]) {
+                a.r.pos[n] = -1;
+                if (a.loss) a.loss[n] = 0.f;
+                if (a.lse) a.lse[n] = 0.f;
+                continue;
+            }
+            const int at = cnt[i * 16 + wave] + __popcll(vote[i] & (((uint64_t)1 << lane) - 1));
+            a.r.pos[n] = at;
+            a.r.idx[at] = (int32_t)n;
+            int32_t want = -1;
+            if (a.targets) {
+                const int64_t v = target_of(a, n);
+                want = v >= 0 && v < a.V ? (int32_t)v : -1;
+                a.r.target[at] = want;
+            }
+            if (a.gout) {
+                a.r.g[at] = want < 0 ? 0.f : a.gout[a.gout_rows ? n : 0] / by;
+                a.r.lse[at] = a.lse_in[n];
+            }
+        }
     }
-    if (t == 0) { *a.r.live = live; *a.r.scale = scale; }
+    __syncthreads();
+    const int live = base;
+    if (t == 0) {
+        if (a.mean && live > 0) scale /= (float)live;
+        *a.r.live = live;
+        *a.r.scale = scale * a.hit;
+    }
     // packed rows up to the end of the last tile: no gradient
     if (a.gout)
         for (int i = live + t; i < (live + kRowPad - 1) / kRowPad * kRowPad; i += 1024) { a.r.g[i] = 0.f; a.r.lse[i] = 0.f; a.r.target[i] = -1; }
 }
 
 // ---- epilogues ------------------------------------------------------------------------------------------------------
+// exp(z - ref) = 2^(z log2 e - ref log2 e): one multiply-add and the hardware's exponential.  The error is that of the argument,
+// 2^-24 |z| log2 e and the like for ref: z and ref are of the size of logits.
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ inline float exp2_of(float v) { return __builtin_amdgcn_exp2f(v); }
+
 struct Logits {              // what every product z = x W^T needs behind the accumulators
     const void* bias;        // [V] or NULL
     int32_t btype, v0, V;    // the product's W rows are outputs v0 .., V is the number of outputs that exist
@@ -870,40 +1036,53 @@ struct StatsArgs {
 template <class T, bool BIG> __global__ void __launch_bounds__(Shape<BIG>::kThreads, BIG ? 2 : 2) stats_kernel(StatsArgs a) {
     using S = Shape<BIG>;
     using Tl = Tile<T, S::BM, S::BN, S::WM, S::WN, false, false>;
-    __shared__ __align__(16) char lds[Tl::kLds];
-    __shared__ float bias[S::BM];
+    char* lds = tile_lds;
+    __shared__ __align__(16) float bias[S::BM];
     Tl t;
     if (!t.place(a.p)) return;
     stage_bias(a.l, t.tm * S::BM, S::BM, bias);
-    t.run(a.p, lds);
-    __syncthreads();
+    t.run(a.p, lds, bias);
     const int64_t at = (int64_t)(t.tm * S::WM + t.wm) * a.pitch;
+    const int first = t.m(0, 0) - 4 * (t.lane >> 5);             // of the wave's outputs
+    const bool whole = a.l.v0 + first + S::BM / S::WM <= a.l.V;
 #pragma unroll
     for (int j = 0; j < Tl::NI; ++j) {
-        const int c = t.n(j), want = a.target && c < t.live ? a.target[c] - a.l.v0 : -1;
-        float top = -INFINITY, all = 0.f, zt = 0.f;
-        bool here = false;
+        const int c = t.n(j);
+        if (a.target) {                                          // the target's logit, where it is among the wave's
+            const int want = c < t.live ? a.target[c] - a.l.v0 - first : -1;
+#pragma unroll
+            for (int i = 0; i < Tl::MI; ++i)
+                if (__any((want >> 5) == i))
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (want == t.m(i, e) - first) a.zt[c] = t.acc[i][j][e];
+        }
+        float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < Tl::MI; ++i)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int m = t.m(i, e);
-                const float z = t.acc[i][j][e] + bias[m - t.tm * S::BM];
-                t.acc[i][j][e] = z;
-                top = fmaxf(top, z);
-                if (a.all) all += a.l.v0 + m < a.l.V ? z : 0.f;
-                if (m == want) { zt = z; here = true; }
-            }
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, t.acc[i][j][e]);
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float ref = top == -INFINITY ? 0.f : top;          // a row of -inf: its exponentials are 0, not NaN
-        float sum = 0.f;
+        const float ref = top == -INFINITY ? 0.f : top * kLog2e;  // a row of -inf: its exponentials are 0, not NaN
+        float sum = 0.f, sum2 = 0.f;
 #pragma unroll
         for (int i = 0; i < Tl::MI; ++i)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) sum += __expf(t.acc[i][j][e] - ref);
+            for (int e = 0; e < 16; e += 2) {
+                sum += exp2_of(fmaf(t.acc[i][j][e], kLog2e, -ref));
+                sum2 += exp2_of(fmaf(t.acc[i][j][e + 1], kLog2e, -ref));
+            }
+        sum += sum2;
         sum += __shfl_xor(sum, 32);
-        if (a.all) all += __shfl_xor(all, 32);
-        if (here) a.zt[c] = zt;
+        float all = 0.f;
+        if (a.all) {
+#pragma unroll
+            for (int i = 0; i < Tl::MI; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    all += whole | (a.l.v0 + t.m(i, e) < a.l.V) ? t.acc[i][j][e] : 0.f;
+            all += __shfl_xor(all, 32);
+        }
         if (t.lane < 32 && c < a.pitch) {
             a.top[at + c] = top;
             a.sum[at + c] = sum;
@@ -921,16 +1100,32 @@ struct JoinArgs {
     float smoothing;
     float *lse, *loss;
 };
+// 16 rows a workgroup, 16 threads a row: each joins every 16th tile, then they meet in LDS
 __global__ void __launch_bounds__(256) join_kernel(JoinArgs a) {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c >= (a.live ? (int64_t)*a.live : a.N)) return;
-    float top = -INFINITY;
-    for (int q = 0; q < a.tiles; ++q) top = fmaxf(top, a.top[q * a.pitch + c]);
-    float sum = 0.f, all = 0.f;
-    for (int q = 0; q < a.tiles; ++q) {
-        const float m = a.top[q * a.pitch + c];
-        sum += a.sum[q * a.pitch + c] * (m == -INFINITY ? 1.f : __expf(m - top));     // (-inf: its sum is 0, or NaN)
-        if (a.all) all += a.all[q * a.pitch + c];
+    __shared__ float tops[16][17], sums[16][17], alls[16][17];
+    const int r = threadIdx.x & 15, k = threadIdx.x >> 4;
+    const int64_t c = (int64_t)blockIdx.x * 16 + r, rows = a.live ? (int64_t)*a.live : a.N;
+    if ((int64_t)blockIdx.x * 16 >= rows) return;
+    auto join = [](float& top, float& sum, float m, float s) {
+        // (a part whose largest is -inf adds its sum as it is: 0, or NaN where its logits were no numbers)
+        const float high = fmaxf(top, m);
+        sum = sum * (top == -INFINITY ? 1.f : __expf(top - high)) + s * (m == -INFINITY ? 1.f : __expf(m - high));
+        top = high;
+    };
+    float top = -INFINITY, sum = 0.f, all = 0.f;
+    if (c < rows)
+        for (int q = k; q < a.tiles; q += 16) {
+            join(top, sum, a.top[q * a.pitch + c], a.sum[q * a.pitch + c]);
+            if (a.all) all += a.all[q * a.pitch + c];
+        }
+    tops[k][r] = top;
+    sums[k][r] = sum;
+    alls[k][r] = all;
+    __syncthreads();
+    if (k != 0 || c >= rows) return;
+    for (int i = 1; i < 16; ++i) {
+        join(top, sum, tops[i][r], sums[i][r]);
+        all += alls[i][r];
     }
     const float lse = (top == -INFINITY ? 0.f : top) + logf(sum);
     const int64_t n = a.idx ? a.idx[c] : c;
@@ -972,7 +1167,7 @@ struct LogProbArgs {
 template <class T, bool BIG> __global__ void __launch_bounds__(Shape<BIG>::kThreads, 2) log_prob_kernel(LogProbArgs a) {
     using S = Shape<BIG>;
     using Tl = Tile<T, S::BM, S::BN, S::WM, S::WN, false, false>;
-    __shared__ __align__(16) char lds[Tl::kLds];
+    char* lds = tile_lds;
     __shared__ float bias[S::BN], lse[S::BM];
     Tl t;
     if (!t.place(a.p)) return;
@@ -1034,38 +1229,44 @@ template <class X, bool BIG> __global__ void __launch_bounds__(Shape<BIG>::kThre
     using T = typename Half<X>::type;
     using S = Shape<BIG>;
     using Tl = Tile<T, S::BM, S::BN, S::WM, S::WN, false, false>;
-    __shared__ __align__(16) char lds[Tl::kLds];
+    char* lds = tile_lds;
     __shared__ __align__(16) float bias[S::BM];
     Tl t;
     if (!t.place(a.p)) return;
     stage_bias(a.l, t.tm * S::BM, S::BM, bias);
-    t.run(a.p, lds);
-    __syncthreads();
+    t.run(a.p, lds, bias);
     // relative to g_max (1 - e): (p - e / V) / (1 - e) - [v = target]
     const float even = a.smoothing / (float)a.outputs, share = a.smoothing < 1.f ? 1.f / (1.f - a.smoothing) : 1.f;
     const float hit = a.smoothing < 1.f ? 1.f : 0.f;
+    const int first = t.m(0, 0) - 4 * (t.lane >> 5);
+    const bool whole = a.l.v0 + first + S::BM / S::WM <= a.l.V;
 #pragma unroll
     for (int j = 0; j < Tl::NI; ++j) {
         const int c = t.n(j);
         const bool in = c < t.live;
-        const float g = in ? a.g[c] : 0.f, lse = in ? a.lse[c] : 0.f, ref = lse == -INFINITY ? 0.f : lse;
-        const int want = in ? a.target[c] - a.l.v0 : -1;
+        const float g = in ? a.g[c] : 0.f, lse = in ? a.lse[c] : 0.f, ref = lse == -INFINITY ? 0.f : lse * kLog2e;
+        const int want = in ? a.target[c] - a.l.v0 - first : -1;
         const bool dead = g == 0.f || lse == -INFINITY;
+        const float up = g * share, down = up * even, own = dead ? 0.f : g * hit;
         uint16_t* row = a.dz + (int64_t)c * parts_of<X>() * a.pitch;
 #pragma unroll
-        for (int i = 0; i < Tl::MI; ++i)
+        for (int i = 0; i < Tl::MI; ++i) {
+            const bool near = __any((want >> 5) == i);           // a target is among these 32 outputs
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int m = t.m(i, q * 4);
                 float d[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float z = t.acc[i][j][q * 4 + e] + bias[m - t.tm * S::BM + e];
-                    d[e] = g * ((__expf(z - ref) - even) * share - (m + e == want ? hit : 0.f));
-                    if (dead || a.l.v0 + m + e >= a.l.V) d[e] = 0.f;
+                    const float u = fmaf(exp2_of(fmaf(t.acc[i][j][q * 4 + e], kLog2e, -ref)), up, -down);
+                    d[e] = dead | (!whole & (a.l.v0 + m + e >= a.l.V)) ? 0.f : u;
                 }
+                if (near)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) d[e] -= want == m - first + e ? own : 0.f;
                 if (m < a.pitch) store_dz4<X>(row, a.pitch, m, d);
             }
+        }
     }
 }
 
@@ -1087,7 +1288,7 @@ struct GradArgs {
 template <class T, bool BIG, bool BK, bool COLSUM> __global__ void __launch_bounds__(Shape<BIG>::kThreads, 2) grad_kernel(GradArgs a) {
     using S = Shape<BIG>;
     using Tl = Tile<T, S::BM, S::BN, S::WM, S::WN, true, BK, COLSUM>;
-    __shared__ __align__(16) char lds[Tl::kLds];
+    char* lds = tile_lds;
     Tl t;
     if (!t.place(a.p)) return;
     t.run(a.p, lds);
@@ -1335,6 +1536,22 @@ void set_parts(Product* p, int type, int64_t aplane, int64_t bplane) {
     }
 }
 unsigned grid_of(const Product& p) { return (unsigned)(ceil_div((int64_t)p.mtiles * p.ntiles * p.splits, 8) * 8); }
+// A kernel over tiles.  Above 64 KB a kernel has to be told once per device how much LDS a launch may ask for.
+template <class S, auto kernel, class A> int launch_tiles(const A& args, hipStream_t st) {
+    if (S::kLds > 65536) {
+        static std::atomic<uint64_t> told{0};
+        int dev = 0;
+        HIP_TRY(hipGetDevice(&dev));
+        const uint64_t bit = (uint64_t)1 << (dev & 63);
+        if (!(told.load(std::memory_order_relaxed) & bit)) {
+            HIP_TRY(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds));
+            told.fetch_or(bit, std::memory_order_relaxed);
+        }
+    }
+    kernel<<<grid_of(args.p), S::kThreads, S::kLds, st>>>(args);
+    HIP_TRY(hipGetLastError());
+    return WF_OK;
+}
 template <class F> void with_half(int type, F&& f) { if (type == WF_F16) f(f16()); else f(bf16()); }
 template <class F> void with_big(bool big, F&& f) { if (big) f(std::true_type()); else f(std::false_type()); }
 
@@ -1366,6 +1583,7 @@ int linear_check(const char* who, const void* x, int64_t ldx, int64_t N, const v
 
 int run_stats(const LinearPlan& p, const Operand& w, const Operand& x, const void* bias, int btype, const int32_t* live,
               const int32_t* target, bool all, hipStream_t st) {
+    int rc = WF_OK;
     StatsArgs s = {};
     s.p = {w, x, p.fwd.mt, p.fwd.nt, p.Dp / kBK, 1, {}, {}, live, 0, 1};
     set_parts(&s.p, p.type, p.Dp, p.Dp);
@@ -1373,10 +1591,10 @@ int run_stats(const LinearPlan& p, const Operand& w, const Operand& x, const voi
     s.top = p.top; s.sum = p.sum; s.all = all ? p.all : nullptr; s.pitch = p.Npad; s.target = target; s.zt = p.zt;
     with_half(p.type, [&](auto t) {
         with_big(p.fwd.big, [&](auto b) {
-            stats_kernel<decltype(t), decltype(b)::value><<<grid_of(s.p), Shape<decltype(b)::value>::kThreads, 0, st>>>(s);
+            rc = launch_tiles<Shape<decltype(b)::value>, stats_kernel<decltype(t), decltype(b)::value>>(s, st);
         });
     });
-    HIP_TRY(hipGetLastError());
+    if (rc) return rc;
     return WF_OK;
 }
 
@@ -1386,6 +1604,7 @@ int run_grads(const LinearPlan& p, const Operand& w, int piece, const GradOut& o
     const int64_t v0 = piece * p.width, width = std::min<int64_t>(p.width, p.V - v0);
     const Operand x = packed_x(p);
     const int64_t zld = p.parts * p.pitch;
+    int rc = WF_OK;
     if (o.dx) {
         GradArgs g = {};
         Operand wv = {(const uint16_t*)w.p + v0 * w.ld, w.ld, (int32_t)width, w.cols};
@@ -1395,10 +1614,10 @@ int run_grads(const LinearPlan& p, const Operand& w, int piece, const GradOut& o
         g.M = p.D; g.N = p.N; g.part = p.part_x; g.add = piece > 0; g.scale = p.rows.scale; g.out = o.dx; g.otype = p.type; g.idx = p.rows.idx;
         with_half(p.type, [&](auto t) {
             with_big(p.dx.big, [&](auto b) {
-                grad_kernel<decltype(t), decltype(b)::value, false, false><<<grid_of(g.p), Shape<decltype(b)::value>::kThreads, 0, st>>>(g);
+                rc = launch_tiles<Shape<decltype(b)::value>, grad_kernel<decltype(t), decltype(b)::value, false, false>>(g, st);
             });
         });
-        HIP_TRY(hipGetLastError());
+        if (rc) return rc;
         if (p.part_x && piece == p.pieces - 1) {
             FoldArgs f = {p.part_x, nullptr, p.rows.scale, p.dx.splits, p.D, p.N, p.rows.live, p.rows.idx, o.dx, nullptr, p.type, 0};
             fold_kernel<<<(unsigned)std::min<int64_t>(ceil_div(p.N * p.D, 1024), 2048), 256, 0, st>>>(f);
@@ -1419,10 +1638,10 @@ int run_grads(const LinearPlan& p, const Operand& w, int piece, const GradOut& o
         if (!o.dw) g.p.mtiles = 1;
         with_half(p.type, [&](auto t) {
             with_big(p.dw.big, [&](auto b) {
-                grad_kernel<decltype(t), decltype(b)::value, true, true><<<grid_of(g.p), Shape<decltype(b)::value>::kThreads, 0, st>>>(g);
+                rc = launch_tiles<Shape<decltype(b)::value>, grad_kernel<decltype(t), decltype(b)::value, true, true>>(g, st);
             });
         });
-        HIP_TRY(hipGetLastError());
+        if (rc) return rc;
         if (p.part_w) {
             FoldArgs f = {p.part_w, g.colpart, p.rows.scale, p.dw.splits, g.M, width, nullptr, nullptr, g.out, g.colout, p.type, o.btype};
             fold_kernel<<<(unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(width * p.D, 1024), 2048)), 256, 0, st>>>(f);
@@ -1471,7 +1690,7 @@ extern "C" int wf_linear_log_softmax(const void* x, int64_t ldx, int64_t N, int3
     }
     if ((rc = run_stats(p, w, xo, bias, bias_type, nullptr, nullptr, false, st))) return rc;
     JoinArgs j = {p.top, p.sum, nullptr, nullptr, p.Npad, N, p.fwd.mt * 2, V, nullptr, nullptr, nullptr, 0.f, p.zt, nullptr};
-    join_kernel<<<(unsigned)ceil_div(N, 256), 256, 0, st>>>(j);
+    join_kernel<<<(unsigned)ceil_div(N, 16), 256, 0, st>>>(j);
     LogProbArgs l = {};
     l.p = {xo, w, p.logp.mt, p.logp.nt, p.Dp / kBK, 1, {}, {}, nullptr, 0, 1};
     set_parts(&l.p, type, p.Dp, p.Dp);
@@ -1479,10 +1698,10 @@ extern "C" int wf_linear_log_softmax(const void* x, int64_t ldx, int64_t N, int3
     l.lse = p.zt; l.out = log_probs; l.N = N;
     with_half(type, [&](auto t) {
         with_big(p.logp.big, [&](auto b) {
-            log_prob_kernel<decltype(t), decltype(b)::value><<<grid_of(l.p), Shape<decltype(b)::value>::kThreads, 0, st>>>(l);
+            rc = launch_tiles<Shape<decltype(b)::value>, log_prob_kernel<decltype(t), decltype(b)::value>>(l, st);
         });
     });
-    HIP_TRY(hipGetLastError());
+    if (rc) return rc;
     return WF_OK;
 }
 
@@ -1536,7 +1755,7 @@ extern "C" int wf_linear_cross_entropy(const void* x, int64_t ldx, int64_t N, in
     if ((rc = run_stats(p, w, packed_x(p), bias, bias_type, p.rows.live, p.rows.target, smoothing != 0.f, st))) return rc;
     JoinArgs j = {p.top, p.sum, smoothing != 0.f ? p.all : nullptr, p.zt, p.Npad, N, p.fwd.mt * 2, V, p.rows.live, p.rows.idx,
                   p.rows.target, smoothing, lse, loss};
-    join_kernel<<<(unsigned)ceil_div(N, 256), 256, 0, st>>>(j);
+    join_kernel<<<(unsigned)ceil_div(N, 16), 256, 0, st>>>(j);
     if (total) total_kernel<<<1, 1024, 0, st>>>(loss, N, p.rows.live, mean, total);
     HIP_TRY(hipGetLastError());
     return WF_OK;
@@ -1573,10 +1792,10 @@ extern "C" int wf_linear_cross_entropy_backward(const float* grad, int32_t grad_
         z.target = p.rows.target; z.g = p.rows.g; z.lse = p.rows.lse; z.smoothing = smoothing; z.outputs = V; z.dz = p.dzp; z.pitch = p.pitch;
         with_type(type, [&](auto t) {
             with_big(p.dz.big, [&](auto b) {
-                dz_kernel<decltype(t), decltype(b)::value><<<grid_of(z.p), Shape<decltype(b)::value>::kThreads, 0, st>>>(z);
+                rc = launch_tiles<Shape<decltype(b)::value>, dz_kernel<decltype(t), decltype(b)::value>>(z, st);
             });
         });
-        HIP_TRY(hipGetLastError());
+        if (rc) return rc;
         if ((rc = run_grads(p, w, piece, {dx, dweight, dbias, bias_type}, st))) return rc;
     }
     return WF_OK;
