@@ -1204,6 +1204,38 @@ struct DzArgs {
     uint16_t* dz;            // [Npad][planes][pitch]
     int64_t pitch;
 };
+// A wave's 32 rows n by 32 MI columns m, out of the accumulators' layout (a lane holds 4 neighbouring columns of one row: 16 or
+// 8 bytes a request) into whole rows (512 or 256 neighbouring bytes), through 4 KB of LDS per 32 columns that only this wave
+// uses: LDS serves a wave in order, no barrier is needed.  get(i, q): columns 32 i + 8 q + 4 (lane / 32) .. + 3 of row
+// lane % 32; put(row, column, values).  Chunks are permuted by row against bank conflicts.
+template <int MI, class G, class P> __device__ inline void rows_out(char* w, int lane, G&& get, P&& put) {
+    constexpr int C = MI * 8;                        // 16-byte chunks of a row
+    const int row = lane & 31;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) *(v4f*)(w + row * (C * 16) + (((i * 8 + q * 2 + (lane >> 5)) ^ (row & (C - 1))) * 16)) = get(i, q);
+#pragma unroll
+    for (int k = 0; k < MI * 4; ++k) {
+        const int r = (k * 64 + lane) / C, c = (k * 64 + lane) % C;
+        put(r, c * 4, *(const v4f*)(w + r * (C * 16) + ((c ^ (r & (C - 1))) * 16)));
+    }
+}
+typedef uint16_t v4h __attribute__((ext_vector_type(4)));
+typedef uint16_t v8h __attribute__((ext_vector_type(8)));
+template <int MI, class G, class P> __device__ inline void rows_out16(char* w, int lane, G&& get, P&& put) {
+    constexpr int C = MI * 4;
+    const int row = lane & 31;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) *(v4h*)(w + row * (C * 16) + (((i * 4 + q) ^ (row & (C - 1))) * 16) + (lane >> 5) * 8) = get(i, q);
+#pragma unroll
+    for (int k = 0; k < MI * 2; ++k) {
+        const int r = (k * 64 + lane) / C, c = (k * 64 + lane) % C;
+        put(r, c * 8, *(const v8h*)(w + r * (C * 16) + ((c ^ (r & (C - 1))) * 16)));
+    }
+}
 // 16-bit planes of four neighbouring values
 template <class T> __device__ inline void store_dz4(uint16_t* row, int64_t pitch, int v, const float (&d)[4]) {
     if constexpr (parts_of<T>() == 1) {
@@ -1240,6 +1272,8 @@ template <class X, bool BIG> __global__ void __launch_bounds__(Shape<BIG>::kThre
     const float hit = a.smoothing < 1.f ? 1.f : 0.f;
     const int first = t.m(0, 0) - 4 * (t.lane >> 5);
     const bool whole = a.l.v0 + first + S::BM / S::WM <= a.l.V;
+    __syncthreads();                                             // the tiles are read: their LDS takes the results
+    char* mine = lds + (t.wm + t.wn * S::WM) * 16384;
 #pragma unroll
     for (int j = 0; j < Tl::NI; ++j) {
         const int c = t.n(j);
@@ -1248,25 +1282,35 @@ template <class X, bool BIG> __global__ void __launch_bounds__(Shape<BIG>::kThre
         const int want = in ? a.target[c] - a.l.v0 - first : -1;
         const bool dead = g == 0.f || lse == -INFINITY;
         const float up = g * share, down = up * even, own = dead ? 0.f : g * hit;
-        uint16_t* row = a.dz + (int64_t)c * parts_of<X>() * a.pitch;
 #pragma unroll
         for (int i = 0; i < Tl::MI; ++i) {
             const bool near = __any((want >> 5) == i);           // a target is among these 32 outputs
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int m = t.m(i, q * 4);
-                float d[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float u = fmaf(exp2_of(fmaf(t.acc[i][j][q * 4 + e], kLog2e, -ref)), up, -down);
-                    d[e] = dead | (!whole & (a.l.v0 + m + e >= a.l.V)) ? 0.f : u;
-                }
-                if (near)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) d[e] -= want == m - first + e ? own : 0.f;
-                if (m < a.pitch) store_dz4<X>(row, a.pitch, m, d);
+            for (int e = 0; e < 16; ++e) {
+                const float u = fmaf(exp2_of(fmaf(t.acc[i][j][e], kLog2e, -ref)), up, -down);
+                t.acc[i][j][e] = dead | (!whole & (a.l.v0 + t.m(i, e) >= a.l.V)) ? 0.f : u;
             }
+            if (near)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) t.acc[i][j][e] -= want == t.m(i, e) - first ? own : 0.f;
         }
+        const int row0 = c - (t.lane & 31);
+        if constexpr (parts_of<X>() == 1)
+            rows_out16<Tl::MI>(mine, t.lane, [&](int i, int q) {
+                v4h h;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) h[e] = bits16<X>(t.acc[i][j][q * 4 + e]);
+                return h;
+            }, [&](int r, int m, v8h h) {
+                if (first + m < a.pitch) *(v8h*)(a.dz + (int64_t)(row0 + r) * a.pitch + first + m) = h;
+            });
+        else
+            rows_out<Tl::MI>(mine, t.lane, [&](int i, int q) {
+                return v4f{t.acc[i][j][q * 4], t.acc[i][j][q * 4 + 1], t.acc[i][j][q * 4 + 2], t.acc[i][j][q * 4 + 3]};
+            }, [&](int r, int m, v4f d) {
+                const float v[4] = {d[0], d[1], d[2], d[3]};
+                if (first + m < a.pitch) store_dz4<X>(a.dz + (int64_t)(row0 + r) * parts_of<X>() * a.pitch, a.pitch, first + m, v);
+            });
     }
 }
 
@@ -1294,44 +1338,46 @@ template <class T, bool BIG, bool BK, bool COLSUM> __global__ void __launch_boun
     t.run(a.p, lds);
     const float scale = a.part ? 1.f : *a.scale;
     const int64_t N = a.p.live && !a.p.live_is_k ? min(a.N, (int64_t)t.live) : a.N;
+    const int first = t.m(0, 0) - 4 * (t.lane >> 5);
+    __syncthreads();
+    char* mine = lds + (t.wm + t.wn * S::WM) * 16384;
 #pragma unroll
     for (int j = 0; j < Tl::NI; ++j) {
-        const int n = t.n(j);
-        if (n >= N) continue;
-        if constexpr (COLSUM)
-            if ((a.colpart || a.colout) && t.tm == 0 && t.wm == 0 && t.lane < 32) {
+        const int n0 = t.n(j) - (t.lane & 31);
+        if constexpr (COLSUM) {
+            const int n = t.n(j);
+            if ((a.colpart || a.colout) && t.tm == 0 && t.wm == 0 && t.lane < 32 && n < N) {
                 if (a.part) a.colpart[(int64_t)t.split * a.N + n] = t.colsum[j][0];
                 else store_any(a.colout, a.ctype, n, t.colsum[j][0] * *a.scale);
             }
+        }
+        rows_out<Tl::MI>(mine, t.lane, [&](int i, int q) {
+            return v4f{t.acc[i][j][q * 4], t.acc[i][j][q * 4 + 1], t.acc[i][j][q * 4 + 2], t.acc[i][j][q * 4 + 3]};
+        }, [&](int r, int k, v4f d) {
+            const int n = n0 + r, m = first + k, left = a.M - m;
+            if (n >= N || left <= 0) return;
+            if (a.part) {
+                float* at = a.part + ((int64_t)t.split * a.N + n) * a.M + m;
+                Pack<float, 4> v;
+                if (a.add) v = load_n<float, 4>(at, left);
 #pragma unroll
-        for (int i = 0; i < Tl::MI; ++i)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int m = t.m(i, q * 4);
-                if (m >= a.M) continue;
-                const int left = a.M - m;
-                if (a.part) {
-                    float* at = a.part + ((int64_t)t.split * a.N + n) * a.M + m;
+                for (int e = 0; e < 4; ++e) v.v[e] = (a.add ? v.v[e] : 0.f) + d[e];
+                store_n<float, 4>(at, v, left);
+            } else {
+                const int64_t at = (a.idx ? a.idx[n] : n) * (int64_t)a.M + m;
+                if (a.otype == WF_F32) {
                     Pack<float, 4> v;
-                    if (a.add) v = load_n<float, 4>(at, left);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v.v[e] = (a.add ? v.v[e] : 0.f) + t.acc[i][j][q * 4 + e];
-                    store_n<float, 4>(at, v, left);
+                    for (int e = 0; e < 4; ++e) v.v[e] = d[e] * scale;
+                    store_n<float, 4>((float*)a.out + at, v, left);
                 } else {
-                    const int64_t r = (a.idx ? a.idx[n] : n) * (int64_t)a.M + m;
-                    if (a.otype == WF_F32) {
-                        Pack<float, 4> v;
+                    Pack<T, 4> v;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) v.v[e] = t.acc[i][j][q * 4 + e] * scale;
-                        store_n<float, 4>((float*)a.out + r, v, left);
-                    } else {
-                        Pack<T, 4> v;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) v.v[e] = (T)(t.acc[i][j][q * 4 + e] * scale);
-                        store_n<T, 4>((T*)a.out + r, v, left);
-                    }
+                    for (int e = 0; e < 4; ++e) v.v[e] = (T)(d[e] * scale);
+                    store_n<T, 4>((T*)a.out + at, v, left);
                 }
             }
+        });
     }
 }
 
