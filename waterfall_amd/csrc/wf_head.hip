@@ -901,108 +901,96 @@ struct RowsArgs {
     const float* gout;       // backward: incoming gradient, one for all rows or per row
     int gout_rows, mean;
     const float* lse_in;
+    int narrow;              // log-softmax backward in fp16: the gradients are scaled by peak's largest
     float hit;               // backward: 1 - smoothing, or 1 where that is 0
 };
 __device__ inline int64_t target_of(const RowsArgs& a, int64_t n) {
     return a.target_wide ? ((const int64_t*)a.targets)[n] : (int64_t)((const int32_t*)a.targets)[n];
 }
-// One workgroup walks the rows 16 x 1024 at a time: row n = i 1024 + thread of a chunk, all 16 flags of a thread loaded at
-// once, counted by wave votes; a prefix over the (i, wave) counts gives every live row its place.
-constexpr int kRowsPer = 16;
-__global__ void __launch_bounds__(1024) rows_kernel(RowsArgs a) {
-    __shared__ int cnt[kRowsPer * 16];
+// At most 64 workgroups, a run of rows each.  A workgroup counts the live rows before its run by itself (flags are a few bytes a
+// row and come from L2: no hand-over between workgroups, no second launch) and walks its run 1024 rows at a time by wave votes.
+constexpr int kRowRuns = 64;
+__global__ void __launch_bounds__(1024) rows_kernel(RowsArgs a, int64_t run) {
+    __shared__ int cnt[16];
     __shared__ float top[16];
-    __shared__ int base;
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
+    const int64_t from = blockIdx.x * run, to = min(a.N, from + run);
+    const bool last = blockIdx.x + 1 == gridDim.x;
     auto alive = [&](int64_t n) { return a.targets ? target_of(a, n) != a.ignore : a.peak[n] != 0.f; };
     // What a 16-bit gradient of a logit is relative to.  Cross entropy: the largest incoming gradient, times the target's own
     // share 1 - smoothing: where all rows weigh the same, the entry of a target is then -1 + p / (1 - smoothing) and not some
     // number whose rounding is the same in every row and adds up over them.  Log-probabilities: a power of two near the largest
     // incoming gradient.  fp16 needs either to stay inside its range: what then falls below its 2^-24 is below that of a row's.
     float scale = 0.f;
-    if (a.peak || a.gout) {
+    if (a.gout && !a.gout_rows) {
+        scale = fabsf(a.gout[0]);
+    } else if (a.gout || (a.narrow && last)) {
         float peak = 0.f;
-        if (a.gout && !a.gout_rows) peak = fabsf(a.gout[0]);
-        else
-            for (int64_t n = t; n < a.N; n += 1024)
-                if (a.peak || alive(n)) peak = fmaxf(peak, a.peak ? a.peak[n] : fabsf(a.gout[n]));
+        for (int64_t n = t; n < a.N; n += 1024)
+            if (a.narrow || alive(n)) peak = fmaxf(peak, a.narrow ? a.peak[n] : fabsf(a.gout[n]));
         peak = wave_max(peak);
         if (lane == 0) top[wave] = peak;
         __syncthreads();
         for (int i = 0; i < 16; ++i) scale = fmaxf(scale, top[i]);
     }
     if (!(scale > 0.f && scale < INFINITY)) scale = 1.f;
-    else if (a.peak) {
+    else if (a.narrow) {
         int e = 0;
         (void)frexpf(scale, &e);
         scale = ldexpf(1.f, max(-100, min(100, e)));
     }
     const float by = scale;
-    if (t == 0) base = 0;
-    for (int64_t n0 = 0; n0 < a.N; n0 += kRowsPer * 1024) {
-        uint64_t vote[kRowsPer];
-        bool is[kRowsPer];
-#pragma unroll
-        for (int i = 0; i < kRowsPer; ++i) {
-            const int64_t n = n0 + i * 1024 + t;
-            is[i] = n < a.N && alive(n);
-        }
-        __syncthreads();                   // (base is written; the counts' last readers are done)
-#pragma unroll
-        for (int i = 0; i < kRowsPer; ++i) {
-            vote[i] = __ballot(is[i]);
-            if (lane == 0) cnt[i * 16 + wave] = __popcll(vote[i]);
-        }
+    int base = 0;
+    if (from > 0) {
+        int c = 0;
+#pragma unroll 8
+        for (int64_t n = t; n < from; n += 1024) c += alive(n);
+        for (int o = 32; o; o >>= 1) c += __shfl_xor(c, o);
+        if (lane == 0) cnt[wave] = c;
         __syncthreads();
-        if (wave == 0) {                   // inclusive prefix of 256 counts, four to a lane
-            int v[4], s = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) { s += cnt[lane * 4 + j]; v[j] = s; }
-            int before = s;
-            for (int o = 1; o < 64; o <<= 1) { const int u = __shfl_up(before, o); if (lane >= o) before += u; }
-            before -= s;
-            const int b = base;
-            int all = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) { const int c = cnt[lane * 4 + j]; cnt[lane * 4 + j] = b + before + v[j] - c; all = b + before + v[j]; }
-            if (lane == 63) base = all;
-        }
+        for (int i = 0; i < 16; ++i) base += cnt[i];
+    }
+    for (int64_t n0 = from; n0 < to; n0 += 1024) {
+        const int64_t n = n0 + t;
+        const bool is = n < to && alive(n);
+        const uint64_t vote = __ballot(is);
+        __syncthreads();                   // (the counts' last readers are done)
+        if (lane == 0) cnt[wave] = __popcll(vote);
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kRowsPer; ++i) {
-            const int64_t n = n0 + i * 1024 + t;
-            if (n >= a.N) break;
-            if (!is[i]) {
-                a.r.pos[n] = -1;
-                if (a.loss) a.loss[n] = 0.f;
-                if (a.lse) a.lse[n] = 0.f;
-                continue;
-            }
-            const int at = cnt[i * 16 + wave] + __popcll(vote[i] & (((uint64_t)1 << lane) - 1));
-            a.r.pos[n] = at;
-            a.r.idx[at] = (int32_t)n;
-            int32_t want = -1;
-            if (a.targets) {
-                const int64_t v = target_of(a, n);
-                want = v >= 0 && v < a.V ? (int32_t)v : -1;
-                a.r.target[at] = want;
-            }
-            if (a.gout) {
-                a.r.g[at] = want < 0 ? 0.f : a.gout[a.gout_rows ? n : 0] / by;
-                a.r.lse[at] = a.lse_in[n];
-            }
+        int at = base + __popcll(vote & (((uint64_t)1 << lane) - 1));
+        for (int i = 0; i < 16; ++i) {
+            at += i < wave ? cnt[i] : 0;
+            base += cnt[i];
+        }
+        if (n >= to) continue;
+        if (!is) {
+            a.r.pos[n] = -1;
+            if (a.loss) a.loss[n] = 0.f;
+            if (a.lse) a.lse[n] = 0.f;
+            continue;
+        }
+        a.r.pos[n] = at;
+        a.r.idx[at] = (int32_t)n;
+        int32_t want = -1;
+        if (a.targets) {
+            const int64_t v = target_of(a, n);
+            want = v >= 0 && v < a.V ? (int32_t)v : -1;
+            a.r.target[at] = want;
+        }
+        if (a.gout) {
+            a.r.g[at] = want < 0 ? 0.f : a.gout[a.gout_rows ? n : 0] / by;
+            a.r.lse[at] = a.lse_in[n];
         }
     }
-    __syncthreads();
-    const int live = base;
+    if (!last) return;
     if (t == 0) {
-        if (a.mean && live > 0) scale /= (float)live;
-        *a.r.live = live;
+        if (a.mean && base > 0) scale /= (float)base;
+        *a.r.live = base;
         *a.r.scale = scale * a.hit;
     }
     // packed rows up to the end of the last tile: no gradient
     if (a.gout)
-        for (int i = live + t; i < (live + kRowPad - 1) / kRowPad * kRowPad; i += 1024) { a.r.g[i] = 0.f; a.r.lse[i] = 0.f; a.r.target[i] = -1; }
+        for (int i = base + t; i < (base + kRowPad - 1) / kRowPad * kRowPad; i += 1024) { a.r.g[i] = 0.f; a.r.lse[i] = 0.f; a.r.target[i] = -1; }
 }
 
 // ---- epilogues ------------------------------------------------------------------------------------------------------
@@ -1100,22 +1088,30 @@ struct JoinArgs {
     float smoothing;
     float *lse, *loss;
 };
+__device__ inline void join_stats(float& top, float& sum, float m, float s) {
+    // (a part whose largest is -inf adds its sum as it is: 0, or NaN where its logits were no numbers)
+    const float high = fmaxf(top, m);
+    sum = sum * (top == -INFINITY ? 1.f : __expf(top - high)) + s * (m == -INFINITY ? 1.f : __expf(m - high));
+    top = high;
+}
+__device__ inline float row_loss(float lse, float zt, float all, int V, int target, float smoothing) {
+    if (target < 0) return NAN;                               // a target that is no output: loud, and no read out of range
+    if (lse == -INFINITY) return INFINITY;                    // every output is masked: as unlikely as a target can be
+    float loss = lse;
+    if (smoothing != 1.f) loss -= (1.f - smoothing) * zt;
+    if (smoothing != 0.f) loss -= smoothing * (all / (float)V);
+    return loss;
+}
 // 16 rows a workgroup, 16 threads a row: each joins every 16th tile, then they meet in LDS
 __global__ void __launch_bounds__(256) join_kernel(JoinArgs a) {
     __shared__ float tops[16][17], sums[16][17], alls[16][17];
     const int r = threadIdx.x & 15, k = threadIdx.x >> 4;
     const int64_t c = (int64_t)blockIdx.x * 16 + r, rows = a.live ? (int64_t)*a.live : a.N;
     if ((int64_t)blockIdx.x * 16 >= rows) return;
-    auto join = [](float& top, float& sum, float m, float s) {
-        // (a part whose largest is -inf adds its sum as it is: 0, or NaN where its logits were no numbers)
-        const float high = fmaxf(top, m);
-        sum = sum * (top == -INFINITY ? 1.f : __expf(top - high)) + s * (m == -INFINITY ? 1.f : __expf(m - high));
-        top = high;
-    };
     float top = -INFINITY, sum = 0.f, all = 0.f;
     if (c < rows)
         for (int q = k; q < a.tiles; q += 16) {
-            join(top, sum, a.top[q * a.pitch + c], a.sum[q * a.pitch + c]);
+            join_stats(top, sum, a.top[q * a.pitch + c], a.sum[q * a.pitch + c]);
             if (a.all) all += a.all[q * a.pitch + c];
         }
     tops[k][r] = top;
@@ -1124,39 +1120,232 @@ __global__ void __launch_bounds__(256) join_kernel(JoinArgs a) {
     __syncthreads();
     if (k != 0 || c >= rows) return;
     for (int i = 1; i < 16; ++i) {
-        join(top, sum, tops[i][r], sums[i][r]);
+        join_stats(top, sum, tops[i][r], sums[i][r]);
         all += alls[i][r];
     }
     const float lse = (top == -INFINITY ? 0.f : top) + logf(sum);
     const int64_t n = a.idx ? a.idx[c] : c;
     a.lse[n] = lse;
-    if (a.loss) {
-        const int t = a.target[c];
-        float loss = NAN;                                     // a target that is no output: loud, and no read out of range
-        if (t >= 0) {
-            loss = lse;
-            if (a.smoothing != 1.f) loss -= (1.f - a.smoothing) * a.zt[c];
-            if (a.smoothing != 0.f) loss -= a.smoothing * (all / (float)a.V);
-            if (lse == -INFINITY) loss = INFINITY;            // every output is masked: as unlikely as a target can be
-        }
-        a.loss[n] = loss;
-    }
+    if (a.loss) a.loss[n] = row_loss(lse, a.zt[c], all, a.V, a.target[c], a.smoothing);
 }
-__global__ void __launch_bounds__(1024) total_kernel(const float* loss, int64_t N, const int32_t* live, int mean, float* out) {
+// sum of the losses, over the number of rows whose target is not `ignore` where `mean`
+__global__ void __launch_bounds__(1024) total_kernel(const float* loss, int64_t N, const void* targets, int wide, int64_t ignore, int mean, float* out) {
     __shared__ float s[16];
+    __shared__ int c[16];
     float v = 0.f;
-    for (int64_t n = threadIdx.x; n < N; n += 1024) v += loss[n];
+    int k = 0;
+    for (int64_t n = threadIdx.x; n < N; n += 1024) {
+        v += loss[n];
+        if (mean) k += (wide ? ((const int64_t*)targets)[n] : (int64_t)((const int32_t*)targets)[n]) != ignore;
+    }
     v = wave_sum(v);
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+    for (int o = 32; o; o >>= 1) k += __shfl_xor(k, o);
+    if ((threadIdx.x & 63) == 0) { s[threadIdx.x >> 6] = v; c[threadIdx.x >> 6] = k; }
     __syncthreads();
     if (threadIdx.x == 0) {
         v = 0.f;
-        for (int i = 0; i < 16; ++i) v += s[i];
-        if (mean && live) v /= (float)max(1, *live);
-        *out = v;
+        k = 0;
+        for (int i = 0; i < 16; ++i) { v += s[i]; k += c[i]; }
+        *out = mean ? v / (float)max(1, k) : v;
     }
 }
 
+// ---- few rows, or few outputs ---------------------------------------------------------------------------------------
+// A chunk of a stream (N small: the time is one read of W) or a table of characters or phones (V small: one read of x).  A
+// workgroup has 32 rows by 32 MV outputs; its 4 waves take every fourth step of 16 K each, straight from memory into the matrix
+// instructions' registers (fp32 is split there), without a tile in LDS and without packed operands; their sums meet in LDS.
+// Where one workgroup sees all outputs of its rows it ends them itself: the whole call is this one launch.
+struct SmallArgs {
+    const void *x, *w;
+    int64_t ldx, ldw, N;
+    int32_t D;
+    Logits l;
+    float *top, *sum, *all;  // [gridDim.x][pitch], or NULL where a workgroup sees all outputs
+    int64_t pitch;
+    float* out;              // log-probabilities: [N][V]; z where a later launch ends the rows
+    const void* targets;     // cross entropy
+    int32_t target_wide;
+    int64_t ignore;
+    float smoothing;
+    float *zt, *lse, *loss;
+};
+template <class X> __device__ inline void split_frag(const Pack<X, 8>& v, typename Mfma<typename Half<X>::type>::v8 (&f)[parts_of<X>()]) {
+    if constexpr (parts_of<X>() == 1) {
+        __builtin_memcpy(&f[0], &v, 16);
+    } else {
+        Pack<uint16_t, 8> h[3];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const Split3 s = split3(v.v[i]);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) h[p].v[i] = s.h[p];
+        }
+#pragma unroll
+        for (int p = 0; p < 3; ++p) __builtin_memcpy(&f[p], &h[p], 16);
+    }
+}
+__device__ inline int32_t small_target(const void* targets, int wide, int64_t ignore, int64_t n, int V, bool* dead) {
+    const int64_t t = wide ? ((const int64_t*)targets)[n] : (int64_t)((const int32_t*)targets)[n];
+    *dead = t == ignore;
+    return t >= 0 && t < V ? (int32_t)t : -1;
+}
+template <class X, int MV> __global__ void __launch_bounds__(256) small_kernel(SmallArgs a) {
+    using T = typename Half<X>::type;
+    constexpr int P = parts_of<X>(), U = P == 1 ? 4 : 2;      // steps whose loads are under way together
+    __shared__ __align__(16) float part[4][MV][4][64][4];     // [wave][m][q][lane][e]
+    __shared__ float wtop[4][32], wsum[4][32], wall[4][32], wzt[32];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int v0 = blockIdx.x * 32 * MV, kl = (lane >> 5) * 8;
+    const int64_t n0 = (int64_t)blockIdx.y * 32, n = n0 + (lane & 31);
+    const X* xr = (const X*)a.x + min(n, a.N - 1) * a.ldx;
+    const X* wr[MV];
+#pragma unroll
+    for (int m = 0; m < MV; ++m) wr[m] = (const X*)a.w + (int64_t)min(v0 + m * 32 + (lane & 31), a.l.V - 1) * a.ldw;
+    v16f acc[MV];
+#pragma unroll
+    for (int m = 0; m < MV; ++m) acc[m] = v16f{};
+    for (int k0 = wave * 16 + kl; k0 - kl < a.D; k0 += 64 * U) {
+        Pack<X, 8> xv[U], wv[U][MV];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = k0 + u * 64;
+            xv[u] = load_n<X, 8>(xr + k, a.D - k);
+#pragma unroll
+            for (int m = 0; m < MV; ++m) wv[u][m] = load_n<X, 8>(wr[m] + k, a.D - k);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            typename Mfma<T>::v8 xf[P], wf[P];
+            split_frag<X>(xv[u], xf);
+#pragma unroll
+            for (int m = 0; m < MV; ++m) {
+                split_frag<X>(wv[u][m], wf);
+                if constexpr (P == 1) {
+                    acc[m] = Mfma<T>::mul(wf[0], xf[0], acc[m]);
+                } else {
+                    acc[m] = Mfma<T>::mul(wf[2], xf[0], acc[m]);
+                    acc[m] = Mfma<T>::mul(wf[1], xf[1], acc[m]);
+                    acc[m] = Mfma<T>::mul(wf[0], xf[2], acc[m]);
+                    acc[m] = Mfma<T>::mul(wf[1], xf[0], acc[m]);
+                    acc[m] = Mfma<T>::mul(wf[0], xf[1], acc[m]);
+                    acc[m] = Mfma<T>::mul(wf[0], xf[0], acc[m]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < MV; ++m)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) *(v4f*)part[wave][m][q][lane] = v4f{acc[m][q * 4], acc[m][q * 4 + 1], acc[m][q * 4 + 2], acc[m][q * 4 + 3]};
+    if (threadIdx.x < 32) wzt[threadIdx.x] = 0.f;
+    __syncthreads();
+    // wave q ends quarter q of every 32 outputs: v0 + 32 m + 8 q + 4 (lane / 32) .. + 3 of row lane % 32
+    bool dead = false;
+    const int want = a.targets && n < a.N ? small_target(a.targets, a.target_wide, a.ignore, n, a.l.V, &dead) : -1;
+    v4f z[MV];
+    float top = -INFINITY, all = 0.f;
+#pragma unroll
+    for (int m = 0; m < MV; ++m) {
+        z[m] = (*(const v4f*)part[0][m][wave][lane] + *(const v4f*)part[1][m][wave][lane]) +
+               (*(const v4f*)part[2][m][wave][lane] + *(const v4f*)part[3][m][wave][lane]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int v = v0 + m * 32 + wave * 8 + (lane >> 5) * 4 + e;
+            const bool in = v < a.l.V;
+            z[m][e] = in ? z[m][e] + (a.l.bias ? load_any(a.l.bias, a.l.btype, v) : 0.f) : -INFINITY;
+            top = fmaxf(top, z[m][e]);
+            all += in ? z[m][e] : 0.f;
+            if (v == want) { if (a.top) a.zt[n] = z[m][e]; else wzt[lane & 31] = z[m][e]; }
+        }
+    }
+    top = fmaxf(top, __shfl_xor(top, 32));
+    all += __shfl_xor(all, 32);
+    if (lane < 32) { wtop[wave][lane] = top; wall[wave][lane] = all; }
+    __syncthreads();
+    top = fmaxf(fmaxf(wtop[0][lane & 31], wtop[1][lane & 31]), fmaxf(wtop[2][lane & 31], wtop[3][lane & 31]));
+    const float ref = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+#pragma unroll
+    for (int m = 0; m < MV; ++m)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += __expf(z[m][e] - ref);
+    sum += __shfl_xor(sum, 32);
+    if (lane < 32) wsum[wave][lane] = sum;
+    __syncthreads();
+    const int r = lane & 31;
+    sum = (wsum[0][r] + wsum[1][r]) + (wsum[2][r] + wsum[3][r]);
+    all = (wall[0][r] + wall[1][r]) + (wall[2][r] + wall[3][r]);
+    if (n >= a.N) return;
+    float lse = 0.f;
+    if (a.top) {
+        if (wave == 0 && lane < 32) {
+            const int64_t at = blockIdx.x * a.pitch + n;
+            a.top[at] = top;
+            a.sum[at] = sum;
+            if (a.all) a.all[at] = all;
+        }
+    } else {
+        lse = ref + logf(sum);
+        if (a.loss && wave == 0 && lane < 32) {
+            a.lse[n] = dead ? 0.f : lse;
+            a.loss[n] = dead ? 0.f : row_loss(lse, wzt[r], all, a.l.V, want, a.smoothing);
+        }
+    }
+    if (a.out) {
+        const float minus = lse == -INFINITY ? 0.f : lse;    // a row of -inf stays one
+#pragma unroll
+        for (int m = 0; m < MV; ++m) {
+            const int v = v0 + m * 32 + wave * 8 + (lane >> 5) * 4;
+            Pack<float, 4> o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o.v[e] = z[m][e] - minus;
+            store_n<float, 4>(a.out + n * a.l.V + v, o, a.l.V - v);
+        }
+    }
+}
+// Ends the rows of several workgroups: out (4096 values of a row a workgroup) -= lse; loss and lse.
+__global__ void __launch_bounds__(256) small_end_kernel(SmallArgs a, int tiles) {
+    __shared__ float tops[4], sums[4], alls[4];
+    const int64_t n = blockIdx.y;
+    float* out = a.out + n * a.l.V;
+    const int v0 = blockIdx.x * 4096 + threadIdx.x;
+    float z[16];                                              // under way while the row's statistics are joined
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i] = a.out && v0 + i * 256 < a.l.V ? out[v0 + i * 256] : 0.f;
+    float top = -INFINITY, sum = 0.f, all = 0.f;
+    for (int q = threadIdx.x; q < tiles; q += 256) {
+        join_stats(top, sum, a.top[q * a.pitch + n], a.sum[q * a.pitch + n]);
+        if (a.all) all += a.all[q * a.pitch + n];
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        const float m = __shfl_xor(top, o), s = __shfl_xor(sum, o);
+        join_stats(top, sum, m, s);
+    }
+    all = wave_sum(all);
+    if ((threadIdx.x & 63) == 0) { tops[threadIdx.x >> 6] = top; sums[threadIdx.x >> 6] = sum; alls[threadIdx.x >> 6] = all; }
+    __syncthreads();
+    top = tops[0];
+    sum = sums[0];
+    all = alls[0];
+    for (int i = 1; i < 4; ++i) { join_stats(top, sum, tops[i], sums[i]); all += alls[i]; }
+    const float lse = (top == -INFINITY ? 0.f : top) + logf(sum);
+    if (a.loss && blockIdx.x == 0 && threadIdx.x == 0) {
+        bool dead = false;
+        const int want = small_target(a.targets, a.target_wide, a.ignore, n, a.l.V, &dead);
+        a.lse[n] = dead ? 0.f : lse;
+        a.loss[n] = dead ? 0.f : row_loss(lse, want < 0 ? 0.f : a.zt[n], all, a.l.V, want, a.smoothing);
+    }
+    if (a.out && lse != -INFINITY)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (v0 + i * 256 < a.l.V) out[v0 + i * 256] = z[i] - lse;
+}
+
+// z - lse, from logits that are computed again: at D 512 that costs less than writing z, reading it and writing it once more (a
+// pass over the box is 62 us at 16000 x 5001, the product 80).  Plain 4-byte stores: 32 lanes fill 128 bytes of a row, whose
+// start is as unaligned as V is odd (16-byte stores of whole rows through LDS: 143 against 135 us, non-temporal ones: 203;
+// 128 x 128 tiles, two workgroups a CU: 158).
 struct LogProbArgs {
     Product p;               // A = x, B = W: a lane is one output, 32 of them make 128 bytes of a row
     Logits l;
@@ -1394,78 +1583,122 @@ __global__ void __launch_bounds__(256) fold_kernel(FoldArgs a) {
     const int64_t N = a.live ? min(a.N, (int64_t)*a.live) : a.N;
     const float scale = *a.scale;
     const int64_t all = N * a.M, stride = a.N * a.M;
-    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < all; i += (int64_t)gridDim.x * 1024) {
-        const int left = (int)min((int64_t)4, all - i);
-        Pack<float, 4> v = load_n<float, 4>(a.part + i, left);
-        for (int s = 1; s < a.splits; ++s) {
-            const auto w = load_n<float, 4>(a.part + s * stride + i, left);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v.v[e] += w.v[e];
+    auto put = [&](int64_t k, float v) { store_any(a.out, a.otype, a.idx ? a.idx[k / a.M] * (int64_t)a.M + k % a.M : k, v * scale); };
+    if (a.splits >= 16) {
+        // few elements, many parts: 32 elements a workgroup, each summed by 8 threads that meet in LDS
+        __shared__ float s[8][32];
+        const int c = threadIdx.x & 31, q = threadIdx.x >> 5;
+        for (int64_t i0 = (int64_t)blockIdx.x * 32; i0 < all; i0 += (int64_t)gridDim.x * 32) {
+            const int64_t i = i0 + c;
+            float v = 0.f;
+            if (i < all)
+#pragma unroll 8
+                for (int k = q; k < a.splits; k += 8) v += a.part[k * stride + i];
+            s[q][c] = v;
+            __syncthreads();
+            if (q == 0 && i < all) put(i, ((s[0][c] + s[1][c]) + (s[2][c] + s[3][c])) + ((s[4][c] + s[5][c]) + (s[6][c] + s[7][c])));
+            __syncthreads();
         }
+    } else {
+        for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < all; i += (int64_t)gridDim.x * 1024) {
+            const int left = (int)min((int64_t)4, all - i);
+            Pack<float, 4> v = load_n<float, 4>(a.part + i, left);
+            for (int s = 1; s < a.splits; ++s) {
+                const auto w = load_n<float, 4>(a.part + s * stride + i, left);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (e >= left) break;
-            const int64_t k = i + e;
-            store_any(a.out, a.otype, a.idx ? a.idx[k / a.M] * (int64_t)a.M + k % a.M : k, v.v[e] * scale);
+                for (int e = 0; e < 4; ++e) v.v[e] += w.v[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e < left) put(i + e, v.v[e]);
         }
     }
-    if (a.colout)
-        for (int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x; n < N; n += (int64_t)gridDim.x * 256) {
-            float v = a.colpart[n];
-            for (int s = 1; s < a.splits; ++s) v += a.colpart[s * a.N + n];
-            store_any(a.colout, a.ctype, n, v * scale);
+    if (a.colout)                      // a wave a column sum
+        for (int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); n < N; n += (int64_t)gridDim.x * 4) {
+            float v = 0.f;
+            for (int s = threadIdx.x & 63; s < a.splits; s += 64) v += a.colpart[s * a.N + n];
+            v = wave_sum(v);
+            if ((threadIdx.x & 63) == 0) store_any(a.colout, a.ctype, n, v * scale);
         }
 }
 
 // ---- the gradient that comes into log-probabilities -----------------------------------------------------------------
-// sum and largest magnitude of every row of G; a workgroup a row
-__global__ void __launch_bounds__(256) grad_rows_kernel(const float* G, int64_t ldg, int V, float* sum, float* peak) {
-    __shared__ float s[4], p[4];
-    const float* g = G + blockIdx.x * ldg;
-    float v = 0.f, m = 0.f;
-    for (int i = threadIdx.x * 4; i < V; i += 1024) {
-        const auto q = load_n<float, 4>(g + i, V - i);
+// Which rows of G hold anything: peak[n] = 0 where all of it is zero.  FULL: the largest magnitude (infinite where something is
+// no number); else some value that is not 0, and a row is read up to its first one.  A wave a row.
+template <bool FULL> __global__ void __launch_bounds__(256) grad_rows_kernel(const float* G, int64_t ldg, int64_t N, int V, float* peak) {
+    const int lane = threadIdx.x & 63;
+    const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (n >= N) return;
+    const float* g = G + n * ldg;
+    float m = 0.f;
+    auto look = [&](int v) {
+        const auto q = load_n<float, 4>(g + v + lane * 4, V - v - lane * 4);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { v += q.v[e]; m = fmaxf(m, q.v[e] != q.v[e] ? INFINITY : fabsf(q.v[e])); }
-    }
-    v = wave_sum(v);
+        for (int e = 0; e < 4; ++e) m = fmaxf(m, q.v[e] != q.v[e] ? INFINITY : fabsf(q.v[e]));
+    };
+    look(0);
+    for (int v = 256; v < V && (FULL || !__any(m != 0.f)); v += 2048)
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (v + u * 256 < V) look(v + u * 256);
     m = wave_max(m);
-    if ((threadIdx.x & 63) == 0) { s[threadIdx.x >> 6] = v; p[threadIdx.x >> 6] = m; }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        sum[blockIdx.x] = (s[0] + s[1]) + (s[2] + s[3]);
-        peak[blockIdx.x] = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
-    }
+    if (lane == 0) peak[n] = m;
 }
-// dz = G - exp(lp) sum(G) of the live rows and the outputs [v0, v0 + width), packed; a workgroup a packed row
+// dz = G - exp(lp) sum(G) of the live rows, packed.  TPR threads a row, which stays in registers between its sum and its result
+// (R pieces of 4 a thread); R = 0: rows that do not fit are read twice.
 struct LogDzArgs {
-    const float *G, *lp, *sum, *scale;
+    const float *G, *lp, *scale;
     int64_t ldg;
     const int32_t *live, *idx;
-    int32_t V, v0, width;
+    int32_t V;
     uint16_t* dz;
     int64_t pitch;
 };
-template <class X> __global__ void __launch_bounds__(256) log_dz_kernel(LogDzArgs a) {
-    const int64_t c = blockIdx.x;
+template <class X, int TPR, int R> __global__ void __launch_bounds__(256) log_dz_kernel(LogDzArgs a) {
+    __shared__ float part[4];
+    const int t = threadIdx.x % TPR;
+    const int64_t c = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
     const int live = *a.live;
-    if (c >= (int64_t)(live + kRowPad - 1) / kRowPad * kRowPad) return;
+    if (c >= (int64_t)(live + kRowPad - 1) / kRowPad * kRowPad) return;      // (256 rows, whole workgroups)
     uint16_t* row = a.dz + c * parts_of<X>() * a.pitch;
     const bool in = c < live;
     const int64_t n = in ? a.idx[c] : 0;
-    const float* g = a.G + n * a.ldg + a.v0;
-    const float* lp = a.lp + n * a.V + a.v0;
-    const float s = in ? a.sum[n] : 0.f, inv = 1.f / *a.scale;
-    const int width = in ? a.width : 0;
-    for (int v = threadIdx.x * 4; v < a.pitch; v += 1024) {
-        float d[4] = {0.f, 0.f, 0.f, 0.f};
-        if (v < width) {
-            const auto q = load_n<float, 4>(g + v, width - v);
-            const auto l = load_n<float, 4>(lp + v, width - v);
+    const float* g = a.G + n * a.ldg;
+    const float* lp = a.lp + n * a.V;
+    const int V = in ? a.V : 0;
+    const float inv = 1.f / *a.scale;
+    Pack<float, 4> gv[R ? R : 1], lv[R ? R : 1];
+    float s = 0.f;
+    if constexpr (R > 0) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) d[e] = v + e < width ? (q.v[e] - __expf(l.v[e]) * s) * inv : 0.f;
+        for (int i = 0; i < R; ++i) gv[i] = load_n<float, 4>(g + (i * TPR + t) * 4, V - (i * TPR + t) * 4);
+#pragma unroll
+        for (int i = 0; i < R; ++i) lv[i] = load_n<float, 4>(lp + (i * TPR + t) * 4, V - (i * TPR + t) * 4);
+#pragma unroll
+        for (int i = 0; i < R; ++i) s += (gv[i].v[0] + gv[i].v[1]) + (gv[i].v[2] + gv[i].v[3]);
+    } else {
+        for (int v = t * 4; v < V; v += TPR * 4) {
+            const auto q = load_n<float, 4>(g + v, V - v);
+            s += (q.v[0] + q.v[1]) + (q.v[2] + q.v[3]);
         }
-        store_dz4<X>(row, a.pitch, v, d);
+    }
+    s = wave_sum(s);
+    if constexpr (TPR > 64) {
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+        __syncthreads();
+        s = (part[0] + part[1]) + (part[2] + part[3]);
+    }
+    auto put = [&](int v, const Pack<float, 4>& q, const Pack<float, 4>& l) {
+        float d[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[e] = v + e < V ? (q.v[e] - __expf(l.v[e]) * s) * inv : 0.f;
+        if (v < a.pitch) store_dz4<X>(row, a.pitch, v, d);
+    };
+    if constexpr (R > 0) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) put((i * TPR + t) * 4, gv[i], lv[i]);
+    } else {
+        for (int v = t * 4; v < a.pitch; v += TPR * 4) put(v, load_n<float, 4>(g + v, V - v), load_n<float, 4>(lp + v, V - v));
     }
 }
 
@@ -1487,7 +1720,7 @@ Grid plan_grid(int64_t m, int64_t n, int64_t its, bool may_split) {
     for (int big = 0; big < 2; ++big) {
         const int64_t b = big ? 256 : 128, mt = ceil_div(m, b), nt = ceil_div(n, b);
         const int64_t slots = big ? kCUs : 2 * kCUs;
-        for (int64_t s = 1; s == 1 || (may_split && s <= 32 && its / s >= 8); ++s) {
+        for (int64_t s = 1; s == 1 || (may_split && s <= 128 && its / s >= 8); ++s) {
             const double cost = (double)ceil_div(mt * nt * s, slots) * (big ? 4.0 : 2 * 1.15) * (double)(ceil_div(its, s) + 6);
             if (least == 0 || cost < least) { least = cost; best = {big != 0, (int)mt, (int)nt, (int)s}; }
         }
@@ -1505,6 +1738,12 @@ struct Arena {               // carves the workspace; with base == NULL it only 
     }
 };
 
+// Few rows or few outputs: up to 64 rows (two reads of W at most) or up to 128 outputs.  Measured on both sides, forward, D 512:
+// SMALL_FIGURES
+constexpr int kSmallRows = 64, kSmallOutputs = 128;
+bool is_small(int64_t N, int32_t V) { return N <= kSmallRows || V <= kSmallOutputs; }
+int small_mv(int32_t V) { return V <= 32 || V > kSmallOutputs ? 1 : V <= 64 ? 2 : 4; }
+
 enum { kLogFwd = 0, kLogBwd = 1, kCeFwd = 2, kCeBwd = 3 };
 struct LinearPlan {
     int what, D, V, type, parts, Dp;
@@ -1513,7 +1752,7 @@ struct LinearPlan {
     Grid fwd, logp, dz, dx, dw;
     Rows rows;
     uint16_t *xp, *wp, *dzp;
-    float *top, *sum, *all, *zt, *gsum, *gpeak, *part_x, *part_w, *part_c;
+    float *top, *sum, *all, *zt, *gpeak, *part_x, *part_w, *part_c;
     size_t bytes;
 };
 int make_linear_plan(int what, int64_t N, int32_t D, int32_t V, int32_t type, void* ws, LinearPlan* out) {
@@ -1529,6 +1768,18 @@ int make_linear_plan(int what, int64_t N, int32_t D, int32_t V, int32_t type, vo
     p.Npad = std::max<int64_t>(kRowPad, round_up(N, kRowPad));
     const bool bwd = what == kLogBwd || what == kCeBwd;
     Arena a = {(char*)ws};
+    if (!bwd && is_small(N, V)) {
+        if (V > kSmallOutputs) {
+            const size_t q = (size_t)ceil_div(V, 32) * kSmallRows;
+            p.top = a.take<float>(q);
+            p.sum = a.take<float>(q);
+            p.all = a.take<float>(q);
+            p.zt = a.take<float>(kSmallRows);
+        }
+        p.bytes = a.used + 256;
+        *out = p;
+        return WF_OK;
+    }
     p.rows.live = a.take<int32_t>(1);
     p.rows.scale = a.take<float>(1);
     p.rows.pos = a.take<int32_t>(N);
@@ -1549,7 +1800,8 @@ int make_linear_plan(int what, int64_t N, int32_t D, int32_t V, int32_t type, vo
         else p.zt = a.take<float>(p.Npad);            // lse
     } else {
         const int64_t fit = std::max<int64_t>(kRowPad, (int64_t)(kPieceBytes / ((size_t)p.Npad * p.parts * 2)) / kRowPad * kRowPad);
-        p.pieces = (int)ceil_div(V, fit);
+        // (log-probabilities: their own box and their gradient's are four times a 16-bit one; its rows are read once)
+        p.pieces = what == kLogBwd ? 1 : (int)ceil_div(V, fit);
         p.width = p.pitch = round_up(ceil_div(V, p.pieces), kRowPad);
         p.pieces = (int)ceil_div(V, p.width);
         p.dzp = a.take<uint16_t>((size_t)p.Npad * p.parts * p.pitch);
@@ -1559,7 +1811,7 @@ int make_linear_plan(int what, int64_t N, int32_t D, int32_t V, int32_t type, vo
         if (p.dx.splits > 1 || p.pieces > 1) p.part_x = a.take<float>((size_t)p.dx.splits * N * D);
         if (p.dw.splits > 1) p.part_w = a.take<float>((size_t)p.dw.splits * p.width * D);
         p.part_c = a.take<float>((size_t)p.dw.splits * p.width);
-        if (what == kLogBwd) { p.gsum = a.take<float>(N); p.gpeak = a.take<float>(N); }
+        if (what == kLogBwd) p.gpeak = a.take<float>(N);
     }
     p.bytes = a.used + 256;
     *out = p;
@@ -1620,6 +1872,11 @@ int weight_operand(const LinearPlan& p, const void* w, int64_t ldw, hipStream_t 
 }
 Operand packed_x(const LinearPlan& p) { return {p.xp, (int64_t)p.parts * p.Dp, (int32_t)p.Npad, p.Dp}; }
 
+void run_rows(const RowsArgs& r, hipStream_t st) {
+    const int64_t run = round_up(ceil_div(r.N, kRowRuns), 1024);
+    rows_kernel<<<(unsigned)ceil_div(r.N, run), 1024, 0, st>>>(r, run);
+}
+
 int linear_check(const char* who, const void* x, int64_t ldx, int64_t N, const void* w, int64_t ldw, const void* bias, int32_t btype) {
     if (!w || (N > 0 && !x)) return wf_fail(WF_EINVAL, "%s: null pointer", who);
     if (ldx < 0 || ldw < 0) return wf_fail(WF_EINVAL, "%s: negative row stride", who);
@@ -1644,7 +1901,24 @@ int run_stats(const LinearPlan& p, const Operand& w, const Operand& x, const voi
     return WF_OK;
 }
 
+// the forward pass of few rows or few outputs
+int run_small(const LinearPlan& p, SmallArgs a, hipStream_t st) {
+    const int mv = small_mv(p.V), tiles = (int)ceil_div(p.V, 32 * mv);
+    a.top = p.top; a.sum = p.sum; a.all = a.smoothing != 0.f ? p.all : nullptr; a.zt = p.zt; a.pitch = kSmallRows;
+    const dim3 grid((unsigned)tiles, (unsigned)ceil_div(p.N, 32));
+    with_type(p.type, [&](auto t) {
+        using X = decltype(t);
+        if (mv == 1) small_kernel<X, 1><<<grid, 256, 0, st>>>(a);
+        else if (mv == 2) small_kernel<X, 2><<<grid, 256, 0, st>>>(a);
+        else small_kernel<X, 4><<<grid, 256, 0, st>>>(a);
+    });
+    if (p.top) small_end_kernel<<<dim3(a.out ? (unsigned)ceil_div(p.V, 4096) : 1, (unsigned)p.N), 256, 0, st>>>(a, tiles);
+    HIP_TRY(hipGetLastError());
+    return WF_OK;
+}
+
 // dx, dW, db from a piece's dz, then the next piece: dx is summed over the pieces, dW and db are final per piece
+unsigned fold_grid(int64_t elements, int splits) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(elements, splits >= 16 ? 32 : 1024), 2048)); }
 struct GradOut { void *dx, *dw, *db; int btype; };
 int run_grads(const LinearPlan& p, const Operand& w, int piece, const GradOut& o, hipStream_t st) {
     const int64_t v0 = piece * p.width, width = std::min<int64_t>(p.width, p.V - v0);
@@ -1666,7 +1940,7 @@ int run_grads(const LinearPlan& p, const Operand& w, int piece, const GradOut& o
         if (rc) return rc;
         if (p.part_x && piece == p.pieces - 1) {
             FoldArgs f = {p.part_x, nullptr, p.rows.scale, p.dx.splits, p.D, p.N, p.rows.live, p.rows.idx, o.dx, nullptr, p.type, 0};
-            fold_kernel<<<(unsigned)std::min<int64_t>(ceil_div(p.N * p.D, 1024), 2048), 256, 0, st>>>(f);
+            fold_kernel<<<fold_grid(p.N * p.D, f.splits), 256, 0, st>>>(f);
             HIP_TRY(hipGetLastError());
         }
     }
@@ -1690,7 +1964,7 @@ int run_grads(const LinearPlan& p, const Operand& w, int piece, const GradOut& o
         if (rc) return rc;
         if (p.part_w) {
             FoldArgs f = {p.part_w, g.colpart, p.rows.scale, p.dw.splits, g.M, width, nullptr, nullptr, g.out, g.colout, p.type, o.btype};
-            fold_kernel<<<(unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(width * p.D, 1024), 2048)), 256, 0, st>>>(f);
+            fold_kernel<<<fold_grid(width * p.D, f.splits), 256, 0, st>>>(f);
             HIP_TRY(hipGetLastError());
         }
     }
@@ -1728,6 +2002,11 @@ extern "C" int wf_linear_log_softmax(const void* x, int64_t ldx, int64_t N, int3
     if (N == 0) return WF_OK;
     if (!log_probs) return wf_fail(WF_EINVAL, "wf_linear_log_softmax: null pointer");
     hipStream_t st = (hipStream_t)stream;
+    if (is_small(N, V)) {
+        SmallArgs s = {};
+        s.x = x; s.w = weight; s.ldx = ldx; s.ldw = ldw; s.N = N; s.D = D; s.l = {bias, bias_type, 0, V}; s.out = log_probs;
+        return run_small(p, s, st);
+    }
     Operand w, xo = {x, ldx, (int32_t)N, p.Dp};
     if ((rc = weight_operand(p, weight, ldw, st, &w))) return rc;
     if (!direct_rows(x, ldx, D, type)) {
@@ -1764,20 +2043,24 @@ extern "C" int wf_linear_log_softmax_backward(const float* log_probs, const floa
     if (!log_probs || !grad || ldg < 0) return wf_fail(WF_EINVAL, "wf_linear_log_softmax_backward: null pointer");
     Operand w;
     if ((rc = weight_operand(p, weight, ldw, st, &w))) return rc;
-    grad_rows_kernel<<<(unsigned)N, 256, 0, st>>>(grad, ldg, V, p.gsum, p.gpeak);
+    const unsigned blocks = (unsigned)ceil_div(N, 4);
+    if (type == WF_F16) grad_rows_kernel<true><<<blocks, 256, 0, st>>>(grad, ldg, N, V, p.gpeak);
+    else grad_rows_kernel<false><<<blocks, 256, 0, st>>>(grad, ldg, N, V, p.gpeak);
     RowsArgs r = {};
-    r.r = p.rows; r.N = N; r.V = V; r.peak = p.gpeak; r.hit = 1.f;
-    rows_kernel<<<1, 1024, 0, st>>>(r);
+    r.r = p.rows; r.N = N; r.V = V; r.peak = p.gpeak; r.hit = 1.f; r.narrow = type == WF_F16;
+    run_rows(r, st);
     if ((rc = pack_rows({x, ldx, N, D, p.Dp, p.rows.pos, p.rows.live, p.xp, dx, 1}, type, st))) return rc;
-    for (int piece = 0; piece < p.pieces; ++piece) {
-        const int64_t v0 = piece * p.width;
-        LogDzArgs z = {grad, log_probs, p.gsum, p.rows.scale, ldg, p.rows.live, p.rows.idx, V, (int32_t)v0,
-                       (int32_t)std::min<int64_t>(p.width, V - v0), p.dzp, p.pitch};
-        with_type(type, [&](auto t) { log_dz_kernel<decltype(t)><<<(unsigned)p.Npad, 256, 0, st>>>(z); });
-        HIP_TRY(hipGetLastError());
-        if ((rc = run_grads(p, w, piece, {dx, dweight, dbias, bias_type}, st))) return rc;
-    }
-    return WF_OK;
+    LogDzArgs z = {grad, log_probs, p.rows.scale, ldg, p.rows.live, p.rows.idx, V, p.dzp, p.pitch};
+    with_type(type, [&](auto t) {
+        using X = decltype(t);
+        if (p.pitch <= 256) log_dz_kernel<X, 64, 1><<<(unsigned)(p.Npad / 4), 256, 0, st>>>(z);
+        else if (p.pitch <= 1024) log_dz_kernel<X, 64, 4><<<(unsigned)(p.Npad / 4), 256, 0, st>>>(z);
+        else if (p.pitch <= 6144) log_dz_kernel<X, 256, 6><<<(unsigned)p.Npad, 256, 0, st>>>(z);
+        else if (p.pitch <= 16384) log_dz_kernel<X, 256, 16><<<(unsigned)p.Npad, 256, 0, st>>>(z);
+        else log_dz_kernel<X, 256, 0><<<(unsigned)p.Npad, 256, 0, st>>>(z);
+    });
+    HIP_TRY(hipGetLastError());
+    return run_grads(p, w, 0, {dx, dweight, dbias, bias_type}, st);
 }
 
 extern "C" int wf_linear_cross_entropy(const void* x, int64_t ldx, int64_t N, int32_t D, const void* weight, int64_t ldw, int32_t V,
@@ -1792,17 +2075,26 @@ extern "C" int wf_linear_cross_entropy(const void* x, int64_t ldx, int64_t N, in
     hipStream_t st = (hipStream_t)stream;
     if (N == 0) return zero_fill(total, 1, WF_F32, st);
     if (!targets || !loss || !lse) return wf_fail(WF_EINVAL, "wf_linear_cross_entropy: null pointer");
+    if (is_small(N, V)) {
+        SmallArgs s = {};
+        s.x = x; s.w = weight; s.ldx = ldx; s.ldw = ldw; s.N = N; s.D = D; s.l = {bias, bias_type, 0, V};
+        s.targets = targets; s.target_wide = targets_wide; s.ignore = ignore_index; s.smoothing = smoothing; s.lse = lse; s.loss = loss;
+        if ((rc = run_small(p, s, st))) return rc;
+        if (total) total_kernel<<<1, 1024, 0, st>>>(loss, N, targets, targets_wide, ignore_index, mean, total);
+        HIP_TRY(hipGetLastError());
+        return WF_OK;
+    }
     Operand w;
     if ((rc = weight_operand(p, weight, ldw, st, &w))) return rc;
     RowsArgs r = {};
     r.r = p.rows; r.N = N; r.V = V; r.targets = targets; r.target_wide = targets_wide; r.ignore = ignore_index; r.loss = loss; r.lse = lse;
-    rows_kernel<<<1, 1024, 0, st>>>(r);
+    run_rows(r, st);
     if ((rc = pack_rows({x, ldx, N, D, p.Dp, p.rows.pos, p.rows.live, p.xp, nullptr, 1}, type, st))) return rc;
     if ((rc = run_stats(p, w, packed_x(p), bias, bias_type, p.rows.live, p.rows.target, smoothing != 0.f, st))) return rc;
     JoinArgs j = {p.top, p.sum, smoothing != 0.f ? p.all : nullptr, p.zt, p.Npad, N, p.fwd.mt * 2, V, p.rows.live, p.rows.idx,
                   p.rows.target, smoothing, lse, loss};
     join_kernel<<<(unsigned)ceil_div(N, 16), 256, 0, st>>>(j);
-    if (total) total_kernel<<<1, 1024, 0, st>>>(loss, N, p.rows.live, mean, total);
+    if (total) total_kernel<<<1, 1024, 0, st>>>(loss, N, targets, targets_wide, ignore_index, mean, total);
     HIP_TRY(hipGetLastError());
     return WF_OK;
 }
@@ -1826,7 +2118,7 @@ extern "C" int wf_linear_cross_entropy_backward(const float* grad, int32_t grad_
     RowsArgs r = {};
     r.r = p.rows; r.N = N; r.V = V; r.targets = targets; r.target_wide = targets_wide; r.ignore = ignore_index;
     r.gout = grad; r.gout_rows = grad_rows; r.mean = mean; r.lse_in = lse; r.hit = smoothing < 1.f ? 1.f - smoothing : 1.f;
-    rows_kernel<<<1, 1024, 0, st>>>(r);
+    run_rows(r, st);
     if ((rc = pack_rows({x, ldx, N, D, p.Dp, p.rows.pos, p.rows.live, p.xp, dx, 1}, type, st))) return rc;
     for (int piece = 0; piece < p.pieces; ++piece) {
         const int64_t v0 = piece * p.width, width = std::min<int64_t>(p.width, V - v0);

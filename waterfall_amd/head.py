@@ -10,13 +10,14 @@ entropy on the same projection, is a kernel of the library with its own gradient
 ``OutputHead`` is the module over them.  All run on the current stream of the tensors' device and can be captured in a graph.
 """
 import ctypes as C
+import functools
 
 import torch
 from torch import nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .graph import _on, _ptr, _stream
+from .graph import _on
 
 __all__ = ["layer_norm", "dropout", "linear_log_softmax", "linear_cross_entropy", "OutputHead"]
 
@@ -37,10 +38,23 @@ def _check(t, name, like=None, dtype=None):
     return t
 
 
+# The calls' host time counts: a backward pass runs on the autograd engine's own thread, where every Python operation takes
+# several times as long, with the forward's device and stream current.  Pointers go to the library as plain integers, what forward knows already is kept for backward.
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _raw_stream(device):
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def _rows(t):
     """(t as rows of its last dimension with unit stride inside a row, elements from row to row).  A view where the leading
     dimensions collapse into one, a contiguous copy otherwise."""
     D = t.shape[-1]
+    if t.is_contiguous():
+        return t, D
     n = t.numel() // D if D else 0
     if t.stride(-1) != 1 and D > 1:
         t = t.contiguous()
@@ -51,44 +65,55 @@ def _rows(t):
     return v, v.stride(0) if n > 1 else D
 
 
+@functools.lru_cache(maxsize=256)
+def _norm_bytes(N, D, t):
+    n = C.c_size_t(0)
+    _lib.check(_lib.lib().wf_layer_norm_backward_workspace_bytes(N, D, t, C.byref(n)))
+    return n.value
+
+
+def _wanted(*tensors):
+    """Whether a gradient may be asked for: without one the call skips autograd's own work (a third of a short call)."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _norm(x, weight, bias, eps, keep):
+    dev, D = x.device, x.shape[-1]
+    v, ld = _rows(x)
+    N = x.numel() // D
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    stats = torch.empty((N, 2), dtype=torch.float32, device=dev) if keep else None
+    params = weight if weight is not None else bias
+    pdtype = x.dtype if params is None else params.dtype
+    with _on(dev):
+        _lib.check(_lib.lib().wf_layer_norm(v.data_ptr(), ld, N, D, _TYPES[x.dtype], _p(weight), _p(bias), _TYPES[pdtype], eps,
+                                            y.data_ptr(), _p(stats), _raw_stream(dev)))
+    return y, v, ld, N, D, pdtype, stats
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        lib, dev = _lib.lib(), x.device
-        v, ld = _rows(x)
-        N, D = v.shape
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        keep = any(ctx.needs_input_grad)
-        stats = torch.empty((N, 2), dtype=torch.float32, device=dev) if keep else None
-        params = weight if weight is not None else bias
-        ptype = _TYPES[params.dtype if params is not None else x.dtype]
-        with _on(dev):
-            _lib.check(lib.wf_layer_norm(_ptr(v), ld, N, D, _TYPES[x.dtype], _ptr(weight), _ptr(bias), ptype, eps, _ptr(y),
-                                         _ptr(stats), _stream(dev)))
-        if keep:
-            ctx.save_for_backward(x, weight, stats)
-            ctx.ptype, ctx.bias = ptype, bias is not None
+        y, v, ld, N, D, pdtype, stats = _norm(x, weight, bias, eps, True)
+        need = ctx.needs_input_grad
+        ctx.save_for_backward(v, weight, stats)
+        ctx.rest = (x.shape, ld, N, D, pdtype, weight is not None and need[1], bias is not None and need[2])
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weight, stats = ctx.saved_tensors
-        lib, dev = _lib.lib(), x.device
-        v, ld = _rows(x)
+        v, weight, stats = ctx.saved_tensors
+        shape, ld, N, D, pdtype, want_w, want_b = ctx.rest
+        dev, t = v.device, _TYPES[v.dtype]
         g, ldg = _rows(dy)
-        N, D = v.shape
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        pt = next(k for k, n in _TYPES.items() if n == ctx.ptype)
-        dw = torch.empty(D, dtype=pt, device=dev) if weight is not None and ctx.needs_input_grad[1] else None
-        db = torch.empty(D, dtype=pt, device=dev) if ctx.bias and ctx.needs_input_grad[2] else None
-        ws, n = None, C.c_size_t(0)
-        if dw is not None or db is not None:
-            _lib.check(lib.wf_layer_norm_backward_workspace_bytes(N, D, _TYPES[x.dtype], C.byref(n)))
-            ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
-        with _on(dev):
-            _lib.check(lib.wf_layer_norm_backward(_ptr(g), ldg, _ptr(v), ld, N, D, _TYPES[x.dtype], _ptr(weight), ctx.ptype,
-                                                  _ptr(stats), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), n.value, _stream(dev)))
+        dx = torch.empty(shape, dtype=v.dtype, device=dev)
+        dw = torch.empty(D, dtype=pdtype, device=dev) if want_w else None
+        db = torch.empty(D, dtype=pdtype, device=dev) if want_b else None
+        n = _norm_bytes(N, D, t) if want_w or want_b else 0
+        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        _lib.check(_lib.lib().wf_layer_norm_backward(g.data_ptr(), ldg, v.data_ptr(), ld, N, D, t, _p(weight), _TYPES[pdtype],
+                                                     stats.data_ptr(), dx.data_ptr(), _p(dw), _p(db), _p(ws), n, _raw_stream(dev)))
         return dx, dw, db, None
 
 
@@ -109,33 +134,37 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
                 raise ValueError(f"layer_norm: {name} has shape {tuple(t.shape)}, expected {tuple(x.shape[-1:])}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError(f"layer_norm: weight is {weight.dtype}, bias is {bias.dtype}")
-    return _LayerNorm.apply(x, None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous(),
-                            float(eps))
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    if _wanted(x, weight, bias):
+        return _LayerNorm.apply(x, weight, bias, float(eps))
+    return _norm(x, weight, bias, float(eps), False)[0]
 
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, p, seed):
-        ctx.p = p
         if isinstance(seed, torch.Tensor):
             ctx.save_for_backward(seed)
-            ctx.seed = None
+            ctx.rest = (p, None)
         else:
-            ctx.seed = seed
+            ctx.rest = (p, seed)
         return _drop(x, p, seed)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        return _drop(dy, ctx.p, ctx.saved_tensors[0] if ctx.seed is None else ctx.seed), None, None
+        p, seed = ctx.rest
+        return _drop(dy, p, ctx.saved_tensors[0] if seed is None else seed), None, None
 
 
 def _drop(x, p, seed):
-    x = x.contiguous()
-    y = torch.empty_like(x)
-    key, at = (0, seed) if isinstance(seed, torch.Tensor) else (seed, None)
-    with _on(x.device):
-        _lib.check(_lib.lib().wf_dropout(_ptr(x), x.numel(), _TYPES[x.dtype], p, key, _ptr(at), _ptr(y), _stream(x.device)))
+    if not x.is_contiguous():
+        x = x.contiguous()
+    y, dev = torch.empty_like(x), x.device
+    key, at = (0, seed.data_ptr()) if isinstance(seed, torch.Tensor) else (seed, None)
+    with _on(dev):
+        _lib.check(_lib.lib().wf_dropout(x.data_ptr(), x.numel(), _TYPES[x.dtype], p, key, at, y.data_ptr(), _raw_stream(dev)))
     return y
 
 
@@ -158,7 +187,7 @@ def dropout(x, p, seed):
             raise ValueError(f"dropout: seed is on {seed.device}, x is on {x.device}")
     else:
         seed = int(seed) & 0xFFFFFFFFFFFFFFFF
-    return _Dropout.apply(x, p, seed)
+    return _Dropout.apply(x, p, seed) if _wanted(x) else _drop(x, p, seed)
 
 
 # ---- the projection ---------------------------------------------------------------------------------------------------
@@ -166,10 +195,11 @@ def dropout(x, p, seed):
 _LOG_FWD, _LOG_BWD, _CE_FWD, _CE_BWD = range(4)
 
 
-def _linear_ws(what, N, D, V, x):
+@functools.lru_cache(maxsize=256)
+def _linear_bytes(what, N, D, V, dtype):
     n = C.c_size_t(0)
-    _lib.check(_lib.lib().wf_linear_workspace_bytes(what, N, D, V, _TYPES[x.dtype], C.byref(n)))
-    return torch.empty(n.value, dtype=torch.uint8, device=x.device), n.value
+    _lib.check(_lib.lib().wf_linear_workspace_bytes(what, N, D, V, _TYPES[dtype], C.byref(n)))
+    return n.value
 
 
 def _check_linear(who, x, weight, bias):
@@ -185,44 +215,49 @@ def _check_linear(who, x, weight, bias):
             raise ValueError(f"{who}: bias has shape {tuple(bias.shape)}, expected [{weight.shape[0]}]")
 
 
-def _linear_args(x, weight, bias):
-    """(what keeps the tensors alive, the arguments x .. type)"""
+def _linear_args(x, weight):
+    """x and weight as rows, and the arguments x .. type of the library's calls"""
     v, ldx = _rows(x)
     w, ldw = _rows(weight)
-    N, D = v.shape
-    return (v, w), (_ptr(v), ldx, N, D, _ptr(w), ldw, w.shape[0], _TYPES[x.dtype])
+    D = x.shape[-1]
+    return v, w, (v.data_ptr(), ldx, x.numel() // D, D, w.data_ptr(), ldw, weight.shape[0], _TYPES[x.dtype])
+
+
+def _log_softmax(x, weight, bias):
+    dev = x.device
+    v, w, a = _linear_args(x, weight)
+    V = a[6]
+    bt = _TYPES[bias.dtype] if bias is not None else 0
+    lp = torch.empty(x.shape[:-1] + (V,), dtype=torch.float32, device=dev)
+    n = _linear_bytes(_LOG_FWD, a[2], a[3], V, x.dtype)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        _lib.check(_lib.lib().wf_linear_log_softmax(*a, _p(bias), bt, lp.data_ptr(), ws.data_ptr(), n, _raw_stream(dev)))
+    return lp, v, w, a, bt
 
 
 class _LinearLogSoftmax(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
-        dev = x.device
-        keep, a = _linear_args(x, weight, bias)
-        N, D, V = a[2], a[3], a[6]
-        bt = _TYPES[bias.dtype] if bias is not None else 0
-        lp = torch.empty(x.shape[:-1] + (V,), dtype=torch.float32, device=dev)
-        with _on(dev):
-            ws, n = _linear_ws(_LOG_FWD, N, D, V, x)
-            _lib.check(_lib.lib().wf_linear_log_softmax(*a, _ptr(bias), bt, _ptr(lp), _ptr(ws), n, _stream(dev)))
-        ctx.save_for_backward(x, weight, bias, lp)
+        lp, v, w, a, bt = _log_softmax(x, weight, bias)
+        ctx.save_for_backward(v, w, bias, lp)
+        ctx.rest = (x.shape, weight.shape, a, bt)
         return lp
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        x, weight, bias, lp = ctx.saved_tensors
-        dev = x.device
-        keep, a = _linear_args(x, weight, bias)
-        N, D, V = a[2], a[3], a[6]
+        v, w, bias, lp = ctx.saved_tensors
+        xshape, wshape, a, bt = ctx.rest
+        dev, need = v.device, ctx.needs_input_grad
         g, ldg = _rows(grad)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if ctx.needs_input_grad[0] else None
-        dw = torch.empty(weight.shape, dtype=x.dtype, device=dev) if ctx.needs_input_grad[1] else None
-        db = torch.empty(V, dtype=bias.dtype, device=dev) if ctx.needs_input_grad[2] else None
-        with _on(dev):
-            ws, n = _linear_ws(_LOG_BWD, N, D, V, x)
-            _lib.check(_lib.lib().wf_linear_log_softmax_backward(
-                _ptr(lp), _ptr(g), ldg, *a, _TYPES[bias.dtype] if bias is not None else 0, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), n,
-                _stream(dev)))
+        dx = torch.empty(xshape, dtype=v.dtype, device=dev) if need[0] else None
+        dw = torch.empty(wshape, dtype=v.dtype, device=dev) if need[1] else None
+        db = torch.empty(wshape[:1], dtype=bias.dtype, device=dev) if need[2] else None
+        n = _linear_bytes(_LOG_BWD, a[2], a[3], a[6], v.dtype)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        _lib.check(_lib.lib().wf_linear_log_softmax_backward(lp.data_ptr(), g.data_ptr(), ldg, *a, bt, _p(dx), _p(dw), _p(db),
+                                                             ws.data_ptr(), n, _raw_stream(dev)))
         return dx, dw, db
 
 
@@ -235,46 +270,51 @@ def linear_log_softmax(x, weight, bias=None):
     utterance's end) are left out whatever they hold; 16-bit types round the gradient of a logit to x's type before it enters
     the products."""
     _check_linear("linear_log_softmax", x, weight, bias)
-    return _LinearLogSoftmax.apply(x, weight, None if bias is None else bias.contiguous())
+    bias = None if bias is None else bias.contiguous()
+    return _LinearLogSoftmax.apply(x, weight, bias) if _wanted(x, weight, bias) else _log_softmax(x, weight, bias)[0]
+
+
+def _entropy(x, weight, targets, bias, ignore_index, smoothing, reduction):
+    dev = x.device
+    v, w, a = _linear_args(x, weight)
+    N = a[2]
+    bt = _TYPES[bias.dtype] if bias is not None else 0
+    rest = (_p(bias), bt, targets.data_ptr(), 1 if targets.dtype == torch.int64 else 0, ignore_index, smoothing)
+    rows, mean = 1 if reduction == "none" else 0, 1 if reduction == "mean" else 0
+    loss = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    lse = torch.empty(N, dtype=torch.float32, device=dev)
+    total = None if rows else torch.empty((), dtype=torch.float32, device=dev)
+    n = _linear_bytes(_CE_FWD, N, a[3], a[6], x.dtype)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        _lib.check(_lib.lib().wf_linear_cross_entropy(*a, *rest, loss.data_ptr(), lse.data_ptr(), _p(total), mean, ws.data_ptr(), n,
+                                                      _raw_stream(dev)))
+    return loss if rows else total, v, w, a, rest, rows, mean, lse
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, targets, bias, ignore_index, smoothing, reduction):
-        dev = x.device
-        keep, a = _linear_args(x, weight, bias)
-        N, D, V = a[2], a[3], a[6]
-        ctx.rest = (_TYPES[bias.dtype] if bias is not None else 0, 1 if targets.dtype == torch.int64 else 0, ignore_index, smoothing)
-        ctx.reduction = reduction
-        bt, wide = ctx.rest[:2]
-        loss = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
-        lse = torch.empty(N, dtype=torch.float32, device=dev)
-        total = torch.empty((), dtype=torch.float32, device=dev) if reduction != "none" else None
-        with _on(dev):
-            ws, n = _linear_ws(_CE_FWD, N, D, V, x)
-            _lib.check(_lib.lib().wf_linear_cross_entropy(*a, _ptr(bias), bt, _ptr(targets), wide, ignore_index, smoothing, _ptr(loss),
-                                                          _ptr(lse), _ptr(total), 1 if reduction == "mean" else 0, _ptr(ws), n,
-                                                          _stream(dev)))
-        ctx.save_for_backward(x, weight, targets, bias, lse)
-        return loss if total is None else total
+        loss, v, w, a, rest, rows, mean, lse = _entropy(x, weight, targets, bias, ignore_index, smoothing, reduction)
+        ctx.save_for_backward(v, w, targets, bias, lse)
+        ctx.rest = (x.shape, weight.shape, a, rest, rows, mean)
+        return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        x, weight, targets, bias, lse = ctx.saved_tensors
-        dev = x.device
-        keep, a = _linear_args(x, weight, bias)
-        N, D, V = a[2], a[3], a[6]
-        bt, wide, ignore_index, smoothing = ctx.rest
-        g = grad.contiguous()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if ctx.needs_input_grad[0] else None
-        dw = torch.empty(weight.shape, dtype=x.dtype, device=dev) if ctx.needs_input_grad[1] else None
-        db = torch.empty(V, dtype=bias.dtype, device=dev) if ctx.needs_input_grad[3] else None
-        with _on(dev):
-            ws, n = _linear_ws(_CE_BWD, N, D, V, x)
-            _lib.check(_lib.lib().wf_linear_cross_entropy_backward(
-                _ptr(g), 1 if ctx.reduction == "none" else 0, 1 if ctx.reduction == "mean" else 0, _ptr(lse), *a, _ptr(bias), bt,
-                _ptr(targets), wide, ignore_index, smoothing, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), n, _stream(dev)))
+        v, w, targets, bias, lse = ctx.saved_tensors
+        xshape, wshape, a, rest, rows, mean = ctx.rest
+        dev, need = v.device, ctx.needs_input_grad
+        if not grad.is_contiguous():
+            grad = grad.contiguous()
+        dx = torch.empty(xshape, dtype=v.dtype, device=dev) if need[0] else None
+        dw = torch.empty(wshape, dtype=v.dtype, device=dev) if need[1] else None
+        db = torch.empty(wshape[:1], dtype=bias.dtype, device=dev) if need[3] else None
+        n = _linear_bytes(_CE_BWD, a[2], a[3], a[6], v.dtype)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        _lib.check(_lib.lib().wf_linear_cross_entropy_backward(grad.data_ptr(), rows, mean, lse.data_ptr(), *a, *rest, _p(dx), _p(dw),
+                                                               _p(db), ws.data_ptr(), n, _raw_stream(dev)))
         return dx, dw, None, db, None, None, None
 
 
@@ -298,8 +338,9 @@ def linear_cross_entropy(x, weight, targets, bias=None, ignore_index=-1, label_s
         raise ValueError(f"linear_cross_entropy: label_smoothing must be in [0, 1], got {label_smoothing}")
     if reduction not in ("none", "sum", "mean"):
         raise ValueError(f"linear_cross_entropy: unknown reduction {reduction!r}")
-    return _LinearCrossEntropy.apply(x, weight, targets.contiguous(), None if bias is None else bias.contiguous(), int(ignore_index),
-                                     float(label_smoothing), reduction)
+    args = (x, weight, targets.contiguous(), None if bias is None else bias.contiguous(), int(ignore_index), float(label_smoothing),
+            reduction)
+    return _LinearCrossEntropy.apply(*args) if _wanted(x, weight, bias) else _entropy(*args)[0]
 
 
 class OutputHead(nn.Module):
