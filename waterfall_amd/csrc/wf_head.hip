@@ -821,43 +821,13 @@ template <class T> __device__ inline uint16_t bits16(float v) {
     return u;
 }
 
-// Rows of D elements into packed operand rows: planes of Dp (a multiple of 64, zeros behind D).  pos == NULL: row n goes to
-// row n.  Else row n goes to row pos[n]; pos[n] < 0: the row is dead -- it is left out, and its row of `clear` (the gradient
-// of x) becomes 0.  256 rows more of the grid clear the packed rows from the last live one to the next multiple of 256.
-struct PackArgs {
-    const void* src;
-    int64_t ld, N;
-    int D, Dp;
-    const int32_t *pos, *live;
-    uint16_t* dst;
-    void* clear;
-    int tail;                // the grid has the 256 rows more
-};
-template <class T> __global__ void __launch_bounds__(256) pack_kernel(PackArgs a) {
+// A row of D elements into a packed operand row: planes of Dp (a multiple of 64) with zeros behind D, by one wave.  src == NULL:
+// zeros.
+template <class T> __device__ inline void pack_row(uint16_t* y, const T* x, int D, int Dp, int lane) {
     constexpr int P = parts_of<T>(), VEC = 8;
-    const int lane = threadIdx.x & 63;
-    const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    int64_t c = n;
-    int D = a.D;
-    if (n >= a.N) {
-        if (!a.tail) return;
-        const int live = a.live ? *a.live : (int)a.N;
-        c = live + (n - a.N);
-        if (c >= (live + kRowPad - 1) / kRowPad * kRowPad) return;
-        D = 0;
-    } else if (a.pos) {
-        c = a.pos[n];
-        if (c < 0) {
-            if (a.clear)
-                for (int d = lane; d < a.D; d += 64) ((T*)a.clear)[n * a.D + d] = (T)0.f;
-            return;
-        }
-    }
-    const T* x = (const T*)a.src + n * a.ld;
-    uint16_t* y = a.dst + c * (int64_t)P * a.Dp;
-    for (int d = lane * VEC; d < a.Dp; d += 64 * VEC) {
+    for (int d = lane * VEC; d < Dp; d += 64 * VEC) {
         Pack<T, VEC> v;
-        if (D > d) v = load_n<T, VEC>(x + d, D - d);
+        if (x && D > d) v = load_n<T, VEC>(x + d, D - d);
         else
 #pragma unroll
             for (int i = 0; i < VEC; ++i) v.v[i] = (T)0.f;
@@ -872,7 +842,7 @@ template <class T> __global__ void __launch_bounds__(256) pack_kernel(PackArgs a
                 for (int p = 0; p < 3; ++p) h[p].v[i] = s.h[p];
             }
 #pragma unroll
-            for (int p = 0; p < 3; ++p) __builtin_memcpy(y + (size_t)p * a.Dp + d, &h[p], sizeof(h[p]));
+            for (int p = 0; p < 3; ++p) __builtin_memcpy(y + (size_t)p * Dp + d, &h[p], sizeof(h[p]));
         }
     }
 }
@@ -883,16 +853,19 @@ template <class T> __global__ void __launch_bounds__(256) pack_kernel(PackArgs a
 struct Rows {                // in the workspace
     int32_t* live;           // [1] number of live rows
     float* scale;            // [1] what the gradients of logits are relative to when they are rounded to 16 bits
-    int32_t* pos;            // [N] packed row of row n, -1: dead
     int32_t* idx;            // [Npad] row of packed row c
     int32_t* target;         // [Npad] its target, -1: none that is in range
     float* g;                // [Npad] its incoming gradient relative to the largest
     float* lse;              // [Npad]
 };
-struct RowsArgs {
+struct PrepArgs {
     Rows r;
-    int64_t N;
-    int V;
+    int64_t N, ldx, ldw;
+    int D, Dp, V;
+    const void *x, *w;
+    uint16_t *xp, *wp;       // packed operands, or NULL where they are used as they lie
+    int all;                 // every row is live and stays where it is (log-softmax forward): x and W are packed, no more
+    void* dx;                // backward: the gradient of x; its dead rows become 0
     const void* targets;     // cross entropy: row n is live iff targets[n] != ignore
     int target_wide;
     int64_t ignore;
@@ -903,20 +876,57 @@ struct RowsArgs {
     const float* lse_in;
     int narrow;              // log-softmax backward in fp16: the gradients are scaled by peak's largest
     float hit;               // backward: 1 - smoothing, or 1 where that is 0
+    int row_blocks, tail_blocks;         // workgroups over the rows, over the rows behind the last live one, then over W
+    int32_t* count;          // per kCountRows rows: how many are live, and the largest |gradient|; NULL: every workgroup looks itself
+    float* most;
 };
-__device__ inline int64_t target_of(const RowsArgs& a, int64_t n) {
+__device__ inline int64_t target_of(const PrepArgs& a, int64_t n) {
     return a.target_wide ? ((const int64_t*)a.targets)[n] : (int64_t)((const int32_t*)a.targets)[n];
 }
-// At most 64 workgroups, a run of rows each.  A workgroup counts the live rows before its run by itself (flags are a few bytes a
-// row and come from L2: no hand-over between workgroups, no second launch) and walks its run 1024 rows at a time by wave votes.
-constexpr int kRowRuns = 64;
-__global__ void __launch_bounds__(1024) rows_kernel(RowsArgs a, int64_t run) {
-    __shared__ int cnt[16];
-    __shared__ float top[16];
+__device__ inline bool row_alive(const PrepArgs& a, int64_t n) { return a.targets ? target_of(a, n) != a.ignore : a.peak[n] != 0.f; }
+__device__ inline float row_peak(const PrepArgs& a, int64_t n) { return a.narrow ? a.peak[n] : row_alive(a, n) ? fabsf(a.gout[n]) : 0.f; }
+
+// Everything before the products in one launch.  A workgroup of rows counts the live rows before its own by itself (no hand-over
+// between workgroups), gives its live rows their places by a wave's vote and packs them; others do the same for the up to 255
+// packed rows behind the last live one, which become zeros; the rest pack W.  Up to kCountedRows rows the flags themselves are
+// counted; beyond, a first launch counts every 256 of them (16000 rows: 27 us in one launch, COUNTED_TIME in two).
+constexpr int kPrepRows = 16;        // rows a workgroup packs
+constexpr int kCountRows = 256, kCountedRows = 2048;
+__global__ void __launch_bounds__(kCountRows) count_kernel(PrepArgs a) {
+    __shared__ int c[4];
+    __shared__ float m[4];
+    const int64_t n = (int64_t)blockIdx.x * kCountRows + threadIdx.x;
+    const int wave = threadIdx.x >> 6;
+    const uint64_t vote = __ballot(n < a.N && row_alive(a, n));
+    const float peak = wave_max((a.gout_rows || a.narrow) && n < a.N ? row_peak(a, n) : 0.f);
+    if ((threadIdx.x & 63) == 0) { c[wave] = __popcll(vote); m[wave] = peak; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        a.count[blockIdx.x] = (c[0] + c[1]) + (c[2] + c[3]);
+        a.most[blockIdx.x] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+    }
+}
+template <class T> __global__ void __launch_bounds__(256) prep_kernel(PrepArgs a) {
+    constexpr int P = parts_of<T>();
+    __shared__ float top[4];
+    __shared__ int cnt[4], place[kPrepRows];
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
-    const int64_t from = blockIdx.x * run, to = min(a.N, from + run);
-    const bool last = blockIdx.x + 1 == gridDim.x;
-    auto alive = [&](int64_t n) { return a.targets ? target_of(a, n) != a.ignore : a.peak[n] != 0.f; };
+    int b = blockIdx.x;
+    if (b >= a.row_blocks + a.tail_blocks) {
+        const int64_t v0 = (int64_t)(b - a.row_blocks - a.tail_blocks) * kPrepRows;
+#pragma unroll
+        for (int i = wave; i < kPrepRows; i += 4)
+            if (v0 + i < a.V) pack_row<T>(a.wp + (v0 + i) * P * a.Dp, (const T*)a.w + (v0 + i) * a.ldw, a.D, a.Dp, lane);
+        return;
+    }
+    const bool tail = b >= a.row_blocks;
+    const int64_t from = tail ? a.N : (int64_t)b * kPrepRows, to = min(a.N, from + kPrepRows);
+    if (a.all) {
+#pragma unroll
+        for (int i = wave; i < kPrepRows; i += 4)
+            if (from + i < to) pack_row<T>(a.xp + (from + i) * P * a.Dp, (const T*)a.x + (from + i) * a.ldx, a.D, a.Dp, lane);
+        return;
+    }
     // What a 16-bit gradient of a logit is relative to.  Cross entropy: the largest incoming gradient, times the target's own
     // share 1 - smoothing: where all rows weigh the same, the entry of a target is then -1 + p / (1 - smoothing) and not some
     // number whose rounding is the same in every row and adds up over them.  Log-probabilities: a power of two near the largest
@@ -924,14 +934,16 @@ __global__ void __launch_bounds__(1024) rows_kernel(RowsArgs a, int64_t run) {
     float scale = 0.f;
     if (a.gout && !a.gout_rows) {
         scale = fabsf(a.gout[0]);
-    } else if (a.gout || (a.narrow && last)) {
+    } else if (a.gout || (a.narrow && tail)) {
         float peak = 0.f;
-        for (int64_t n = t; n < a.N; n += 1024)
-            if (a.narrow || alive(n)) peak = fmaxf(peak, a.narrow ? a.peak[n] : fabsf(a.gout[n]));
+        if (a.count)
+            for (int64_t i = t; i * kCountRows < a.N; i += 256) peak = fmaxf(peak, a.most[i]);
+        else
+            for (int64_t n = t; n < a.N; n += 256) peak = fmaxf(peak, row_peak(a, n));
         peak = wave_max(peak);
         if (lane == 0) top[wave] = peak;
         __syncthreads();
-        for (int i = 0; i < 16; ++i) scale = fmaxf(scale, top[i]);
+        scale = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
     }
     if (!(scale > 0.f && scale < INFINITY)) scale = 1.f;
     else if (a.narrow) {
@@ -939,58 +951,64 @@ __global__ void __launch_bounds__(1024) rows_kernel(RowsArgs a, int64_t run) {
         (void)frexpf(scale, &e);
         scale = ldexpf(1.f, max(-100, min(100, e)));
     }
-    const float by = scale;
-    int base = 0;
-    if (from > 0) {
-        int c = 0;
-#pragma unroll 8
-        for (int64_t n = t; n < from; n += 1024) c += alive(n);
-        for (int o = 32; o; o >>= 1) c += __shfl_xor(c, o);
-        if (lane == 0) cnt[wave] = c;
-        __syncthreads();
-        for (int i = 0; i < 16; ++i) base += cnt[i];
+    int c = 0;
+    int64_t seen = 0;                      // rows whose count is known
+    if (a.count) {
+        seen = from / kCountRows * kCountRows;
+        for (int64_t i = t; i < from / kCountRows; i += 256) c += a.count[i];
     }
-    for (int64_t n0 = from; n0 < to; n0 += 1024) {
-        const int64_t n = n0 + t;
-        const bool is = n < to && alive(n);
-        const uint64_t vote = __ballot(is);
-        __syncthreads();                   // (the counts' last readers are done)
-        if (lane == 0) cnt[wave] = __popcll(vote);
-        __syncthreads();
-        int at = base + __popcll(vote & (((uint64_t)1 << lane) - 1));
-        for (int i = 0; i < 16; ++i) {
-            at += i < wave ? cnt[i] : 0;
-            base += cnt[i];
+    for (int64_t n = seen + t; n < from; n += 256) c += row_alive(a, n);
+    for (int o = 32; o; o >>= 1) c += __shfl_xor(c, o);
+    if (lane == 0) cnt[wave] = c;
+    __syncthreads();
+    int base = (cnt[0] + cnt[1]) + (cnt[2] + cnt[3]);
+    if (tail) {
+        const int end = (base + kRowPad - 1) / kRowPad * kRowPad;
+        b -= a.row_blocks;
+        if (b == 0 && t == 0) {
+            *a.r.live = base;
+            *a.r.scale = (a.mean && base > 0 ? scale / (float)base : scale) * a.hit;
         }
-        if (n >= to) continue;
-        if (!is) {
-            a.r.pos[n] = -1;
+        for (int i = wave; i < kPrepRows; i += 4) {
+            const int at = base + b * kPrepRows + i;
+            if (at >= end) break;
+            pack_row<T>(a.xp + (int64_t)at * P * a.Dp, nullptr, a.D, a.Dp, lane);
+            if (a.gout && lane == 0) { a.r.g[at] = 0.f; a.r.lse[at] = 0.f; a.r.target[at] = -1; }
+        }
+        return;
+    }
+    if (wave == 0) {
+        const int64_t n = from + lane;
+        const bool in = lane < kPrepRows && n < to, is = in && row_alive(a, n);
+        const uint64_t vote = __ballot(is);
+        const int at = base + __popcll(vote & (((uint64_t)1 << lane) - 1));
+        if (lane < kPrepRows) place[lane] = is ? at : in ? -1 : -2;
+        if (is) {
+            a.r.idx[at] = (int32_t)n;
+            int32_t want = -1;
+            if (a.targets) {
+                const int64_t v = target_of(a, n);
+                want = v >= 0 && v < a.V ? (int32_t)v : -1;
+                a.r.target[at] = want;
+            }
+            if (a.gout) {
+                a.r.g[at] = want < 0 ? 0.f : a.gout[a.gout_rows ? n : 0] / scale;
+                a.r.lse[at] = a.lse_in[n];
+            }
+        } else if (in) {
             if (a.loss) a.loss[n] = 0.f;
             if (a.lse) a.lse[n] = 0.f;
-            continue;
-        }
-        a.r.pos[n] = at;
-        a.r.idx[at] = (int32_t)n;
-        int32_t want = -1;
-        if (a.targets) {
-            const int64_t v = target_of(a, n);
-            want = v >= 0 && v < a.V ? (int32_t)v : -1;
-            a.r.target[at] = want;
-        }
-        if (a.gout) {
-            a.r.g[at] = want < 0 ? 0.f : a.gout[a.gout_rows ? n : 0] / by;
-            a.r.lse[at] = a.lse_in[n];
         }
     }
-    if (!last) return;
-    if (t == 0) {
-        if (a.mean && base > 0) scale /= (float)base;
-        *a.r.live = base;
-        *a.r.scale = scale * a.hit;
+    __syncthreads();
+#pragma unroll
+    for (int i = wave; i < kPrepRows; i += 4) {
+        const int at = place[i];
+        const int64_t n = from + i;
+        if (at >= 0) pack_row<T>(a.xp + (int64_t)at * P * a.Dp, (const T*)a.x + n * a.ldx, a.D, a.Dp, lane);
+        else if (at == -1 && a.dx)
+            for (int d = lane; d < a.D; d += 64) ((T*)a.dx)[n * a.D + d] = (T)0.f;
     }
-    // packed rows up to the end of the last tile: no gradient
-    if (a.gout)
-        for (int i = base + t; i < (base + kRowPad - 1) / kRowPad * kRowPad; i += 1024) { a.r.g[i] = 0.f; a.r.lse[i] = 0.f; a.r.target[i] = -1; }
 }
 
 // ---- epilogues ------------------------------------------------------------------------------------------------------
@@ -1087,6 +1105,7 @@ struct JoinArgs {
     const int32_t *live, *idx, *target;
     float smoothing;
     float *lse, *loss;
+    float* share;            // sums of the workgroups' losses, or NULL
 };
 __device__ inline void join_stats(float& top, float& sum, float m, float s) {
     // (a part whose largest is -inf adds its sum as it is: 0, or NaN where its logits were no numbers)
@@ -1102,9 +1121,10 @@ __device__ inline float row_loss(float lse, float zt, float all, int V, int targ
     if (smoothing != 0.f) loss -= smoothing * (all / (float)V);
     return loss;
 }
-// 16 rows a workgroup, 16 threads a row: each joins every 16th tile, then they meet in LDS
+// 16 rows a workgroup, 16 threads a row: each joins every 16th tile, then they meet in LDS.  (The total in the same launch, by the
+// workgroup that is done last, took 18 us more at 1000 workgroups: each one's release empties its die's L2.)
 __global__ void __launch_bounds__(256) join_kernel(JoinArgs a) {
-    __shared__ float tops[16][17], sums[16][17], alls[16][17];
+    __shared__ float tops[16][17], sums[16][17], alls[16][17], loss[16];
     const int r = threadIdx.x & 15, k = threadIdx.x >> 4;
     const int64_t c = (int64_t)blockIdx.x * 16 + r, rows = a.live ? (int64_t)*a.live : a.N;
     if ((int64_t)blockIdx.x * 16 >= rows) return;
@@ -1117,16 +1137,41 @@ __global__ void __launch_bounds__(256) join_kernel(JoinArgs a) {
     tops[k][r] = top;
     sums[k][r] = sum;
     alls[k][r] = all;
+    if (k == 0) loss[r] = 0.f;
     __syncthreads();
-    if (k != 0 || c >= rows) return;
-    for (int i = 1; i < 16; ++i) {
-        join_stats(top, sum, tops[i][r], sums[i][r]);
-        all += alls[i][r];
+    if (k == 0 && c < rows) {
+        for (int i = 1; i < 16; ++i) {
+            join_stats(top, sum, tops[i][r], sums[i][r]);
+            all += alls[i][r];
+        }
+        const float lse = (top == -INFINITY ? 0.f : top) + logf(sum);
+        const int64_t n = a.idx ? a.idx[c] : c;
+        a.lse[n] = lse;
+        if (a.loss) a.loss[n] = loss[r] = row_loss(lse, a.zt[c], all, a.V, a.target[c], a.smoothing);
     }
-    const float lse = (top == -INFINITY ? 0.f : top) + logf(sum);
-    const int64_t n = a.idx ? a.idx[c] : c;
-    a.lse[n] = lse;
-    if (a.loss) a.loss[n] = row_loss(lse, a.zt[c], all, a.V, a.target[c], a.smoothing);
+    if (!a.share) return;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        float v = 0.f;
+        for (int i = 0; i < 16; ++i) v += loss[i];
+        a.share[blockIdx.x] = v;
+    }
+}
+// the sum of the workgroups' shares, over the number of rows where `mean` (0 rows: 0)
+__global__ void __launch_bounds__(1024) shares_kernel(const float* share, const int32_t* live, int mean, float* out) {
+    __shared__ float s[16];
+    const int rows = *live, n = (rows + 15) / 16;
+    float v = 0.f;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += 1024) v += share[i];
+    v = wave_sum(v);
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        v = 0.f;
+        for (int i = 0; i < 16; ++i) v += s[i];
+        *out = mean && rows > 0 ? v / (float)rows : v;
+    }
 }
 // sum of the losses, over the number of rows whose target is not `ignore` where `mean`
 __global__ void __launch_bounds__(1024) total_kernel(const float* loss, int64_t N, const void* targets, int wide, int64_t ignore, int mean, float* out) {
@@ -1134,6 +1179,7 @@ __global__ void __launch_bounds__(1024) total_kernel(const float* loss, int64_t 
     __shared__ int c[16];
     float v = 0.f;
     int k = 0;
+#pragma unroll 4
     for (int64_t n = threadIdx.x; n < N; n += 1024) {
         v += loss[n];
         if (mean) k += (wide ? ((const int64_t*)targets)[n] : (int64_t)((const int32_t*)targets)[n]) != ignore;
@@ -1751,8 +1797,10 @@ struct LinearPlan {
     int pieces;
     Grid fwd, logp, dz, dx, dw;
     Rows rows;
+    int32_t* count;
+    float* most;
     uint16_t *xp, *wp, *dzp;
-    float *top, *sum, *all, *zt, *gpeak, *part_x, *part_w, *part_c;
+    float *top, *sum, *all, *zt, *share, *gpeak, *part_x, *part_w, *part_c;
     size_t bytes;
 };
 int make_linear_plan(int what, int64_t N, int32_t D, int32_t V, int32_t type, void* ws, LinearPlan* out) {
@@ -1782,7 +1830,8 @@ int make_linear_plan(int what, int64_t N, int32_t D, int32_t V, int32_t type, vo
     }
     p.rows.live = a.take<int32_t>(1);
     p.rows.scale = a.take<float>(1);
-    p.rows.pos = a.take<int32_t>(N);
+    p.count = a.take<int32_t>(ceil_div(N, kCountRows) + 1);
+    p.most = a.take<float>(ceil_div(N, kCountRows) + 1);
     p.rows.idx = a.take<int32_t>(p.Npad);
     p.rows.target = a.take<int32_t>(p.Npad);
     p.rows.g = a.take<float>(p.Npad);
@@ -1796,7 +1845,7 @@ int make_linear_plan(int what, int64_t N, int32_t D, int32_t V, int32_t type, vo
         const size_t q = (size_t)p.fwd.mt * 2 * p.Npad;
         p.top = a.take<float>(q);
         p.sum = a.take<float>(q);
-        if (what == kCeFwd) { p.all = a.take<float>(q); p.zt = a.take<float>(p.Npad); }
+        if (what == kCeFwd) { p.all = a.take<float>(q); p.zt = a.take<float>(p.Npad); p.share = a.take<float>(p.Npad / 16); }
         else p.zt = a.take<float>(p.Npad);            // lse
     } else {
         const int64_t fit = std::max<int64_t>(kRowPad, (int64_t)(kPieceBytes / ((size_t)p.Npad * p.parts * 2)) / kRowPad * kRowPad);
@@ -1856,26 +1905,27 @@ template <class F> void with_big(bool big, F&& f) { if (big) f(std::true_type())
 bool direct_rows(const void* p, int64_t ld, int64_t D, int type) {   // usable as an operand where it lies
     return type != WF_F32 && D % kBK == 0 && ld % 8 == 0 && (uintptr_t)p % 16 == 0;
 }
-int pack_rows(const PackArgs& a, int type, hipStream_t st) {
-    with_type(type, [&](auto t) { pack_kernel<decltype(t)><<<(unsigned)ceil_div(a.N + kRowPad, 4), 256, 0, st>>>(a); });
-    HIP_TRY(hipGetLastError());
-    return WF_OK;
-}
-// W as an operand: where it lies, or packed
-int weight_operand(const LinearPlan& p, const void* w, int64_t ldw, hipStream_t st, Operand* o) {
-    if (direct_rows(w, ldw, p.D, p.type)) { *o = {w, ldw, p.V, p.Dp}; return WF_OK; }
-    *o = {p.wp, (int64_t)p.parts * p.Dp, p.V, p.Dp};
-    PackArgs a = {w, ldw, p.V, p.D, p.Dp, nullptr, nullptr, p.wp, nullptr, 0};
-    with_type(p.type, [&](auto t) { pack_kernel<decltype(t)><<<(unsigned)ceil_div(p.V, 4), 256, 0, st>>>(a); });   // (no rows behind W)
+// Packs what has to be packed and places the rows; *w is W as an operand, where it lies or packed.
+int run_prep(const LinearPlan& p, PrepArgs a, const void* x, int64_t ldx, const void* w, int64_t ldw, hipStream_t st, Operand* wo) {
+    const bool direct = direct_rows(w, ldw, p.D, p.type);
+    if (direct) *wo = {w, ldw, p.V, p.Dp};
+    else *wo = {p.wp, (int64_t)p.parts * p.Dp, p.V, p.Dp};
+    a.r = p.rows; a.N = p.N; a.ldx = ldx; a.ldw = ldw; a.D = p.D; a.Dp = p.Dp; a.V = p.V; a.x = x; a.w = w;
+    a.wp = direct ? nullptr : p.wp;
+    a.row_blocks = a.xp ? (int)ceil_div(p.N, kPrepRows) : 0;
+    a.tail_blocks = a.all ? 0 : kRowPad / kPrepRows;
+    const unsigned blocks = (unsigned)(a.row_blocks + a.tail_blocks + (direct ? 0 : ceil_div(p.V, kPrepRows)));
+    if (!blocks) return WF_OK;
+    if (!a.all && p.N > kCountedRows) {
+        a.count = p.count;
+        a.most = p.most;
+        count_kernel<<<(unsigned)ceil_div(p.N, kCountRows), kCountRows, 0, st>>>(a);
+    }
+    with_type(p.type, [&](auto t) { prep_kernel<decltype(t)><<<blocks, 256, 0, st>>>(a); });
     HIP_TRY(hipGetLastError());
     return WF_OK;
 }
 Operand packed_x(const LinearPlan& p) { return {p.xp, (int64_t)p.parts * p.Dp, (int32_t)p.Npad, p.Dp}; }
-
-void run_rows(const RowsArgs& r, hipStream_t st) {
-    const int64_t run = round_up(ceil_div(r.N, kRowRuns), 1024);
-    rows_kernel<<<(unsigned)ceil_div(r.N, run), 1024, 0, st>>>(r, run);
-}
 
 int linear_check(const char* who, const void* x, int64_t ldx, int64_t N, const void* w, int64_t ldw, const void* bias, int32_t btype) {
     if (!w || (N > 0 && !x)) return wf_fail(WF_EINVAL, "%s: null pointer", who);
@@ -2008,13 +2058,16 @@ extern "C" int wf_linear_log_softmax(const void* x, int64_t ldx, int64_t N, int3
         return run_small(p, s, st);
     }
     Operand w, xo = {x, ldx, (int32_t)N, p.Dp};
-    if ((rc = weight_operand(p, weight, ldw, st, &w))) return rc;
+    PrepArgs r = {};
+    r.all = 1;
     if (!direct_rows(x, ldx, D, type)) {
-        xo = packed_x(p);
-        if ((rc = pack_rows({x, ldx, N, D, p.Dp, nullptr, nullptr, p.xp, nullptr, 1}, type, st))) return rc;
+        r.xp = p.xp;
+        xo = {p.xp, (int64_t)p.parts * p.Dp, (int32_t)N, p.Dp};
     }
+    if ((rc = run_prep(p, r, x, ldx, weight, ldw, st, &w))) return rc;
     if ((rc = run_stats(p, w, xo, bias, bias_type, nullptr, nullptr, false, st))) return rc;
-    JoinArgs j = {p.top, p.sum, nullptr, nullptr, p.Npad, N, p.fwd.mt * 2, V, nullptr, nullptr, nullptr, 0.f, p.zt, nullptr};
+    JoinArgs j = {};
+    j.top = p.top; j.sum = p.sum; j.pitch = p.Npad; j.N = N; j.tiles = p.fwd.mt * 2; j.V = V; j.lse = p.zt;
     join_kernel<<<(unsigned)ceil_div(N, 16), 256, 0, st>>>(j);
     LogProbArgs l = {};
     l.p = {xo, w, p.logp.mt, p.logp.nt, p.Dp / kBK, 1, {}, {}, nullptr, 0, 1};
@@ -2041,15 +2094,13 @@ extern "C" int wf_linear_log_softmax_backward(const float* log_probs, const floa
     hipStream_t st = (hipStream_t)stream;
     if (N == 0) return (rc = zero_fill(dweight, (int64_t)V * D, type, st)) ? rc : zero_fill(dbias, V, bias_type, st);
     if (!log_probs || !grad || ldg < 0) return wf_fail(WF_EINVAL, "wf_linear_log_softmax_backward: null pointer");
-    Operand w;
-    if ((rc = weight_operand(p, weight, ldw, st, &w))) return rc;
     const unsigned blocks = (unsigned)ceil_div(N, 4);
     if (type == WF_F16) grad_rows_kernel<true><<<blocks, 256, 0, st>>>(grad, ldg, N, V, p.gpeak);
     else grad_rows_kernel<false><<<blocks, 256, 0, st>>>(grad, ldg, N, V, p.gpeak);
-    RowsArgs r = {};
-    r.r = p.rows; r.N = N; r.V = V; r.peak = p.gpeak; r.hit = 1.f; r.narrow = type == WF_F16;
-    run_rows(r, st);
-    if ((rc = pack_rows({x, ldx, N, D, p.Dp, p.rows.pos, p.rows.live, p.xp, dx, 1}, type, st))) return rc;
+    Operand w;
+    PrepArgs r = {};
+    r.xp = p.xp; r.dx = dx; r.peak = p.gpeak; r.hit = 1.f; r.narrow = type == WF_F16;
+    if ((rc = run_prep(p, r, x, ldx, weight, ldw, st, &w))) return rc;
     LogDzArgs z = {grad, log_probs, p.rows.scale, ldg, p.rows.live, p.rows.idx, V, p.dzp, p.pitch};
     with_type(type, [&](auto t) {
         using X = decltype(t);
@@ -2085,16 +2136,16 @@ extern "C" int wf_linear_cross_entropy(const void* x, int64_t ldx, int64_t N, in
         return WF_OK;
     }
     Operand w;
-    if ((rc = weight_operand(p, weight, ldw, st, &w))) return rc;
-    RowsArgs r = {};
-    r.r = p.rows; r.N = N; r.V = V; r.targets = targets; r.target_wide = targets_wide; r.ignore = ignore_index; r.loss = loss; r.lse = lse;
-    run_rows(r, st);
-    if ((rc = pack_rows({x, ldx, N, D, p.Dp, p.rows.pos, p.rows.live, p.xp, nullptr, 1}, type, st))) return rc;
+    PrepArgs r = {};
+    r.xp = p.xp; r.targets = targets; r.target_wide = targets_wide; r.ignore = ignore_index; r.loss = loss; r.lse = lse; r.hit = 1.f;
+    if ((rc = run_prep(p, r, x, ldx, weight, ldw, st, &w))) return rc;
     if ((rc = run_stats(p, w, packed_x(p), bias, bias_type, p.rows.live, p.rows.target, smoothing != 0.f, st))) return rc;
-    JoinArgs j = {p.top, p.sum, smoothing != 0.f ? p.all : nullptr, p.zt, p.Npad, N, p.fwd.mt * 2, V, p.rows.live, p.rows.idx,
-                  p.rows.target, smoothing, lse, loss};
+    JoinArgs j = {};
+    j.top = p.top; j.sum = p.sum; j.all = smoothing != 0.f ? p.all : nullptr; j.zt = p.zt; j.pitch = p.Npad; j.N = N;
+    j.tiles = p.fwd.mt * 2; j.V = V; j.live = p.rows.live; j.idx = p.rows.idx; j.target = p.rows.target; j.smoothing = smoothing;
+    j.lse = lse; j.loss = loss; j.share = total ? p.share : nullptr;
     join_kernel<<<(unsigned)ceil_div(N, 16), 256, 0, st>>>(j);
-    if (total) total_kernel<<<1, 1024, 0, st>>>(loss, N, targets, targets_wide, ignore_index, mean, total);
+    if (total) shares_kernel<<<1, 1024, 0, st>>>(p.share, p.rows.live, mean, total);
     HIP_TRY(hipGetLastError());
     return WF_OK;
 }
@@ -2114,12 +2165,10 @@ extern "C" int wf_linear_cross_entropy_backward(const float* grad, int32_t grad_
     if (N == 0) return (rc = zero_fill(dweight, (int64_t)V * D, type, st)) ? rc : zero_fill(dbias, V, bias_type, st);
     if (!targets || !grad || !lse) return wf_fail(WF_EINVAL, "wf_linear_cross_entropy_backward: null pointer");
     Operand w;
-    if ((rc = weight_operand(p, weight, ldw, st, &w))) return rc;
-    RowsArgs r = {};
-    r.r = p.rows; r.N = N; r.V = V; r.targets = targets; r.target_wide = targets_wide; r.ignore = ignore_index;
+    PrepArgs r = {};
+    r.xp = p.xp; r.dx = dx; r.targets = targets; r.target_wide = targets_wide; r.ignore = ignore_index;
     r.gout = grad; r.gout_rows = grad_rows; r.mean = mean; r.lse_in = lse; r.hit = smoothing < 1.f ? 1.f - smoothing : 1.f;
-    run_rows(r, st);
-    if ((rc = pack_rows({x, ldx, N, D, p.Dp, p.rows.pos, p.rows.live, p.xp, dx, 1}, type, st))) return rc;
+    if ((rc = run_prep(p, r, x, ldx, weight, ldw, st, &w))) return rc;
     for (int piece = 0; piece < p.pieces; ++piece) {
         const int64_t v0 = piece * p.width, width = std::min<int64_t>(p.width, V - v0);
         DzArgs z = {};
