@@ -889,7 +889,7 @@ __device__ inline float row_peak(const PrepArgs& a, int64_t n) { return a.narrow
 // Everything before the products in one launch.  A workgroup of rows counts the live rows before its own by itself (no hand-over
 // between workgroups), gives its live rows their places by a wave's vote and packs them; others do the same for the up to 255
 // packed rows behind the last live one, which become zeros; the rest pack W.  Up to kCountedRows rows the flags themselves are
-// counted; beyond, a first launch counts every 256 of them (16000 rows: 27 us in one launch, COUNTED_TIME in two).
+// counted; beyond, a first launch counts every 256 of them (16000 x 512 bf16: 27 us in one launch, 11 in two).
 constexpr int kPrepRows = 16;        // rows a workgroup packs
 constexpr int kCountRows = 256, kCountedRows = 2048;
 __global__ void __launch_bounds__(kCountRows) count_kernel(PrepArgs a) {
@@ -1214,7 +1214,31 @@ struct SmallArgs {
     int64_t ignore;
     float smoothing;
     float *zt, *lse, *loss;
+    // gradients of the logits instead: of the packed rows, see dz_kernel
+    const int32_t *live, *idx, *want;
+    const float *g, *glse;
+    uint16_t* dz;
+    int64_t zpitch;
 };
+// 16-bit planes of four neighbouring values
+template <class T> __device__ inline void store_dz4(uint16_t* row, int64_t pitch, int v, const float (&d)[4]) {
+    if constexpr (parts_of<T>() == 1) {
+        Pack<uint16_t, 4> h;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h.v[i] = bits16<T>(d[i]);
+        __builtin_memcpy(row + v, &h, 8);
+    } else {
+        Pack<uint16_t, 4> h[3];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const Split3 s = split3(d[i]);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) h[p].v[i] = s.h[p];
+        }
+#pragma unroll
+        for (int p = 0; p < 3; ++p) __builtin_memcpy(row + p * pitch + v, &h[p], 8);
+    }
+}
 template <class X> __device__ inline void split_frag(const Pack<X, 8>& v, typename Mfma<typename Half<X>::type>::v8 (&f)[parts_of<X>()]) {
     if constexpr (parts_of<X>() == 1) {
         __builtin_memcpy(&f[0], &v, 16);
@@ -1235,7 +1259,7 @@ __device__ inline int32_t small_target(const void* targets, int wide, int64_t ig
     *dead = t == ignore;
     return t >= 0 && t < V ? (int32_t)t : -1;
 }
-template <class X, int MV> __global__ void __launch_bounds__(256) small_kernel(SmallArgs a) {
+template <class X, int MV, bool DZ> __global__ void __launch_bounds__(256) small_kernel(SmallArgs a) {
     using T = typename Half<X>::type;
     constexpr int P = parts_of<X>(), U = P == 1 ? 4 : 2;      // steps whose loads are under way together
     __shared__ __align__(16) float part[4][MV][4][64][4];     // [wave][m][q][lane][e]
@@ -1243,7 +1267,9 @@ template <class X, int MV> __global__ void __launch_bounds__(256) small_kernel(S
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int v0 = blockIdx.x * 32 * MV, kl = (lane >> 5) * 8;
     const int64_t n0 = (int64_t)blockIdx.y * 32, n = n0 + (lane & 31);
-    const X* xr = (const X*)a.x + min(n, a.N - 1) * a.ldx;
+    const int live = DZ ? *a.live : 0;
+    if (DZ && n0 >= (live + kBK - 1) / kBK * kBK) return;     // rows that no product reads
+    const X* xr = (const X*)a.x + (DZ ? (int64_t)(n < live ? a.idx[n] : 0) : min(n, a.N - 1)) * a.ldx;
     const X* wr[MV];
 #pragma unroll
     for (int m = 0; m < MV; ++m) wr[m] = (const X*)a.w + (int64_t)min(v0 + m * 32 + (lane & 31), a.l.V - 1) * a.ldw;
@@ -1286,6 +1312,29 @@ template <class X, int MV> __global__ void __launch_bounds__(256) small_kernel(S
     if (threadIdx.x < 32) wzt[threadIdx.x] = 0.f;
     __syncthreads();
     // wave q ends quarter q of every 32 outputs: v0 + 32 m + 8 q + 4 (lane / 32) .. + 3 of row lane % 32
+    if constexpr (DZ) {
+        const float share = a.smoothing < 1.f ? 1.f / (1.f - a.smoothing) : 1.f, hit = a.smoothing < 1.f ? 1.f : 0.f;
+        const float g = n < live ? a.g[n] : 0.f, lse = n < live ? a.glse[n] : 0.f, ref = lse == -INFINITY ? 0.f : lse;
+        const int target = n < live ? a.want[n] : -1;
+        const bool none = g == 0.f || lse == -INFINITY;
+        const float even = a.smoothing / (float)a.l.V;
+#pragma unroll
+        for (int m = 0; m < MV; ++m) {
+            const v4f s = (*(const v4f*)part[0][m][wave][lane] + *(const v4f*)part[1][m][wave][lane]) +
+                          (*(const v4f*)part[2][m][wave][lane] + *(const v4f*)part[3][m][wave][lane]);
+            const int v = v0 + m * 32 + wave * 8 + (lane >> 5) * 4;
+            float d[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool in = v + e < a.l.V;
+                const float z = in && a.l.bias ? s[e] + load_any(a.l.bias, a.l.btype, v + e) : s[e];
+                const float u = g * ((__expf(z - ref) - even) * share - (v + e == target ? hit : 0.f));
+                d[e] = none | !in ? 0.f : u;
+            }
+            if (v < a.zpitch) store_dz4<X>(a.dz + n * P * a.zpitch, a.zpitch, v, d);
+        }
+        return;
+    }
     bool dead = false;
     const int want = a.targets && n < a.N ? small_target(a.targets, a.target_wide, a.ignore, n, a.l.V, &dead) : -1;
     v4f z[MV];
@@ -1469,25 +1518,6 @@ template <int MI, class G, class P> __device__ inline void rows_out16(char* w, i
     for (int k = 0; k < MI * 2; ++k) {
         const int r = (k * 64 + lane) / C, c = (k * 64 + lane) % C;
         put(r, c * 8, *(const v8h*)(w + r * (C * 16) + ((c ^ (r & (C - 1))) * 16)));
-    }
-}
-// 16-bit planes of four neighbouring values
-template <class T> __device__ inline void store_dz4(uint16_t* row, int64_t pitch, int v, const float (&d)[4]) {
-    if constexpr (parts_of<T>() == 1) {
-        Pack<uint16_t, 4> h;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) h.v[i] = bits16<T>(d[i]);
-        __builtin_memcpy(row + v, &h, 8);
-    } else {
-        Pack<uint16_t, 4> h[3];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const Split3 s = split3(d[i]);
-#pragma unroll
-            for (int p = 0; p < 3; ++p) h[p].v[i] = s.h[p];
-        }
-#pragma unroll
-        for (int p = 0; p < 3; ++p) __builtin_memcpy(row + p * pitch + v, &h[p], 8);
     }
 }
 // d loss / d z of a piece of the outputs from logits that are computed again: g (p - (1 - e) [v = target] - e / V), rounded to
@@ -1784,10 +1814,16 @@ struct Arena {               // carves the workspace; with base == NULL it only 
     }
 };
 
-// Few rows or few outputs: up to 64 rows (two reads of W at most) or up to 128 outputs.  Measured on both sides, forward, D 512:
-// SMALL_FIGURES
-constexpr int kSmallRows = 64, kSmallOutputs = 128;
-bool is_small(int64_t N, int32_t V) { return N <= kSmallRows || V <= kSmallOutputs; }
+// Logits straight from memory (small_kernel) or by tiles: a table of at most 128 outputs is always small, else the work decides.
+// Forward with log-probabilities, us, small / tiles, at N of V 5001, D 512: fp32 1: 15 / 74, 256: 36 / 83, 512: 57 / 87, 1024: 99 /
+// 107; bf16 1: 9.5 / 20, 64: 13 / 24, 256: 22 / 24, 512: 35 / 26; of V 15001, D 1024: fp32 64: 47 / 172, 512: 256 / 241, bf16 64:
+// 27 / 38, 256: 78 / 45; of V 500, D 256: bf16 2048: 16 / 19.
+constexpr int kSmallOutputs = 128;
+constexpr double kSmallWork = 0.7e9, kSmallWorkF32 = 1.6e9;      // N V D
+bool is_small(int64_t N, int32_t D, int32_t V, int type) {
+    if (V <= kSmallOutputs) return N <= 32 * 65535;          // (workgroups in a launch's second dimension)
+    return N <= 65535 && (double)N * V * D <= (type == WF_F32 ? kSmallWorkF32 : kSmallWork);
+}
 int small_mv(int32_t V) { return V <= 32 || V > kSmallOutputs ? 1 : V <= 64 ? 2 : 4; }
 
 enum { kLogFwd = 0, kLogBwd = 1, kCeFwd = 2, kCeBwd = 3 };
@@ -1795,6 +1831,7 @@ struct LinearPlan {
     int what, D, V, type, parts, Dp;
     int64_t N, Npad, pitch, width;      // width: outputs of a piece, pitch: its padded row
     int pieces;
+    bool small;
     Grid fwd, logp, dz, dx, dw;
     Rows rows;
     int32_t* count;
@@ -1816,13 +1853,14 @@ int make_linear_plan(int what, int64_t N, int32_t D, int32_t V, int32_t type, vo
     p.Npad = std::max<int64_t>(kRowPad, round_up(N, kRowPad));
     const bool bwd = what == kLogBwd || what == kCeBwd;
     Arena a = {(char*)ws};
-    if (!bwd && is_small(N, V)) {
+    p.small = is_small(N, D, V, type);
+    if (!bwd && p.small) {
         if (V > kSmallOutputs) {
-            const size_t q = (size_t)ceil_div(V, 32) * kSmallRows;
+            const size_t q = (size_t)ceil_div(V, 32) * N;
             p.top = a.take<float>(q);
             p.sum = a.take<float>(q);
             p.all = a.take<float>(q);
-            p.zt = a.take<float>(kSmallRows);
+            p.zt = a.take<float>(N);
         }
         p.bytes = a.used + 256;
         *out = p;
@@ -1853,6 +1891,7 @@ int make_linear_plan(int what, int64_t N, int32_t D, int32_t V, int32_t type, vo
         p.pieces = what == kLogBwd ? 1 : (int)ceil_div(V, fit);
         p.width = p.pitch = round_up(ceil_div(V, p.pieces), kRowPad);
         p.pieces = (int)ceil_div(V, p.width);
+        p.small = p.small && p.pieces == 1;
         p.dzp = a.take<uint16_t>((size_t)p.Npad * p.parts * p.pitch);
         p.dz = plan_grid(p.width, N, dits, false);
         p.dx = plan_grid(D, N, products * p.pitch / kBK, true);
@@ -1954,13 +1993,13 @@ int run_stats(const LinearPlan& p, const Operand& w, const Operand& x, const voi
 // the forward pass of few rows or few outputs
 int run_small(const LinearPlan& p, SmallArgs a, hipStream_t st) {
     const int mv = small_mv(p.V), tiles = (int)ceil_div(p.V, 32 * mv);
-    a.top = p.top; a.sum = p.sum; a.all = a.smoothing != 0.f ? p.all : nullptr; a.zt = p.zt; a.pitch = kSmallRows;
+    a.top = p.top; a.sum = p.sum; a.all = a.smoothing != 0.f ? p.all : nullptr; a.zt = p.zt; a.pitch = p.N;
     const dim3 grid((unsigned)tiles, (unsigned)ceil_div(p.N, 32));
     with_type(p.type, [&](auto t) {
         using X = decltype(t);
-        if (mv == 1) small_kernel<X, 1><<<grid, 256, 0, st>>>(a);
-        else if (mv == 2) small_kernel<X, 2><<<grid, 256, 0, st>>>(a);
-        else small_kernel<X, 4><<<grid, 256, 0, st>>>(a);
+        if (mv == 1) small_kernel<X, 1, false><<<grid, 256, 0, st>>>(a);
+        else if (mv == 2) small_kernel<X, 2, false><<<grid, 256, 0, st>>>(a);
+        else small_kernel<X, 4, false><<<grid, 256, 0, st>>>(a);
     });
     if (p.top) small_end_kernel<<<dim3(a.out ? (unsigned)ceil_div(p.V, 4096) : 1, (unsigned)p.N), 256, 0, st>>>(a, tiles);
     HIP_TRY(hipGetLastError());
@@ -2052,7 +2091,7 @@ extern "C" int wf_linear_log_softmax(const void* x, int64_t ldx, int64_t N, int3
     if (N == 0) return WF_OK;
     if (!log_probs) return wf_fail(WF_EINVAL, "wf_linear_log_softmax: null pointer");
     hipStream_t st = (hipStream_t)stream;
-    if (is_small(N, V)) {
+    if (p.small) {
         SmallArgs s = {};
         s.x = x; s.w = weight; s.ldx = ldx; s.ldw = ldw; s.N = N; s.D = D; s.l = {bias, bias_type, 0, V}; s.out = log_probs;
         return run_small(p, s, st);
@@ -2126,7 +2165,7 @@ extern "C" int wf_linear_cross_entropy(const void* x, int64_t ldx, int64_t N, in
     hipStream_t st = (hipStream_t)stream;
     if (N == 0) return zero_fill(total, 1, WF_F32, st);
     if (!targets || !loss || !lse) return wf_fail(WF_EINVAL, "wf_linear_cross_entropy: null pointer");
-    if (is_small(N, V)) {
+    if (p.small) {
         SmallArgs s = {};
         s.x = x; s.w = weight; s.ldx = ldx; s.ldw = ldw; s.N = N; s.D = D; s.l = {bias, bias_type, 0, V};
         s.targets = targets; s.target_wide = targets_wide; s.ignore = ignore_index; s.smoothing = smoothing; s.lse = lse; s.loss = loss;
@@ -2177,7 +2216,20 @@ extern "C" int wf_linear_cross_entropy_backward(const float* grad, int32_t grad_
         set_parts(&z.p, type, p.Dp, p.Dp);
         z.l = {bias, bias_type, (int32_t)v0, (int32_t)(v0 + width)};
         z.target = p.rows.target; z.g = p.rows.g; z.lse = p.rows.lse; z.smoothing = smoothing; z.outputs = V; z.dz = p.dzp; z.pitch = p.pitch;
-        with_type(type, [&](auto t) {
+        if (p.small) {
+            SmallArgs s = {};
+            s.x = x; s.w = weight; s.ldx = ldx; s.ldw = ldw; s.N = N; s.D = D; s.l = {bias, bias_type, 0, V}; s.smoothing = smoothing;
+            s.live = p.rows.live; s.idx = p.rows.idx; s.want = p.rows.target; s.g = p.rows.g; s.glse = p.rows.lse; s.dz = p.dzp; s.zpitch = p.pitch;
+            const int mv = small_mv(V);
+            const dim3 grid((unsigned)ceil_div(round_up(V, kBK), 32 * mv), (unsigned)ceil_div(round_up(N, kBK), 32));
+            with_type(type, [&](auto t) {
+                using X = decltype(t);
+                if (mv == 1) small_kernel<X, 1, true><<<grid, 256, 0, st>>>(s);
+                else if (mv == 2) small_kernel<X, 2, true><<<grid, 256, 0, st>>>(s);
+                else small_kernel<X, 4, true><<<grid, 256, 0, st>>>(s);
+            });
+            HIP_TRY(hipGetLastError());
+        } else with_type(type, [&](auto t) {
             with_big(p.dz.big, [&](auto b) {
                 rc = launch_tiles<Shape<decltype(b)::value>, dz_kernel<decltype(t), decltype(b)::value>>(z, st);
             });
