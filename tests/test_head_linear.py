@@ -419,7 +419,7 @@ def test_the_projection_refuses_what_it_cannot_do():
     import ctypes as C
     lib, n = _lib.lib(), C.c_size_t(0)
     for what, N, D, V, t, rc in ((0, 5, 8, 3, 0, 0), (4, 5, 8, 3, 0, -1), (0, -1, 8, 3, 0, -1), (1, 5, 0, 3, 0, -1), (2, 5, 8, 0, 0, -1),
-                                 (3, 5, 8, 3, 9, -1), (0, 1 << 31, 8, 3, 0, -5), (0, 5, 1 << 21, 3, 0, -5), (0, 5, 8, 1 << 25, 0, -5)):
+                                 (3, 5, 8, 3, 9, -1), (0, 1 << 31, 8, 3, 0, -5), (0, 5, 1 << 21, 3, 0, -5), (0, 5, 8, (1 << 21) + 1, 0, -5)):
         assert lib.wf_linear_workspace_bytes(what, N, D, V, t, C.byref(n)) == rc, (what, N, D, V, t)
     # too small a workspace, null pointers, a bad smoothing: an error before anything is launched
     assert lib.wf_linear_log_softmax(1, 8, 2, 8, 1, 8, 3, 0, None, 0, 1, 256, 10, None) == -2

@@ -797,21 +797,26 @@ template <class T> constexpr int parts_of() { return sizeof(T) == 4 ? 3 : 1; }  
 template <class T> struct Half { typedef T type; };
 template <> struct Half<float> { typedef bf16 type; };
 
-// v in three bf16 parts of 8 significand bits each, by truncation; the parts below a value that is not finite are 0
-struct Split3 { uint16_t h[3]; };
-__device__ inline Split3 split3(float v) {
-    Split3 s;
-    const uint32_t a = __float_as_uint(v) & 0xffff0000u;
-    s.h[0] = (uint16_t)(a >> 16);
-    if ((a & 0x7f800000u) == 0x7f800000u) {          // keeps a NaN a NaN when its upper significand bits are 0
-        if (v != v) s.h[0] |= 0x40;
-        s.h[1] = s.h[2] = 0;
-        return s;
+// W values in three bf16 parts of 8 significand bits each, by truncation: exact, v = first + second + third, two neighbours to a
+// word by one byte permutation.  (Infinity - infinity: a value that is not finite has parts that are no numbers.)
+template <int W> struct Split3 { uint32_t h[3][W / 2]; };
+template <int W> __device__ inline Split3<W> split3(const float (&v)[W]) {
+    Split3<W> s;
+#pragma unroll
+    for (int i = 0; i < W; i += 2) {
+        float r[2];
+        uint32_t u[2];
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                if (p == 0) r[e] = v[i + e];
+                else r[e] -= __uint_as_float(u[e] & 0xffff0000u);
+                u[e] = __float_as_uint(r[e]);
+            }
+            s.h[p][i / 2] = __builtin_amdgcn_perm(u[1], u[0], 0x07060302);
+        }
     }
-    const float r = v - __uint_as_float(a);
-    const uint32_t b = __float_as_uint(r) & 0xffff0000u;
-    s.h[1] = (uint16_t)(b >> 16);
-    s.h[2] = (uint16_t)(__float_as_uint(r - __uint_as_float(b)) >> 16);
     return s;
 }
 template <class T> __device__ inline uint16_t bits16(float v) {
@@ -834,15 +839,9 @@ template <class T> __device__ inline void pack_row(uint16_t* y, const T* x, int 
         if constexpr (P == 1) {
             __builtin_memcpy(y + d, &v, sizeof(v));
         } else {
-            Pack<uint16_t, VEC> h[3];
+            const auto s = split3(v.v);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const Split3 s = split3(v.v[i]);
-#pragma unroll
-                for (int p = 0; p < 3; ++p) h[p].v[i] = s.h[p];
-            }
-#pragma unroll
-            for (int p = 0; p < 3; ++p) __builtin_memcpy(y + (size_t)p * Dp + d, &h[p], sizeof(h[p]));
+            for (int p = 0; p < 3; ++p) __builtin_memcpy(y + (size_t)p * Dp + d, s.h[p], sizeof(s.h[p]));
         }
     }
 }
@@ -1228,30 +1227,18 @@ template <class T> __device__ inline void store_dz4(uint16_t* row, int64_t pitch
         for (int i = 0; i < 4; ++i) h.v[i] = bits16<T>(d[i]);
         __builtin_memcpy(row + v, &h, 8);
     } else {
-        Pack<uint16_t, 4> h[3];
+        const auto s = split3(d);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const Split3 s = split3(d[i]);
-#pragma unroll
-            for (int p = 0; p < 3; ++p) h[p].v[i] = s.h[p];
-        }
-#pragma unroll
-        for (int p = 0; p < 3; ++p) __builtin_memcpy(row + p * pitch + v, &h[p], 8);
+        for (int p = 0; p < 3; ++p) __builtin_memcpy(row + p * pitch + v, s.h[p], 8);
     }
 }
 template <class X> __device__ inline void split_frag(const Pack<X, 8>& v, typename Mfma<typename Half<X>::type>::v8 (&f)[parts_of<X>()]) {
     if constexpr (parts_of<X>() == 1) {
         __builtin_memcpy(&f[0], &v, 16);
     } else {
-        Pack<uint16_t, 8> h[3];
+        const auto s = split3(v.v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const Split3 s = split3(v.v[i]);
-#pragma unroll
-            for (int p = 0; p < 3; ++p) h[p].v[i] = s.h[p];
-        }
-#pragma unroll
-        for (int p = 0; p < 3; ++p) __builtin_memcpy(&f[p], &h[p], 16);
+        for (int p = 0; p < 3; ++p) __builtin_memcpy(&f[p], s.h[p], 16);
     }
 }
 __device__ inline int32_t small_target(const void* targets, int wide, int64_t ignore, int64_t n, int V, bool* dead) {
@@ -1843,7 +1830,8 @@ struct LinearPlan {
 int make_linear_plan(int what, int64_t N, int32_t D, int32_t V, int32_t type, void* ws, LinearPlan* out) {
     if (!known_type(type)) return wf_fail(WF_EINVAL, "wf_linear: unknown element type");
     if (N < 0 || D < 1 || V < 1) return wf_fail(WF_EINVAL, "wf_linear: bad size (N %lld, D %d, V %d)", (long long)N, D, V);
-    if (N > (1 << 30) || D > (1 << 20) || V > (1 << 24) || ceil_div(N, 128) * ceil_div(V, 128) > (1 << 29))
+    // (a tile's offsets are 32 bits: 256 rows of at most 2^22 x 2 bytes x 3 parts of an operand)
+    if (N > (1 << 30) || D > (1 << 20) || V > (1 << 21) || ceil_div(N, 128) * ceil_div(V, 128) > (1 << 29))
         return wf_fail(WF_EUNSUPPORTED, "wf_linear: N %lld, D %d, V %d is beyond what one call takes", (long long)N, D, V);
     LinearPlan p = {};
     p.what = what; p.N = N; p.D = D; p.V = V; p.type = type;
@@ -1942,7 +1930,7 @@ template <class F> void with_half(int type, F&& f) { if (type == WF_F16) f(f16()
 template <class F> void with_big(bool big, F&& f) { if (big) f(std::true_type()); else f(std::false_type()); }
 
 bool direct_rows(const void* p, int64_t ld, int64_t D, int type) {   // usable as an operand where it lies
-    return type != WF_F32 && D % kBK == 0 && ld % 8 == 0 && (uintptr_t)p % 16 == 0;
+    return type != WF_F32 && D % kBK == 0 && ld % 8 == 0 && ld <= (1 << 22) && (uintptr_t)p % 16 == 0;
 }
 // Packs what has to be packed and places the rows; *w is W as an operand, where it lies or packed.
 int run_prep(const LinearPlan& p, PrepArgs a, const void* x, int64_t ldx, const void* w, int64_t ldw, hipStream_t st, Operand* wo) {

@@ -38,8 +38,9 @@ def _check(t, name, like=None, dtype=None):
     return t
 
 
-# The calls' host time counts: a backward pass runs on the autograd engine's own thread, where every Python operation takes
-# several times as long, with the forward's device and stream current.  Pointers go to the library as plain integers, what forward knows already is kept for backward.
+# The calls' host time counts: a backward pass runs on the autograd engine's own thread (with the forward's device and stream
+# current), where every Python operation takes several times as long.  Pointers go to the library as plain integers; they and
+# the strides are taken from the saved tensors again, which hooks may have moved in between.
 
 def _p(t):
     return None if t is None else t.data_ptr()
@@ -97,15 +98,16 @@ class _LayerNorm(torch.autograd.Function):
         y, v, ld, N, D, pdtype, stats = _norm(x, weight, bias, eps, True)
         need = ctx.needs_input_grad
         ctx.save_for_backward(v, weight, stats)
-        ctx.rest = (x.shape, ld, N, D, pdtype, weight is not None and need[1], bias is not None and need[2])
+        ctx.rest = (x.shape, N, D, pdtype, weight is not None and need[1], bias is not None and need[2])
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         v, weight, stats = ctx.saved_tensors
-        shape, ld, N, D, pdtype, want_w, want_b = ctx.rest
+        shape, N, D, pdtype, want_w, want_b = ctx.rest
         dev, t = v.device, _TYPES[v.dtype]
+        v, ld = _rows(v)
         g, ldg = _rows(dy)
         dx = torch.empty(shape, dtype=v.dtype, device=dev)
         dw = torch.empty(D, dtype=pdtype, device=dev) if want_w else None
@@ -223,6 +225,11 @@ def _linear_args(x, weight):
     return v, w, (v.data_ptr(), ldx, x.numel() // D, D, w.data_ptr(), ldw, weight.shape[0], _TYPES[x.dtype])
 
 
+def _entropy_args(bias, targets, rest):
+    """the arguments bias .. smoothing; rest: (ignore_index, smoothing)"""
+    return (_p(bias), _TYPES[bias.dtype] if bias is not None else 0, targets.data_ptr(), 1 if targets.dtype == torch.int64 else 0) + rest
+
+
 def _log_softmax(x, weight, bias):
     dev = x.device
     v, w, a = _linear_args(x, weight)
@@ -241,14 +248,16 @@ class _LinearLogSoftmax(torch.autograd.Function):
     def forward(ctx, x, weight, bias):
         lp, v, w, a, bt = _log_softmax(x, weight, bias)
         ctx.save_for_backward(v, w, bias, lp)
-        ctx.rest = (x.shape, weight.shape, a, bt)
+        ctx.shapes = (x.shape, weight.shape)
         return lp
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         v, w, bias, lp = ctx.saved_tensors
-        xshape, wshape, a, bt = ctx.rest
+        xshape, wshape = ctx.shapes
+        v, w, a = _linear_args(v, w)
+        bt = _TYPES[bias.dtype] if bias is not None else 0
         dev, need = v.device, ctx.needs_input_grad
         g, ldg = _rows(grad)
         dx = torch.empty(xshape, dtype=v.dtype, device=dev) if need[0] else None
@@ -278,8 +287,7 @@ def _entropy(x, weight, targets, bias, ignore_index, smoothing, reduction):
     dev = x.device
     v, w, a = _linear_args(x, weight)
     N = a[2]
-    bt = _TYPES[bias.dtype] if bias is not None else 0
-    rest = (_p(bias), bt, targets.data_ptr(), 1 if targets.dtype == torch.int64 else 0, ignore_index, smoothing)
+    rest = (ignore_index, smoothing)
     rows, mean = 1 if reduction == "none" else 0, 1 if reduction == "mean" else 0
     loss = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
     lse = torch.empty(N, dtype=torch.float32, device=dev)
@@ -287,24 +295,25 @@ def _entropy(x, weight, targets, bias, ignore_index, smoothing, reduction):
     n = _linear_bytes(_CE_FWD, N, a[3], a[6], x.dtype)
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
     with _on(dev):
-        _lib.check(_lib.lib().wf_linear_cross_entropy(*a, *rest, loss.data_ptr(), lse.data_ptr(), _p(total), mean, ws.data_ptr(), n,
-                                                      _raw_stream(dev)))
-    return loss if rows else total, v, w, a, rest, rows, mean, lse
+        _lib.check(_lib.lib().wf_linear_cross_entropy(*a, *_entropy_args(bias, targets, rest), loss.data_ptr(), lse.data_ptr(),
+                                                      _p(total), mean, ws.data_ptr(), n, _raw_stream(dev)))
+    return loss if rows else total, v, w, rest, rows, mean, lse
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, targets, bias, ignore_index, smoothing, reduction):
-        loss, v, w, a, rest, rows, mean, lse = _entropy(x, weight, targets, bias, ignore_index, smoothing, reduction)
+        loss, v, w, rest, rows, mean, lse = _entropy(x, weight, targets, bias, ignore_index, smoothing, reduction)
         ctx.save_for_backward(v, w, targets, bias, lse)
-        ctx.rest = (x.shape, weight.shape, a, rest, rows, mean)
+        ctx.rest = (x.shape, weight.shape, rest, rows, mean)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         v, w, targets, bias, lse = ctx.saved_tensors
-        xshape, wshape, a, rest, rows, mean = ctx.rest
+        xshape, wshape, rest, rows, mean = ctx.rest
+        v, w, a = _linear_args(v, w)
         dev, need = v.device, ctx.needs_input_grad
         if not grad.is_contiguous():
             grad = grad.contiguous()
@@ -313,8 +322,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
         db = torch.empty(wshape[:1], dtype=bias.dtype, device=dev) if need[3] else None
         n = _linear_bytes(_CE_BWD, a[2], a[3], a[6], v.dtype)
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        _lib.check(_lib.lib().wf_linear_cross_entropy_backward(grad.data_ptr(), rows, mean, lse.data_ptr(), *a, *rest, _p(dx), _p(dw),
-                                                               _p(db), ws.data_ptr(), n, _raw_stream(dev)))
+        _lib.check(_lib.lib().wf_linear_cross_entropy_backward(grad.data_ptr(), rows, mean, lse.data_ptr(), *a,
+                                                               *_entropy_args(bias, targets, rest), _p(dx), _p(dw), _p(db),
+                                                               ws.data_ptr(), n, _raw_stream(dev)))
         return dx, dw, None, db, None, None, None
 
 
