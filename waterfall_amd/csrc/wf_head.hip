@@ -1085,7 +1085,7 @@ template <class T, bool BIG> __global__ void __launch_bounds__(Shape<BIG>::kThre
             for (int i = 0; i < Tl::MI; ++i)
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                    all += whole | (a.l.v0 + t.m(i, e) < a.l.V) ? t.acc[i][j][e] : 0.f;
+                    all += (whole | (a.l.v0 + t.m(i, e) < a.l.V)) ? t.acc[i][j][e] : 0.f;
             all += __shfl_xor(all, 32);
         }
         if (t.lane < 32 && c < a.pitch) {
@@ -1316,7 +1316,7 @@ template <class X, int MV, bool DZ> __global__ void __launch_bounds__(256) small
                 const bool in = v + e < a.l.V;
                 const float z = in && a.l.bias ? s[e] + load_any(a.l.bias, a.l.btype, v + e) : s[e];
                 const float u = g * ((__expf(z - ref) - even) * share - (v + e == target ? hit : 0.f));
-                d[e] = none | !in ? 0.f : u;
+                d[e] = (none | !in) ? 0.f : u;
             }
             if (v < a.zpitch) store_dz4<X>(a.dz + n * P * a.zpitch, a.zpitch, v, d);
         }

@@ -9,12 +9,8 @@ entropy on the same projection, is a kernel of the library with its own gradient
 
 ``OutputHead`` is the module over them.  All run on the current stream of the tensors' device and can be captured in a graph.
 """
-import ctypes as C
-import functools
-
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .graph import _on
@@ -38,85 +34,34 @@ def _check(t, name, like=None, dtype=None):
     return t
 
 
-# The calls' host time counts: a backward pass runs on the autograd engine's own thread (with the forward's device and stream
-# current), where every Python operation takes several times as long.  Pointers go to the library as plain integers; they and
-# the strides are taken from the saved tensors again, which hooks may have moved in between.
+# The autograd nodes are C++ (csrc/wf_head_torch.cpp over the C entry points): short calls are bound by the host.
 
-def _p(t):
-    return None if t is None else t.data_ptr()
+_ext = None
 
 
-def _raw_stream(device):
-    return torch._C._cuda_getCurrentRawStream(device.index)
+def _nodes():
+    global _ext
+    if _ext is None:
+        _lib.lib()
+        try:
+            from . import _head
+        except ImportError as e:
+            raise _lib.WfError(f"waterfall_amd/_head.so cannot be loaded ({e}): build it first "
+                               "(python -c 'import __graft_entry__ as g; g.build()').") from None
+        _ext = _head
+    return _ext
 
 
-def _rows(t):
-    """(t as rows of its last dimension with unit stride inside a row, elements from row to row).  A view where the leading
-    dimensions collapse into one, a contiguous copy otherwise."""
-    D = t.shape[-1]
-    if t.is_contiguous():
-        return t, D
-    n = t.numel() // D if D else 0
-    if t.stride(-1) != 1 and D > 1:
-        t = t.contiguous()
-    try:
-        v = t.view(n, D)
-    except RuntimeError:
-        v = t.contiguous().view(n, D)
-    return v, v.stride(0) if n > 1 else D
-
-
-@functools.lru_cache(maxsize=256)
-def _norm_bytes(N, D, t):
-    n = C.c_size_t(0)
-    _lib.check(_lib.lib().wf_layer_norm_backward_workspace_bytes(N, D, t, C.byref(n)))
-    return n.value
-
-
-def _wanted(*tensors):
-    """Whether a gradient may be asked for: without one the call skips autograd's own work (a third of a short call)."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-def _norm(x, weight, bias, eps, keep):
-    dev, D = x.device, x.shape[-1]
-    v, ld = _rows(x)
-    N = x.numel() // D
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    stats = torch.empty((N, 2), dtype=torch.float32, device=dev) if keep else None
-    params = weight if weight is not None else bias
-    pdtype = x.dtype if params is None else params.dtype
+def _run(name, x, *args):
+    """One of the nodes on x's device and its current stream."""
+    dev = x.device
     with _on(dev):
-        _lib.check(_lib.lib().wf_layer_norm(v.data_ptr(), ld, N, D, _TYPES[x.dtype], _p(weight), _p(bias), _TYPES[pdtype], eps,
-                                            y.data_ptr(), _p(stats), _raw_stream(dev)))
-    return y, v, ld, N, D, pdtype, stats
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, v, ld, N, D, pdtype, stats = _norm(x, weight, bias, eps, True)
-        need = ctx.needs_input_grad
-        ctx.save_for_backward(v, weight, stats)
-        ctx.rest = (x.shape, N, D, pdtype, weight is not None and need[1], bias is not None and need[2])
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        v, weight, stats = ctx.saved_tensors
-        shape, N, D, pdtype, want_w, want_b = ctx.rest
-        dev, t = v.device, _TYPES[v.dtype]
-        v, ld = _rows(v)
-        g, ldg = _rows(dy)
-        dx = torch.empty(shape, dtype=v.dtype, device=dev)
-        dw = torch.empty(D, dtype=pdtype, device=dev) if want_w else None
-        db = torch.empty(D, dtype=pdtype, device=dev) if want_b else None
-        n = _norm_bytes(N, D, t) if want_w or want_b else 0
-        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-        _lib.check(_lib.lib().wf_layer_norm_backward(g.data_ptr(), ldg, v.data_ptr(), ld, N, D, t, _p(weight), _TYPES[pdtype],
-                                                     stats.data_ptr(), dx.data_ptr(), _p(dw), _p(db), _p(ws), n, _raw_stream(dev)))
-        return dx, dw, db, None
+        try:
+            return getattr(_ext or _nodes(), name)(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+        except RuntimeError as e:
+            if str(e).startswith("libwfdwfst error"):
+                raise _lib.WfError(str(e).split("\n")[0]) from None
+            raise
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -136,38 +81,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
                 raise ValueError(f"layer_norm: {name} has shape {tuple(t.shape)}, expected {tuple(x.shape[-1:])}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError(f"layer_norm: weight is {weight.dtype}, bias is {bias.dtype}")
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    if _wanted(x, weight, bias):
-        return _LayerNorm.apply(x, weight, bias, float(eps))
-    return _norm(x, weight, bias, float(eps), False)[0]
-
-
-class _Dropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, p, seed):
-        if isinstance(seed, torch.Tensor):
-            ctx.save_for_backward(seed)
-            ctx.rest = (p, None)
-        else:
-            ctx.rest = (p, seed)
-        return _drop(x, p, seed)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        p, seed = ctx.rest
-        return _drop(dy, p, ctx.saved_tensors[0] if seed is None else seed), None, None
-
-
-def _drop(x, p, seed):
-    if not x.is_contiguous():
-        x = x.contiguous()
-    y, dev = torch.empty_like(x), x.device
-    key, at = (0, seed.data_ptr()) if isinstance(seed, torch.Tensor) else (seed, None)
-    with _on(dev):
-        _lib.check(_lib.lib().wf_dropout(x.data_ptr(), x.numel(), _TYPES[x.dtype], p, key, at, y.data_ptr(), _raw_stream(dev)))
-    return y
+    return _run("layer_norm", x, x, None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous(),
+                float(eps))
 
 
 def dropout(x, p, seed):
@@ -187,22 +102,11 @@ def dropout(x, p, seed):
             raise TypeError("dropout: seed must be an integer or an int64 tensor of one element")
         if seed.device != x.device:
             raise ValueError(f"dropout: seed is on {seed.device}, x is on {x.device}")
-    else:
-        seed = int(seed) & 0xFFFFFFFFFFFFFFFF
-    return _Dropout.apply(x, p, seed) if _wanted(x) else _drop(x, p, seed)
+        return _run("dropout", x, x, p, 0, seed)
+    return _run("dropout", x, x, p, int(seed) & 0xFFFFFFFFFFFFFFFF, None)
 
 
 # ---- the projection ---------------------------------------------------------------------------------------------------
-
-_LOG_FWD, _LOG_BWD, _CE_FWD, _CE_BWD = range(4)
-
-
-@functools.lru_cache(maxsize=256)
-def _linear_bytes(what, N, D, V, dtype):
-    n = C.c_size_t(0)
-    _lib.check(_lib.lib().wf_linear_workspace_bytes(what, N, D, V, _TYPES[dtype], C.byref(n)))
-    return n.value
-
 
 def _check_linear(who, x, weight, bias):
     _check(x, "x")
@@ -217,59 +121,6 @@ def _check_linear(who, x, weight, bias):
             raise ValueError(f"{who}: bias has shape {tuple(bias.shape)}, expected [{weight.shape[0]}]")
 
 
-def _linear_args(x, weight):
-    """x and weight as rows, and the arguments x .. type of the library's calls"""
-    v, ldx = _rows(x)
-    w, ldw = _rows(weight)
-    D = x.shape[-1]
-    return v, w, (v.data_ptr(), ldx, x.numel() // D, D, w.data_ptr(), ldw, weight.shape[0], _TYPES[x.dtype])
-
-
-def _entropy_args(bias, targets, rest):
-    """the arguments bias .. smoothing; rest: (ignore_index, smoothing)"""
-    return (_p(bias), _TYPES[bias.dtype] if bias is not None else 0, targets.data_ptr(), 1 if targets.dtype == torch.int64 else 0) + rest
-
-
-def _log_softmax(x, weight, bias):
-    dev = x.device
-    v, w, a = _linear_args(x, weight)
-    V = a[6]
-    bt = _TYPES[bias.dtype] if bias is not None else 0
-    lp = torch.empty(x.shape[:-1] + (V,), dtype=torch.float32, device=dev)
-    n = _linear_bytes(_LOG_FWD, a[2], a[3], V, x.dtype)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        _lib.check(_lib.lib().wf_linear_log_softmax(*a, _p(bias), bt, lp.data_ptr(), ws.data_ptr(), n, _raw_stream(dev)))
-    return lp, v, w, a, bt
-
-
-class _LinearLogSoftmax(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias):
-        lp, v, w, a, bt = _log_softmax(x, weight, bias)
-        ctx.save_for_backward(v, w, bias, lp)
-        ctx.shapes = (x.shape, weight.shape)
-        return lp
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        v, w, bias, lp = ctx.saved_tensors
-        xshape, wshape = ctx.shapes
-        v, w, a = _linear_args(v, w)
-        bt = _TYPES[bias.dtype] if bias is not None else 0
-        dev, need = v.device, ctx.needs_input_grad
-        g, ldg = _rows(grad)
-        dx = torch.empty(xshape, dtype=v.dtype, device=dev) if need[0] else None
-        dw = torch.empty(wshape, dtype=v.dtype, device=dev) if need[1] else None
-        db = torch.empty(wshape[:1], dtype=bias.dtype, device=dev) if need[2] else None
-        n = _linear_bytes(_LOG_BWD, a[2], a[3], a[6], v.dtype)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        _lib.check(_lib.lib().wf_linear_log_softmax_backward(lp.data_ptr(), g.data_ptr(), ldg, *a, bt, _p(dx), _p(dw), _p(db),
-                                                             ws.data_ptr(), n, _raw_stream(dev)))
-        return dx, dw, db
-
-
 def linear_log_softmax(x, weight, bias=None):
     """log_softmax(x weight^T + bias) as float32 [..., V]: the log-probabilities that ``DenseFsaVec`` takes.
 
@@ -279,53 +130,10 @@ def linear_log_softmax(x, weight, bias=None):
     utterance's end) are left out whatever they hold; 16-bit types round the gradient of a logit to x's type before it enters
     the products."""
     _check_linear("linear_log_softmax", x, weight, bias)
-    bias = None if bias is None else bias.contiguous()
-    return _LinearLogSoftmax.apply(x, weight, bias) if _wanted(x, weight, bias) else _log_softmax(x, weight, bias)[0]
+    return _run("linear_log_softmax", x, x, weight, None if bias is None else bias.contiguous())
 
 
-def _entropy(x, weight, targets, bias, ignore_index, smoothing, reduction):
-    dev = x.device
-    v, w, a = _linear_args(x, weight)
-    N = a[2]
-    rest = (ignore_index, smoothing)
-    rows, mean = 1 if reduction == "none" else 0, 1 if reduction == "mean" else 0
-    loss = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
-    lse = torch.empty(N, dtype=torch.float32, device=dev)
-    total = None if rows else torch.empty((), dtype=torch.float32, device=dev)
-    n = _linear_bytes(_CE_FWD, N, a[3], a[6], x.dtype)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        _lib.check(_lib.lib().wf_linear_cross_entropy(*a, *_entropy_args(bias, targets, rest), loss.data_ptr(), lse.data_ptr(),
-                                                      _p(total), mean, ws.data_ptr(), n, _raw_stream(dev)))
-    return loss if rows else total, v, w, rest, rows, mean, lse
-
-
-class _LinearCrossEntropy(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, targets, bias, ignore_index, smoothing, reduction):
-        loss, v, w, rest, rows, mean, lse = _entropy(x, weight, targets, bias, ignore_index, smoothing, reduction)
-        ctx.save_for_backward(v, w, targets, bias, lse)
-        ctx.rest = (x.shape, weight.shape, rest, rows, mean)
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        v, w, targets, bias, lse = ctx.saved_tensors
-        xshape, wshape, rest, rows, mean = ctx.rest
-        v, w, a = _linear_args(v, w)
-        dev, need = v.device, ctx.needs_input_grad
-        if not grad.is_contiguous():
-            grad = grad.contiguous()
-        dx = torch.empty(xshape, dtype=v.dtype, device=dev) if need[0] else None
-        dw = torch.empty(wshape, dtype=v.dtype, device=dev) if need[1] else None
-        db = torch.empty(wshape[:1], dtype=bias.dtype, device=dev) if need[3] else None
-        n = _linear_bytes(_CE_BWD, a[2], a[3], a[6], v.dtype)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        _lib.check(_lib.lib().wf_linear_cross_entropy_backward(grad.data_ptr(), rows, mean, lse.data_ptr(), *a,
-                                                               *_entropy_args(bias, targets, rest), _p(dx), _p(dw), _p(db),
-                                                               ws.data_ptr(), n, _raw_stream(dev)))
-        return dx, dw, None, db, None, None, None
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 
 def linear_cross_entropy(x, weight, targets, bias=None, ignore_index=-1, label_smoothing=0.0, reduction="mean"):
@@ -346,11 +154,10 @@ def linear_cross_entropy(x, weight, targets, bias=None, ignore_index=-1, label_s
         raise ValueError(f"linear_cross_entropy: targets have shape {tuple(targets.shape)}, expected {tuple(x.shape[:-1])}")
     if not 0.0 <= float(label_smoothing) <= 1.0:
         raise ValueError(f"linear_cross_entropy: label_smoothing must be in [0, 1], got {label_smoothing}")
-    if reduction not in ("none", "sum", "mean"):
+    if reduction not in _REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: unknown reduction {reduction!r}")
-    args = (x, weight, targets.contiguous(), None if bias is None else bias.contiguous(), int(ignore_index), float(label_smoothing),
-            reduction)
-    return _LinearCrossEntropy.apply(*args) if _wanted(x, weight, bias) else _entropy(*args)[0]
+    return _run("linear_cross_entropy", x, x, weight, targets.contiguous(), None if bias is None else bias.contiguous(),
+                int(ignore_index), float(label_smoothing), _REDUCTIONS[reduction])
 
 
 class OutputHead(nn.Module):
