@@ -971,7 +971,7 @@ template <class T> __global__ void __launch_bounds__(256) prep_kernel(PrepArgs a
         for (int i = wave; i < kPrepRows; i += 4) {
             const int at = base + b * kPrepRows + i;
             if (at >= end) break;
-            pack_row<T>(a.xp + (int64_t)at * P * a.Dp, nullptr, a.D, a.Dp, lane);
+            if (a.xp) pack_row<T>(a.xp + (int64_t)at * P * a.Dp, nullptr, a.D, a.Dp, lane);
             if (a.gout && lane == 0) { a.r.g[at] = 0.f; a.r.lse[at] = 0.f; a.r.target[at] = -1; }
         }
         return;
@@ -1004,7 +1004,7 @@ template <class T> __global__ void __launch_bounds__(256) prep_kernel(PrepArgs a
     for (int i = wave; i < kPrepRows; i += 4) {
         const int at = place[i];
         const int64_t n = from + i;
-        if (at >= 0) pack_row<T>(a.xp + (int64_t)at * P * a.Dp, (const T*)a.x + n * a.ldx, a.D, a.Dp, lane);
+        if (at >= 0) { if (a.xp) pack_row<T>(a.xp + (int64_t)at * P * a.Dp, (const T*)a.x + n * a.ldx, a.D, a.Dp, lane); }
         else if (at == -1 && a.dx)
             for (int d = lane; d < a.D; d += 64) ((T*)a.dx)[n * a.D + d] = (T)0.f;
     }
@@ -1216,7 +1216,7 @@ struct SmallArgs {
     // gradients of the logits instead: of the packed rows, see dz_kernel
     const int32_t *live, *idx, *want;
     const float *g, *glse;
-    uint16_t* dz;
+    void* dz;                // [.][zpitch] of x's type
     int64_t zpitch;
 };
 // 16-bit planes of four neighbouring values
@@ -1248,7 +1248,7 @@ __device__ inline int32_t small_target(const void* targets, int wide, int64_t ig
 }
 template <class X, int MV, bool DZ> __global__ void __launch_bounds__(256) small_kernel(SmallArgs a) {
     using T = typename Half<X>::type;
-    constexpr int P = parts_of<X>(), U = P == 1 ? 4 : 2;      // steps whose loads are under way together
+    constexpr int P = parts_of<X>(), U = P == 1 || MV == 2 ? 4 : 2;      // steps whose loads are under way together
     __shared__ __align__(16) float part[4][MV][4][64][4];     // [wave][m][q][lane][e]
     __shared__ float wtop[4][32], wsum[4][32], wall[4][32], wzt[32];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1263,14 +1263,18 @@ template <class X, int MV, bool DZ> __global__ void __launch_bounds__(256) small
     v16f acc[MV];
 #pragma unroll
     for (int m = 0; m < MV; ++m) acc[m] = v16f{};
-    for (int k0 = wave * 16 + kl; k0 - kl < a.D; k0 += 64 * U) {
+    // (a load under a condition has to be waited for before the zeros of the other lanes may go into its registers: whole steps
+    // are loaded without one)
+    auto group = [&](int k0, auto u_, auto full_) {
+        constexpr int U = decltype(u_)::value;
+        constexpr bool FULL = decltype(full_)::value;
         Pack<X, 8> xv[U], wv[U][MV];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int k = k0 + u * 64;
-            xv[u] = load_n<X, 8>(xr + k, a.D - k);
+            xv[u] = load_n<X, 8>(xr + k, FULL ? 8 : a.D - k);
 #pragma unroll
-            for (int m = 0; m < MV; ++m) wv[u][m] = load_n<X, 8>(wr[m] + k, a.D - k);
+            for (int m = 0; m < MV; ++m) wv[u][m] = load_n<X, 8>(wr[m] + k, FULL ? 8 : a.D - k);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -1291,7 +1295,11 @@ template <class X, int MV, bool DZ> __global__ void __launch_bounds__(256) small
                 }
             }
         }
-    }
+    };
+    int k0 = wave * 16;
+    for (; k0 + (U - 1) * 64 + 16 <= a.D; k0 += U * 64) group(k0 + kl, std::integral_constant<int, U>(), std::true_type());
+    for (; k0 + 16 <= a.D; k0 += 64) group(k0 + kl, std::integral_constant<int, 1>(), std::true_type());
+    if (k0 < a.D) group(k0 + kl, std::integral_constant<int, 1>(), std::false_type());
 #pragma unroll
     for (int m = 0; m < MV; ++m)
 #pragma unroll
@@ -1318,7 +1326,10 @@ template <class X, int MV, bool DZ> __global__ void __launch_bounds__(256) small
                 const float u = g * ((__expf(z - ref) - even) * share - (v + e == target ? hit : 0.f));
                 d[e] = (none | !in) ? 0.f : u;
             }
-            if (v < a.zpitch) store_dz4<X>(a.dz + n * P * a.zpitch, a.zpitch, v, d);
+            Pack<X, 4> o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o.v[e] = (X)d[e];
+            if (v < a.zpitch) store_n<X, 4>((X*)a.dz + n * a.zpitch + v, o, 4);
         }
         return;
     }
@@ -1422,6 +1433,215 @@ __global__ void __launch_bounds__(256) small_end_kernel(SmallArgs a, int tiles) 
 #pragma unroll
         for (int i = 0; i < 16; ++i)
             if (v0 + i * 256 < a.l.V) out[v0 + i * 256] = z[i] - lse;
+}
+
+// Gradients of the same sizes, C[m][d] = sum over k of A(k, m) B(k, d), straight from memory as well:
+//   dx (ROWS):  m a live row, k an output: A = dz in its rows, 8 neighbours of k a load; B = W
+//   dW:         m an output, k a live row: A = dz, B = x's rows where they lie
+// The rows of W and x run across k: a lane collects the 8 k of its place in a matrix instruction with 8 loads.  It takes two
+// neighbours of a row at a time, its columns in two instructions, so 32 lanes read 256 bytes (fp32) and write as many.  The 4
+// waves take every fourth step of 16 k, their sums meet in LDS, long k is split over workgroups too.
+struct SmallGradArgs {
+    const void *dz, *b;
+    int64_t N;               // rows that exist
+    uint32_t zld, ldb;       // bytes
+    const int32_t *live, *idx;
+    int32_t V, D;
+    float *part, *colpart;   // [splits][N or V][D], [splits][V], or NULL: straight to the outputs
+    const float* scale;
+    void *out, *colout;
+    int32_t ctype;
+};
+template <class X, bool ROWS> __global__ void __launch_bounds__(256, 2) small_grad_kernel(SmallGradArgs a) {
+    using T = typename Half<X>::type;
+    constexpr int P = parts_of<X>(), NM = ROWS ? 1 : 2;       // dW: two neighbours of m a lane as well
+    __shared__ __align__(16) float meet[2][4][4][64][4];      // [turn][wave][q][lane][e]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, at = lane & 31;
+    const int live = *a.live, M = ROWS ? live : a.V, K = ROWS ? a.V : live;
+    const int64_t m0 = (int64_t)blockIdx.y * 32 * NM;
+    const int d0 = blockIdx.x * 64, d = d0 + at * 2;
+    if (m0 >= M) return;
+    const bool col = !ROWS && a.colout && blockIdx.x == 0;
+    const int steps = (K + 15) / 16, per = (steps + gridDim.z - 1) / gridDim.z, s1 = min(steps, (int)(blockIdx.z + 1) * per), end = min(K, s1 * 16);
+    // (dz has whole 64 outputs in every row: what is behind the last output or row is not used)
+    const char* zp = (const char*)a.dz + (ROWS ? min(m0 + at, (int64_t)M - 1) * a.zld : (m0 + at * 2) * (int64_t)sizeof(X));
+    const char* bp = (const char*)a.b + (int64_t)min(d, a.D - 1) * sizeof(X);
+    const int left = a.D - d;
+    v16f acc[NM][2], ones[NM];
+#pragma unroll
+    for (int i = 0; i < NM; ++i) ones[i] = acc[i][0] = acc[i][1] = v16f{};
+    typename Mfma<T>::v8 one;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) one[e] = (T)1.f;
+    // U steps from s on, loads first; FULL: all of their k and all 64 columns exist
+    auto group = [&](int s, auto u_, auto full_) {
+        constexpr int U = decltype(u_)::value;
+        constexpr bool FULL = decltype(full_)::value;
+        Pack<X, 8> av[U][NM], bv[U][2];
+        int row[U][8];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int k = (s + u * 4) * 16 + half * 8 + e, ke = FULL ? k : min(k, end - 1);
+                row[u][e] = ROWS ? ke : a.idx[ke];
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = (s + u * 4) * 16 + half * 8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const X* p = (const X*)(bp + (uint64_t)(uint32_t)row[u][e] * a.ldb);
+                const auto b = FULL ? load_n<X, 2>(p, 2) : load_n<X, 2>(p, k + e < end ? left : 0);
+                bv[u][0].v[e] = b.v[0];
+                bv[u][1].v[e] = b.v[1];
+            }
+            if constexpr (ROWS) {
+                av[u][0] = load_n<X, 8>((const X*)zp + k, FULL ? 8 : end - k);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const X* p = (const X*)(zp + (uint64_t)(uint32_t)(k + e) * a.zld);
+                    const auto z = load_n<X, 2>(p, FULL || k + e < end ? 2 : 0);
+                    av[u][0].v[e] = z.v[0];
+                    av[u][1].v[e] = z.v[1];
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            typename Mfma<T>::v8 bf[2][P];
+            split_frag<X>(bv[u][0], bf[0]);
+            split_frag<X>(bv[u][1], bf[1]);
+#pragma unroll
+            for (int i = 0; i < NM; ++i) {
+                typename Mfma<T>::v8 af[P];
+                split_frag<X>(av[u][i], af);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    if constexpr (P == 3) {
+                        acc[i][j] = Mfma<T>::mul(af[2], bf[j][0], acc[i][j]);
+                        acc[i][j] = Mfma<T>::mul(af[1], bf[j][1], acc[i][j]);
+                        acc[i][j] = Mfma<T>::mul(af[0], bf[j][2], acc[i][j]);
+                        acc[i][j] = Mfma<T>::mul(af[1], bf[j][0], acc[i][j]);
+                        acc[i][j] = Mfma<T>::mul(af[0], bf[j][1], acc[i][j]);
+                    }
+                    acc[i][j] = Mfma<T>::mul(af[0], bf[j][0], acc[i][j]);
+                }
+                if (col)
+#pragma unroll
+                    for (int p = P - 1; p >= 0; --p) ones[i] = Mfma<T>::mul(af[p], one, ones[i]);
+            }
+        }
+    };
+    using std::integral_constant;
+    int s = (int)blockIdx.z * per + wave;
+    if (d0 + 64 <= a.D) {
+        for (; (s + 4) * 16 + 16 <= end; s += 8) group(s, integral_constant<int, 2>(), std::true_type());
+        if (s * 16 + 16 <= end) { group(s, integral_constant<int, 1>(), std::true_type()); s += 4; }
+    }
+    for (; s < s1; s += 4) group(s, integral_constant<int, 1>(), std::false_type());
+    // wave q ends quarter q: 8 q + 4 half + e of 32, a lane two columns
+    const float scale = a.part ? 1.f : *a.scale;
+    int turn = 0;
+    auto join = [&](const v16f& c) {
+        float(*t)[4][64][4] = meet[turn];
+        turn ^= 1;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) *(v4f*)t[wave][q][lane] = v4f{c[q * 4], c[q * 4 + 1], c[q * 4 + 2], c[q * 4 + 3]};
+        __syncthreads();                                      // (two buffers: one barrier a turn)
+        return (*(const v4f*)t[0][wave][lane] + *(const v4f*)t[1][wave][lane]) + (*(const v4f*)t[2][wave][lane] + *(const v4f*)t[3][wave][lane]);
+    };
+#pragma unroll
+    for (int i = 0; i < NM; ++i) {
+        const v4f c0 = join(acc[i][0]), c1 = join(acc[i][1]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int64_t m = m0 + (wave * 8 + half * 4 + e) * NM + i;
+            if (m >= M || left <= 0) continue;
+            if (a.part) store_n<float, 2>(a.part + ((int64_t)blockIdx.z * (ROWS ? a.N : a.V) + m) * a.D + d, Pack<float, 2>{{c0[e], c1[e]}}, left);
+            else if (a.out) store_n<X, 2>((X*)a.out + (ROWS ? a.idx[m] : m) * a.D + d, Pack<X, 2>{{(X)(c0[e] * scale), (X)(c1[e] * scale)}}, left);
+        }
+        if (col) {
+            const v4f c = join(ones[i]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int64_t m = m0 + (wave * 8 + half * 4 + e) * NM + i;
+                if (at || m >= M) continue;
+                if (a.part) a.colpart[(int64_t)blockIdx.z * a.V + m] = c[e];
+                else store_any(a.colout, a.ctype, m, c[e] * scale);
+            }
+        }
+    }
+}
+
+// dx of a small table: W's fragments of 64 columns (all KS steps of k; 32 columns where an fp32 table has more than 64 outputs)
+// stay in a wave's registers while it walks over tiles of 32 rows; the next tile's dz is under way meanwhile.
+template <class X, int KS> __global__ void __launch_bounds__(256, 2) small_dx_kernel(SmallGradArgs a) {
+    using T = typename Half<X>::type;
+    constexpr int P = parts_of<X>(), NN = P == 3 && KS > 4 ? 1 : 2;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, at = lane & 31;
+    const int live = *a.live, tiles = (live + 31) / 32, step = gridDim.y * 4;
+    int t = blockIdx.y * 4 + wave;
+    if (t >= tiles) return;
+    Pack<X, 8> zv[KS];
+    auto load = [&](int tile) {                               // (dz has KS * 16 outputs, zeros behind the last; behind the last row: another row)
+        const X* z = (const X*)((const char*)a.dz + (uint64_t)(uint32_t)min(tile * 32 + at, live - 1) * a.zld) + half * 8;
+#pragma unroll
+        for (int u = 0; u < KS; ++u) zv[u] = load_n<X, 8>(z + u * 16, 8);
+    };
+    load(t);
+    const int d = (blockIdx.x * 32 + at) * NN, left = a.D - d;
+    const X* w = (const X*)a.b + min(d, a.D - 1);
+    const bool whole = (int)(blockIdx.x + 1) * 32 * NN <= a.D;
+    typename Mfma<T>::v8 wf[NN][KS][P];
+#pragma unroll
+    for (int u = 0; u < KS; ++u) {
+        Pack<X, 8> v[NN];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int k = u * 16 + half * 8 + e;
+            const X* p = (const X*)((const char*)w + (uint64_t)(uint32_t)min(k, a.V - 1) * a.ldb);
+            const auto q = whole ? load_n<X, NN>(p, NN) : load_n<X, NN>(p, left);
+#pragma unroll
+            for (int j = 0; j < NN; ++j) v[j].v[e] = k < a.V ? q.v[j] : (X)0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < NN; ++j) split_frag<X>(v[j], wf[j][u]);
+    }
+    const float scale = *a.scale;
+    for (; t < tiles; t += step) {
+        v16f acc[NN];
+#pragma unroll
+        for (int j = 0; j < NN; ++j) acc[j] = v16f{};
+        typename Mfma<T>::v8 zf[KS][P];
+#pragma unroll
+        for (int u = 0; u < KS; ++u) split_frag<X>(zv[u], zf[u]);
+        if (t + step < tiles) load(t + step);
+#pragma unroll
+        for (int u = 0; u < KS; ++u)
+#pragma unroll
+            for (int j = 0; j < NN; ++j) {
+                if constexpr (P == 3) {
+                    acc[j] = Mfma<T>::mul(zf[u][2], wf[j][u][0], acc[j]);
+                    acc[j] = Mfma<T>::mul(zf[u][1], wf[j][u][1], acc[j]);
+                    acc[j] = Mfma<T>::mul(zf[u][0], wf[j][u][2], acc[j]);
+                    acc[j] = Mfma<T>::mul(zf[u][1], wf[j][u][0], acc[j]);
+                    acc[j] = Mfma<T>::mul(zf[u][0], wf[j][u][1], acc[j]);
+                }
+                acc[j] = Mfma<T>::mul(zf[u][0], wf[j][u][0], acc[j]);
+            }
+        if (left <= 0) continue;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int m = t * 32 + e / 4 * 8 + half * 4 + e % 4;
+            if (m >= live) continue;
+            Pack<X, NN> o;
+#pragma unroll
+            for (int j = 0; j < NN; ++j) o.v[j] = (X)(acc[j][e] * scale);
+            store_n<X, NN>((X*)a.out + (int64_t)a.idx[m] * a.D + d, o, left);
+        }
+    }
 }
 
 // z - lse, from logits that are computed again: at D 512 that costs less than writing z, reading it and writing it once more (a
@@ -1713,7 +1933,7 @@ struct LogDzArgs {
     const float *G, *lp, *scale;
     int64_t ldg;
     const int32_t *live, *idx;
-    int32_t V;
+    int32_t V, plain;        // plain: rows of X, for small_grad_kernel
     uint16_t* dz;
     int64_t pitch;
 };
@@ -1755,7 +1975,9 @@ template <class X, int TPR, int R> __global__ void __launch_bounds__(256) log_dz
         float d[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) d[e] = v + e < V ? (q.v[e] - __expf(l.v[e]) * s) * inv : 0.f;
-        if (v < a.pitch) store_dz4<X>(row, a.pitch, v, d);
+        if (v >= a.pitch) return;
+        if (std::is_same<X, float>::value && a.plain) __builtin_memcpy((float*)a.dz + c * a.pitch + v, d, 16);
+        else store_dz4<X>(row, a.pitch, v, d);
     };
     if constexpr (R > 0) {
 #pragma unroll
@@ -1811,6 +2033,11 @@ bool is_small(int64_t N, int32_t D, int32_t V, int type) {
     if (V <= kSmallOutputs) return N <= 32 * 65535;          // (workgroups in a launch's second dimension)
     return N <= 65535 && (double)N * V * D <= (type == WF_F32 ? kSmallWorkF32 : kSmallWork);
 }
+// A product of small_grad_kernel that has fewer than 4 workgroups per CU is split over k while a wave keeps 4 steps.
+int small_splits(int64_t mt, int64_t D, int64_t K) {
+    const int64_t tiles = std::max<int64_t>(1, mt) * ceil_div(D, 64);
+    return (int)std::max<int64_t>(1, std::min<int64_t>({4 * kCUs / tiles, ceil_div(K, 16 * 16), 128}));
+}
 int small_mv(int32_t V) { return V <= 32 || V > kSmallOutputs ? 1 : V <= 64 ? 2 : 4; }
 
 enum { kLogFwd = 0, kLogBwd = 1, kCeFwd = 2, kCeBwd = 3 };
@@ -1819,6 +2046,7 @@ struct LinearPlan {
     int64_t N, Npad, pitch, width;      // width: outputs of a piece, pitch: its padded row
     int pieces;
     bool small;
+    int sx, sw;                         // K splits of small_grad_kernel
     Grid fwd, logp, dz, dx, dw;
     Rows rows;
     int32_t* count;
@@ -1862,6 +2090,19 @@ int make_linear_plan(int what, int64_t N, int32_t D, int32_t V, int32_t type, vo
     p.rows.target = a.take<int32_t>(p.Npad);
     p.rows.g = a.take<float>(p.Npad);
     p.rows.lse = a.take<float>(p.Npad);
+    if (bwd && p.small) {
+        p.pitch = round_up(V, 64);
+        p.dzp = a.take<uint16_t>((size_t)p.Npad * p.pitch * (type == WF_F32 ? 2 : 1));
+        p.sx = V > kSmallOutputs ? small_splits(ceil_div(N, 32), D, V) : 1;
+        p.sw = small_splits(ceil_div(V, 64), D, N);
+        if (p.sx > 1) p.part_x = a.take<float>((size_t)p.sx * N * D);
+        if (p.sw > 1) p.part_w = a.take<float>((size_t)p.sw * V * D);
+        p.part_c = a.take<float>((size_t)p.sw * V);
+        if (what == kLogBwd) p.gpeak = a.take<float>(N);
+        p.bytes = a.used + 256;
+        *out = p;
+        return WF_OK;
+    }
     p.xp = a.take<uint16_t>((size_t)p.Npad * p.parts * p.Dp);
     p.wp = a.take<uint16_t>((size_t)V * p.parts * p.Dp);
     const int64_t dits = (int64_t)products * p.Dp / kBK;
@@ -1879,7 +2120,6 @@ int make_linear_plan(int what, int64_t N, int32_t D, int32_t V, int32_t type, vo
         p.pieces = what == kLogBwd ? 1 : (int)ceil_div(V, fit);
         p.width = p.pitch = round_up(ceil_div(V, p.pieces), kRowPad);
         p.pieces = (int)ceil_div(V, p.width);
-        p.small = p.small && p.pieces == 1;
         p.dzp = a.take<uint16_t>((size_t)p.Npad * p.parts * p.pitch);
         p.dz = plan_grid(p.width, N, dits, false);
         p.dx = plan_grid(D, N, products * p.pitch / kBK, true);
@@ -1934,12 +2174,12 @@ bool direct_rows(const void* p, int64_t ld, int64_t D, int type) {   // usable a
 }
 // Packs what has to be packed and places the rows; *w is W as an operand, where it lies or packed.
 int run_prep(const LinearPlan& p, PrepArgs a, const void* x, int64_t ldx, const void* w, int64_t ldw, hipStream_t st, Operand* wo) {
-    const bool direct = direct_rows(w, ldw, p.D, p.type);
+    const bool direct = !p.wp || direct_rows(w, ldw, p.D, p.type);
     if (direct) *wo = {w, ldw, p.V, p.Dp};
     else *wo = {p.wp, (int64_t)p.parts * p.Dp, p.V, p.Dp};
     a.r = p.rows; a.N = p.N; a.ldx = ldx; a.ldw = ldw; a.D = p.D; a.Dp = p.Dp; a.V = p.V; a.x = x; a.w = w;
     a.wp = direct ? nullptr : p.wp;
-    a.row_blocks = a.xp ? (int)ceil_div(p.N, kPrepRows) : 0;
+    a.row_blocks = a.xp || !a.all ? (int)ceil_div(p.N, kPrepRows) : 0;
     a.tail_blocks = a.all ? 0 : kRowPad / kPrepRows;
     const unsigned blocks = (unsigned)(a.row_blocks + a.tail_blocks + (direct ? 0 : ceil_div(p.V, kPrepRows)));
     if (!blocks) return WF_OK;
@@ -1957,6 +2197,7 @@ Operand packed_x(const LinearPlan& p) { return {p.xp, (int64_t)p.parts * p.Dp, (
 int linear_check(const char* who, const void* x, int64_t ldx, int64_t N, const void* w, int64_t ldw, const void* bias, int32_t btype) {
     if (!w || (N > 0 && !x)) return wf_fail(WF_EINVAL, "%s: null pointer", who);
     if (ldx < 0 || ldw < 0) return wf_fail(WF_EINVAL, "%s: negative row stride", who);
+    if (ldx >= (1 << 30) || ldw >= (1 << 30)) return wf_fail(WF_EUNSUPPORTED, "%s: row stride of 2^30 elements or more", who);
     if (bias && !known_type(btype)) return wf_fail(WF_EINVAL, "%s: unknown element type", who);
     return WF_OK;
 }
@@ -1994,9 +2235,45 @@ int run_small(const LinearPlan& p, SmallArgs a, hipStream_t st) {
     return WF_OK;
 }
 
-// dx, dW, db from a piece's dz, then the next piece: dx is summed over the pieces, dW and db are final per piece
-unsigned fold_grid(int64_t elements, int splits) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(elements, splits >= 16 ? 32 : 1024), 2048)); }
 struct GradOut { void *dx, *dw, *db; int btype; };
+unsigned fold_grid(int64_t elements, int splits) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(elements, splits >= 16 ? 32 : 1024), 2048)); }
+// the gradients of few rows or few outputs
+int run_small_grads(const LinearPlan& p, const void* x, int64_t ldx, const void* w, int64_t ldw, const GradOut& o, hipStream_t st) {
+    with_type(p.type, [&](auto t) {
+        using X = decltype(t);
+        SmallGradArgs g = {p.dzp, w, p.N, (uint32_t)(p.pitch * sizeof(X)), (uint32_t)(ldw * sizeof(X)), p.rows.live, p.rows.idx, p.V, p.D, p.part_x, nullptr, p.rows.scale, o.dx, nullptr, 0};
+        if (o.dx) {
+            if (p.V <= kSmallOutputs) {
+                const int columns = p.V > 64 && p.type == WF_F32 ? 32 : 64;
+                const unsigned x = (unsigned)ceil_div(p.D, columns), most = std::max(1u, 2 * kCUs / x);
+                const dim3 grid(x, std::min<unsigned>((unsigned)ceil_div(p.N, 128), most));
+                if (p.V <= 64) small_dx_kernel<X, 4><<<grid, 256, 0, st>>>(g);
+                else small_dx_kernel<X, 8><<<grid, 256, 0, st>>>(g);
+            } else {
+                const dim3 grid((unsigned)ceil_div(p.D, 64), (unsigned)ceil_div(p.N, 32), (unsigned)p.sx);
+                small_grad_kernel<X, true><<<grid, 256, 0, st>>>(g);
+            }
+            if (p.part_x) {
+                FoldArgs f = {p.part_x, nullptr, p.rows.scale, p.sx, p.D, p.N, p.rows.live, p.rows.idx, o.dx, nullptr, p.type, 0};
+                fold_kernel<<<fold_grid(p.N * p.D, f.splits), 256, 0, st>>>(f);
+            }
+        }
+        if (o.dw || o.db) {
+            g.b = x; g.ldb = (uint32_t)(ldx * sizeof(X)); g.part = p.part_w; g.colpart = p.part_c; g.out = o.dw; g.colout = o.db; g.ctype = o.btype;
+            const dim3 grid(o.dw ? (unsigned)ceil_div(p.D, 64) : 1, (unsigned)ceil_div(p.V, 64), (unsigned)p.sw);
+            small_grad_kernel<X, false><<<grid, 256, 0, st>>>(g);
+            if (p.part_w) {
+                const int M = o.dw ? p.D : 0;
+                FoldArgs f = {p.part_w, p.part_c, p.rows.scale, p.sw, M, p.V, nullptr, nullptr, o.dw, o.db, p.type, o.btype};
+                fold_kernel<<<fold_grid((int64_t)p.V * p.D, f.splits), 256, 0, st>>>(f);
+            }
+        }
+    });
+    HIP_TRY(hipGetLastError());
+    return WF_OK;
+}
+
+// dx, dW, db from a piece's dz, then the next piece: dx is summed over the pieces, dW and db are final per piece
 int run_grads(const LinearPlan& p, const Operand& w, int piece, const GradOut& o, hipStream_t st) {
     const int64_t v0 = piece * p.width, width = std::min<int64_t>(p.width, p.V - v0);
     const Operand x = packed_x(p);
@@ -2128,7 +2405,7 @@ extern "C" int wf_linear_log_softmax_backward(const float* log_probs, const floa
     PrepArgs r = {};
     r.xp = p.xp; r.dx = dx; r.peak = p.gpeak; r.hit = 1.f; r.narrow = type == WF_F16;
     if ((rc = run_prep(p, r, x, ldx, weight, ldw, st, &w))) return rc;
-    LogDzArgs z = {grad, log_probs, p.rows.scale, ldg, p.rows.live, p.rows.idx, V, p.dzp, p.pitch};
+    LogDzArgs z = {grad, log_probs, p.rows.scale, ldg, p.rows.live, p.rows.idx, V, p.small, p.dzp, p.pitch};
     with_type(type, [&](auto t) {
         using X = decltype(t);
         if (p.pitch <= 256) log_dz_kernel<X, 64, 1><<<(unsigned)(p.Npad / 4), 256, 0, st>>>(z);
@@ -2138,6 +2415,7 @@ extern "C" int wf_linear_log_softmax_backward(const float* log_probs, const floa
         else log_dz_kernel<X, 256, 0><<<(unsigned)p.Npad, 256, 0, st>>>(z);
     });
     HIP_TRY(hipGetLastError());
+    if (p.small) return run_small_grads(p, x, ldx, weight, ldw, {dx, dweight, dbias, bias_type}, st);
     return run_grads(p, w, 0, {dx, dweight, dbias, bias_type}, st);
 }
 
@@ -2196,6 +2474,21 @@ extern "C" int wf_linear_cross_entropy_backward(const float* grad, int32_t grad_
     r.xp = p.xp; r.dx = dx; r.targets = targets; r.target_wide = targets_wide; r.ignore = ignore_index;
     r.gout = grad; r.gout_rows = grad_rows; r.mean = mean; r.lse_in = lse; r.hit = smoothing < 1.f ? 1.f - smoothing : 1.f;
     if ((rc = run_prep(p, r, x, ldx, weight, ldw, st, &w))) return rc;
+    if (p.small) {
+        SmallArgs s = {};
+        s.x = x; s.w = weight; s.ldx = ldx; s.ldw = ldw; s.N = N; s.D = D; s.l = {bias, bias_type, 0, V}; s.smoothing = smoothing;
+        s.live = p.rows.live; s.idx = p.rows.idx; s.want = p.rows.target; s.g = p.rows.g; s.glse = p.rows.lse; s.dz = p.dzp; s.zpitch = p.pitch;
+        const int mv = small_mv(V);
+        const dim3 grid((unsigned)ceil_div(round_up(V, kBK), 32 * mv), (unsigned)ceil_div(round_up(N, kBK), 32));
+        with_type(type, [&](auto t) {
+            using X = decltype(t);
+            if (mv == 1) small_kernel<X, 1, true><<<grid, 256, 0, st>>>(s);
+            else if (mv == 2) small_kernel<X, 2, true><<<grid, 256, 0, st>>>(s);
+            else small_kernel<X, 4, true><<<grid, 256, 0, st>>>(s);
+        });
+        HIP_TRY(hipGetLastError());
+        return run_small_grads(p, x, ldx, weight, ldw, {dx, dweight, dbias, bias_type}, st);
+    }
     for (int piece = 0; piece < p.pieces; ++piece) {
         const int64_t v0 = piece * p.width, width = std::min<int64_t>(p.width, V - v0);
         DzArgs z = {};
@@ -2204,20 +2497,7 @@ extern "C" int wf_linear_cross_entropy_backward(const float* grad, int32_t grad_
         set_parts(&z.p, type, p.Dp, p.Dp);
         z.l = {bias, bias_type, (int32_t)v0, (int32_t)(v0 + width)};
         z.target = p.rows.target; z.g = p.rows.g; z.lse = p.rows.lse; z.smoothing = smoothing; z.outputs = V; z.dz = p.dzp; z.pitch = p.pitch;
-        if (p.small) {
-            SmallArgs s = {};
-            s.x = x; s.w = weight; s.ldx = ldx; s.ldw = ldw; s.N = N; s.D = D; s.l = {bias, bias_type, 0, V}; s.smoothing = smoothing;
-            s.live = p.rows.live; s.idx = p.rows.idx; s.want = p.rows.target; s.g = p.rows.g; s.glse = p.rows.lse; s.dz = p.dzp; s.zpitch = p.pitch;
-            const int mv = small_mv(V);
-            const dim3 grid((unsigned)ceil_div(round_up(V, kBK), 32 * mv), (unsigned)ceil_div(round_up(N, kBK), 32));
-            with_type(type, [&](auto t) {
-                using X = decltype(t);
-                if (mv == 1) small_kernel<X, 1, true><<<grid, 256, 0, st>>>(s);
-                else if (mv == 2) small_kernel<X, 2, true><<<grid, 256, 0, st>>>(s);
-                else small_kernel<X, 4, true><<<grid, 256, 0, st>>>(s);
-            });
-            HIP_TRY(hipGetLastError());
-        } else with_type(type, [&](auto t) {
+        with_type(type, [&](auto t) {
             with_big(p.dz.big, [&](auto b) {
                 rc = launch_tiles<Shape<decltype(b)::value>, dz_kernel<decltype(t), decltype(b)::value>>(z, st);
             });
