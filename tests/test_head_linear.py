@@ -24,7 +24,11 @@ gpu = pytest.mark.gpu
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
 # one of everything; below and above a tile of 128 / 256, odd ones, a K tail, a K that is not a multiple of 8
 SIZES = [(1, 1, 1), (1, 512, 5001), (3, 64, 2), (5, 7, 59), (64, 65, 128), (127, 72, 129), (128, 128, 256), (129, 257, 255),
-         (300, 64, 513), (513, 192, 300), (1000, 80, 59), (2, 1030, 1), (296, 257, 5001)]
+         (300, 64, 513), (513, 192, 300), (1000, 80, 59), (2, 1030, 1), (296, 257, 5001),
+         # outputs in whole 64s and around them, features around the 32 and 64 columns of a workgroup, splits over many rows
+         (40, 33, 64), (100, 63, 65), (5000, 31, 33), (4099, 95, 127),
+         # more work than the direct kernels take: tiles, with rows, outputs and features that end inside one
+         (300, 1031, 6007), (700, 641, 5003), (2049, 257, 4099), (20003, 700, 131)]
 
 
 def k_error(dtype, K):
@@ -425,11 +429,29 @@ def test_the_projection_refuses_what_it_cannot_do():
     assert lib.wf_linear_log_softmax(1, 8, 2, 8, 1, 8, 3, 0, None, 0, 1, 256, 10, None) == -2
     assert lib.wf_linear_log_softmax(None, 8, 2, 8, 1, 8, 3, 0, None, 0, 1, 256, 1 << 40, None) == -1
     assert lib.wf_linear_log_softmax(1, 8, 2, 8, 1, -8, 3, 0, None, 0, 1, 256, 1 << 40, None) == -1
+    assert lib.wf_linear_log_softmax(1, 1 << 30, 2, 8, 1, 8, 3, 0, None, 0, 1, 256, 1 << 40, None) == -5
+    assert lib.wf_linear_cross_entropy(1, 8, 2, 8, 1, 1 << 30, 3, 0, None, 0, 1, 1, -1, 0.0, 1, 1, None, 0, 256, 1 << 40, None) == -5
     assert lib.wf_linear_cross_entropy(1, 8, 2, 8, 1, 8, 3, 0, None, 0, 1, 1, -1, 1.5, 1, 1, None, 0, 256, 1 << 40, None) == -1
     assert lib.wf_linear_cross_entropy(1, 8, 2, 8, 1, 8, 3, 0, None, 0, None, 1, -1, 0.0, 1, 1, None, 0, 256, 1 << 40, None) == -1
     assert lib.wf_linear_cross_entropy(1, 8, 2, 8, 1, 8, 3, 0, 1, 8, 1, 1, -1, 0.0, 1, 1, None, 0, 256, 1 << 40, None) == -1
     assert lib.wf_linear_cross_entropy_backward(1, 0, 0, None, 1, 8, 2, 8, 1, 8, 3, 0, None, 0, 1, 1, -1, 0.0, 1, 1, None, 256, 1 << 40, None) == -1
     assert lib.wf_linear_log_softmax_backward(1, None, 3, 1, 8, 2, 8, 1, 8, 3, 0, 0, 1, 1, None, 256, 1 << 40, None) == -1
+
+
+@gpu
+def test_rows_that_lie_more_than_2_30_elements_apart():
+    big = torch.empty((1 << 30) + 64, dtype=torch.bfloat16, device=DEV)
+    x = big.as_strided((2, 64), (1 << 30, 1))
+    c = Case(2, 64, 40, torch.bfloat16)
+    x.copy_(c.x)
+    y = x.detach().requires_grad_()
+    out = wf.linear_cross_entropy(y, c.w, c.t)
+    assert torch.equal(out, wf.linear_cross_entropy(c.x, c.w, c.t))
+    dx, = torch.autograd.grad(out, y)
+    d = c.x.detach().requires_grad_()
+    assert torch.equal(dx, torch.autograd.grad(wf.linear_cross_entropy(d, c.w, c.t), d)[0])
+    same = c.x[:1].expand(5, 64)                                             # the other end: one row five times
+    assert torch.equal(wf.linear_log_softmax(same, c.w), wf.linear_log_softmax(same.contiguous(), c.w))
 
 
 @gpu

@@ -2030,7 +2030,7 @@ struct Arena {               // carves the workspace; with base == NULL it only 
 constexpr int kSmallOutputs = 128;
 constexpr double kSmallWork = 0.7e9, kSmallWorkF32 = 1.6e9;      // N V D
 bool is_small(int64_t N, int32_t D, int32_t V, int type) {
-    if (V <= kSmallOutputs) return N <= 32 * 65535;          // (workgroups in a launch's second dimension)
+    if (V <= kSmallOutputs) return N <= (1 << 21) - 64;      // (workgroups in a launch's second dimension)
     return N <= 65535 && (double)N * V * D <= (type == WF_F32 ? kSmallWorkF32 : kSmallWork);
 }
 // A product of small_grad_kernel that has fewer than 4 workgroups per CU is split over k while a wave keeps 4 steps.
@@ -2069,7 +2069,7 @@ int make_linear_plan(int what, int64_t N, int32_t D, int32_t V, int32_t type, vo
     p.Npad = std::max<int64_t>(kRowPad, round_up(N, kRowPad));
     const bool bwd = what == kLogBwd || what == kCeBwd;
     Arena a = {(char*)ws};
-    p.small = is_small(N, D, V, type);
+    p.small = is_small(N, D, V, type) && (!bwd || (size_t)N * round_up(V, 64) * (type == WF_F32 ? 4 : 2) <= kPieceBytes);
     if (!bwd && p.small) {
         if (V > kSmallOutputs) {
             const size_t q = (size_t)ceil_div(V, 32) * N;

@@ -27,6 +27,8 @@ void check(int rc) { TORCH_CHECK(rc == WF_OK, "libwfdwfst error ", rc, ": ", wf_
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor workspace(size_t n, const Tensor& like) { return at::empty({(int64_t)n}, like.options().dtype(at::kByte)); }
 
+constexpr int64_t kMaxStride = (int64_t)1 << 30;                // elements between rows that the entry points take
+
 // Rows of the last dimension with unit stride inside a row, `ld` elements apart: t itself where its leading dimensions collapse
 // into one, else a contiguous copy.
 struct Rows {
@@ -40,7 +42,8 @@ struct Rows {
             const auto s = at::detail::computeStride(x.sizes(), x.strides(), to);
             if (s && (d == 1 || (*s)[1] == 1)) {
                 ld = n > 1 ? (*s)[0] : d;
-                return;
+                if (ld < kMaxStride) return;
+                ld = d;
             }
         }
         t = x.contiguous();
