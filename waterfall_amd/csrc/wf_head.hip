@@ -2023,14 +2023,18 @@ struct Arena {               // carves the workspace; with base == NULL it only 
     }
 };
 
-// Logits straight from memory (small_kernel) or by tiles: a table of at most 128 outputs is always small, else the work decides.
-// Forward with log-probabilities, us, small / tiles, at N of V 5001, D 512: fp32 1: 15 / 74, 256: 36 / 83, 512: 57 / 87, 1024: 99 /
-// 107; bf16 1: 9.5 / 20, 64: 13 / 24, 256: 22 / 24, 512: 35 / 26; of V 15001, D 1024: fp32 64: 47 / 172, 512: 256 / 241, bf16 64:
-// 27 / 38, 256: 78 / 45; of V 500, D 256: bf16 2048: 16 / 19.
+// Straight from memory (small_kernel, small_grad_kernel, small_dx_kernel) or by tiles: a table of at most 128 outputs (gradients in
+// 16 bits: 64) is always small, else the work decides.  us, small / tiles, at N of V 5001, D 512 unless said:
+//   log-probabilities: fp32 1: 15 / 74, 256: 36 / 83, 512: 57 / 87, 1024: 99 / 107; bf16 1: 9.5 / 20, 64: 13 / 24, 256: 22 / 24,
+//     512: 35 / 26; of V 15001, D 1024: fp32 64: 47 / 172, 512: 256 / 241, bf16 64: 27 / 38, 256: 78 / 45
+//   gradients of cross entropy: fp32 8: 36 / 75, 256: 72 / 104, 512: 109 / 122; bf16 8: 24 / 38, 128: 35 / 43, 256: 45 / 46, 512:
+//     65 / 55; of V 15001, D 1024: fp32 64: 104 / 169, 256: 267 / 246, bf16 64: 67 / 62; of V 59: 16000: fp32 67 / 115, bf16 48 / 57,
+//     100000: 279 / 580, 174 / 212; of V 128: 16000: 99 / 123, 66 / 59
 constexpr int kSmallOutputs = 128;
 constexpr double kSmallWork = 0.7e9, kSmallWorkF32 = 1.6e9;      // N V D
-bool is_small(int64_t N, int32_t D, int32_t V, int type) {
-    if (V <= kSmallOutputs) return N <= (1 << 21) - 64;      // (workgroups in a launch's second dimension)
+bool is_small(int64_t N, int32_t D, int32_t V, int type, bool bwd) {
+    if (bwd && (size_t)N * round_up(V, 64) * (type == WF_F32 ? 4 : 2) > kPieceBytes) return false;
+    if (V <= (bwd && type != WF_F32 ? kSmallOutputs / 2 : kSmallOutputs)) return N <= (1 << 21) - 64;      // (workgroups in a launch's second dimension)
     return N <= 65535 && (double)N * V * D <= (type == WF_F32 ? kSmallWorkF32 : kSmallWork);
 }
 // A product of small_grad_kernel that has fewer than 4 workgroups per CU is split over k while a wave keeps 4 steps.
@@ -2069,7 +2073,7 @@ int make_linear_plan(int what, int64_t N, int32_t D, int32_t V, int32_t type, vo
     p.Npad = std::max<int64_t>(kRowPad, round_up(N, kRowPad));
     const bool bwd = what == kLogBwd || what == kCeBwd;
     Arena a = {(char*)ws};
-    p.small = is_small(N, D, V, type) && (!bwd || (size_t)N * round_up(V, 64) * (type == WF_F32 ? 4 : 2) <= kPieceBytes);
+    p.small = is_small(N, D, V, type, bwd);
     if (!bwd && p.small) {
         if (V > kSmallOutputs) {
             const size_t q = (size_t)ceil_div(V, 32) * N;
@@ -2245,7 +2249,8 @@ int run_small_grads(const LinearPlan& p, const void* x, int64_t ldx, const void*
         if (o.dx) {
             if (p.V <= kSmallOutputs) {
                 const int columns = p.V > 64 && p.type == WF_F32 ? 32 : 64;
-                const unsigned x = (unsigned)ceil_div(p.D, columns), most = std::max(1u, 2 * kCUs / x);
+                // (as many workgroups as are resident: an fp32 wave holds 203 registers, a 16-bit one 99)
+                const unsigned x = (unsigned)ceil_div(p.D, columns), most = std::max(1u, (p.type == WF_F32 ? 2 : 4) * kCUs / x);
                 const dim3 grid(x, std::min<unsigned>((unsigned)ceil_div(p.N, 128), most));
                 if (p.V <= 64) small_dx_kernel<X, 4><<<grid, 256, 0, st>>>(g);
                 else small_dx_kernel<X, 8><<<grid, 256, 0, st>>>(g);
