@@ -105,6 +105,9 @@ __device__ inline void store_any(void* p, int type, int64_t i, float v) {
 //   dx = rstd (g - mean(g) - xh mean(g xh)),   dw = sum_n dy xh,   db = sum_n dy;
 // every thread keeps the dw / db sums of its own columns in registers over the rows its workgroup walks, one partial row
 // per workgroup goes to the workspace and a second kernel adds the partial rows in a fixed order (no atomics).
+//
+// Bound by HBM: 48000 x 1024 fp32 forward 75 us (5.2 TB/s, what a large copy reaches), backward 120 (4.9) + 5 for the fold;
+// 16000 x 512 bf16 9.7 + 12.5 + 3.9 us; one row of 512 2.4 us, a launch.
 
 constexpr int kLnVecs = 4;                 // 16-byte pieces of a row that a lane holds at most
 template <class T> constexpr int vec_of() { return 16 / (int)sizeof(T); }
@@ -305,7 +308,8 @@ __global__ void __launch_bounds__(1024) layer_norm_fold_kernel(const float* part
 // Element i (row-major) is kept iff word i % 4 of Philox4x32-7 (Salmon, Moraes, Dror, Shaw: Parallel random numbers: as easy
 // as 1, 2, 3; 2011 -- seven rounds are the fewest the authors found to pass every test of BigCrush) under the key `seed` and
 // the counter i / 4 is at least p 2^32; kept elements are multiplied by 1 / (1 - p), the others are exactly 0 whatever they
-// hold.  The mask is a function of (seed, i): backward computes it again, nothing is stored.
+// hold.  The mask is a function of (seed, i): backward computes it again, nothing is stored.  Bound by HBM: 16000 x 1024 bf16
+// 14 us (4.7 TB/s); 2331 x 515 fp32 3.7 us.
 struct Philox { uint32_t w[4]; };
 __device__ inline Philox philox7(uint64_t counter, uint64_t key) {
     uint32_t c0 = (uint32_t)counter, c1 = (uint32_t)(counter >> 32), c2 = 0, c3 = 0;
@@ -469,6 +473,10 @@ extern "C" int wf_dropout(const void* x, int64_t n, int32_t type, double p, uint
 // 64 different banks: chunk c of row r sits at c ^ (r / 2) % 8 (16 rows of 128 bytes at the same c), and at c ^ 4 (r % 4) where
 // K is the row (4 rows by 64 bytes).  The permutation is applied to the global address, since the direct load writes LDS in
 // lane order.  (Permutations that spread only 128 bytes, r % 8 and 2 (r % 4), had half of all LDS cycles lost to conflicts.)
+//
+// Bound by the matrix cores with K long (z of 14000 x 15001, D 1024 bf16: 464 us, 930 TFLOP/s; dW of that size 940 a piece) and by
+// prologue, epilogue and the last round of the chip with K short (16000 x 5001, D 512: 97 us, 846 TFLOP/s).  A large product of
+// the vendor's library reaches 1412 on this card, 684 and 1021 at these two sizes.
 
 struct Operand {
     const void* p;           // 16-bit elements
@@ -1037,7 +1045,8 @@ struct StatsArgs {
     float* zt;               // its logit
 };
 // Row statistics of z, tile by tile: A = W (a lane's registers run along the outputs), B = x (a lane is one row): the softmax
-// sums are register loops and one exchange between the lane halves.
+// sums are register loops and one exchange between the lane halves.  97 us at 16000 x 5001, D 512 bf16, 464 at 14000 x 15001,
+// D 1024.
 template <class T, bool BIG> __global__ void __launch_bounds__(Shape<BIG>::kThreads, BIG ? 2 : 2) stats_kernel(StatsArgs a) {
     using S = Shape<BIG>;
     using Tl = Tile<T, S::BM, S::BN, S::WM, S::WN, false, false>;
@@ -1199,7 +1208,10 @@ __global__ void __launch_bounds__(1024) total_kernel(const float* loss, int64_t 
 // A chunk of a stream (N small: the time is one read of W) or a table of characters or phones (V small: one read of x).  A
 // workgroup has 32 rows by 32 MV outputs; its 4 waves take every fourth step of 16 K each, straight from memory into the matrix
 // instructions' registers (fp32 is split there), without a tile in LDS and without packed operands; their sums meet in LDS.
-// Where one workgroup sees all outputs of its rows it ends them itself: the whole call is this one launch.
+// 4 rows of V 5001, D 512 bf16: 5.4 us and 5.4 for the end of the rows; 16000 x 59, D 512 fp32: 20 us, of which the reading of x is 6
+// and the splitting of fp32 operands 6.5 (rows brought to LDS in whole 256-byte pieces first: 18 us there, 22.4 against 20.9 at
+// 296 x 5001, D 257; 64 outputs a workgroup at that size: 23).  Where one workgroup sees all outputs of its rows it ends them
+// itself: the whole call is this one launch.
 struct SmallArgs {
     const void *x, *w;
     int64_t ldx, ldw, N;
@@ -1440,7 +1452,8 @@ __global__ void __launch_bounds__(256) small_end_kernel(SmallArgs a, int tiles) 
 //   dW:         m an output, k a live row: A = dz, B = x's rows where they lie
 // The rows of W and x run across k: a lane collects the 8 k of its place in a matrix instruction with 8 loads.  It takes two
 // neighbours of a row at a time, its columns in two instructions, so 32 lanes read 256 bytes (fp32) and write as many.  The 4
-// waves take every fourth step of 16 k, their sums meet in LDS, long k is split over workgroups too.
+// waves take every fourth step of 16 k, their sums meet in LDS, long k is split over workgroups too.  296 x 5001, D 257 fp32: dx 16
+// us, dW 18; 16000 x 59, D 512: dW 15.6.
 struct SmallGradArgs {
     const void *dz, *b;
     int64_t N;               // rows that exist
@@ -1576,7 +1589,8 @@ template <class X, bool ROWS> __global__ void __launch_bounds__(256, 2) small_gr
 }
 
 // dx of a small table: W's fragments of 64 columns (all KS steps of k; 32 columns where an fp32 table has more than 64 outputs)
-// stay in a wave's registers while it walks over tiles of 32 rows; the next tile's dz is under way meanwhile.
+// stay in a wave's registers while it walks over tiles of 32 rows; the next tile's dz is under way meanwhile.  16000 x 59, D 512
+// fp32: 22 us (the writing of dx alone: 6).
 template <class X, int KS> __global__ void __launch_bounds__(256, 2) small_dx_kernel(SmallGradArgs a) {
     using T = typename Half<X>::type;
     constexpr int P = parts_of<X>(), NN = P == 3 && KS > 4 ? 1 : 2;
@@ -1728,7 +1742,8 @@ template <int MI, class G, class P> __device__ inline void rows_out16(char* w, i
     }
 }
 // d loss / d z of a piece of the outputs from logits that are computed again: g (p - (1 - e) [v = target] - e / V), rounded to
-// the type of x for the products that follow (fp32: exact parts), as a 16-bit training step's stored gradients are.
+// the type of x for the products that follow (fp32: exact parts), as a 16-bit training step's stored gradients are.  The product
+// once more and a box of 16 bits written: 14000 x 5001, D 512 bf16 121 us, of which 28 are that box at the rate of a copy.
 template <class X, bool BIG> __global__ void __launch_bounds__(Shape<BIG>::kThreads, 2) dz_kernel(DzArgs a) {
     using T = typename Half<X>::type;
     using S = Shape<BIG>;
@@ -1800,7 +1815,8 @@ struct GradArgs {
     void* colout;
     int32_t ctype;
 };
-// C[n][m] for a gradient: m runs along features (registers: 4 neighbours), n along rows of x or of W.
+// C[n][m] for a gradient: m runs along features (registers: 4 neighbours), n along rows of x or of W.  14000 x 5001, D 512 bf16: dx
+// 102 us, dW 87.
 template <class T, bool BIG, bool BK, bool COLSUM> __global__ void __launch_bounds__(Shape<BIG>::kThreads, 2) grad_kernel(GradArgs a) {
     using S = Shape<BIG>;
     using Tl = Tile<T, S::BM, S::BN, S::WM, S::WN, true, BK, COLSUM>;
@@ -1853,7 +1869,8 @@ template <class T, bool BIG, bool BK, bool COLSUM> __global__ void __launch_boun
     }
 }
 
-// out[row(n)][m] = scale * sum over splits of part[s][n][m], and the same for the column sums
+// out[row(n)][m] = scale * sum over splits of part[s][n][m], and the same for the column sums (dW of 5001 x 512 in its splits: 14
+// us, a read of what the product wrote)
 struct FoldArgs {
     const float *part, *colpart, *scale;
     int32_t splits, M;
@@ -1907,7 +1924,8 @@ __global__ void __launch_bounds__(256) fold_kernel(FoldArgs a) {
 
 // ---- the gradient that comes into log-probabilities -----------------------------------------------------------------
 // Which rows of G hold anything: peak[n] = 0 where all of it is zero.  FULL: the largest magnitude (infinite where something is
-// no number); else some value that is not 0, and a row is read up to its first one.  A wave a row.
+// no number); else some value that is not 0, and a row is read up to its first one.  A wave a row.  16000 x 5001, an eighth of the
+// rows zero: 25 us, the reading of those.
 template <bool FULL> __global__ void __launch_bounds__(256) grad_rows_kernel(const float* G, int64_t ldg, int64_t N, int V, float* peak) {
     const int lane = threadIdx.x & 63;
     const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -1928,7 +1946,8 @@ template <bool FULL> __global__ void __launch_bounds__(256) grad_rows_kernel(con
     if (lane == 0) peak[n] = m;
 }
 // dz = G - exp(lp) sum(G) of the live rows, packed.  TPR threads a row, which stays in registers between its sum and its result
-// (R pieces of 4 a thread); R = 0: rows that do not fit are read twice.
+// (R pieces of 4 a thread); R = 0: rows that do not fit are read twice.  Bound by HBM: 14000 of 16000 x 5001 to bf16 149 us (4.7
+// TB/s).
 struct LogDzArgs {
     const float *G, *lp, *scale;
     int64_t ldg;
