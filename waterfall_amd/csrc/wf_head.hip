@@ -474,8 +474,8 @@ extern "C" int wf_dropout(const void* x, int64_t n, int32_t type, double p, uint
 // K is the row (4 rows by 64 bytes).  The permutation is applied to the global address, since the direct load writes LDS in
 // lane order.  (Permutations that spread only 128 bytes, r % 8 and 2 (r % 4), had half of all LDS cycles lost to conflicts.)
 //
-// Bound by the matrix cores with K long (z of 14000 x 15001, D 1024 bf16: 464 us, 930 TFLOP/s; dW of that size 940 a piece) and by
-// prologue, epilogue and the last round of the chip with K short (16000 x 5001, D 512: 97 us, 846 TFLOP/s).  A large product of
+// Bound by the matrix cores with K long (z of 14000 x 15001, D 1024 bf16: 450 us, 956 TFLOP/s; dW of that size 1000) and by
+// prologue, epilogue and the last round of the chip with K short (16000 x 5001, D 512: 95 us, 862 TFLOP/s).  A large product of
 // the vendor's library reaches 1412 on this card, 684 and 1021 at these two sizes.
 
 struct Operand {
@@ -1086,7 +1086,7 @@ struct StatsArgs {
     float* zt;               // its logit
 };
 // Row statistics of z, tile by tile: A = W (a lane's registers run along the outputs), B = x (a lane is one row): the softmax
-// sums are register loops and one exchange between the lane halves.  97 us at 16000 x 5001, D 512 bf16, 464 at 14000 x 15001,
+// sums are register loops and one exchange between the lane halves.  95 us at 16000 x 5001, D 512 bf16, 450 at 14000 x 15001,
 // D 1024.
 template <class T, bool BIG> __global__ void __launch_bounds__(Shape<BIG>::kThreads, BIG ? 2 : 2) stats_kernel(StatsArgs a) {
     using S = Shape<BIG>;
@@ -1783,7 +1783,7 @@ template <class T, bool BIG> __global__ void __launch_bounds__(Shape<BIG>::kThre
     }
     // d loss / d z of a piece of the outputs from logits that are computed again: g (p - (1 - e) [v = target] - e / V), rounded to
     // the type of x for the products that follow (fp32: exact parts), as a 16-bit training step's stored gradients are.  The product
-    // once more and a box of 16 bits written: 14000 x 5001, D 512 bf16 121 us, of which 28 are that box at the rate of a copy.
+    // once more and a box of 16 bits written: 14000 x 5001, D 512 bf16 108 us, of which 28 are that box at the rate of a copy.
     template <class X, bool BIG> __global__ void __launch_bounds__(Shape<BIG>::kThreads, 2) dz_kernel(DzArgs a) {
         using T = typename Half<X>::type;
         using S = Shape<BIG>;
@@ -1855,7 +1855,7 @@ template <class T, bool BIG> __global__ void __launch_bounds__(Shape<BIG>::kThre
         int32_t ctype;
     };
     // C[n][m] for a gradient: m runs along features (registers: 4 neighbours), n along rows of x or of W.  14000 x 5001, D 512 bf16: dx
-    // 102 us, dW 87.
+    // 99 us, dW 85.
     template <class T, bool BIG, bool BK, bool COLSUM> __global__ void __launch_bounds__(Shape<BIG>::kThreads, 2) grad_kernel(GradArgs a) {
         using S = Shape<BIG>;
         using Tl = Tile<T, S::BM, S::BN, S::WM, S::WN, true, BK, COLSUM>;
