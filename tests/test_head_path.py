@@ -127,6 +127,25 @@ def test_saved_tensors_that_hooks_moved(dtype):
         assert torch.equal(p, q)
 
 
+def test_saved_tensors_that_come_back_as_something_else():
+    """Hooks that hand back other devices, types or sizes: an error on the host, nothing is launched."""
+    x, w = torch.randn(4, 64, device=DEV, requires_grad=True), torch.randn(50, 64, device=DEV, requires_grad=True)
+    t, one = torch.randint(0, 50, (4,), device=DEV), torch.ones(64, device=DEV)
+    for wrong in (lambda v: v.cpu(), lambda v: v.double() if v.is_floating_point() else v.short(), lambda v: v.reshape(-1)[:-1] if v.numel() > 1 else v.short()):
+        for f in (lambda: wf.layer_norm(x, one, one), lambda: wf.linear_log_softmax(x, w), lambda: wf.linear_cross_entropy(x, w, t),
+                  lambda: wf.dropout(x, 0.5, torch.tensor([3], device=DEV))):
+            with torch.autograd.graph.saved_tensors_hooks(lambda v: v, wrong):
+                y = f()
+                with pytest.raises(RuntimeError, match="came back"):
+                    y.sum().backward()
+    # other strides are fine
+    with torch.autograd.graph.saved_tensors_hooks(lambda v: v, lambda v: torch.stack((v, v), -1)[..., 0]):
+        got = torch.autograd.grad(wf.linear_cross_entropy(wf.layer_norm(x, one, one), w, t), (x, w))
+    want = torch.autograd.grad(wf.linear_cross_entropy(wf.layer_norm(x, one, one), w, t), (x, w))
+    for p, q in zip(got, want):
+        assert torch.equal(p, q)
+
+
 def test_what_autograd_has_to_notice():
     x = torch.randn(4, 64, device=DEV, requires_grad=True)
     w = torch.randn(50, 64, device=DEV, requires_grad=True)

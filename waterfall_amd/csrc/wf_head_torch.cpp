@@ -64,6 +64,15 @@ variable_list once(variable_list grads) {
         if (g.defined()) g = out[k++];
     return grads;
 }
+// A saved tensor as hooks hand it back: it has to be where the gradient is, of the type and size it had.
+const Tensor& back(const Tensor& t, const Tensor& grad, int64_t type, int64_t n) {
+    TORCH_CHECK(!t.defined() || (t.device() == grad.device() && (int64_t)t.scalar_type() == type && t.numel() == n),
+                "waterfall_amd.head: a saved tensor came back on another device, of another type or with another size");
+    return t;
+}
+Tensor back_whole(const Tensor& t, const Tensor& grad, int64_t type, int64_t n) { return back(t, grad, type, n).defined() ? t.contiguous() : t; }
+int64_t of(const Tensor& t) { return t.defined() ? (int64_t)t.scalar_type() : 0; }
+constexpr int64_t kF32 = (int64_t)at::kFloat;
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 void* as_stream(int64_t s) { return (void*)(uintptr_t)s; }
 
@@ -80,15 +89,15 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
                             (float*)ptr(stats), as_stream(stream)));
         if (keep) {
             ctx->save_for_backward({v.t, weight, stats});
-            ctx->saved_data["a"] = std::vector<int64_t>{wants(weight), wants(bias), (int64_t)par.scalar_type(), stream};
+            ctx->saved_data["a"] = std::vector<int64_t>{wants(weight), wants(bias), of(par), stream, of(x), v.n, v.d};
         }
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         const auto a = ctx->saved_data["a"].toIntVector();
-        const Rows v(saved[0]), g(grads[0]);
-        const Tensor& weight = saved[1];
+        const Rows v(back(saved[0], grads[0], a[4], a[5] * a[6])), g(grads[0]);
+        const Tensor weight = back_whole(saved[1], grads[0], a[2], a[6]), stats = back_whole(saved[2], grads[0], kF32, a[5] * 2);
         Tensor dx = at::empty(v.t.sizes(), v.t.options()), dw, db, ws;
         const auto par = v.t.options().dtype((at::ScalarType)a[2]);
         size_t n = 0;
@@ -100,7 +109,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         }
         const int ptype = (at::ScalarType)a[2] == at::kFloat ? WF_F32 : (at::ScalarType)a[2] == at::kHalf ? WF_F16 : WF_BF16;
         check(wf_layer_norm_backward(g.p(), g.ld, v.p(), v.ld, v.n, (int32_t)v.d, type_of(v.t), ptr(weight), ptype,
-                                     (const float*)saved[2].data_ptr(), dx.data_ptr(), ptr(dw), ptr(db), ptr(ws), n, as_stream(a[3])));
+                                     (const float*)stats.data_ptr(), dx.data_ptr(), ptr(dw), ptr(db), ptr(ws), n, as_stream(a[3])));
         return once({dx, dw, db, Tensor(), Tensor()});
     }
 };
@@ -120,7 +129,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto a = ctx->saved_data["a"].toIntVector();
-        const Tensor dx = drop(grads[0], ctx->saved_data["p"].toDouble(), (uint64_t)a[0], ctx->get_saved_variables()[0], a[1]);
+        const Tensor dx = drop(grads[0], ctx->saved_data["p"].toDouble(), (uint64_t)a[0], back(ctx->get_saved_variables()[0], grads[0], (int64_t)at::kLong, 1), a[1]);
         return once({dx, Tensor(), Tensor(), Tensor(), Tensor()});
     }
 };
@@ -155,14 +164,14 @@ struct LogSoftmax : torch::autograd::Function<LogSoftmax> {
         check(wf_linear_log_softmax(v.p(), v.ld, v.n, (int32_t)v.d, w.p(), w.ld, (int32_t)w.n, type_of(x), ptr(bias),
                                     bias.defined() ? type_of(bias) : WF_F32, (float*)lp.data_ptr(), ws.data_ptr(), n, as_stream(stream)));
         ctx->save_for_backward({v.t, w.t, bias, lp});
-        ctx->saved_data["a"] = std::vector<int64_t>{wants(x), wants(weight), wants(bias), stream};
+        ctx->saved_data["a"] = std::vector<int64_t>{wants(x), wants(weight), wants(bias), stream, of(x), of(bias), v.n, v.d, w.n};
         return lp;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         const auto a = ctx->saved_data["a"].toIntVector();
-        const Rows v(saved[0]), w(saved[1]), g(grads[0]);
-        const Tensor &bias = saved[2], &lp = saved[3];
+        const Rows v(back(saved[0], grads[0], a[4], a[6] * a[7])), w(back(saved[1], grads[0], a[4], a[8] * a[7])), g(grads[0]);
+        const Tensor bias = back(saved[2], grads[0], a[5], a[8]), lp = back_whole(saved[3], grads[0], kF32, a[6] * a[8]);
         const Grads o(a, v, w, bias);
         const size_t n = linear_bytes(kLogBwd, v, w);
         const Tensor ws = workspace(n, v.t);
@@ -189,19 +198,21 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
                                       (float)smoothing, (float*)loss.data_ptr(), (float*)lse.data_ptr(), (float*)ptr(total),
                                       reduction == kMean, ws.data_ptr(), n, as_stream(stream)));
         ctx->save_for_backward({v.t, w.t, targets, bias, lse});
-        ctx->saved_data["a"] = std::vector<int64_t>{wants(x), wants(weight), wants(bias), stream, ignore, reduction};
+        ctx->saved_data["a"] = std::vector<int64_t>{wants(x), wants(weight), wants(bias), stream, ignore, reduction, of(x), of(bias),
+                                                    of(targets), v.n, v.d, w.n};
         ctx->saved_data["s"] = smoothing;
         return total.defined() ? total : loss;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         const auto a = ctx->saved_data["a"].toIntVector();
-        const Rows v(saved[0]), w(saved[1]);
-        const Tensor &targets = saved[2], &bias = saved[3], g = grads[0].contiguous();
+        const Rows v(back(saved[0], grads[0], a[6], a[9] * a[10])), w(back(saved[1], grads[0], a[6], a[11] * a[10]));
+        const Tensor targets = back_whole(saved[2], grads[0], a[8], a[9]), bias = back_whole(saved[3], grads[0], a[7], a[11]);
+        const Tensor lse = back_whole(saved[4], grads[0], kF32, a[9]), g = grads[0].contiguous();
         const Grads o(a, v, w, bias);
         const size_t n = linear_bytes(kCeBwd, v, w);
         const Tensor ws = workspace(n, v.t);
-        check(wf_linear_cross_entropy_backward((const float*)g.data_ptr(), a[5] == kNone, a[5] == kMean, (const float*)saved[4].data_ptr(),
+        check(wf_linear_cross_entropy_backward((const float*)g.data_ptr(), a[5] == kNone, a[5] == kMean, (const float*)lse.data_ptr(),
                                                v.p(), v.ld, v.n, (int32_t)v.d, w.p(), w.ld, (int32_t)w.n, type_of(v.t), ptr(bias),
                                                bias.defined() ? type_of(bias) : WF_F32, targets.data_ptr(),
                                                targets.scalar_type() == at::kLong, a[4], (float)ctx->saved_data["s"].toDouble(), ptr(o.dx),
