@@ -455,6 +455,62 @@ def test_rows_that_lie_more_than_2_30_elements_apart():
 
 
 @gpu
+def test_boxes_and_rows_beyond_2_31_elements():
+    dtype, u = torch.bfloat16, U[torch.bfloat16]
+    N, D, V = 429500, 64, 5001                                                # N V passes 2^31
+    c = Case(N, D, V, dtype)
+    with torch.no_grad():
+        G = torch.empty(N, V, device=DEV)
+        for n in range(0, N, 20000):
+            G[n:n + 20000].normal_(std=0.01)
+        G[::7] = 0
+    leaves = [t.requires_grad_() for t in (c.x, c.w, c.b)]
+    lp = wf.linear_log_softmax(*leaves)
+    dx, dw, db = torch.autograd.grad(lp, leaves, G)
+    lp = lp.detach()
+    want = [torch.zeros(V, D, device=DEV, dtype=torch.float64) for _ in range(3)] + [torch.zeros(V, device=DEV, dtype=torch.float64) for _ in range(3)]
+    with torch.no_grad():
+        for n in range(0, N, 20000):
+            part = Case.__new__(Case)
+            part.x, part.w, part.b, part.dtype, part.D, part.V = c.x[n:n + 20000].detach(), c.w.detach(), c.b.detach(), dtype, D, V
+            part.N = part.x.shape[0]
+            z, lse, e, el = part.logits()
+            within(lp[n:n + 20000], z - lse, e + el + 2.0 ** -24 * (z - lse).abs(), ("log_probs", n))
+            del z, lse, e, el
+            dz, edz = dz_of_log_softmax(part, G[n:n + 20000])
+            within(dx[n:n + 20000], *part.products(dz, edz)[0], ("dx", n))
+            edz = edz + u * (dz.abs() + edz)
+            x = part.x.double()
+            for k, (m, b) in enumerate(((dz, x), (edz, x.abs()), (dz.abs(), x.abs()))):
+                want[k] += m.t() @ b
+                want[3 + k] += m.sum(0)
+            del dz, edz
+        for got, (w, spread, size), what in ((dw, want[:3], "dweight"), (db, want[3:], "dbias")):
+            bound = spread + k_error(dtype, N) * size
+            within(got, w, bound + u * (w.abs() + bound), what)
+    del G, lp, c, leaves, dx
+    torch.cuda.empty_cache()
+    N, D, V = (1 << 21) - 64, 1040, 50                                        # N D passes 2^31: the most rows the direct kernels take
+    g = torch.Generator(device=DEV).manual_seed(5)
+    x = torch.empty(N, D, dtype=dtype, device=DEV).normal_(generator=g)
+    few = Case(300, D, V, dtype)
+    at = torch.cat((torch.arange(100), torch.arange(N // 2, N // 2 + 100), torch.arange(N - 100, N))).to(DEV)
+    x[at] = few.x
+    t = torch.full((N,), -1, device=DEV)
+    t[at] = few.t
+    assert torch.equal(wf.linear_log_softmax(x, few.w, few.b)[at], wf.linear_log_softmax(few.x, few.w, few.b))
+    y = x.detach().requires_grad_()
+    w, b = few.w.detach().requires_grad_(), few.b.detach().requires_grad_()
+    got = torch.autograd.grad(wf.linear_cross_entropy(y, w, t, b), (y, w, b))
+    f = few.x.detach().requires_grad_()
+    ref = torch.autograd.grad(wf.linear_cross_entropy(f, w, few.t, b), (f, w, b))
+    assert torch.equal(got[0][at], ref[0])                                    # the same rows, alone in a small batch
+    assert got[0].ne(0).any(1).sum().item() <= 300
+    with torch.no_grad():
+        check_grads(got[1:], few.products(*dz_of_entropy(few, torch.full((300,), 1 / 300, device=DEV), 0.0))[1:], "weights")
+
+
+@gpu
 def test_the_projection_refuses_mismatches():
     x, w, b = torch.zeros(2, 8, device=DEV), torch.zeros(3, 8, device=DEV), torch.zeros(3, device=DEV)
     t = torch.zeros(2, dtype=torch.int64, device=DEV)

@@ -132,6 +132,23 @@ def test_layer_norm_a_row_of_infinities_or_equal_values_stays_in_its_row():
 
 
 @gpu
+def test_layer_norm_beyond_2_31_elements():
+    N, D = 2200000, 1000
+    x = torch.empty(N, D, dtype=torch.bfloat16, device=DEV).normal_()
+    at = torch.cat((torch.arange(50), torch.arange(N // 2, N // 2 + 50), torch.arange(N - 50, N))).to(DEV)
+    w, b = torch.randn(D, device=DEV), torch.randn(D, device=DEV)
+    big, few = x.requires_grad_(), x.detach()[at].requires_grad_()
+    y, z = wf.layer_norm(big, w, b), wf.layer_norm(few, w, b)
+    assert torch.equal(y[at], z)
+    g = torch.randn(150, D, device=DEV).bfloat16()
+    up = torch.zeros_like(x)
+    up[at] = g
+    dx, = torch.autograd.grad(y, big, up)
+    assert torch.equal(dx[at], torch.autograd.grad(z, few, g)[0])
+    assert dx.ne(0).any(1).sum().item() <= 150
+
+
+@gpu
 def test_layer_norm_gradient_against_differences():
     g = torch.Generator().manual_seed(2)
     x, w, b = torch.randn(3, 37, generator=g), torch.randn(37, generator=g), torch.randn(37, generator=g)
