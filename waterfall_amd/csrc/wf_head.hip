@@ -1142,653 +1142,654 @@ template <class T, bool BIG> __global__ void __launch_bounds__(Shape<BIG>::kThre
                 a.sum[at + c] = sum;
                 if (a.all) a.all[at + c] = all;
             }
-        }    });
-    }
+        }
+    });
+}
 
-    // The tiles' statistics of a row joined: lse, and the loss of the row where there are targets.
-    struct JoinArgs {
-        const float *top, *sum, *all, *zt;
-        int64_t pitch, N;
-        int tiles, V;
-        const int32_t *live, *idx, *target;
-        float smoothing;
-        float *lse, *loss;
-        float* share;            // sums of the workgroups' losses, or NULL
-    };
-    __device__ inline void join_stats(float& top, float& sum, float m, float s) {
-        // (a part whose largest is -inf adds its sum as it is: 0, or NaN where its logits were no numbers)
-        const float high = fmaxf(top, m);
-        sum = sum * (top == -INFINITY ? 1.f : __expf(top - high)) + s * (m == -INFINITY ? 1.f : __expf(m - high));
-        top = high;
-    }
-    __device__ inline float row_loss(float lse, float zt, float all, int V, int target, float smoothing) {
-        if (target < 0) return NAN;                               // a target that is no output: loud, and no read out of range
-        if (lse == -INFINITY) return INFINITY;                    // every output is masked: as unlikely as a target can be
-        float loss = lse;
-        if (smoothing != 1.f) loss -= (1.f - smoothing) * zt;
-        if (smoothing != 0.f) loss -= smoothing * (all / (float)V);
-        return loss;
-    }
-    // 16 rows a workgroup, 16 threads a row: each joins every 16th tile, then they meet in LDS.  (The total in the same launch, by the
-    // workgroup that is done last, took 18 us more at 1000 workgroups: each one's release empties its die's L2.)
-    __global__ void __launch_bounds__(256) join_kernel(JoinArgs a) {
-        __shared__ float tops[16][17], sums[16][17], alls[16][17], loss[16];
-        const int r = threadIdx.x & 15, k = threadIdx.x >> 4;
-        const int64_t c = (int64_t)blockIdx.x * 16 + r, rows = a.live ? (int64_t)*a.live : a.N;
-        if ((int64_t)blockIdx.x * 16 >= rows) return;
-        float top = -INFINITY, sum = 0.f, all = 0.f;
-        if (c < rows)
-            for (int q = k; q < a.tiles; q += 16) {
-                join_stats(top, sum, a.top[q * a.pitch + c], a.sum[q * a.pitch + c]);
-                if (a.all) all += a.all[q * a.pitch + c];
-            }
-        tops[k][r] = top;
-        sums[k][r] = sum;
-        alls[k][r] = all;
-        if (k == 0) loss[r] = 0.f;
-        __syncthreads();
-        if (k == 0 && c < rows) {
-            for (int i = 1; i < 16; ++i) {
-                join_stats(top, sum, tops[i][r], sums[i][r]);
-                all += alls[i][r];
-            }
-            const float lse = (top == -INFINITY ? 0.f : top) + logf(sum);
-            const int64_t n = a.idx ? a.idx[c] : c;
-            a.lse[n] = lse;
-            if (a.loss) a.loss[n] = loss[r] = row_loss(lse, a.zt[c], all, a.V, a.target[c], a.smoothing);
+// The tiles' statistics of a row joined: lse, and the loss of the row where there are targets.
+struct JoinArgs {
+    const float *top, *sum, *all, *zt;
+    int64_t pitch, N;
+    int tiles, V;
+    const int32_t *live, *idx, *target;
+    float smoothing;
+    float *lse, *loss;
+    float* share;            // sums of the workgroups' losses, or NULL
+};
+__device__ inline void join_stats(float& top, float& sum, float m, float s) {
+    // (a part whose largest is -inf adds its sum as it is: 0, or NaN where its logits were no numbers)
+    const float high = fmaxf(top, m);
+    sum = sum * (top == -INFINITY ? 1.f : __expf(top - high)) + s * (m == -INFINITY ? 1.f : __expf(m - high));
+    top = high;
+}
+__device__ inline float row_loss(float lse, float zt, float all, int V, int target, float smoothing) {
+    if (target < 0) return NAN;                               // a target that is no output: loud, and no read out of range
+    if (lse == -INFINITY) return INFINITY;                    // every output is masked: as unlikely as a target can be
+    float loss = lse;
+    if (smoothing != 1.f) loss -= (1.f - smoothing) * zt;
+    if (smoothing != 0.f) loss -= smoothing * (all / (float)V);
+    return loss;
+}
+// 16 rows a workgroup, 16 threads a row: each joins every 16th tile, then they meet in LDS.  (The total in the same launch, by the
+// workgroup that is done last, took 18 us more at 1000 workgroups: each one's release empties its die's L2.)
+__global__ void __launch_bounds__(256) join_kernel(JoinArgs a) {
+    __shared__ float tops[16][17], sums[16][17], alls[16][17], loss[16];
+    const int r = threadIdx.x & 15, k = threadIdx.x >> 4;
+    const int64_t c = (int64_t)blockIdx.x * 16 + r, rows = a.live ? (int64_t)*a.live : a.N;
+    if ((int64_t)blockIdx.x * 16 >= rows) return;
+    float top = -INFINITY, sum = 0.f, all = 0.f;
+    if (c < rows)
+        for (int q = k; q < a.tiles; q += 16) {
+            join_stats(top, sum, a.top[q * a.pitch + c], a.sum[q * a.pitch + c]);
+            if (a.all) all += a.all[q * a.pitch + c];
         }
-        if (!a.share) return;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            float v = 0.f;
-            for (int i = 0; i < 16; ++i) v += loss[i];
-            a.share[blockIdx.x] = v;
+    tops[k][r] = top;
+    sums[k][r] = sum;
+    alls[k][r] = all;
+    if (k == 0) loss[r] = 0.f;
+    __syncthreads();
+    if (k == 0 && c < rows) {
+        for (int i = 1; i < 16; ++i) {
+            join_stats(top, sum, tops[i][r], sums[i][r]);
+            all += alls[i][r];
         }
+        const float lse = (top == -INFINITY ? 0.f : top) + logf(sum);
+        const int64_t n = a.idx ? a.idx[c] : c;
+        a.lse[n] = lse;
+        if (a.loss) a.loss[n] = loss[r] = row_loss(lse, a.zt[c], all, a.V, a.target[c], a.smoothing);
     }
-    // the sum of the workgroups' shares, over the number of rows where `mean` (0 rows: 0)
-    __global__ void __launch_bounds__(1024) shares_kernel(const float* share, const int32_t* live, int mean, float* out) {
-        __shared__ float s[16];
-        const int rows = *live, n = (rows + 15) / 16;
+    if (!a.share) return;
+    __syncthreads();
+    if (threadIdx.x == 0) {
         float v = 0.f;
-#pragma unroll 4
-        for (int i = threadIdx.x; i < n; i += 1024) v += share[i];
-        v = wave_sum(v);
-        if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            v = 0.f;
-            for (int i = 0; i < 16; ++i) v += s[i];
-            *out = mean && rows > 0 ? v / (float)rows : v;
-        }
+        for (int i = 0; i < 16; ++i) v += loss[i];
+        a.share[blockIdx.x] = v;
     }
-    // sum of the losses, over the number of rows whose target is not `ignore` where `mean`
-    __global__ void __launch_bounds__(1024) total_kernel(const float* loss, int64_t N, const void* targets, int wide, int64_t ignore, int mean, float* out) {
-        __shared__ float s[16];
-        __shared__ int c[16];
-        float v = 0.f;
-        int k = 0;
+}
+// the sum of the workgroups' shares, over the number of rows where `mean` (0 rows: 0)
+__global__ void __launch_bounds__(1024) shares_kernel(const float* share, const int32_t* live, int mean, float* out) {
+    __shared__ float s[16];
+    const int rows = *live, n = (rows + 15) / 16;
+    float v = 0.f;
 #pragma unroll 4
-        for (int64_t n = threadIdx.x; n < N; n += 1024) {
-            v += loss[n];
-            if (mean) k += (wide ? ((const int64_t*)targets)[n] : (int64_t)((const int32_t*)targets)[n]) != ignore;
-        }
-        v = wave_sum(v);
-        for (int o = 32; o; o >>= 1) k += __shfl_xor(k, o);
-        if ((threadIdx.x & 63) == 0) { s[threadIdx.x >> 6] = v; c[threadIdx.x >> 6] = k; }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            v = 0.f;
-            k = 0;
-            for (int i = 0; i < 16; ++i) { v += s[i]; k += c[i]; }
-            *out = mean ? v / (float)max(1, k) : v;
-        }
+    for (int i = threadIdx.x; i < n; i += 1024) v += share[i];
+    v = wave_sum(v);
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        v = 0.f;
+        for (int i = 0; i < 16; ++i) v += s[i];
+        *out = mean && rows > 0 ? v / (float)rows : v;
     }
+}
+// sum of the losses, over the number of rows whose target is not `ignore` where `mean`
+__global__ void __launch_bounds__(1024) total_kernel(const float* loss, int64_t N, const void* targets, int wide, int64_t ignore, int mean, float* out) {
+    __shared__ float s[16];
+    __shared__ int c[16];
+    float v = 0.f;
+    int k = 0;
+#pragma unroll 4
+    for (int64_t n = threadIdx.x; n < N; n += 1024) {
+        v += loss[n];
+        if (mean) k += (wide ? ((const int64_t*)targets)[n] : (int64_t)((const int32_t*)targets)[n]) != ignore;
+    }
+    v = wave_sum(v);
+    for (int o = 32; o; o >>= 1) k += __shfl_xor(k, o);
+    if ((threadIdx.x & 63) == 0) { s[threadIdx.x >> 6] = v; c[threadIdx.x >> 6] = k; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        v = 0.f;
+        k = 0;
+        for (int i = 0; i < 16; ++i) { v += s[i]; k += c[i]; }
+        *out = mean ? v / (float)max(1, k) : v;
+    }
+}
 
-    // ---- few rows, or few outputs ---------------------------------------------------------------------------------------
-    // A chunk of a stream (N small: the time is one read of W) or a table of characters or phones (V small: one read of x).  A
-    // workgroup has 32 rows by 32 MV outputs; its 4 waves take every fourth step of 16 K each, straight from memory into the matrix
-    // instructions' registers (fp32 is split there), without a tile in LDS and without packed operands; their sums meet in LDS.
-    // 4 rows of V 5001, D 512 bf16: 5.4 us and 5.4 for the end of the rows; 16000 x 59, D 512 fp32: 20 us, of which the reading of x is 6
-    // and the splitting of fp32 operands 6.5 (rows brought to LDS in whole 256-byte pieces first: 18 us there, 22.4 against 20.9 at
-    // 296 x 5001, D 257; 64 outputs a workgroup at that size: 23).  Where one workgroup sees all outputs of its rows it ends them
-    // itself: the whole call is this one launch.
-    struct SmallArgs {
-        const void *x, *w;
-        int64_t ldx, ldw, N;
-        int32_t D;
-        Logits l;
-        float *top, *sum, *all;  // [gridDim.x][pitch], or NULL where a workgroup sees all outputs
-        int64_t pitch;
-        float* out;              // log-probabilities: [N][V]; z where a later launch ends the rows
-        const void* targets;     // cross entropy
-        int32_t target_wide;
-        int64_t ignore;
-        float smoothing;
-        float *zt, *lse, *loss;
-        // gradients of the logits instead: of the packed rows, see dz_kernel
-        const int32_t *live, *idx, *want;
-        const float *g, *glse;
-        void* dz;                // [.][zpitch] of x's type
-        int64_t zpitch;
-    };
-    // 16-bit planes of four neighbouring values
-    template <class T> __device__ inline void store_dz4(uint16_t* row, int64_t pitch, int v, const float (&d)[4]) {
-        if constexpr (parts_of<T>() == 1) {
-            Pack<uint16_t, 4> h;
+// ---- few rows, or few outputs ---------------------------------------------------------------------------------------
+// A chunk of a stream (N small: the time is one read of W) or a table of characters or phones (V small: one read of x).  A
+// workgroup has 32 rows by 32 MV outputs; its 4 waves take every fourth step of 16 K each, straight from memory into the matrix
+// instructions' registers (fp32 is split there), without a tile in LDS and without packed operands; their sums meet in LDS.
+// 4 rows of V 5001, D 512 bf16: 5.4 us and 5.4 for the end of the rows; 16000 x 59, D 512 fp32: 20 us, of which the reading of x is 6
+// and the splitting of fp32 operands 6.5 (rows brought to LDS in whole 256-byte pieces first: 18 us there, 22.4 against 20.9 at
+// 296 x 5001, D 257; 64 outputs a workgroup at that size: 23).  Where one workgroup sees all outputs of its rows it ends them
+// itself: the whole call is this one launch.
+struct SmallArgs {
+    const void *x, *w;
+    int64_t ldx, ldw, N;
+    int32_t D;
+    Logits l;
+    float *top, *sum, *all;  // [gridDim.x][pitch], or NULL where a workgroup sees all outputs
+    int64_t pitch;
+    float* out;              // log-probabilities: [N][V]; z where a later launch ends the rows
+    const void* targets;     // cross entropy
+    int32_t target_wide;
+    int64_t ignore;
+    float smoothing;
+    float *zt, *lse, *loss;
+    // gradients of the logits instead: of the packed rows, see dz_kernel
+    const int32_t *live, *idx, *want;
+    const float *g, *glse;
+    void* dz;                // [.][zpitch] of x's type
+    int64_t zpitch;
+};
+// 16-bit planes of four neighbouring values
+template <class T> __device__ inline void store_dz4(uint16_t* row, int64_t pitch, int v, const float (&d)[4]) {
+    if constexpr (parts_of<T>() == 1) {
+        Pack<uint16_t, 4> h;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) h.v[i] = bits16<T>(d[i]);
-            __builtin_memcpy(row + v, &h, 8);
-        } else {
-            const auto s = split3(d);
+        for (int i = 0; i < 4; ++i) h.v[i] = bits16<T>(d[i]);
+        __builtin_memcpy(row + v, &h, 8);
+    } else {
+        const auto s = split3(d);
 #pragma unroll
-            for (int p = 0; p < 3; ++p) __builtin_memcpy(row + p * pitch + v, s.h[p], 8);
+        for (int p = 0; p < 3; ++p) __builtin_memcpy(row + p * pitch + v, s.h[p], 8);
+    }
+}
+template <class X> __device__ inline void split_frag(const Pack<X, 8>& v, typename Mfma<typename Half<X>::type>::v8 (&f)[parts_of<X>()]) {
+    if constexpr (parts_of<X>() == 1) {
+        __builtin_memcpy(&f[0], &v, 16);
+    } else {
+        const auto s = split3(v.v);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) __builtin_memcpy(&f[p], s.h[p], 16);
+    }
+}
+__device__ inline int32_t small_target(const void* targets, int wide, int64_t ignore, int64_t n, int V, bool* dead) {
+    const int64_t t = wide ? ((const int64_t*)targets)[n] : (int64_t)((const int32_t*)targets)[n];
+    *dead = t == ignore;
+    return t >= 0 && t < V ? (int32_t)t : -1;
+}
+template <class X, int MV, bool DZ> __global__ void __launch_bounds__(256) small_kernel(SmallArgs a) {
+    using T = typename Half<X>::type;
+    constexpr int P = parts_of<X>(), U = P == 1 || MV == 2 ? 4 : 2;      // steps whose loads are under way together
+    __shared__ __align__(16) float part[4][MV][4][64][4];     // [wave][m][q][lane][e]
+    __shared__ float wtop[4][32], wsum[4][32], wall[4][32], wzt[32];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int v0 = blockIdx.x * 32 * MV, kl = (lane >> 5) * 8;
+    const int64_t n0 = (int64_t)blockIdx.y * 32, n = n0 + (lane & 31);
+    const int live = DZ ? *a.live : 0;
+    if (DZ && n0 >= (live + kBK - 1) / kBK * kBK) return;     // rows that no product reads
+    const X* xr = (const X*)a.x + (DZ ? (int64_t)(n < live ? a.idx[n] : 0) : min(n, a.N - 1)) * a.ldx;
+    const X* wr[MV];
+#pragma unroll
+    for (int m = 0; m < MV; ++m) wr[m] = (const X*)a.w + (int64_t)min(v0 + m * 32 + (lane & 31), a.l.V - 1) * a.ldw;
+    v16f acc[MV];
+#pragma unroll
+    for (int m = 0; m < MV; ++m) acc[m] = v16f{};
+    // (a load under a condition has to be waited for before the zeros of the other lanes may go into its registers: whole steps
+    // are loaded without one)
+    auto group = [&](int k0, auto u_, auto full_) {
+        constexpr int U = decltype(u_)::value;
+        constexpr bool FULL = decltype(full_)::value;
+        Pack<X, 8> xv[U], wv[U][MV];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = k0 + u * 64;
+            xv[u] = load_n<X, 8>(xr + k, FULL ? 8 : a.D - k);
+#pragma unroll
+            for (int m = 0; m < MV; ++m) wv[u][m] = load_n<X, 8>(wr[m] + k, FULL ? 8 : a.D - k);
         }
-    }
-    template <class X> __device__ inline void split_frag(const Pack<X, 8>& v, typename Mfma<typename Half<X>::type>::v8 (&f)[parts_of<X>()]) {
-        if constexpr (parts_of<X>() == 1) {
-            __builtin_memcpy(&f[0], &v, 16);
-        } else {
-            const auto s = split3(v.v);
 #pragma unroll
-            for (int p = 0; p < 3; ++p) __builtin_memcpy(&f[p], s.h[p], 16);
-        }
-    }
-    __device__ inline int32_t small_target(const void* targets, int wide, int64_t ignore, int64_t n, int V, bool* dead) {
-        const int64_t t = wide ? ((const int64_t*)targets)[n] : (int64_t)((const int32_t*)targets)[n];
-        *dead = t == ignore;
-        return t >= 0 && t < V ? (int32_t)t : -1;
-    }
-    template <class X, int MV, bool DZ> __global__ void __launch_bounds__(256) small_kernel(SmallArgs a) {
-        using T = typename Half<X>::type;
-        constexpr int P = parts_of<X>(), U = P == 1 || MV == 2 ? 4 : 2;      // steps whose loads are under way together
-        __shared__ __align__(16) float part[4][MV][4][64][4];     // [wave][m][q][lane][e]
-        __shared__ float wtop[4][32], wsum[4][32], wall[4][32], wzt[32];
-        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        const int v0 = blockIdx.x * 32 * MV, kl = (lane >> 5) * 8;
-        const int64_t n0 = (int64_t)blockIdx.y * 32, n = n0 + (lane & 31);
-        const int live = DZ ? *a.live : 0;
-        if (DZ && n0 >= (live + kBK - 1) / kBK * kBK) return;     // rows that no product reads
-        const X* xr = (const X*)a.x + (DZ ? (int64_t)(n < live ? a.idx[n] : 0) : min(n, a.N - 1)) * a.ldx;
-        const X* wr[MV];
-#pragma unroll
-        for (int m = 0; m < MV; ++m) wr[m] = (const X*)a.w + (int64_t)min(v0 + m * 32 + (lane & 31), a.l.V - 1) * a.ldw;
-        v16f acc[MV];
-#pragma unroll
-        for (int m = 0; m < MV; ++m) acc[m] = v16f{};
-        // (a load under a condition has to be waited for before the zeros of the other lanes may go into its registers: whole steps
-        // are loaded without one)
-        auto group = [&](int k0, auto u_, auto full_) {
-            constexpr int U = decltype(u_)::value;
-            constexpr bool FULL = decltype(full_)::value;
-            Pack<X, 8> xv[U], wv[U][MV];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int k = k0 + u * 64;
-                xv[u] = load_n<X, 8>(xr + k, FULL ? 8 : a.D - k);
-#pragma unroll
-                for (int m = 0; m < MV; ++m) wv[u][m] = load_n<X, 8>(wr[m] + k, FULL ? 8 : a.D - k);
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                typename Mfma<T>::v8 xf[P], wf[P];
-                split_frag<X>(xv[u], xf);
-#pragma unroll
-                for (int m = 0; m < MV; ++m) {
-                    split_frag<X>(wv[u][m], wf);
-                    if constexpr (P == 1) {
-                        acc[m] = Mfma<T>::mul(wf[0], xf[0], acc[m]);
-                    } else {
-                        acc[m] = Mfma<T>::mul(wf[2], xf[0], acc[m]);
-                        acc[m] = Mfma<T>::mul(wf[1], xf[1], acc[m]);
-                        acc[m] = Mfma<T>::mul(wf[0], xf[2], acc[m]);
-                        acc[m] = Mfma<T>::mul(wf[1], xf[0], acc[m]);
-                        acc[m] = Mfma<T>::mul(wf[0], xf[1], acc[m]);
-                        acc[m] = Mfma<T>::mul(wf[0], xf[0], acc[m]);
-                    }
-                }
-            }
-        };
-        int k0 = wave * 16;
-        for (; k0 + (U - 1) * 64 + 16 <= a.D; k0 += U * 64) group(k0 + kl, std::integral_constant<int, U>(), std::true_type());
-        for (; k0 + 16 <= a.D; k0 += 64) group(k0 + kl, std::integral_constant<int, 1>(), std::true_type());
-        if (k0 < a.D) group(k0 + kl, std::integral_constant<int, 1>(), std::false_type());
-#pragma unroll
-        for (int m = 0; m < MV; ++m)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) *(v4f*)part[wave][m][q][lane] = v4f{acc[m][q * 4], acc[m][q * 4 + 1], acc[m][q * 4 + 2], acc[m][q * 4 + 3]};
-        if (threadIdx.x < 32) wzt[threadIdx.x] = 0.f;
-        __syncthreads();
-        // wave q ends quarter q of every 32 outputs: v0 + 32 m + 8 q + 4 (lane / 32) .. + 3 of row lane % 32
-        if constexpr (DZ) {
-            const float share = a.smoothing < 1.f ? 1.f / (1.f - a.smoothing) : 1.f, hit = a.smoothing < 1.f ? 1.f : 0.f;
-            const float g = n < live ? a.g[n] : 0.f, lse = n < live ? a.glse[n] : 0.f, ref = lse == -INFINITY ? 0.f : lse;
-            const int target = n < live ? a.want[n] : -1;
-            const bool none = g == 0.f || lse == -INFINITY;
-            const float even = a.smoothing / (float)a.l.V;
+        for (int u = 0; u < U; ++u) {
+            typename Mfma<T>::v8 xf[P], wf[P];
+            split_frag<X>(xv[u], xf);
 #pragma unroll
             for (int m = 0; m < MV; ++m) {
-                const v4f s = (*(const v4f*)part[0][m][wave][lane] + *(const v4f*)part[1][m][wave][lane]) +
-                              (*(const v4f*)part[2][m][wave][lane] + *(const v4f*)part[3][m][wave][lane]);
-                const int v = v0 + m * 32 + wave * 8 + (lane >> 5) * 4;
-                float d[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const bool in = v + e < a.l.V;
-                    const float z = in && a.l.bias ? s[e] + load_any(a.l.bias, a.l.btype, v + e) : s[e];
-                    const float u = g * ((__expf(z - ref) - even) * share - (v + e == target ? hit : 0.f));
-                    d[e] = (none | !in) ? 0.f : u;
+                split_frag<X>(wv[u][m], wf);
+                if constexpr (P == 1) {
+                    acc[m] = Mfma<T>::mul(wf[0], xf[0], acc[m]);
+                } else {
+                    acc[m] = Mfma<T>::mul(wf[2], xf[0], acc[m]);
+                    acc[m] = Mfma<T>::mul(wf[1], xf[1], acc[m]);
+                    acc[m] = Mfma<T>::mul(wf[0], xf[2], acc[m]);
+                    acc[m] = Mfma<T>::mul(wf[1], xf[0], acc[m]);
+                    acc[m] = Mfma<T>::mul(wf[0], xf[1], acc[m]);
+                    acc[m] = Mfma<T>::mul(wf[0], xf[0], acc[m]);
                 }
-                Pack<X, 4> o;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o.v[e] = (X)d[e];
-                if (v < a.zpitch) store_n<X, 4>((X*)a.dz + n * a.zpitch + v, o, 4);
             }
-            return;
         }
-        bool dead = false;
-        const int want = a.targets && n < a.N ? small_target(a.targets, a.target_wide, a.ignore, n, a.l.V, &dead) : -1;
-        v4f z[MV];
-        float top = -INFINITY, all = 0.f;
+    };
+    int k0 = wave * 16;
+    for (; k0 + (U - 1) * 64 + 16 <= a.D; k0 += U * 64) group(k0 + kl, std::integral_constant<int, U>(), std::true_type());
+    for (; k0 + 16 <= a.D; k0 += 64) group(k0 + kl, std::integral_constant<int, 1>(), std::true_type());
+    if (k0 < a.D) group(k0 + kl, std::integral_constant<int, 1>(), std::false_type());
+#pragma unroll
+    for (int m = 0; m < MV; ++m)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) *(v4f*)part[wave][m][q][lane] = v4f{acc[m][q * 4], acc[m][q * 4 + 1], acc[m][q * 4 + 2], acc[m][q * 4 + 3]};
+    if (threadIdx.x < 32) wzt[threadIdx.x] = 0.f;
+    __syncthreads();
+    // wave q ends quarter q of every 32 outputs: v0 + 32 m + 8 q + 4 (lane / 32) .. + 3 of row lane % 32
+    if constexpr (DZ) {
+        const float share = a.smoothing < 1.f ? 1.f / (1.f - a.smoothing) : 1.f, hit = a.smoothing < 1.f ? 1.f : 0.f;
+        const float g = n < live ? a.g[n] : 0.f, lse = n < live ? a.glse[n] : 0.f, ref = lse == -INFINITY ? 0.f : lse;
+        const int target = n < live ? a.want[n] : -1;
+        const bool none = g == 0.f || lse == -INFINITY;
+        const float even = a.smoothing / (float)a.l.V;
 #pragma unroll
         for (int m = 0; m < MV; ++m) {
-            z[m] = (*(const v4f*)part[0][m][wave][lane] + *(const v4f*)part[1][m][wave][lane]) +
-                   (*(const v4f*)part[2][m][wave][lane] + *(const v4f*)part[3][m][wave][lane]);
+            const v4f s = (*(const v4f*)part[0][m][wave][lane] + *(const v4f*)part[1][m][wave][lane]) +
+                          (*(const v4f*)part[2][m][wave][lane] + *(const v4f*)part[3][m][wave][lane]);
+            const int v = v0 + m * 32 + wave * 8 + (lane >> 5) * 4;
+            float d[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int v = v0 + m * 32 + wave * 8 + (lane >> 5) * 4 + e;
-                const bool in = v < a.l.V;
-                z[m][e] = in ? z[m][e] + (a.l.bias ? load_any(a.l.bias, a.l.btype, v) : 0.f) : -INFINITY;
-                top = fmaxf(top, z[m][e]);
-                all += in ? z[m][e] : 0.f;
-                if (v == want) { if (a.top) a.zt[n] = z[m][e]; else wzt[lane & 31] = z[m][e]; }
+                const bool in = v + e < a.l.V;
+                const float z = in && a.l.bias ? s[e] + load_any(a.l.bias, a.l.btype, v + e) : s[e];
+                const float u = g * ((__expf(z - ref) - even) * share - (v + e == target ? hit : 0.f));
+                d[e] = (none | !in) ? 0.f : u;
             }
+            Pack<X, 4> o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o.v[e] = (X)d[e];
+            if (v < a.zpitch) store_n<X, 4>((X*)a.dz + n * a.zpitch + v, o, 4);
         }
-        top = fmaxf(top, __shfl_xor(top, 32));
-        all += __shfl_xor(all, 32);
-        if (lane < 32) { wtop[wave][lane] = top; wall[wave][lane] = all; }
-        __syncthreads();
-        top = fmaxf(fmaxf(wtop[0][lane & 31], wtop[1][lane & 31]), fmaxf(wtop[2][lane & 31], wtop[3][lane & 31]));
-        const float ref = top == -INFINITY ? 0.f : top;
-        float sum = 0.f;
+        return;
+    }
+    bool dead = false;
+    const int want = a.targets && n < a.N ? small_target(a.targets, a.target_wide, a.ignore, n, a.l.V, &dead) : -1;
+    v4f z[MV];
+    float top = -INFINITY, all = 0.f;
 #pragma unroll
-        for (int m = 0; m < MV; ++m)
+    for (int m = 0; m < MV; ++m) {
+        z[m] = (*(const v4f*)part[0][m][wave][lane] + *(const v4f*)part[1][m][wave][lane]) +
+               (*(const v4f*)part[2][m][wave][lane] + *(const v4f*)part[3][m][wave][lane]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum += __expf(z[m][e] - ref);
-        sum += __shfl_xor(sum, 32);
-        if (lane < 32) wsum[wave][lane] = sum;
-        __syncthreads();
-        const int r = lane & 31;
-        sum = (wsum[0][r] + wsum[1][r]) + (wsum[2][r] + wsum[3][r]);
-        all = (wall[0][r] + wall[1][r]) + (wall[2][r] + wall[3][r]);
-        if (n >= a.N) return;
-        float lse = 0.f;
-        if (a.top) {
-            if (wave == 0 && lane < 32) {
-                const int64_t at = blockIdx.x * a.pitch + n;
-                a.top[at] = top;
-                a.sum[at] = sum;
-                if (a.all) a.all[at] = all;
-            }
-        } else {
-            lse = ref + logf(sum);
-            if (a.loss && wave == 0 && lane < 32) {
-                a.lse[n] = dead ? 0.f : lse;
-                a.loss[n] = dead ? 0.f : row_loss(lse, wzt[r], all, a.l.V, want, a.smoothing);
-            }
-        }
-        if (a.out) {
-            const float minus = lse == -INFINITY ? 0.f : lse;    // a row of -inf stays one
-#pragma unroll
-            for (int m = 0; m < MV; ++m) {
-                const int v = v0 + m * 32 + wave * 8 + (lane >> 5) * 4;
-                Pack<float, 4> o;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o.v[e] = z[m][e] - minus;
-                store_n<float, 4>(a.out + n * a.l.V + v, o, a.l.V - v);
-            }
+        for (int e = 0; e < 4; ++e) {
+            const int v = v0 + m * 32 + wave * 8 + (lane >> 5) * 4 + e;
+            const bool in = v < a.l.V;
+            z[m][e] = in ? z[m][e] + (a.l.bias ? load_any(a.l.bias, a.l.btype, v) : 0.f) : -INFINITY;
+            top = fmaxf(top, z[m][e]);
+            all += in ? z[m][e] : 0.f;
+            if (v == want) { if (a.top) a.zt[n] = z[m][e]; else wzt[lane & 31] = z[m][e]; }
         }
     }
-    // Ends the rows of several workgroups: out (4096 values of a row a workgroup) -= lse; loss and lse.
-    __global__ void __launch_bounds__(256) small_end_kernel(SmallArgs a, int tiles) {
-        __shared__ float tops[4], sums[4], alls[4];
-        const int64_t n = blockIdx.y;
-        float* out = a.out + n * a.l.V;
-        const int v0 = blockIdx.x * 4096 + threadIdx.x;
-        float z[16];                                              // under way while the row's statistics are joined
+    top = fmaxf(top, __shfl_xor(top, 32));
+    all += __shfl_xor(all, 32);
+    if (lane < 32) { wtop[wave][lane] = top; wall[wave][lane] = all; }
+    __syncthreads();
+    top = fmaxf(fmaxf(wtop[0][lane & 31], wtop[1][lane & 31]), fmaxf(wtop[2][lane & 31], wtop[3][lane & 31]));
+    const float ref = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) z[i] = a.out && v0 + i * 256 < a.l.V ? out[v0 + i * 256] : 0.f;
-        float top = -INFINITY, sum = 0.f, all = 0.f;
-        for (int q = threadIdx.x; q < tiles; q += 256) {
-            join_stats(top, sum, a.top[q * a.pitch + n], a.sum[q * a.pitch + n]);
-            if (a.all) all += a.all[q * a.pitch + n];
-        }
+    for (int m = 0; m < MV; ++m)
 #pragma unroll
-        for (int o = 32; o; o >>= 1) {
-            const float m = __shfl_xor(top, o), s = __shfl_xor(sum, o);
-            join_stats(top, sum, m, s);
+        for (int e = 0; e < 4; ++e) sum += __expf(z[m][e] - ref);
+    sum += __shfl_xor(sum, 32);
+    if (lane < 32) wsum[wave][lane] = sum;
+    __syncthreads();
+    const int r = lane & 31;
+    sum = (wsum[0][r] + wsum[1][r]) + (wsum[2][r] + wsum[3][r]);
+    all = (wall[0][r] + wall[1][r]) + (wall[2][r] + wall[3][r]);
+    if (n >= a.N) return;
+    float lse = 0.f;
+    if (a.top) {
+        if (wave == 0 && lane < 32) {
+            const int64_t at = blockIdx.x * a.pitch + n;
+            a.top[at] = top;
+            a.sum[at] = sum;
+            if (a.all) a.all[at] = all;
         }
-        all = wave_sum(all);
-        if ((threadIdx.x & 63) == 0) { tops[threadIdx.x >> 6] = top; sums[threadIdx.x >> 6] = sum; alls[threadIdx.x >> 6] = all; }
-        __syncthreads();
-        top = tops[0];
-        sum = sums[0];
-        all = alls[0];
-        for (int i = 1; i < 4; ++i) { join_stats(top, sum, tops[i], sums[i]); all += alls[i]; }
-        const float lse = (top == -INFINITY ? 0.f : top) + logf(sum);
-        if (a.loss && blockIdx.x == 0 && threadIdx.x == 0) {
-            bool dead = false;
-            const int want = small_target(a.targets, a.target_wide, a.ignore, n, a.l.V, &dead);
+    } else {
+        lse = ref + logf(sum);
+        if (a.loss && wave == 0 && lane < 32) {
             a.lse[n] = dead ? 0.f : lse;
-            a.loss[n] = dead ? 0.f : row_loss(lse, want < 0 ? 0.f : a.zt[n], all, a.l.V, want, a.smoothing);
+            a.loss[n] = dead ? 0.f : row_loss(lse, wzt[r], all, a.l.V, want, a.smoothing);
         }
-        if (a.out && lse != -INFINITY)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (v0 + i * 256 < a.l.V) out[v0 + i * 256] = z[i] - lse;
     }
-
-    // Gradients of the same sizes, C[m][d] = sum over k of A(k, m) B(k, d), straight from memory as well:
-    //   dx (ROWS):  m a live row, k an output: A = dz in its rows, 8 neighbours of k a load; B = W
-    //   dW:         m an output, k a live row: A = dz, B = x's rows where they lie
-    // The rows of W and x run across k: a lane collects the 8 k of its place in a matrix instruction with 8 loads.  It takes two
-    // neighbours of a row at a time, its columns in two instructions, so 32 lanes read 256 bytes (fp32) and write as many.  The 4
-    // waves take every fourth step of 16 k, their sums meet in LDS, long k is split over workgroups too.  296 x 5001, D 257 fp32: dx 16
-    // us, dW 18; 16000 x 59, D 512: dW 15.6.
-    struct SmallGradArgs {
-        const void *dz, *b;
-        int64_t N;               // rows that exist
-        uint32_t zld, ldb;       // bytes
-        const int32_t *live, *idx;
-        int32_t V, D;
-        float *part, *colpart;   // [splits][N or V][D], [splits][V], or NULL: straight to the outputs
-        const float* scale;
-        void *out, *colout;
-        int32_t ctype;
-    };
-    template <class X, bool ROWS> __global__ void __launch_bounds__(256, 2) small_grad_kernel(SmallGradArgs a) {
-        using T = typename Half<X>::type;
-        constexpr int P = parts_of<X>(), NM = ROWS ? 1 : 2;       // dW: two neighbours of m a lane as well
-        __shared__ __align__(16) float meet[2][4][4][64][4];      // [turn][wave][q][lane][e]
-        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, at = lane & 31;
-        const int live = *a.live, M = ROWS ? live : a.V, K = ROWS ? a.V : live;
-        const int64_t m0 = (int64_t)blockIdx.y * 32 * NM;
-        const int d0 = blockIdx.x * 64, d = d0 + at * 2;
-        if (m0 >= M) return;
-        const bool col = !ROWS && a.colout && blockIdx.x == 0;
-        const int steps = (K + 15) / 16, per = (steps + gridDim.z - 1) / gridDim.z, s1 = min(steps, (int)(blockIdx.z + 1) * per), end = min(K, s1 * 16);
-        // (dz has whole 64 outputs in every row: what is behind the last output or row is not used)
-        const char* zp = (const char*)a.dz + (ROWS ? min(m0 + at, (int64_t)M - 1) * a.zld : (m0 + at * 2) * (int64_t)sizeof(X));
-        const char* bp = (const char*)a.b + (int64_t)min(d, a.D - 1) * sizeof(X);
-        const int left = a.D - d;
-        v16f acc[NM][2], ones[NM];
+    if (a.out) {
+        const float minus = lse == -INFINITY ? 0.f : lse;    // a row of -inf stays one
 #pragma unroll
-        for (int i = 0; i < NM; ++i) ones[i] = acc[i][0] = acc[i][1] = v16f{};
-        typename Mfma<T>::v8 one;
+        for (int m = 0; m < MV; ++m) {
+            const int v = v0 + m * 32 + wave * 8 + (lane >> 5) * 4;
+            Pack<float, 4> o;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) one[e] = (T)1.f;
-        // U steps from s on, loads first; FULL: all of their k and all 64 columns exist
-        auto group = [&](int s, auto u_, auto full_) {
-            constexpr int U = decltype(u_)::value;
-            constexpr bool FULL = decltype(full_)::value;
-            Pack<X, 8> av[U][NM], bv[U][2];
-            int row[U][8];
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int k = (s + u * 4) * 16 + half * 8 + e, ke = FULL ? k : min(k, end - 1);
-                    row[u][e] = ROWS ? ke : a.idx[ke];
-                }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int k = (s + u * 4) * 16 + half * 8;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const X* p = (const X*)(bp + (uint64_t)(uint32_t)row[u][e] * a.ldb);
-                    const auto b = FULL ? load_n<X, 2>(p, 2) : load_n<X, 2>(p, k + e < end ? left : 0);
-                    bv[u][0].v[e] = b.v[0];
-                    bv[u][1].v[e] = b.v[1];
-                }
-                if constexpr (ROWS) {
-                    av[u][0] = load_n<X, 8>((const X*)zp + k, FULL ? 8 : end - k);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const X* p = (const X*)(zp + (uint64_t)(uint32_t)(k + e) * a.zld);
-                        const auto z = load_n<X, 2>(p, FULL || k + e < end ? 2 : 0);
-                        av[u][0].v[e] = z.v[0];
-                        av[u][1].v[e] = z.v[1];
-                    }
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                typename Mfma<T>::v8 bf[2][P];
-                split_frag<X>(bv[u][0], bf[0]);
-                split_frag<X>(bv[u][1], bf[1]);
-#pragma unroll
-                for (int i = 0; i < NM; ++i) {
-                    typename Mfma<T>::v8 af[P];
-                    split_frag<X>(av[u][i], af);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        if constexpr (P == 3) {
-                            acc[i][j] = Mfma<T>::mul(af[2], bf[j][0], acc[i][j]);
-                            acc[i][j] = Mfma<T>::mul(af[1], bf[j][1], acc[i][j]);
-                            acc[i][j] = Mfma<T>::mul(af[0], bf[j][2], acc[i][j]);
-                            acc[i][j] = Mfma<T>::mul(af[1], bf[j][0], acc[i][j]);
-                            acc[i][j] = Mfma<T>::mul(af[0], bf[j][1], acc[i][j]);
-                        }
-                        acc[i][j] = Mfma<T>::mul(af[0], bf[j][0], acc[i][j]);
-                    }
-                    if (col)
-#pragma unroll
-                        for (int p = P - 1; p >= 0; --p) ones[i] = Mfma<T>::mul(af[p], one, ones[i]);
-                }
-            }
-        };
-        using std::integral_constant;
-        int s = (int)blockIdx.z * per + wave;
-        if (d0 + 64 <= a.D) {
-            for (; (s + 4) * 16 + 16 <= end; s += 8) group(s, integral_constant<int, 2>(), std::true_type());
-            if (s * 16 + 16 <= end) { group(s, integral_constant<int, 1>(), std::true_type()); s += 4; }
+            for (int e = 0; e < 4; ++e) o.v[e] = z[m][e] - minus;
+            store_n<float, 4>(a.out + n * a.l.V + v, o, a.l.V - v);
         }
-        for (; s < s1; s += 4) group(s, integral_constant<int, 1>(), std::false_type());
-        // wave q ends quarter q: 8 q + 4 half + e of 32, a lane two columns
-        const float scale = a.part ? 1.f : *a.scale;
-        int turn = 0;
-        auto join = [&](const v16f& c) {
-            float(*t)[4][64][4] = meet[turn];
-            turn ^= 1;
+    }
+}
+// Ends the rows of several workgroups: out (4096 values of a row a workgroup) -= lse; loss and lse.
+__global__ void __launch_bounds__(256) small_end_kernel(SmallArgs a, int tiles) {
+    __shared__ float tops[4], sums[4], alls[4];
+    const int64_t n = blockIdx.y;
+    float* out = a.out + n * a.l.V;
+    const int v0 = blockIdx.x * 4096 + threadIdx.x;
+    float z[16];                                              // under way while the row's statistics are joined
 #pragma unroll
-            for (int q = 0; q < 4; ++q) *(v4f*)t[wave][q][lane] = v4f{c[q * 4], c[q * 4 + 1], c[q * 4 + 2], c[q * 4 + 3]};
-            __syncthreads();                                      // (two buffers: one barrier a turn)
-            return (*(const v4f*)t[0][wave][lane] + *(const v4f*)t[1][wave][lane]) + (*(const v4f*)t[2][wave][lane] + *(const v4f*)t[3][wave][lane]);
-        };
+    for (int i = 0; i < 16; ++i) z[i] = a.out && v0 + i * 256 < a.l.V ? out[v0 + i * 256] : 0.f;
+    float top = -INFINITY, sum = 0.f, all = 0.f;
+    for (int q = threadIdx.x; q < tiles; q += 256) {
+        join_stats(top, sum, a.top[q * a.pitch + n], a.sum[q * a.pitch + n]);
+        if (a.all) all += a.all[q * a.pitch + n];
+    }
 #pragma unroll
-        for (int i = 0; i < NM; ++i) {
-            const v4f c0 = join(acc[i][0]), c1 = join(acc[i][1]);
+    for (int o = 32; o; o >>= 1) {
+        const float m = __shfl_xor(top, o), s = __shfl_xor(sum, o);
+        join_stats(top, sum, m, s);
+    }
+    all = wave_sum(all);
+    if ((threadIdx.x & 63) == 0) { tops[threadIdx.x >> 6] = top; sums[threadIdx.x >> 6] = sum; alls[threadIdx.x >> 6] = all; }
+    __syncthreads();
+    top = tops[0];
+    sum = sums[0];
+    all = alls[0];
+    for (int i = 1; i < 4; ++i) { join_stats(top, sum, tops[i], sums[i]); all += alls[i]; }
+    const float lse = (top == -INFINITY ? 0.f : top) + logf(sum);
+    if (a.loss && blockIdx.x == 0 && threadIdx.x == 0) {
+        bool dead = false;
+        const int want = small_target(a.targets, a.target_wide, a.ignore, n, a.l.V, &dead);
+        a.lse[n] = dead ? 0.f : lse;
+        a.loss[n] = dead ? 0.f : row_loss(lse, want < 0 ? 0.f : a.zt[n], all, a.l.V, want, a.smoothing);
+    }
+    if (a.out && lse != -INFINITY)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (v0 + i * 256 < a.l.V) out[v0 + i * 256] = z[i] - lse;
+}
+
+// Gradients of the same sizes, C[m][d] = sum over k of A(k, m) B(k, d), straight from memory as well:
+//   dx (ROWS):  m a live row, k an output: A = dz in its rows, 8 neighbours of k a load; B = W
+//   dW:         m an output, k a live row: A = dz, B = x's rows where they lie
+// The rows of W and x run across k: a lane collects the 8 k of its place in a matrix instruction with 8 loads.  It takes two
+// neighbours of a row at a time, its columns in two instructions, so 32 lanes read 256 bytes (fp32) and write as many.  The 4
+// waves take every fourth step of 16 k, their sums meet in LDS, long k is split over workgroups too.  296 x 5001, D 257 fp32: dx 16
+// us, dW 18; 16000 x 59, D 512: dW 15.6.
+struct SmallGradArgs {
+    const void *dz, *b;
+    int64_t N;               // rows that exist
+    uint32_t zld, ldb;       // bytes
+    const int32_t *live, *idx;
+    int32_t V, D;
+    float *part, *colpart;   // [splits][N or V][D], [splits][V], or NULL: straight to the outputs
+    const float* scale;
+    void *out, *colout;
+    int32_t ctype;
+};
+template <class X, bool ROWS> __global__ void __launch_bounds__(256, 2) small_grad_kernel(SmallGradArgs a) {
+    using T = typename Half<X>::type;
+    constexpr int P = parts_of<X>(), NM = ROWS ? 1 : 2;       // dW: two neighbours of m a lane as well
+    __shared__ __align__(16) float meet[2][4][4][64][4];      // [turn][wave][q][lane][e]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, at = lane & 31;
+    const int live = *a.live, M = ROWS ? live : a.V, K = ROWS ? a.V : live;
+    const int64_t m0 = (int64_t)blockIdx.y * 32 * NM;
+    const int d0 = blockIdx.x * 64, d = d0 + at * 2;
+    if (m0 >= M) return;
+    const bool col = !ROWS && a.colout && blockIdx.x == 0;
+    const int steps = (K + 15) / 16, per = (steps + gridDim.z - 1) / gridDim.z, s1 = min(steps, (int)(blockIdx.z + 1) * per), end = min(K, s1 * 16);
+    // (dz has whole 64 outputs in every row: what is behind the last output or row is not used)
+    const char* zp = (const char*)a.dz + (ROWS ? min(m0 + at, (int64_t)M - 1) * a.zld : (m0 + at * 2) * (int64_t)sizeof(X));
+    const char* bp = (const char*)a.b + (int64_t)min(d, a.D - 1) * sizeof(X);
+    const int left = a.D - d;
+    v16f acc[NM][2], ones[NM];
+#pragma unroll
+    for (int i = 0; i < NM; ++i) ones[i] = acc[i][0] = acc[i][1] = v16f{};
+    typename Mfma<T>::v8 one;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) one[e] = (T)1.f;
+    // U steps from s on, loads first; FULL: all of their k and all 64 columns exist
+    auto group = [&](int s, auto u_, auto full_) {
+        constexpr int U = decltype(u_)::value;
+        constexpr bool FULL = decltype(full_)::value;
+        Pack<X, 8> av[U][NM], bv[U][2];
+        int row[U][8];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int k = (s + u * 4) * 16 + half * 8 + e, ke = FULL ? k : min(k, end - 1);
+                row[u][e] = ROWS ? ke : a.idx[ke];
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = (s + u * 4) * 16 + half * 8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const X* p = (const X*)(bp + (uint64_t)(uint32_t)row[u][e] * a.ldb);
+                const auto b = FULL ? load_n<X, 2>(p, 2) : load_n<X, 2>(p, k + e < end ? left : 0);
+                bv[u][0].v[e] = b.v[0];
+                bv[u][1].v[e] = b.v[1];
+            }
+            if constexpr (ROWS) {
+                av[u][0] = load_n<X, 8>((const X*)zp + k, FULL ? 8 : end - k);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const X* p = (const X*)(zp + (uint64_t)(uint32_t)(k + e) * a.zld);
+                    const auto z = load_n<X, 2>(p, FULL || k + e < end ? 2 : 0);
+                    av[u][0].v[e] = z.v[0];
+                    av[u][1].v[e] = z.v[1];
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            typename Mfma<T>::v8 bf[2][P];
+            split_frag<X>(bv[u][0], bf[0]);
+            split_frag<X>(bv[u][1], bf[1]);
+#pragma unroll
+            for (int i = 0; i < NM; ++i) {
+                typename Mfma<T>::v8 af[P];
+                split_frag<X>(av[u][i], af);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    if constexpr (P == 3) {
+                        acc[i][j] = Mfma<T>::mul(af[2], bf[j][0], acc[i][j]);
+                        acc[i][j] = Mfma<T>::mul(af[1], bf[j][1], acc[i][j]);
+                        acc[i][j] = Mfma<T>::mul(af[0], bf[j][2], acc[i][j]);
+                        acc[i][j] = Mfma<T>::mul(af[1], bf[j][0], acc[i][j]);
+                        acc[i][j] = Mfma<T>::mul(af[0], bf[j][1], acc[i][j]);
+                    }
+                    acc[i][j] = Mfma<T>::mul(af[0], bf[j][0], acc[i][j]);
+                }
+                if (col)
+#pragma unroll
+                    for (int p = P - 1; p >= 0; --p) ones[i] = Mfma<T>::mul(af[p], one, ones[i]);
+            }
+        }
+    };
+    using std::integral_constant;
+    int s = (int)blockIdx.z * per + wave;
+    if (d0 + 64 <= a.D) {
+        for (; (s + 4) * 16 + 16 <= end; s += 8) group(s, integral_constant<int, 2>(), std::true_type());
+        if (s * 16 + 16 <= end) { group(s, integral_constant<int, 1>(), std::true_type()); s += 4; }
+    }
+    for (; s < s1; s += 4) group(s, integral_constant<int, 1>(), std::false_type());
+    // wave q ends quarter q: 8 q + 4 half + e of 32, a lane two columns
+    const float scale = a.part ? 1.f : *a.scale;
+    int turn = 0;
+    auto join = [&](const v16f& c) {
+        float(*t)[4][64][4] = meet[turn];
+        turn ^= 1;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) *(v4f*)t[wave][q][lane] = v4f{c[q * 4], c[q * 4 + 1], c[q * 4 + 2], c[q * 4 + 3]};
+        __syncthreads();                                      // (two buffers: one barrier a turn)
+        return (*(const v4f*)t[0][wave][lane] + *(const v4f*)t[1][wave][lane]) + (*(const v4f*)t[2][wave][lane] + *(const v4f*)t[3][wave][lane]);
+    };
+#pragma unroll
+    for (int i = 0; i < NM; ++i) {
+        const v4f c0 = join(acc[i][0]), c1 = join(acc[i][1]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int64_t m = m0 + (wave * 8 + half * 4 + e) * NM + i;
+            if (m >= M || left <= 0) continue;
+            if (a.part) store_n<float, 2>(a.part + ((int64_t)blockIdx.z * (ROWS ? a.N : a.V) + m) * a.D + d, Pack<float, 2>{{c0[e], c1[e]}}, left);
+            else if (a.out) store_n<X, 2>((X*)a.out + (ROWS ? a.idx[m] : m) * a.D + d, Pack<X, 2>{{(X)(c0[e] * scale), (X)(c1[e] * scale)}}, left);
+        }
+        if (col) {
+            const v4f c = join(ones[i]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int64_t m = m0 + (wave * 8 + half * 4 + e) * NM + i;
-                if (m >= M || left <= 0) continue;
-                if (a.part) store_n<float, 2>(a.part + ((int64_t)blockIdx.z * (ROWS ? a.N : a.V) + m) * a.D + d, Pack<float, 2>{{c0[e], c1[e]}}, left);
-                else if (a.out) store_n<X, 2>((X*)a.out + (ROWS ? a.idx[m] : m) * a.D + d, Pack<X, 2>{{(X)(c0[e] * scale), (X)(c1[e] * scale)}}, left);
-            }
-            if (col) {
-                const v4f c = join(ones[i]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int64_t m = m0 + (wave * 8 + half * 4 + e) * NM + i;
-                    if (at || m >= M) continue;
-                    if (a.part) a.colpart[(int64_t)blockIdx.z * a.V + m] = c[e];
-                    else store_any(a.colout, a.ctype, m, c[e] * scale);
-                }
+                if (at || m >= M) continue;
+                if (a.part) a.colpart[(int64_t)blockIdx.z * a.V + m] = c[e];
+                else store_any(a.colout, a.ctype, m, c[e] * scale);
             }
         }
     }
+}
 
-    // dx of a small table: W's fragments of 64 columns (all KS steps of k; 32 columns where an fp32 table has more than 64 outputs)
-    // stay in a wave's registers while it walks over tiles of 32 rows; the next tile's dz is under way meanwhile.  16000 x 59, D 512
-    // fp32: 22 us (the writing of dx alone: 6).
-    template <class X, int KS> __global__ void __launch_bounds__(256, 2) small_dx_kernel(SmallGradArgs a) {
-        using T = typename Half<X>::type;
-        constexpr int P = parts_of<X>(), NN = P == 3 && KS > 4 ? 1 : 2;
-        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, at = lane & 31;
-        const int live = *a.live, tiles = (live + 31) / 32, step = gridDim.y * 4;
-        int t = blockIdx.y * 4 + wave;
-        if (t >= tiles) return;
-        Pack<X, 8> zv[KS];
-        auto load = [&](int tile) {                               // (dz has KS * 16 outputs, zeros behind the last; behind the last row: another row)
-            const X* z = (const X*)((const char*)a.dz + (uint64_t)(uint32_t)min(tile * 32 + at, live - 1) * a.zld) + half * 8;
+// dx of a small table: W's fragments of 64 columns (all KS steps of k; 32 columns where an fp32 table has more than 64 outputs)
+// stay in a wave's registers while it walks over tiles of 32 rows; the next tile's dz is under way meanwhile.  16000 x 59, D 512
+// fp32: 22 us (the writing of dx alone: 6).
+template <class X, int KS> __global__ void __launch_bounds__(256, 2) small_dx_kernel(SmallGradArgs a) {
+    using T = typename Half<X>::type;
+    constexpr int P = parts_of<X>(), NN = P == 3 && KS > 4 ? 1 : 2;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, at = lane & 31;
+    const int live = *a.live, tiles = (live + 31) / 32, step = gridDim.y * 4;
+    int t = blockIdx.y * 4 + wave;
+    if (t >= tiles) return;
+    Pack<X, 8> zv[KS];
+    auto load = [&](int tile) {                               // (dz has KS * 16 outputs, zeros behind the last; behind the last row: another row)
+        const X* z = (const X*)((const char*)a.dz + (uint64_t)(uint32_t)min(tile * 32 + at, live - 1) * a.zld) + half * 8;
 #pragma unroll
-            for (int u = 0; u < KS; ++u) zv[u] = load_n<X, 8>(z + u * 16, 8);
-        };
-        load(t);
-        const int d = (blockIdx.x * 32 + at) * NN, left = a.D - d;
-        const X* w = (const X*)a.b + min(d, a.D - 1);
-        const bool whole = (int)(blockIdx.x + 1) * 32 * NN <= a.D;
-        typename Mfma<T>::v8 wf[NN][KS][P];
-#pragma unroll
-        for (int u = 0; u < KS; ++u) {
-            Pack<X, 8> v[NN];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int k = u * 16 + half * 8 + e;
-                const X* p = (const X*)((const char*)w + (uint64_t)(uint32_t)min(k, a.V - 1) * a.ldb);
-                const auto q = whole ? load_n<X, NN>(p, NN) : load_n<X, NN>(p, left);
-#pragma unroll
-                for (int j = 0; j < NN; ++j) v[j].v[e] = k < a.V ? q.v[j] : (X)0.f;
-            }
-#pragma unroll
-            for (int j = 0; j < NN; ++j) split_frag<X>(v[j], wf[j][u]);
-        }
-        const float scale = *a.scale;
-        for (; t < tiles; t += step) {
-            v16f acc[NN];
-#pragma unroll
-            for (int j = 0; j < NN; ++j) acc[j] = v16f{};
-            typename Mfma<T>::v8 zf[KS][P];
-#pragma unroll
-            for (int u = 0; u < KS; ++u) split_frag<X>(zv[u], zf[u]);
-            if (t + step < tiles) load(t + step);
-#pragma unroll
-            for (int u = 0; u < KS; ++u)
-#pragma unroll
-                for (int j = 0; j < NN; ++j) {
-                    if constexpr (P == 3) {
-                        acc[j] = Mfma<T>::mul(zf[u][2], wf[j][u][0], acc[j]);
-                        acc[j] = Mfma<T>::mul(zf[u][1], wf[j][u][1], acc[j]);
-                        acc[j] = Mfma<T>::mul(zf[u][0], wf[j][u][2], acc[j]);
-                        acc[j] = Mfma<T>::mul(zf[u][1], wf[j][u][0], acc[j]);
-                        acc[j] = Mfma<T>::mul(zf[u][0], wf[j][u][1], acc[j]);
-                    }
-                    acc[j] = Mfma<T>::mul(zf[u][0], wf[j][u][0], acc[j]);
-                }
-            if (left <= 0) continue;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int m = t * 32 + e / 4 * 8 + half * 4 + e % 4;
-                if (m >= live) continue;
-                Pack<X, NN> o;
-#pragma unroll
-                for (int j = 0; j < NN; ++j) o.v[j] = (X)(acc[j][e] * scale);
-                store_n<X, NN>((X*)a.out + (int64_t)a.idx[m] * a.D + d, o, left);
-            }
-        }
-    }
-
-    // z - lse, from logits that are computed again: at D 512 that costs less than writing z, reading it and writing it once more (a
-    // pass over the box is 62 us at 16000 x 5001, the product 80).  Plain 4-byte stores: 32 lanes fill 128 bytes of a row, whose
-    // start is as unaligned as V is odd (16-byte stores of whole rows through LDS: 143 against 135 us, non-temporal ones: 203;
-    // 128 x 128 tiles, two workgroups a CU: 158).
-    struct LogProbArgs {
-        Product p;               // A = x, B = W: a lane is one output, 32 of them make 128 bytes of a row
-        Logits l;
-        const float* lse;
-        float* out;
-        int64_t N;
+        for (int u = 0; u < KS; ++u) zv[u] = load_n<X, 8>(z + u * 16, 8);
     };
-    template <class T, bool BIG> __global__ void __launch_bounds__(Shape<BIG>::kThreads, 2) log_prob_kernel(LogProbArgs a) {
-        using S = Shape<BIG>;
-        using Tl = Tile<T, S::BM, S::BN, S::WM, S::WN, false, false>;
-        char* lds = tile_lds;
-        __shared__ float bias[S::BN], lse[S::BM];
-        Tl t;
-        if (!t.place(a.p)) return;
-        stage_bias(a.l, t.tn * S::BN, S::BN, bias);
-        for (int i = threadIdx.x; i < S::BM; i += S::kThreads) {
-            const int64_t n = (int64_t)t.tm * S::BM + i;
-            const float v = n < a.N ? a.lse[n] : 0.f;
-            lse[i] = v == -INFINITY ? 0.f : v;                   // a row of -inf stays one
+    load(t);
+    const int d = (blockIdx.x * 32 + at) * NN, left = a.D - d;
+    const X* w = (const X*)a.b + min(d, a.D - 1);
+    const bool whole = (int)(blockIdx.x + 1) * 32 * NN <= a.D;
+    typename Mfma<T>::v8 wf[NN][KS][P];
+#pragma unroll
+    for (int u = 0; u < KS; ++u) {
+        Pack<X, 8> v[NN];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int k = u * 16 + half * 8 + e;
+            const X* p = (const X*)((const char*)w + (uint64_t)(uint32_t)min(k, a.V - 1) * a.ldb);
+            const auto q = whole ? load_n<X, NN>(p, NN) : load_n<X, NN>(p, left);
+#pragma unroll
+            for (int j = 0; j < NN; ++j) v[j].v[e] = k < a.V ? q.v[j] : (X)0.f;
         }
-        t.run(a.p, lds);
-        __syncthreads();
 #pragma unroll
-        for (int i = 0; i < Tl::MI; ++i)
+        for (int j = 0; j < NN; ++j) split_frag<X>(v[j], wf[j][u]);
+    }
+    const float scale = *a.scale;
+    for (; t < tiles; t += step) {
+        v16f acc[NN];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int64_t n = t.m(i, e);
-                if (n >= a.N) continue;
-                const float l = lse[n - (int64_t)t.tm * S::BM];
+        for (int j = 0; j < NN; ++j) acc[j] = v16f{};
+        typename Mfma<T>::v8 zf[KS][P];
 #pragma unroll
-                for (int j = 0; j < Tl::NI; ++j) {
-                    const int v = t.n(j);
-                    if (v < a.l.V) a.out[n * a.l.V + v] = t.acc[i][j][e] + bias[v - t.tn * S::BN] - l;
+        for (int u = 0; u < KS; ++u) split_frag<X>(zv[u], zf[u]);
+        if (t + step < tiles) load(t + step);
+#pragma unroll
+        for (int u = 0; u < KS; ++u)
+#pragma unroll
+            for (int j = 0; j < NN; ++j) {
+                if constexpr (P == 3) {
+                    acc[j] = Mfma<T>::mul(zf[u][2], wf[j][u][0], acc[j]);
+                    acc[j] = Mfma<T>::mul(zf[u][1], wf[j][u][1], acc[j]);
+                    acc[j] = Mfma<T>::mul(zf[u][0], wf[j][u][2], acc[j]);
+                    acc[j] = Mfma<T>::mul(zf[u][1], wf[j][u][0], acc[j]);
+                    acc[j] = Mfma<T>::mul(zf[u][0], wf[j][u][1], acc[j]);
                 }
+                acc[j] = Mfma<T>::mul(zf[u][0], wf[j][u][0], acc[j]);
             }
+        if (left <= 0) continue;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int m = t * 32 + e / 4 * 8 + half * 4 + e % 4;
+            if (m >= live) continue;
+            Pack<X, NN> o;
+#pragma unroll
+            for (int j = 0; j < NN; ++j) o.v[j] = (X)(acc[j][e] * scale);
+            store_n<X, NN>((X*)a.out + (int64_t)a.idx[m] * a.D + d, o, left);
+        }
     }
+}
 
-    struct DzArgs {
-        Product p;               // A = W's piece, B = the live rows of x
-        Logits l;
-        const int32_t* target;
-        const float *g, *lse;
-        float smoothing;
-        int32_t outputs;         // all of them, not the piece's
-        uint16_t* dz;            // [Npad][planes][pitch]
-        int64_t pitch;
-    };
-    // A wave's 32 rows n by 32 MI columns m, out of the accumulators' layout (a lane holds 4 neighbouring columns of one row: 16 or
-    // 8 bytes a request) into whole rows (512 or 256 neighbouring bytes), through 4 KB of LDS per 32 columns that only this wave
-    // uses: LDS serves a wave in order, no barrier is needed.  get(i, q): columns 32 i + 8 q + 4 (lane / 32) .. + 3 of row
-    // lane % 32; put(row, column, values).  Chunks are permuted by row against bank conflicts.
-    template <int MI, class G, class P> __device__ inline void rows_out(char* w, int lane, G&& get, P&& put) {
-        constexpr int C = MI * 8;                        // 16-byte chunks of a row
-        const int row = lane & 31;
-#pragma unroll
-        for (int i = 0; i < MI; ++i)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) *(v4f*)(w + row * (C * 16) + (((i * 8 + q * 2 + (lane >> 5)) ^ (row & (C - 1))) * 16)) = get(i, q);
-#pragma unroll
-        for (int k = 0; k < MI * 4; ++k) {
-            const int r = (k * 64 + lane) / C, c = (k * 64 + lane) % C;
-            put(r, c * 4, *(const v4f*)(w + r * (C * 16) + ((c ^ (r & (C - 1))) * 16)));
-        }
+// z - lse, from logits that are computed again: at D 512 that costs less than writing z, reading it and writing it once more (a
+// pass over the box is 62 us at 16000 x 5001, the product 80).  Plain 4-byte stores: 32 lanes fill 128 bytes of a row, whose
+// start is as unaligned as V is odd (16-byte stores of whole rows through LDS: 143 against 135 us, non-temporal ones: 203;
+// 128 x 128 tiles, two workgroups a CU: 158).
+struct LogProbArgs {
+    Product p;               // A = x, B = W: a lane is one output, 32 of them make 128 bytes of a row
+    Logits l;
+    const float* lse;
+    float* out;
+    int64_t N;
+};
+template <class T, bool BIG> __global__ void __launch_bounds__(Shape<BIG>::kThreads, 2) log_prob_kernel(LogProbArgs a) {
+    using S = Shape<BIG>;
+    using Tl = Tile<T, S::BM, S::BN, S::WM, S::WN, false, false>;
+    char* lds = tile_lds;
+    __shared__ float bias[S::BN], lse[S::BM];
+    Tl t;
+    if (!t.place(a.p)) return;
+    stage_bias(a.l, t.tn * S::BN, S::BN, bias);
+    for (int i = threadIdx.x; i < S::BM; i += S::kThreads) {
+        const int64_t n = (int64_t)t.tm * S::BM + i;
+        const float v = n < a.N ? a.lse[n] : 0.f;
+        lse[i] = v == -INFINITY ? 0.f : v;                   // a row of -inf stays one
     }
-    typedef uint16_t v4h __attribute__((ext_vector_type(4)));
-    typedef uint16_t v8h __attribute__((ext_vector_type(8)));
-    template <int MI, class G, class P> __device__ inline void rows_out16(char* w, int lane, G&& get, P&& put) {
-        constexpr int C = MI * 4;
-        const int row = lane & 31;
+    t.run(a.p, lds);
+    __syncthreads();
 #pragma unroll
-        for (int i = 0; i < MI; ++i)
+    for (int i = 0; i < Tl::MI; ++i)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) *(v4h*)(w + row * (C * 16) + (((i * 4 + q) ^ (row & (C - 1))) * 16) + (lane >> 5) * 8) = get(i, q);
+        for (int e = 0; e < 16; ++e) {
+            const int64_t n = t.m(i, e);
+            if (n >= a.N) continue;
+            const float l = lse[n - (int64_t)t.tm * S::BM];
 #pragma unroll
-        for (int k = 0; k < MI * 2; ++k) {
-            const int r = (k * 64 + lane) / C, c = (k * 64 + lane) % C;
-            put(r, c * 8, *(const v8h*)(w + r * (C * 16) + ((c ^ (r & (C - 1))) * 16)));
+            for (int j = 0; j < Tl::NI; ++j) {
+                const int v = t.n(j);
+                if (v < a.l.V) a.out[n * a.l.V + v] = t.acc[i][j][e] + bias[v - t.tn * S::BN] - l;
+            }
         }
+}
+
+struct DzArgs {
+    Product p;               // A = W's piece, B = the live rows of x
+    Logits l;
+    const int32_t* target;
+    const float *g, *lse;
+    float smoothing;
+    int32_t outputs;         // all of them, not the piece's
+    uint16_t* dz;            // [Npad][planes][pitch]
+    int64_t pitch;
+};
+// A wave's 32 rows n by 32 MI columns m, out of the accumulators' layout (a lane holds 4 neighbouring columns of one row: 16 or
+// 8 bytes a request) into whole rows (512 or 256 neighbouring bytes), through 4 KB of LDS per 32 columns that only this wave
+// uses: LDS serves a wave in order, no barrier is needed.  get(i, q): columns 32 i + 8 q + 4 (lane / 32) .. + 3 of row
+// lane % 32; put(row, column, values).  Chunks are permuted by row against bank conflicts.
+template <int MI, class G, class P> __device__ inline void rows_out(char* w, int lane, G&& get, P&& put) {
+    constexpr int C = MI * 8;                        // 16-byte chunks of a row
+    const int row = lane & 31;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) *(v4f*)(w + row * (C * 16) + (((i * 8 + q * 2 + (lane >> 5)) ^ (row & (C - 1))) * 16)) = get(i, q);
+#pragma unroll
+    for (int k = 0; k < MI * 4; ++k) {
+        const int r = (k * 64 + lane) / C, c = (k * 64 + lane) % C;
+        put(r, c * 4, *(const v4f*)(w + r * (C * 16) + ((c ^ (r & (C - 1))) * 16)));
     }
-    // d loss / d z of a piece of the outputs from logits that are computed again: g (p - (1 - e) [v = target] - e / V), rounded to
-    // the type of x for the products that follow (fp32: exact parts), as a 16-bit training step's stored gradients are.  The product
-    // once more and a box of 16 bits written: 14000 x 5001, D 512 bf16 108 us, of which 28 are that box at the rate of a copy.
-    template <class X, bool BIG> __global__ void __launch_bounds__(Shape<BIG>::kThreads, 2) dz_kernel(DzArgs a) {
-        using T = typename Half<X>::type;
-        using S = Shape<BIG>;
-        char* lds = tile_lds;
-        __shared__ __align__(16) float bias[S::BM];
+}
+typedef uint16_t v4h __attribute__((ext_vector_type(4)));
+typedef uint16_t v8h __attribute__((ext_vector_type(8)));
+template <int MI, class G, class P> __device__ inline void rows_out16(char* w, int lane, G&& get, P&& put) {
+    constexpr int C = MI * 4;
+    const int row = lane & 31;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) *(v4h*)(w + row * (C * 16) + (((i * 4 + q) ^ (row & (C - 1))) * 16) + (lane >> 5) * 8) = get(i, q);
+#pragma unroll
+    for (int k = 0; k < MI * 2; ++k) {
+        const int r = (k * 64 + lane) / C, c = (k * 64 + lane) % C;
+        put(r, c * 8, *(const v8h*)(w + r * (C * 16) + ((c ^ (r & (C - 1))) * 16)));
+    }
+}
+// d loss / d z of a piece of the outputs from logits that are computed again: g (p - (1 - e) [v = target] - e / V), rounded to
+// the type of x for the products that follow (fp32: exact parts), as a 16-bit training step's stored gradients are.  The product
+// once more and a box of 16 bits written: 14000 x 5001, D 512 bf16 108 us, of which 28 are that box at the rate of a copy.
+template <class X, bool BIG> __global__ void __launch_bounds__(Shape<BIG>::kThreads, 2) dz_kernel(DzArgs a) {
+    using T = typename Half<X>::type;
+    using S = Shape<BIG>;
+    char* lds = tile_lds;
+    __shared__ __align__(16) float bias[S::BM];
     with_tile<T, BIG>(a.p, [&](auto& t) {
         using Tl = std::remove_reference_t<decltype(t)>;
         stage_bias(a.l, t.tm * S::BM, S::BM, bias);
@@ -1837,446 +1838,447 @@ template <class T, bool BIG> __global__ void __launch_bounds__(Shape<BIG>::kThre
                     const float v[4] = {d[0], d[1], d[2], d[3]};
                     if (first + m < a.pitch) store_dz4<X>(a.dz + (int64_t)(row0 + r) * parts_of<X>() * a.pitch, a.pitch, first + m, v);
                 });
-        }    });
-    }
+        }
+    });
+}
 
-    struct GradArgs {
-        Product p;
-        int32_t M;               // columns (features) that exist
-        int64_t N;               // rows that exist
-        float* part;             // [splits][N][M] sums, or NULL: straight to out
-        int32_t add;             // ... added to what is there
-        float* colpart;          // [splits][N] sums of B's rows (the bias' gradient), or NULL
-        const float* scale;
-        void* out;               // [.][M]
-        int32_t otype;
-        const int32_t* idx;      // row of out, or NULL
-        void* colout;
-        int32_t ctype;
-    };
-    // C[n][m] for a gradient: m runs along features (registers: 4 neighbours), n along rows of x or of W.  14000 x 5001, D 512 bf16: dx
-    // 99 us, dW 85.
-    template <class T, bool BIG, bool BK, bool COLSUM> __global__ void __launch_bounds__(Shape<BIG>::kThreads, 2) grad_kernel(GradArgs a) {
-        using S = Shape<BIG>;
-        using Tl = Tile<T, S::BM, S::BN, S::WM, S::WN, true, BK, COLSUM>;
-        char* lds = tile_lds;
-        Tl t;
-        if (!t.place(a.p)) return;
-        t.run(a.p, lds);
-        const float scale = a.part ? 1.f : *a.scale;
-        const int64_t N = a.p.live && !a.p.live_is_k ? min(a.N, (int64_t)t.live) : a.N;
-        const int first = t.m(0, 0) - 4 * (t.lane >> 5);
-        __syncthreads();
-        char* mine = lds + (t.wm + t.wn * S::WM) * 16384;
+struct GradArgs {
+    Product p;
+    int32_t M;               // columns (features) that exist
+    int64_t N;               // rows that exist
+    float* part;             // [splits][N][M] sums, or NULL: straight to out
+    int32_t add;             // ... added to what is there
+    float* colpart;          // [splits][N] sums of B's rows (the bias' gradient), or NULL
+    const float* scale;
+    void* out;               // [.][M]
+    int32_t otype;
+    const int32_t* idx;      // row of out, or NULL
+    void* colout;
+    int32_t ctype;
+};
+// C[n][m] for a gradient: m runs along features (registers: 4 neighbours), n along rows of x or of W.  14000 x 5001, D 512 bf16: dx
+// 99 us, dW 85.
+template <class T, bool BIG, bool BK, bool COLSUM> __global__ void __launch_bounds__(Shape<BIG>::kThreads, 2) grad_kernel(GradArgs a) {
+    using S = Shape<BIG>;
+    using Tl = Tile<T, S::BM, S::BN, S::WM, S::WN, true, BK, COLSUM>;
+    char* lds = tile_lds;
+    Tl t;
+    if (!t.place(a.p)) return;
+    t.run(a.p, lds);
+    const float scale = a.part ? 1.f : *a.scale;
+    const int64_t N = a.p.live && !a.p.live_is_k ? min(a.N, (int64_t)t.live) : a.N;
+    const int first = t.m(0, 0) - 4 * (t.lane >> 5);
+    __syncthreads();
+    char* mine = lds + (t.wm + t.wn * S::WM) * 16384;
 #pragma unroll
-        for (int j = 0; j < Tl::NI; ++j) {
-            const int n0 = t.n(j) - (t.lane & 31);
-            if constexpr (COLSUM) {
-                const int n = t.n(j);
-                if ((a.colpart || a.colout) && t.tm == 0 && t.wm == 0 && t.lane < 32 && n < N) {
-                    if (a.part) a.colpart[(int64_t)t.split * a.N + n] = t.colsum[j][0];
-                    else store_any(a.colout, a.ctype, n, t.colsum[j][0] * *a.scale);
-                }
+    for (int j = 0; j < Tl::NI; ++j) {
+        const int n0 = t.n(j) - (t.lane & 31);
+        if constexpr (COLSUM) {
+            const int n = t.n(j);
+            if ((a.colpart || a.colout) && t.tm == 0 && t.wm == 0 && t.lane < 32 && n < N) {
+                if (a.part) a.colpart[(int64_t)t.split * a.N + n] = t.colsum[j][0];
+                else store_any(a.colout, a.ctype, n, t.colsum[j][0] * *a.scale);
             }
-            rows_out<Tl::MI>(mine, t.lane, [&](int i, int q) {
-                return v4f{t.acc[i][j][q * 4], t.acc[i][j][q * 4 + 1], t.acc[i][j][q * 4 + 2], t.acc[i][j][q * 4 + 3]};
-            }, [&](int r, int k, v4f d) {
-                const int n = n0 + r, m = first + k, left = a.M - m;
-                if (n >= N || left <= 0) return;
-                if (a.part) {
-                    float* at = a.part + ((int64_t)t.split * a.N + n) * a.M + m;
+        }
+        rows_out<Tl::MI>(mine, t.lane, [&](int i, int q) {
+            return v4f{t.acc[i][j][q * 4], t.acc[i][j][q * 4 + 1], t.acc[i][j][q * 4 + 2], t.acc[i][j][q * 4 + 3]};
+        }, [&](int r, int k, v4f d) {
+            const int n = n0 + r, m = first + k, left = a.M - m;
+            if (n >= N || left <= 0) return;
+            if (a.part) {
+                float* at = a.part + ((int64_t)t.split * a.N + n) * a.M + m;
+                Pack<float, 4> v;
+                if (a.add) v = load_n<float, 4>(at, left);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v.v[e] = (a.add ? v.v[e] : 0.f) + d[e];
+                store_n<float, 4>(at, v, left);
+            } else {
+                const int64_t at = (a.idx ? a.idx[n] : n) * (int64_t)a.M + m;
+                if (a.otype == WF_F32) {
                     Pack<float, 4> v;
-                    if (a.add) v = load_n<float, 4>(at, left);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v.v[e] = (a.add ? v.v[e] : 0.f) + d[e];
-                    store_n<float, 4>(at, v, left);
+                    for (int e = 0; e < 4; ++e) v.v[e] = d[e] * scale;
+                    store_n<float, 4>((float*)a.out + at, v, left);
                 } else {
-                    const int64_t at = (a.idx ? a.idx[n] : n) * (int64_t)a.M + m;
-                    if (a.otype == WF_F32) {
-                        Pack<float, 4> v;
+                    Pack<T, 4> v;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) v.v[e] = d[e] * scale;
-                        store_n<float, 4>((float*)a.out + at, v, left);
-                    } else {
-                        Pack<T, 4> v;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) v.v[e] = (T)(d[e] * scale);
-                        store_n<T, 4>((T*)a.out + at, v, left);
-                    }
+                    for (int e = 0; e < 4; ++e) v.v[e] = (T)(d[e] * scale);
+                    store_n<T, 4>((T*)a.out + at, v, left);
                 }
-            });
-        }
+            }
+        });
     }
+}
 
-    // out[row(n)][m] = scale * sum over splits of part[s][n][m], and the same for the column sums (dW of 5001 x 512 in its splits: 14
-    // us, a read of what the product wrote)
-    struct FoldArgs {
-        const float *part, *colpart, *scale;
-        int32_t splits, M;
-        int64_t N;
-        const int32_t *live, *idx;
-        void *out, *colout;
-        int32_t otype, ctype;
-    };
-    __global__ void __launch_bounds__(256) fold_kernel(FoldArgs a) {
-        const int64_t N = a.live ? min(a.N, (int64_t)*a.live) : a.N;
-        const float scale = *a.scale;
-        const int64_t all = N * a.M, stride = a.N * a.M;
-        auto put = [&](int64_t k, float v) { store_any(a.out, a.otype, a.idx ? a.idx[k / a.M] * (int64_t)a.M + k % a.M : k, v * scale); };
-        if (a.splits >= 16) {
-            // few elements, many parts: 32 elements a workgroup, each summed by 8 threads that meet in LDS
-            __shared__ float s[8][32];
-            const int c = threadIdx.x & 31, q = threadIdx.x >> 5;
-            for (int64_t i0 = (int64_t)blockIdx.x * 32; i0 < all; i0 += (int64_t)gridDim.x * 32) {
-                const int64_t i = i0 + c;
-                float v = 0.f;
-                if (i < all)
+// out[row(n)][m] = scale * sum over splits of part[s][n][m], and the same for the column sums (dW of 5001 x 512 in its splits: 14
+// us, a read of what the product wrote)
+struct FoldArgs {
+    const float *part, *colpart, *scale;
+    int32_t splits, M;
+    int64_t N;
+    const int32_t *live, *idx;
+    void *out, *colout;
+    int32_t otype, ctype;
+};
+__global__ void __launch_bounds__(256) fold_kernel(FoldArgs a) {
+    const int64_t N = a.live ? min(a.N, (int64_t)*a.live) : a.N;
+    const float scale = *a.scale;
+    const int64_t all = N * a.M, stride = a.N * a.M;
+    auto put = [&](int64_t k, float v) { store_any(a.out, a.otype, a.idx ? a.idx[k / a.M] * (int64_t)a.M + k % a.M : k, v * scale); };
+    if (a.splits >= 16) {
+        // few elements, many parts: 32 elements a workgroup, each summed by 8 threads that meet in LDS
+        __shared__ float s[8][32];
+        const int c = threadIdx.x & 31, q = threadIdx.x >> 5;
+        for (int64_t i0 = (int64_t)blockIdx.x * 32; i0 < all; i0 += (int64_t)gridDim.x * 32) {
+            const int64_t i = i0 + c;
+            float v = 0.f;
+            if (i < all)
 #pragma unroll 8
-                    for (int k = q; k < a.splits; k += 8) v += a.part[k * stride + i];
-                s[q][c] = v;
-                __syncthreads();
-                if (q == 0 && i < all) put(i, ((s[0][c] + s[1][c]) + (s[2][c] + s[3][c])) + ((s[4][c] + s[5][c]) + (s[6][c] + s[7][c])));
-                __syncthreads();
-            }
-        } else {
-            for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < all; i += (int64_t)gridDim.x * 1024) {
-                const int left = (int)min((int64_t)4, all - i);
-                Pack<float, 4> v = load_n<float, 4>(a.part + i, left);
-                for (int s = 1; s < a.splits; ++s) {
-                    const auto w = load_n<float, 4>(a.part + s * stride + i, left);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v.v[e] += w.v[e];
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (e < left) put(i + e, v.v[e]);
-            }
-        }
-        if (a.colout)                      // a wave a column sum
-            for (int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); n < N; n += (int64_t)gridDim.x * 4) {
-                float v = 0.f;
-                for (int s = threadIdx.x & 63; s < a.splits; s += 64) v += a.colpart[s * a.N + n];
-                v = wave_sum(v);
-                if ((threadIdx.x & 63) == 0) store_any(a.colout, a.ctype, n, v * scale);
-            }
-    }
-
-    // ---- the gradient that comes into log-probabilities -----------------------------------------------------------------
-    // Which rows of G hold anything: peak[n] = 0 where all of it is zero.  FULL: the largest magnitude (infinite where something is
-    // no number); else some value that is not 0, and a row is read up to its first one.  A wave a row.  16000 x 5001, an eighth of the
-    // rows zero: 25 us, the reading of those.
-    template <bool FULL> __global__ void __launch_bounds__(256) grad_rows_kernel(const float* G, int64_t ldg, int64_t N, int V, float* peak) {
-        const int lane = threadIdx.x & 63;
-        const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-        if (n >= N) return;
-        const float* g = G + n * ldg;
-        float m = 0.f;
-        auto look = [&](int v) {
-            const auto q = load_n<float, 4>(g + v + lane * 4, V - v - lane * 4);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) m = fmaxf(m, q.v[e] != q.v[e] ? INFINITY : fabsf(q.v[e]));
-        };
-        look(0);
-        for (int v = 256; v < V && (FULL || !__any(m != 0.f)); v += 2048)
-#pragma unroll
-            for (int u = 0; u < 8; ++u)
-                if (v + u * 256 < V) look(v + u * 256);
-        m = wave_max(m);
-        if (lane == 0) peak[n] = m;
-    }
-    // dz = G - exp(lp) sum(G) of the live rows, packed.  TPR threads a row, which stays in registers between its sum and its result
-    // (R pieces of 4 a thread); R = 0: rows that do not fit are read twice.  Bound by HBM: 14000 of 16000 x 5001 to bf16 149 us (4.7
-    // TB/s).
-    struct LogDzArgs {
-        const float *G, *lp, *scale;
-        int64_t ldg;
-        const int32_t *live, *idx;
-        int32_t V, plain;        // plain: rows of X, for small_grad_kernel
-        uint16_t* dz;
-        int64_t pitch;
-    };
-    template <class X, int TPR, int R> __global__ void __launch_bounds__(256) log_dz_kernel(LogDzArgs a) {
-        __shared__ float part[4];
-        const int t = threadIdx.x % TPR;
-        const int64_t c = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
-        const int live = *a.live;
-        if (c >= (int64_t)(live + kRowPad - 1) / kRowPad * kRowPad) return;      // (256 rows, whole workgroups)
-        uint16_t* row = a.dz + c * parts_of<X>() * a.pitch;
-        const bool in = c < live;
-        const int64_t n = in ? a.idx[c] : 0;
-        const float* g = a.G + n * a.ldg;
-        const float* lp = a.lp + n * a.V;
-        const int V = in ? a.V : 0;
-        const float inv = 1.f / *a.scale;
-        Pack<float, 4> gv[R ? R : 1], lv[R ? R : 1];
-        float s = 0.f;
-        if constexpr (R > 0) {
-#pragma unroll
-            for (int i = 0; i < R; ++i) gv[i] = load_n<float, 4>(g + (i * TPR + t) * 4, V - (i * TPR + t) * 4);
-#pragma unroll
-            for (int i = 0; i < R; ++i) lv[i] = load_n<float, 4>(lp + (i * TPR + t) * 4, V - (i * TPR + t) * 4);
-#pragma unroll
-            for (int i = 0; i < R; ++i) s += (gv[i].v[0] + gv[i].v[1]) + (gv[i].v[2] + gv[i].v[3]);
-        } else {
-            for (int v = t * 4; v < V; v += TPR * 4) {
-                const auto q = load_n<float, 4>(g + v, V - v);
-                s += (q.v[0] + q.v[1]) + (q.v[2] + q.v[3]);
-            }
-        }
-        s = wave_sum(s);
-        if constexpr (TPR > 64) {
-            if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+                for (int k = q; k < a.splits; k += 8) v += a.part[k * stride + i];
+            s[q][c] = v;
             __syncthreads();
-            s = (part[0] + part[1]) + (part[2] + part[3]);
+            if (q == 0 && i < all) put(i, ((s[0][c] + s[1][c]) + (s[2][c] + s[3][c])) + ((s[4][c] + s[5][c]) + (s[6][c] + s[7][c])));
+            __syncthreads();
         }
-        auto put = [&](int v, const Pack<float, 4>& q, const Pack<float, 4>& l) {
-            float d[4];
+    } else {
+        for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < all; i += (int64_t)gridDim.x * 1024) {
+            const int left = (int)min((int64_t)4, all - i);
+            Pack<float, 4> v = load_n<float, 4>(a.part + i, left);
+            for (int s = 1; s < a.splits; ++s) {
+                const auto w = load_n<float, 4>(a.part + s * stride + i, left);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) d[e] = v + e < V ? (q.v[e] - __expf(l.v[e]) * s) * inv : 0.f;
-            if (v >= a.pitch) return;
-            if (std::is_same<X, float>::value && a.plain) __builtin_memcpy((float*)a.dz + c * a.pitch + v, d, 16);
-            else store_dz4<X>(row, a.pitch, v, d);
-        };
-        if constexpr (R > 0) {
+                for (int e = 0; e < 4; ++e) v.v[e] += w.v[e];
+            }
 #pragma unroll
-            for (int i = 0; i < R; ++i) put((i * TPR + t) * 4, gv[i], lv[i]);
-        } else {
-            for (int v = t * 4; v < a.pitch; v += TPR * 4) put(v, load_n<float, 4>(g + v, V - v), load_n<float, 4>(lp + v, V - v));
+            for (int e = 0; e < 4; ++e)
+                if (e < left) put(i + e, v.v[e]);
         }
     }
-
-    // ---- host side --------------------------------------------------------------------------------------------------------
-    namespace {
-    constexpr size_t kPieceBytes = (size_t)256 << 20;      // gradients of logits in hand at a time: what the last-level cache holds
-
-    int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-    int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
-
-    // Tile shape and K splits of a product of m x n over `its` K tiles.  256 x 256 tiles run one per CU at 1.15 times the rate of
-    // 128 x 128 tiles, which run two per CU (measured at 5120 x 16384 x 512: 926 against 837 TFLOP/s; 4096^3: 1172 / 983); the
-    // cheaper of both by rounds of the chip is taken.  A product that does not fill the chip is split over K while a split
-    // keeps 8 K tiles.  A tile's prologue and epilogue cost about 6 K tiles, 12 where it writes partial sums (gradients of cross entropy,
-    // 14400 x 5001, D 512, bf16: 331 us with 6 for both, 310 - 316 with 10 - 20; 1000 rows 70.9, 71.2 - 67.7).
-    struct Grid { bool big; int mt, nt, splits; };
-    Grid plan_grid(int64_t m, int64_t n, int64_t its, bool may_split) {
-        Grid best = {};
-        double least = 0;
-        for (int big = 0; big < 2; ++big) {
-            const int64_t b = big ? 256 : 128, mt = ceil_div(m, b), nt = ceil_div(n, b);
-            const int64_t slots = big ? kCUs : 2 * kCUs;
-            for (int64_t s = 1; s == 1 || (may_split && s <= 128 && its / s >= 8); ++s) {
-                const double cost = (double)ceil_div(mt * nt * s, slots) * (big ? 4.0 : 2 * 1.15) * (double)(ceil_div(its, s) + (s > 1 ? 12 : 6));
-                if (least == 0 || cost < least) { least = cost; best = {big != 0, (int)mt, (int)nt, (int)s}; }
-            }
+    if (a.colout)                      // a wave a column sum
+        for (int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); n < N; n += (int64_t)gridDim.x * 4) {
+            float v = 0.f;
+            for (int s = threadIdx.x & 63; s < a.splits; s += 64) v += a.colpart[s * a.N + n];
+            v = wave_sum(v);
+            if ((threadIdx.x & 63) == 0) store_any(a.colout, a.ctype, n, v * scale);
         }
-        return best;
-    }
+}
 
-    struct Arena {               // carves the workspace; with base == NULL it only counts
-        char* base;
-        size_t used = 0;
-        template <class T> T* take(size_t n) {
-            T* p = base ? (T*)(base + used) : nullptr;
-            used = (used + n * sizeof(T) + 255) & ~(size_t)255;
-            return p;
-        }
+// ---- the gradient that comes into log-probabilities -----------------------------------------------------------------
+// Which rows of G hold anything: peak[n] = 0 where all of it is zero.  FULL: the largest magnitude (infinite where something is
+// no number); else some value that is not 0, and a row is read up to its first one.  A wave a row.  16000 x 5001, an eighth of the
+// rows zero: 25 us, the reading of those.
+template <bool FULL> __global__ void __launch_bounds__(256) grad_rows_kernel(const float* G, int64_t ldg, int64_t N, int V, float* peak) {
+    const int lane = threadIdx.x & 63;
+    const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (n >= N) return;
+    const float* g = G + n * ldg;
+    float m = 0.f;
+    auto look = [&](int v) {
+        const auto q = load_n<float, 4>(g + v + lane * 4, V - v - lane * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = fmaxf(m, q.v[e] != q.v[e] ? INFINITY : fabsf(q.v[e]));
     };
-
-    // Straight from memory (small_kernel, small_grad_kernel, small_dx_kernel) or by tiles: a table of at most 128 outputs (gradients in
-    // 16 bits: 64) is always small, else the work decides.  us, small / tiles, at N of V 5001, D 512 unless said:
-    //   log-probabilities: fp32 1: 15 / 74, 256: 36 / 83, 512: 57 / 87, 1024: 99 / 107; bf16 1: 9.5 / 20, 64: 13 / 24, 256: 22 / 24,
-    //     512: 35 / 26; of V 15001, D 1024: fp32 64: 47 / 172, 512: 256 / 241, bf16 64: 27 / 38, 256: 78 / 45
-    //   gradients of cross entropy: fp32 8: 36 / 75, 256: 72 / 104, 512: 109 / 122; bf16 8: 24 / 38, 128: 35 / 43, 256: 45 / 46, 512:
-    //     65 / 55; of V 15001, D 1024: fp32 64: 104 / 169, 256: 267 / 246, bf16 64: 67 / 62; of V 59: 16000: fp32 67 / 115, bf16 48 / 57,
-    //     100000: 279 / 580, 174 / 212; of V 128: 16000: 99 / 123, 66 / 59
-    constexpr int kSmallOutputs = 128;
-    constexpr double kSmallWork = 0.7e9, kSmallWorkF32 = 1.6e9;      // N V D
-    bool is_small(int64_t N, int32_t D, int32_t V, int type, bool bwd) {
-        if (bwd && (size_t)N * round_up(V, 64) * (type == WF_F32 ? 4 : 2) > kPieceBytes) return false;
-        if (V <= (bwd && type != WF_F32 ? kSmallOutputs / 2 : kSmallOutputs)) return N <= (1 << 21) - 64;      // (workgroups in a launch's second dimension)
-        return N <= 65535 && (double)N * V * D <= (type == WF_F32 ? kSmallWorkF32 : kSmallWork);
+    look(0);
+    for (int v = 256; v < V && (FULL || !__any(m != 0.f)); v += 2048)
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (v + u * 256 < V) look(v + u * 256);
+    m = wave_max(m);
+    if (lane == 0) peak[n] = m;
+}
+// dz = G - exp(lp) sum(G) of the live rows, packed.  TPR threads a row, which stays in registers between its sum and its result
+// (R pieces of 4 a thread); R = 0: rows that do not fit are read twice.  Bound by HBM: 14000 of 16000 x 5001 to bf16 149 us (4.7
+// TB/s).
+struct LogDzArgs {
+    const float *G, *lp, *scale;
+    int64_t ldg;
+    const int32_t *live, *idx;
+    int32_t V, plain;        // plain: rows of X, for small_grad_kernel
+    uint16_t* dz;
+    int64_t pitch;
+};
+template <class X, int TPR, int R> __global__ void __launch_bounds__(256) log_dz_kernel(LogDzArgs a) {
+    __shared__ float part[4];
+    const int t = threadIdx.x % TPR;
+    const int64_t c = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    const int live = *a.live;
+    if (c >= (int64_t)(live + kRowPad - 1) / kRowPad * kRowPad) return;      // (256 rows, whole workgroups)
+    uint16_t* row = a.dz + c * parts_of<X>() * a.pitch;
+    const bool in = c < live;
+    const int64_t n = in ? a.idx[c] : 0;
+    const float* g = a.G + n * a.ldg;
+    const float* lp = a.lp + n * a.V;
+    const int V = in ? a.V : 0;
+    const float inv = 1.f / *a.scale;
+    Pack<float, 4> gv[R ? R : 1], lv[R ? R : 1];
+    float s = 0.f;
+    if constexpr (R > 0) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) gv[i] = load_n<float, 4>(g + (i * TPR + t) * 4, V - (i * TPR + t) * 4);
+#pragma unroll
+        for (int i = 0; i < R; ++i) lv[i] = load_n<float, 4>(lp + (i * TPR + t) * 4, V - (i * TPR + t) * 4);
+#pragma unroll
+        for (int i = 0; i < R; ++i) s += (gv[i].v[0] + gv[i].v[1]) + (gv[i].v[2] + gv[i].v[3]);
+    } else {
+        for (int v = t * 4; v < V; v += TPR * 4) {
+            const auto q = load_n<float, 4>(g + v, V - v);
+            s += (q.v[0] + q.v[1]) + (q.v[2] + q.v[3]);
+        }
     }
-    // A product of small_grad_kernel that has fewer than 4 workgroups per CU is split over k while a wave keeps 4 steps.
-    int small_splits(int64_t mt, int64_t D, int64_t K) {
-        const int64_t tiles = std::max<int64_t>(1, mt) * ceil_div(D, 64);
-        return (int)std::max<int64_t>(1, std::min<int64_t>({4 * kCUs / tiles, ceil_div(K, 16 * 16), 128}));
+    s = wave_sum(s);
+    if constexpr (TPR > 64) {
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+        __syncthreads();
+        s = (part[0] + part[1]) + (part[2] + part[3]);
     }
-    int small_mv(int32_t V) { return V <= 32 || V > kSmallOutputs ? 1 : V <= 64 ? 2 : 4; }
-
-    enum { kLogFwd = 0, kLogBwd = 1, kCeFwd = 2, kCeBwd = 3 };
-    struct LinearPlan {
-        int what, D, V, type, parts, Dp;
-        int64_t N, Npad, pitch, width;      // width: outputs of a piece, pitch: its padded row
-        int pieces;
-        bool small;
-        int sx, sw;                         // K splits of small_grad_kernel
-        Grid fwd, logp, dz, dx, dw;
-        Rows rows;
-        int32_t* count;
-        float* most;
-        uint16_t *xp, *wp, *dzp;
-        float *top, *sum, *all, *zt, *share, *gpeak, *part_x, *part_w, *part_c;
-        size_t bytes;
+    auto put = [&](int v, const Pack<float, 4>& q, const Pack<float, 4>& l) {
+        float d[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[e] = v + e < V ? (q.v[e] - __expf(l.v[e]) * s) * inv : 0.f;
+        if (v >= a.pitch) return;
+        if (std::is_same<X, float>::value && a.plain) __builtin_memcpy((float*)a.dz + c * a.pitch + v, d, 16);
+        else store_dz4<X>(row, a.pitch, v, d);
     };
-    int make_linear_plan(int what, int64_t N, int32_t D, int32_t V, int32_t type, void* ws, LinearPlan* out) {
-        if (!known_type(type)) return wf_fail(WF_EINVAL, "wf_linear: unknown element type");
-        if (N < 0 || D < 1 || V < 1) return wf_fail(WF_EINVAL, "wf_linear: bad size (N %lld, D %d, V %d)", (long long)N, D, V);
-        // (a tile's offsets are 32 bits: 256 rows of at most 2^22 x 2 bytes x 3 parts of an operand)
-        if (N > (1 << 30) || D > (1 << 20) || V > (1 << 21) || ceil_div(N, 128) * ceil_div(V, 128) > (1 << 29))
-            return wf_fail(WF_EUNSUPPORTED, "wf_linear: N %lld, D %d, V %d is beyond what one call takes", (long long)N, D, V);
-        LinearPlan p = {};
-        p.what = what; p.N = N; p.D = D; p.V = V; p.type = type;
-        p.parts = type == WF_F32 ? 3 : 1;
-        const int products = type == WF_F32 ? 6 : 1;
-        p.Dp = (int)round_up(D, kBK);
-        p.Npad = std::max<int64_t>(kRowPad, round_up(N, kRowPad));
-        const bool bwd = what == kLogBwd || what == kCeBwd;
-        Arena a = {(char*)ws};
-        p.small = is_small(N, D, V, type, bwd);
-        if (!bwd && p.small) {
-            if (V > kSmallOutputs) {
-                const size_t q = (size_t)ceil_div(V, 32) * N;
-                p.top = a.take<float>(q);
-                p.sum = a.take<float>(q);
-                p.all = a.take<float>(q);
-                p.zt = a.take<float>(N);
-            }
-            p.bytes = a.used + 256;
-            *out = p;
-            return WF_OK;
+    if constexpr (R > 0) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) put((i * TPR + t) * 4, gv[i], lv[i]);
+    } else {
+        for (int v = t * 4; v < a.pitch; v += TPR * 4) put(v, load_n<float, 4>(g + v, V - v), load_n<float, 4>(lp + v, V - v));
+    }
+}
+
+// ---- host side --------------------------------------------------------------------------------------------------------
+namespace {
+constexpr size_t kPieceBytes = (size_t)256 << 20;      // gradients of logits in hand at a time: what the last-level cache holds
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+
+// Tile shape and K splits of a product of m x n over `its` K tiles.  256 x 256 tiles run one per CU at 1.15 times the rate of
+// 128 x 128 tiles, which run two per CU (measured at 5120 x 16384 x 512: 926 against 837 TFLOP/s; 4096^3: 1172 / 983); the
+// cheaper of both by rounds of the chip is taken.  A product that does not fill the chip is split over K while a split
+// keeps 8 K tiles.  A tile's prologue and epilogue cost about 6 K tiles, 12 where it writes partial sums (gradients of cross entropy,
+// 14400 x 5001, D 512, bf16: 331 us with 6 for both, 310 - 316 with 10 - 20; 1000 rows 70.9, 71.2 - 67.7).
+struct Grid { bool big; int mt, nt, splits; };
+Grid plan_grid(int64_t m, int64_t n, int64_t its, bool may_split) {
+    Grid best = {};
+    double least = 0;
+    for (int big = 0; big < 2; ++big) {
+        const int64_t b = big ? 256 : 128, mt = ceil_div(m, b), nt = ceil_div(n, b);
+        const int64_t slots = big ? kCUs : 2 * kCUs;
+        for (int64_t s = 1; s == 1 || (may_split && s <= 128 && its / s >= 8); ++s) {
+            const double cost = (double)ceil_div(mt * nt * s, slots) * (big ? 4.0 : 2 * 1.15) * (double)(ceil_div(its, s) + (s > 1 ? 12 : 6));
+            if (least == 0 || cost < least) { least = cost; best = {big != 0, (int)mt, (int)nt, (int)s}; }
         }
-        p.rows.live = a.take<int32_t>(1);
-        p.rows.scale = a.take<float>(1);
-        p.count = a.take<int32_t>(ceil_div(N, kCountRows) + 1);
-        p.most = a.take<float>(ceil_div(N, kCountRows) + 1);
-        p.rows.idx = a.take<int32_t>(p.Npad);
-        p.rows.target = a.take<int32_t>(p.Npad);
-        p.rows.g = a.take<float>(p.Npad);
-        p.rows.lse = a.take<float>(p.Npad);
-        if (bwd && p.small) {
-            p.pitch = round_up(V, 64);
-            p.dzp = a.take<uint16_t>((size_t)p.Npad * p.pitch * (type == WF_F32 ? 2 : 1));
-            p.sx = V > kSmallOutputs ? small_splits(ceil_div(N, 32), D, V) : 1;
-            p.sw = small_splits(ceil_div(V, 64), D, N);
-            if (p.sx > 1) p.part_x = a.take<float>((size_t)p.sx * N * D);
-            if (p.sw > 1) p.part_w = a.take<float>((size_t)p.sw * V * D);
-            p.part_c = a.take<float>((size_t)p.sw * V);
-            if (what == kLogBwd) p.gpeak = a.take<float>(N);
-            p.bytes = a.used + 256;
-            *out = p;
-            return WF_OK;
-        }
-        p.xp = a.take<uint16_t>((size_t)p.Npad * p.parts * p.Dp);
-        p.wp = a.take<uint16_t>((size_t)V * p.parts * p.Dp);
-        const int64_t dits = (int64_t)products * p.Dp / kBK;
-        if (!bwd) {
-            p.fwd = plan_grid(V, N, dits, false);
-            p.logp = plan_grid(N, V, dits, false);
-            const size_t q = (size_t)p.fwd.mt * 2 * p.Npad;
+    }
+    return best;
+}
+
+struct Arena {               // carves the workspace; with base == NULL it only counts
+    char* base;
+    size_t used = 0;
+    template <class T> T* take(size_t n) {
+        T* p = base ? (T*)(base + used) : nullptr;
+        used = (used + n * sizeof(T) + 255) & ~(size_t)255;
+        return p;
+    }
+};
+
+// Straight from memory (small_kernel, small_grad_kernel, small_dx_kernel) or by tiles: a table of at most 128 outputs (gradients in
+// 16 bits: 64) is always small, else the work decides.  us, small / tiles, at N of V 5001, D 512 unless said:
+//   log-probabilities: fp32 1: 15 / 74, 256: 36 / 83, 512: 57 / 87, 1024: 99 / 107; bf16 1: 9.5 / 20, 64: 13 / 24, 256: 22 / 24,
+//     512: 35 / 26; of V 15001, D 1024: fp32 64: 47 / 172, 512: 256 / 241, bf16 64: 27 / 38, 256: 78 / 45
+//   gradients of cross entropy: fp32 8: 36 / 75, 256: 72 / 104, 512: 109 / 122; bf16 8: 24 / 38, 128: 35 / 43, 256: 45 / 46, 512:
+//     65 / 55; of V 15001, D 1024: fp32 64: 104 / 169, 256: 267 / 246, bf16 64: 67 / 62; of V 59: 16000: fp32 67 / 115, bf16 48 / 57,
+//     100000: 279 / 580, 174 / 212; of V 128: 16000: 99 / 123, 66 / 59
+constexpr int kSmallOutputs = 128;
+constexpr double kSmallWork = 0.7e9, kSmallWorkF32 = 1.6e9;      // N V D
+bool is_small(int64_t N, int32_t D, int32_t V, int type, bool bwd) {
+    if (bwd && (size_t)N * round_up(V, 64) * (type == WF_F32 ? 4 : 2) > kPieceBytes) return false;
+    if (V <= (bwd && type != WF_F32 ? kSmallOutputs / 2 : kSmallOutputs)) return N <= (1 << 21) - 64;      // (workgroups in a launch's second dimension)
+    return N <= 65535 && (double)N * V * D <= (type == WF_F32 ? kSmallWorkF32 : kSmallWork);
+}
+// A product of small_grad_kernel that has fewer than 4 workgroups per CU is split over k while a wave keeps 4 steps.
+int small_splits(int64_t mt, int64_t D, int64_t K) {
+    const int64_t tiles = std::max<int64_t>(1, mt) * ceil_div(D, 64);
+    return (int)std::max<int64_t>(1, std::min<int64_t>({4 * kCUs / tiles, ceil_div(K, 16 * 16), 128}));
+}
+int small_mv(int32_t V) { return V <= 32 || V > kSmallOutputs ? 1 : V <= 64 ? 2 : 4; }
+
+enum { kLogFwd = 0, kLogBwd = 1, kCeFwd = 2, kCeBwd = 3 };
+struct LinearPlan {
+    int what, D, V, type, parts, Dp;
+    int64_t N, Npad, pitch, width;      // width: outputs of a piece, pitch: its padded row
+    int pieces;
+    bool small;
+    int sx, sw;                         // K splits of small_grad_kernel
+    Grid fwd, logp, dz, dx, dw;
+    Rows rows;
+    int32_t* count;
+    float* most;
+    uint16_t *xp, *wp, *dzp;
+    float *top, *sum, *all, *zt, *share, *gpeak, *part_x, *part_w, *part_c;
+    size_t bytes;
+};
+int make_linear_plan(int what, int64_t N, int32_t D, int32_t V, int32_t type, void* ws, LinearPlan* out) {
+    if (!known_type(type)) return wf_fail(WF_EINVAL, "wf_linear: unknown element type");
+    if (N < 0 || D < 1 || V < 1) return wf_fail(WF_EINVAL, "wf_linear: bad size (N %lld, D %d, V %d)", (long long)N, D, V);
+    // (a tile's offsets are 32 bits: 256 rows of at most 2^22 x 2 bytes x 3 parts of an operand)
+    if (N > (1 << 30) || D > (1 << 20) || V > (1 << 21) || ceil_div(N, 128) * ceil_div(V, 128) > (1 << 29))
+        return wf_fail(WF_EUNSUPPORTED, "wf_linear: N %lld, D %d, V %d is beyond what one call takes", (long long)N, D, V);
+    LinearPlan p = {};
+    p.what = what; p.N = N; p.D = D; p.V = V; p.type = type;
+    p.parts = type == WF_F32 ? 3 : 1;
+    const int products = type == WF_F32 ? 6 : 1;
+    p.Dp = (int)round_up(D, kBK);
+    p.Npad = std::max<int64_t>(kRowPad, round_up(N, kRowPad));
+    const bool bwd = what == kLogBwd || what == kCeBwd;
+    Arena a = {(char*)ws};
+    p.small = is_small(N, D, V, type, bwd);
+    if (!bwd && p.small) {
+        if (V > kSmallOutputs) {
+            const size_t q = (size_t)ceil_div(V, 32) * N;
             p.top = a.take<float>(q);
             p.sum = a.take<float>(q);
-            if (what == kCeFwd) { p.all = a.take<float>(q); p.zt = a.take<float>(p.Npad); p.share = a.take<float>(p.Npad / 16); }
-            else p.zt = a.take<float>(p.Npad);            // lse
-        } else {
-            const int64_t fit = std::max<int64_t>(kRowPad, (int64_t)(kPieceBytes / ((size_t)p.Npad * p.parts * 2)) / kRowPad * kRowPad);
-            // (log-probabilities: their own box and their gradient's are four times a 16-bit one; its rows are read once)
-            p.pieces = what == kLogBwd ? 1 : (int)ceil_div(V, fit);
-            p.width = p.pitch = round_up(ceil_div(V, p.pieces), kRowPad);
-            p.pieces = (int)ceil_div(V, p.width);
-            p.dzp = a.take<uint16_t>((size_t)p.Npad * p.parts * p.pitch);
-            p.dz = plan_grid(p.width, N, dits, false);
-            p.dx = plan_grid(D, N, products * p.pitch / kBK, true);
-            p.dw = plan_grid(D, p.width, products * ceil_div(N, kBK), true);
-            if (p.dx.splits > 1 || p.pieces > 1) p.part_x = a.take<float>((size_t)p.dx.splits * N * D);
-            if (p.dw.splits > 1) p.part_w = a.take<float>((size_t)p.dw.splits * p.width * D);
-            p.part_c = a.take<float>((size_t)p.dw.splits * p.width);
-            if (what == kLogBwd) p.gpeak = a.take<float>(N);
+            p.all = a.take<float>(q);
+            p.zt = a.take<float>(N);
         }
         p.bytes = a.used + 256;
         *out = p;
         return WF_OK;
     }
-    int linear_plan_in(int what, int64_t N, int32_t D, int32_t V, int32_t type, void* ws, size_t bytes, LinearPlan* out) {
-        char* at = (char*)(((uintptr_t)ws + 255) & ~(uintptr_t)255);
-        int rc = make_linear_plan(what, N, D, V, type, at, out);
-        if (rc) return rc;
-        if (!ws || bytes < out->bytes) return wf_fail(WF_ENOSPC, "wf_linear: workspace too small (%zu B given, %zu B needed)", bytes, out->bytes);
+    p.rows.live = a.take<int32_t>(1);
+    p.rows.scale = a.take<float>(1);
+    p.count = a.take<int32_t>(ceil_div(N, kCountRows) + 1);
+    p.most = a.take<float>(ceil_div(N, kCountRows) + 1);
+    p.rows.idx = a.take<int32_t>(p.Npad);
+    p.rows.target = a.take<int32_t>(p.Npad);
+    p.rows.g = a.take<float>(p.Npad);
+    p.rows.lse = a.take<float>(p.Npad);
+    if (bwd && p.small) {
+        p.pitch = round_up(V, 64);
+        p.dzp = a.take<uint16_t>((size_t)p.Npad * p.pitch * (type == WF_F32 ? 2 : 1));
+        p.sx = V > kSmallOutputs ? small_splits(ceil_div(N, 32), D, V) : 1;
+        p.sw = small_splits(ceil_div(V, 64), D, N);
+        if (p.sx > 1) p.part_x = a.take<float>((size_t)p.sx * N * D);
+        if (p.sw > 1) p.part_w = a.take<float>((size_t)p.sw * V * D);
+        p.part_c = a.take<float>((size_t)p.sw * V);
+        if (what == kLogBwd) p.gpeak = a.take<float>(N);
+        p.bytes = a.used + 256;
+        *out = p;
         return WF_OK;
     }
+    p.xp = a.take<uint16_t>((size_t)p.Npad * p.parts * p.Dp);
+    p.wp = a.take<uint16_t>((size_t)V * p.parts * p.Dp);
+    const int64_t dits = (int64_t)products * p.Dp / kBK;
+    if (!bwd) {
+        p.fwd = plan_grid(V, N, dits, false);
+        p.logp = plan_grid(N, V, dits, false);
+        const size_t q = (size_t)p.fwd.mt * 2 * p.Npad;
+        p.top = a.take<float>(q);
+        p.sum = a.take<float>(q);
+        if (what == kCeFwd) { p.all = a.take<float>(q); p.zt = a.take<float>(p.Npad); p.share = a.take<float>(p.Npad / 16); }
+        else p.zt = a.take<float>(p.Npad);            // lse
+    } else {
+        const int64_t fit = std::max<int64_t>(kRowPad, (int64_t)(kPieceBytes / ((size_t)p.Npad * p.parts * 2)) / kRowPad * kRowPad);
+        // (log-probabilities: their own box and their gradient's are four times a 16-bit one; its rows are read once)
+        p.pieces = what == kLogBwd ? 1 : (int)ceil_div(V, fit);
+        p.width = p.pitch = round_up(ceil_div(V, p.pieces), kRowPad);
+        p.pieces = (int)ceil_div(V, p.width);
+        p.dzp = a.take<uint16_t>((size_t)p.Npad * p.parts * p.pitch);
+        p.dz = plan_grid(p.width, N, dits, false);
+        p.dx = plan_grid(D, N, products * p.pitch / kBK, true);
+        p.dw = plan_grid(D, p.width, products * ceil_div(N, kBK), true);
+        if (p.dx.splits > 1 || p.pieces > 1) p.part_x = a.take<float>((size_t)p.dx.splits * N * D);
+        if (p.dw.splits > 1) p.part_w = a.take<float>((size_t)p.dw.splits * p.width * D);
+        p.part_c = a.take<float>((size_t)p.dw.splits * p.width);
+        if (what == kLogBwd) p.gpeak = a.take<float>(N);
+    }
+    p.bytes = a.used + 256;
+    *out = p;
+    return WF_OK;
+}
+int linear_plan_in(int what, int64_t N, int32_t D, int32_t V, int32_t type, void* ws, size_t bytes, LinearPlan* out) {
+    char* at = (char*)(((uintptr_t)ws + 255) & ~(uintptr_t)255);
+    int rc = make_linear_plan(what, N, D, V, type, at, out);
+    if (rc) return rc;
+    if (!ws || bytes < out->bytes) return wf_fail(WF_ENOSPC, "wf_linear: workspace too small (%zu B given, %zu B needed)", bytes, out->bytes);
+    return WF_OK;
+}
 
-    void set_parts(Product* p, int type, int64_t aplane, int64_t bplane) {
-        static const int part_a[6] = {0, 0, 0, 1, 1, 2}, part_b[6] = {0, 1, 2, 0, 1, 0};
-        p->parts = type == WF_F32 ? 6 : 1;
-        for (int i = 0; i < 6; ++i) {
-            p->aoff[i] = (int32_t)(type == WF_F32 ? part_a[i] * aplane : 0);
-            p->boff[i] = (int32_t)(type == WF_F32 ? part_b[i] * bplane : 0);
+void set_parts(Product* p, int type, int64_t aplane, int64_t bplane) {
+    static const int part_a[6] = {0, 0, 0, 1, 1, 2}, part_b[6] = {0, 1, 2, 0, 1, 0};
+    p->parts = type == WF_F32 ? 6 : 1;
+    for (int i = 0; i < 6; ++i) {
+        p->aoff[i] = (int32_t)(type == WF_F32 ? part_a[i] * aplane : 0);
+        p->boff[i] = (int32_t)(type == WF_F32 ? part_b[i] * bplane : 0);
+    }
+}
+unsigned grid_of(const Product& p) { return (unsigned)(ceil_div((int64_t)p.mtiles * p.ntiles * p.splits, 8) * 8); }
+// A kernel over tiles.  Above 64 KB a kernel has to be told once per device how much LDS a launch may ask for.
+template <class S, auto kernel, class A> int launch_tiles(const A& args, hipStream_t st, unsigned spare = 0) {
+    if (S::kLds > 65536) {
+        static std::atomic<uint64_t> told{0};
+        int dev = 0;
+        HIP_TRY(hipGetDevice(&dev));
+        const uint64_t bit = (uint64_t)1 << (dev & 63);
+        if (!(told.load(std::memory_order_relaxed) & bit)) {
+            HIP_TRY(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds));
+            told.fetch_or(bit, std::memory_order_relaxed);
         }
     }
-    unsigned grid_of(const Product& p) { return (unsigned)(ceil_div((int64_t)p.mtiles * p.ntiles * p.splits, 8) * 8); }
-    // A kernel over tiles.  Above 64 KB a kernel has to be told once per device how much LDS a launch may ask for.
-    template <class S, auto kernel, class A> int launch_tiles(const A& args, hipStream_t st, unsigned spare = 0) {
-        if (S::kLds > 65536) {
-            static std::atomic<uint64_t> told{0};
-            int dev = 0;
-            HIP_TRY(hipGetDevice(&dev));
-            const uint64_t bit = (uint64_t)1 << (dev & 63);
-            if (!(told.load(std::memory_order_relaxed) & bit)) {
-                HIP_TRY(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds));
-                told.fetch_or(bit, std::memory_order_relaxed);
-            }
-        }
-        kernel<<<grid_of(args.p) + spare, S::kThreads, S::kLds, st>>>(args);
-        HIP_TRY(hipGetLastError());
-        return WF_OK;
-    }
-    template <class F> void with_half(int type, F&& f) { if (type == WF_F16) f(f16()); else f(bf16()); }
-    template <class F> void with_big(bool big, F&& f) { if (big) f(std::true_type()); else f(std::false_type()); }
+    kernel<<<grid_of(args.p) + spare, S::kThreads, S::kLds, st>>>(args);
+    HIP_TRY(hipGetLastError());
+    return WF_OK;
+}
+template <class F> void with_half(int type, F&& f) { if (type == WF_F16) f(f16()); else f(bf16()); }
+template <class F> void with_big(bool big, F&& f) { if (big) f(std::true_type()); else f(std::false_type()); }
 
-    bool direct_rows(const void* p, int64_t ld, int64_t D, int type) {   // usable as an operand where it lies
-        return type != WF_F32 && D % kBK == 0 && ld % 8 == 0 && ld <= (1 << 22) && (uintptr_t)p % 16 == 0;
+bool direct_rows(const void* p, int64_t ld, int64_t D, int type) {   // usable as an operand where it lies
+    return type != WF_F32 && D % kBK == 0 && ld % 8 == 0 && ld <= (1 << 22) && (uintptr_t)p % 16 == 0;
+}
+// Packs what has to be packed and places the rows; *w is W as an operand, where it lies or packed.
+int run_prep(const LinearPlan& p, PrepArgs a, const void* x, int64_t ldx, const void* w, int64_t ldw, hipStream_t st, Operand* wo) {
+    const bool direct = !p.wp || direct_rows(w, ldw, p.D, p.type);
+    if (direct) *wo = {w, ldw, p.V, p.Dp};
+    else *wo = {p.wp, (int64_t)p.parts * p.Dp, p.V, p.Dp};
+    a.r = p.rows; a.N = p.N; a.ldx = ldx; a.ldw = ldw; a.D = p.D; a.Dp = p.Dp; a.V = p.V; a.x = x; a.w = w;
+    a.wp = direct ? nullptr : p.wp;
+    a.row_blocks = a.xp || !a.all ? (int)ceil_div(p.N, kPrepRows) : 0;
+    a.tail_blocks = a.all ? 0 : kRowPad / kPrepRows;
+    const unsigned blocks = (unsigned)(a.row_blocks + a.tail_blocks + (direct ? 0 : ceil_div(p.V, kPrepRows)));
+    if (!blocks) return WF_OK;
+    if (!a.all && p.N > kCountedRows) {
+        a.count = p.count;
+        a.most = p.most;
+        count_kernel<<<(unsigned)ceil_div(p.N, kCountRows), kCountRows, 0, st>>>(a);
     }
-    // Packs what has to be packed and places the rows; *w is W as an operand, where it lies or packed.
-    int run_prep(const LinearPlan& p, PrepArgs a, const void* x, int64_t ldx, const void* w, int64_t ldw, hipStream_t st, Operand* wo) {
-        const bool direct = !p.wp || direct_rows(w, ldw, p.D, p.type);
-        if (direct) *wo = {w, ldw, p.V, p.Dp};
-        else *wo = {p.wp, (int64_t)p.parts * p.Dp, p.V, p.Dp};
-        a.r = p.rows; a.N = p.N; a.ldx = ldx; a.ldw = ldw; a.D = p.D; a.Dp = p.Dp; a.V = p.V; a.x = x; a.w = w;
-        a.wp = direct ? nullptr : p.wp;
-        a.row_blocks = a.xp || !a.all ? (int)ceil_div(p.N, kPrepRows) : 0;
-        a.tail_blocks = a.all ? 0 : kRowPad / kPrepRows;
-        const unsigned blocks = (unsigned)(a.row_blocks + a.tail_blocks + (direct ? 0 : ceil_div(p.V, kPrepRows)));
-        if (!blocks) return WF_OK;
-        if (!a.all && p.N > kCountedRows) {
-            a.count = p.count;
-            a.most = p.most;
-            count_kernel<<<(unsigned)ceil_div(p.N, kCountRows), kCountRows, 0, st>>>(a);
-        }
-        with_type(p.type, [&](auto t) { prep_kernel<decltype(t)><<<blocks, 256, 0, st>>>(a); });
-        HIP_TRY(hipGetLastError());
-        return WF_OK;
-    }
-    Operand packed_x(const LinearPlan& p) { return {p.xp, (int64_t)p.parts * p.Dp, (int32_t)p.Npad, p.Dp}; }
+    with_type(p.type, [&](auto t) { prep_kernel<decltype(t)><<<blocks, 256, 0, st>>>(a); });
+    HIP_TRY(hipGetLastError());
+    return WF_OK;
+}
+Operand packed_x(const LinearPlan& p) { return {p.xp, (int64_t)p.parts * p.Dp, (int32_t)p.Npad, p.Dp}; }
 
-    int linear_check(const char* who, const void* x, int64_t ldx, int64_t N, const void* w, int64_t ldw, const void* bias, int32_t btype) {
-        if (!w || (N > 0 && !x)) return wf_fail(WF_EINVAL, "%s: null pointer", who);
-        if (ldx < 0 || ldw < 0) return wf_fail(WF_EINVAL, "%s: negative row stride", who);
-        if (ldx >= (1 << 30) || ldw >= (1 << 30)) return wf_fail(WF_EUNSUPPORTED, "%s: row stride of 2^30 elements or more", who);
-        if (bias && !known_type(btype)) return wf_fail(WF_EINVAL, "%s: unknown element type", who);
-        return WF_OK;
-    }
+int linear_check(const char* who, const void* x, int64_t ldx, int64_t N, const void* w, int64_t ldw, const void* bias, int32_t btype) {
+    if (!w || (N > 0 && !x)) return wf_fail(WF_EINVAL, "%s: null pointer", who);
+    if (ldx < 0 || ldw < 0) return wf_fail(WF_EINVAL, "%s: negative row stride", who);
+    if (ldx >= (1 << 30) || ldw >= (1 << 30)) return wf_fail(WF_EUNSUPPORTED, "%s: row stride of 2^30 elements or more", who);
+    if (bias && !known_type(btype)) return wf_fail(WF_EINVAL, "%s: unknown element type", who);
+    return WF_OK;
+}
 
-    int run_stats(const LinearPlan& p, const Operand& w, const Operand& x, const void* bias, int btype, const int32_t* live,
-                  const int32_t* target, bool all, hipStream_t st) {
-        int rc = WF_OK;
-        StatsArgs s = {};
-        s.p = {w, x, p.fwd.mt, p.fwd.nt, p.Dp / kBK, 1, {}, {}, live, 0, 1};
-        set_parts(&s.p, p.type, p.Dp, p.Dp);
-        s.l = {bias, btype, 0, p.V};
-        s.top = p.top; s.sum = p.sum; s.all = all ? p.all : nullptr; s.pitch = p.Npad; s.target = target; s.zt = p.zt;
-        with_half(p.type, [&](auto t) {
-            with_big(p.fwd.big, [&](auto b) {
-                rc = launch_tiles<Shape<decltype(b)::value>, stats_kernel<decltype(t), decltype(b)::value>>(s, st, kCUs / 2);
-            });
+int run_stats(const LinearPlan& p, const Operand& w, const Operand& x, const void* bias, int btype, const int32_t* live,
+              const int32_t* target, bool all, hipStream_t st) {
+    int rc = WF_OK;
+    StatsArgs s = {};
+    s.p = {w, x, p.fwd.mt, p.fwd.nt, p.Dp / kBK, 1, {}, {}, live, 0, 1};
+    set_parts(&s.p, p.type, p.Dp, p.Dp);
+    s.l = {bias, btype, 0, p.V};
+    s.top = p.top; s.sum = p.sum; s.all = all ? p.all : nullptr; s.pitch = p.Npad; s.target = target; s.zt = p.zt;
+    with_half(p.type, [&](auto t) {
+        with_big(p.fwd.big, [&](auto b) {
+            rc = launch_tiles<Shape<decltype(b)::value>, stats_kernel<decltype(t), decltype(b)::value>>(s, st, kCUs / 2);
+        });
     });
     if (rc) return rc;
     return WF_OK;
