@@ -1495,11 +1495,12 @@ __global__ void __launch_bounds__(256) small_end_kernel(SmallArgs a, int tiles) 
 // neighbours of a row at a time, its columns in two instructions, so 32 lanes read 256 bytes (fp32) and write as many.  The 4
 // waves take every fourth step of 16 k, their sums meet in LDS, long k is split over workgroups too.  296 x 5001, D 257 fp32: dx 16
 // us, dW 18; 16000 x 59, D 512: dW 15.6.
+__device__ inline int row_of(int id) { return id ^ (id >> 31); }
 struct SmallGradArgs {
     const void *dz, *b;
     int64_t N;               // rows that exist
     uint32_t zld, ldb;       // bytes
-    const int32_t *live, *idx;
+    const int32_t *live, *idx;           // idx: ~row where a row takes no part and was not left out
     int32_t V, D;
     float *part, *colpart;   // [splits][N or V][D], [splits][V], or NULL: straight to the outputs
     const float* scale;
@@ -1545,10 +1546,11 @@ template <class X, bool ROWS> __global__ void __launch_bounds__(256, 2) small_gr
             const int k = (s + u * 4) * 16 + half * 8;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const X* p = (const X*)(bp + (uint64_t)(uint32_t)row[u][e] * a.ldb);
+                const X* p = (const X*)(bp + (uint64_t)(uint32_t)(ROWS ? row[u][e] : row_of(row[u][e])) * a.ldb);
                 const auto b = FULL ? load_n<X, 2>(p, 2) : load_n<X, 2>(p, k + e < end ? left : 0);
-                bv[u][0].v[e] = b.v[0];
-                bv[u][1].v[e] = b.v[1];
+                const bool dead = !ROWS && row[u][e] < 0;
+                bv[u][0].v[e] = dead ? (X)0.f : b.v[0];
+                bv[u][1].v[e] = dead ? (X)0.f : b.v[1];
             }
             if constexpr (ROWS) {
                 av[u][0] = load_n<X, 8>((const X*)zp + k, FULL ? 8 : end - k);
@@ -1614,7 +1616,11 @@ template <class X, bool ROWS> __global__ void __launch_bounds__(256, 2) small_gr
             const int64_t m = m0 + (wave * 8 + half * 4 + e) * NM + i;
             if (m >= M || left <= 0) continue;
             if (a.part) store_n<float, 2>(a.part + ((int64_t)blockIdx.z * (ROWS ? a.N : a.V) + m) * a.D + d, Pack<float, 2>{{c0[e], c1[e]}}, left);
-            else if (a.out) store_n<X, 2>((X*)a.out + (ROWS ? a.idx[m] : m) * a.D + d, Pack<X, 2>{{(X)(c0[e] * scale), (X)(c1[e] * scale)}}, left);
+            else if (a.out) {
+                const int64_t id = ROWS ? a.idx[m] : m;
+                const Pack<X, 2> o = {{id < 0 ? (X)0.f : (X)(c0[e] * scale), id < 0 ? (X)0.f : (X)(c1[e] * scale)}};
+                store_n<X, 2>((X*)a.out + (id < 0 ? ~id : id) * a.D + d, o, left);
+            }
         }
         if (col) {
             const v4f c = join(ones[i]);
@@ -1691,10 +1697,11 @@ template <class X, int KS> __global__ void __launch_bounds__(256, 2) small_dx_ke
         for (int e = 0; e < 16; ++e) {
             const int m = t * 32 + e / 4 * 8 + half * 4 + e % 4;
             if (m >= live) continue;
+            const int id = a.idx[m];
             Pack<X, NN> o;
 #pragma unroll
-            for (int j = 0; j < NN; ++j) o.v[j] = (X)(acc[j][e] * scale);
-            store_n<X, NN>((X*)a.out + (int64_t)a.idx[m] * a.D + d, o, left);
+            for (int j = 0; j < NN; ++j) o.v[j] = id < 0 ? (X)0.f : (X)(acc[j][e] * scale);
+            store_n<X, NN>((X*)a.out + (int64_t)row_of(id) * a.D + d, o, left);
         }
     }
 }
@@ -1924,7 +1931,10 @@ __global__ void __launch_bounds__(256) fold_kernel(FoldArgs a) {
     const int64_t N = a.live ? min(a.N, (int64_t)*a.live) : a.N;
     const float scale = *a.scale;
     const int64_t all = N * a.M, stride = a.N * a.M;
-    auto put = [&](int64_t k, float v) { store_any(a.out, a.otype, a.idx ? a.idx[k / a.M] * (int64_t)a.M + k % a.M : k, v * scale); };
+    auto put = [&](int64_t k, float v) {
+        const int id = a.idx ? a.idx[k / a.M] : 0;
+        store_any(a.out, a.otype, a.idx ? row_of(id) * (int64_t)a.M + k % a.M : k, id < 0 ? 0.f : v * scale);
+    };
     if (a.splits >= 16) {
         // few elements, many parts: 32 elements a workgroup, each summed by 8 threads that meet in LDS
         __shared__ float s[8][32];
@@ -1994,22 +2004,32 @@ struct LogDzArgs {
     int64_t ldg;
     const int32_t *live, *idx;
     int32_t V, plain;        // plain: rows of X, for small_grad_kernel
+    int64_t N;               // plain, and not fp16 (whose scale has to be known first): all N rows in their places, here it is found
+    int32_t *live_out, *idx_out;         // which of them hold a gradient at all; or NULL
+    float* scale_out;
     uint16_t* dz;
     int64_t pitch;
 };
 template <class X, int TPR, int R> __global__ void __launch_bounds__(256) log_dz_kernel(LogDzArgs a) {
     __shared__ float part[4];
+    __shared__ int held[4];
     const int t = threadIdx.x % TPR;
     const int64_t c = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
-    const int live = *a.live;
+    const bool all = a.idx_out != nullptr;
+    const int live = all ? (int)a.N : *a.live;
     if (c >= (int64_t)(live + kRowPad - 1) / kRowPad * kRowPad) return;      // (256 rows, whole workgroups)
     uint16_t* row = a.dz + c * parts_of<X>() * a.pitch;
     const bool in = c < live;
-    const int64_t n = in ? a.idx[c] : 0;
+    const int64_t n = in ? all ? c : a.idx[c] : 0;
     const float* g = a.G + n * a.ldg;
     const float* lp = a.lp + n * a.V;
     const int V = in ? a.V : 0;
-    const float inv = 1.f / *a.scale;
+    const float inv = all ? 1.f : 1.f / *a.scale;
+    bool some = false;       // (of the thread, then of the row)
+    auto add = [&](const Pack<float, 4>& q) {
+        some |= (q.v[0] != 0.f) | (q.v[1] != 0.f) | (q.v[2] != 0.f) | (q.v[3] != 0.f);
+        return (q.v[0] + q.v[1]) + (q.v[2] + q.v[3]);
+    };
     Pack<float, 4> gv[R ? R : 1], lv[R ? R : 1];
     float s = 0.f;
     if constexpr (R > 0) {
@@ -2018,23 +2038,26 @@ template <class X, int TPR, int R> __global__ void __launch_bounds__(256) log_dz
 #pragma unroll
         for (int i = 0; i < R; ++i) lv[i] = load_n<float, 4>(lp + (i * TPR + t) * 4, V - (i * TPR + t) * 4);
 #pragma unroll
-        for (int i = 0; i < R; ++i) s += (gv[i].v[0] + gv[i].v[1]) + (gv[i].v[2] + gv[i].v[3]);
+        for (int i = 0; i < R; ++i) s += add(gv[i]);
     } else {
-        for (int v = t * 4; v < V; v += TPR * 4) {
-            const auto q = load_n<float, 4>(g + v, V - v);
-            s += (q.v[0] + q.v[1]) + (q.v[2] + q.v[3]);
-        }
+        for (int v = t * 4; v < V; v += TPR * 4) s += add(load_n<float, 4>(g + v, V - v));
     }
     s = wave_sum(s);
+    some = __any(some);
     if constexpr (TPR > 64) {
-        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+        if ((threadIdx.x & 63) == 0) { part[threadIdx.x >> 6] = s; held[threadIdx.x >> 6] = some; }
         __syncthreads();
         s = (part[0] + part[1]) + (part[2] + part[3]);
+        some = (held[0] | held[1] | held[2] | held[3]) != 0;
+    }
+    if (all && t == 0) {
+        if (in) a.idx_out[c] = some ? (int)c : ~(int)c;
+        if (c == 0) { *a.live_out = live; *a.scale_out = 1.f; }
     }
     auto put = [&](int v, const Pack<float, 4>& q, const Pack<float, 4>& l) {
         float d[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) d[e] = v + e < V ? (q.v[e] - __expf(l.v[e]) * s) * inv : 0.f;
+        for (int e = 0; e < 4; ++e) d[e] = (some & (v + e < V)) ? (q.v[e] - __expf(l.v[e]) * s) * inv : 0.f;
         if (v >= a.pitch) return;
         if (std::is_same<X, float>::value && a.plain) __builtin_memcpy((float*)a.dz + c * a.pitch + v, d, 16);
         else store_dz4<X>(row, a.pitch, v, d);
@@ -2465,13 +2488,18 @@ extern "C" int wf_linear_log_softmax_backward(const float* log_probs, const floa
     if (N == 0) return (rc = zero_fill(dweight, (int64_t)V * D, type, st)) ? rc : zero_fill(dbias, V, bias_type, st);
     if (!log_probs || !grad || ldg < 0) return wf_fail(WF_EINVAL, "wf_linear_log_softmax_backward: null pointer");
     const unsigned blocks = (unsigned)ceil_div(N, 4);
-    if (type == WF_F16) grad_rows_kernel<true><<<blocks, 256, 0, st>>>(grad, ldg, N, V, p.gpeak);
-    else grad_rows_kernel<false><<<blocks, 256, 0, st>>>(grad, ldg, N, V, p.gpeak);
+    const bool in_place = p.small && type != WF_F16;
     Operand w;
-    PrepArgs r = {};
-    r.xp = p.xp; r.dx = dx; r.peak = p.gpeak; r.hit = 1.f; r.narrow = type == WF_F16;
-    if ((rc = run_prep(p, r, x, ldx, weight, ldw, st, &w))) return rc;
-    LogDzArgs z = {grad, log_probs, p.rows.scale, ldg, p.rows.live, p.rows.idx, V, p.small, p.dzp, p.pitch};
+    LogDzArgs z = {grad, log_probs, p.rows.scale, ldg, p.rows.live, p.rows.idx, V, p.small, N, nullptr, nullptr, nullptr, p.dzp, p.pitch};
+    if (in_place) {
+        z.live_out = p.rows.live; z.idx_out = p.rows.idx; z.scale_out = p.rows.scale;
+    } else {
+        if (type == WF_F16) grad_rows_kernel<true><<<blocks, 256, 0, st>>>(grad, ldg, N, V, p.gpeak);
+        else grad_rows_kernel<false><<<blocks, 256, 0, st>>>(grad, ldg, N, V, p.gpeak);
+        PrepArgs r = {};
+        r.xp = p.xp; r.dx = dx; r.peak = p.gpeak; r.hit = 1.f; r.narrow = type == WF_F16;
+        if ((rc = run_prep(p, r, x, ldx, weight, ldw, st, &w))) return rc;
+    }
     with_type(type, [&](auto t) {
         using X = decltype(t);
         if (p.pitch <= 256) log_dz_kernel<X, 64, 1><<<(unsigned)(p.Npad / 4), 256, 0, st>>>(z);
