@@ -1611,13 +1611,15 @@ template <class X, bool ROWS> __global__ void __launch_bounds__(256, 2) small_gr
 #pragma unroll
     for (int i = 0; i < NM; ++i) {
         const v4f c0 = join(acc[i][0]), c1 = join(acc[i][1]);
+        Pack<int, 4> ids = {};
+        if constexpr (ROWS) __builtin_memcpy(&ids, a.idx + m0 + wave * 8 + half * 4, 16);       // (idx has whole 256 rows)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int64_t m = m0 + (wave * 8 + half * 4 + e) * NM + i;
             if (m >= M || left <= 0) continue;
             if (a.part) store_n<float, 2>(a.part + ((int64_t)blockIdx.z * (ROWS ? a.N : a.V) + m) * a.D + d, Pack<float, 2>{{c0[e], c1[e]}}, left);
             else if (a.out) {
-                const int64_t id = ROWS ? a.idx[m] : m;
+                const int64_t id = ROWS ? ids.v[e] : m;
                 const Pack<X, 2> o = {{id < 0 ? (X)0.f : (X)(c0[e] * scale), id < 0 ? (X)0.f : (X)(c1[e] * scale)}};
                 store_n<X, 2>((X*)a.out + (id < 0 ? ~id : id) * a.D + d, o, left);
             }
@@ -1637,7 +1639,7 @@ template <class X, bool ROWS> __global__ void __launch_bounds__(256, 2) small_gr
 
 // dx of a small table: W's fragments of 64 columns (all KS steps of k; 32 columns where an fp32 table has more than 64 outputs)
 // stay in a wave's registers while it walks over tiles of 32 rows; the next tile's dz is under way meanwhile.  16000 x 59, D 512
-// fp32: 22 us (the writing of dx alone: 6).
+// fp32: 21 us (the writing of dx alone: 6).
 template <class X, int KS> __global__ void __launch_bounds__(256, 2) small_dx_kernel(SmallGradArgs a) {
     using T = typename Half<X>::type;
     constexpr int P = parts_of<X>(), NN = P == 3 && KS > 4 ? 1 : 2;
@@ -1645,13 +1647,14 @@ template <class X, int KS> __global__ void __launch_bounds__(256, 2) small_dx_ke
     const int live = *a.live, tiles = (live + 31) / 32, step = gridDim.y * 4;
     int t = blockIdx.y * 4 + wave;
     if (t >= tiles) return;
+    constexpr bool AHEAD = P * KS <= 12;                      // (the registers are full otherwise)
     Pack<X, 8> zv[KS];
     auto load = [&](int tile) {                               // (dz has KS * 16 outputs, zeros behind the last; behind the last row: another row)
         const X* z = (const X*)((const char*)a.dz + (uint64_t)(uint32_t)min(tile * 32 + at, live - 1) * a.zld) + half * 8;
 #pragma unroll
         for (int u = 0; u < KS; ++u) zv[u] = load_n<X, 8>(z + u * 16, 8);
     };
-    load(t);
+    if (AHEAD) load(t);
     const int d = (blockIdx.x * 32 + at) * NN, left = a.D - d;
     const X* w = (const X*)a.b + min(d, a.D - 1);
     const bool whole = (int)(blockIdx.x + 1) * 32 * NN <= a.D;
@@ -1663,7 +1666,13 @@ template <class X, int KS> __global__ void __launch_bounds__(256, 2) small_dx_ke
         for (int e = 0; e < 8; ++e) {
             const int k = u * 16 + half * 8 + e;
             const X* p = (const X*)((const char*)w + (uint64_t)(uint32_t)min(k, a.V - 1) * a.ldb);
-            const auto q = whole ? load_n<X, NN>(p, NN) : load_n<X, NN>(p, left);
+            Pack<X, NN> q;
+            if (whole) {
+                q = load_n<X, NN>(p, NN);
+            } else {                                          // (columns behind the last one: the last one again)
+                q.v[0] = p[0];
+                if constexpr (NN == 2) q.v[1] = p[left > 1 ? 1 : 0];
+            }
 #pragma unroll
             for (int j = 0; j < NN; ++j) v[j].v[e] = k < a.V ? q.v[j] : (X)0.f;
         }
@@ -1676,9 +1685,10 @@ template <class X, int KS> __global__ void __launch_bounds__(256, 2) small_dx_ke
 #pragma unroll
         for (int j = 0; j < NN; ++j) acc[j] = v16f{};
         typename Mfma<T>::v8 zf[KS][P];
+        if (!AHEAD) load(t);
 #pragma unroll
         for (int u = 0; u < KS; ++u) split_frag<X>(zv[u], zf[u]);
-        if (t + step < tiles) load(t + step);
+        if (AHEAD && t + step < tiles) load(t + step);
 #pragma unroll
         for (int u = 0; u < KS; ++u)
 #pragma unroll
@@ -1692,12 +1702,15 @@ template <class X, int KS> __global__ void __launch_bounds__(256, 2) small_dx_ke
                 }
                 acc[j] = Mfma<T>::mul(zf[u][0], wf[j][u][0], acc[j]);
             }
+        Pack<int, 16> ids;                                    // all under way before the first store (idx has whole 256 rows)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) __builtin_memcpy(&ids.v[q * 4], a.idx + t * 32 + q * 8 + half * 4, 16);
         if (left <= 0) continue;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             const int m = t * 32 + e / 4 * 8 + half * 4 + e % 4;
+            const int id = ids.v[e];
             if (m >= live) continue;
-            const int id = a.idx[m];
             Pack<X, NN> o;
 #pragma unroll
             for (int j = 0; j < NN; ++j) o.v[j] = id < 0 ? (X)0.f : (X)(acc[j][e] * scale);
@@ -2333,7 +2346,7 @@ int run_small_grads(const LinearPlan& p, const void* x, int64_t ldx, const void*
         if (o.dx) {
             if (p.V <= kSmallOutputs) {
                 const int columns = p.V > 64 && p.type == WF_F32 ? 32 : 64;
-                // (as many workgroups as are resident: an fp32 wave holds 203 registers, a 16-bit one 99)
+                // (as many workgroups as are resident: an fp32 wave holds up to 211 registers, a 16-bit one 107 with 64 outputs)
                 const unsigned x = (unsigned)ceil_div(p.D, columns), most = std::max(1u, (p.type == WF_F32 ? 2 : 4) * kCUs / x);
                 const dim3 grid(x, std::min<unsigned>((unsigned)ceil_div(p.N, 128), most));
                 if (p.V <= 64) small_dx_kernel<X, 4><<<grid, 256, 0, st>>>(g);
