@@ -26,7 +26,7 @@ TYPES = [torch.float32, torch.bfloat16, torch.float16]
 SIZES = [(1, 1, 1), (1, 512, 5001), (3, 64, 2), (5, 7, 59), (64, 65, 128), (127, 72, 129), (128, 128, 256), (129, 257, 255),
          (300, 64, 513), (513, 192, 300), (1000, 80, 59), (2, 1030, 1), (296, 257, 5001),
          # outputs in whole 64s and around them, features around the 32 and 64 columns of a workgroup, splits over many rows
-         (40, 33, 64), (100, 63, 65), (5000, 31, 33), (4099, 95, 127),
+         (40, 33, 64), (100, 63, 65), (5000, 31, 33), (4099, 95, 127), (40000, 33, 50),
          # more work than the direct kernels take: tiles, with rows, outputs and features that end inside one
          (300, 1031, 6007), (700, 641, 5003), (2049, 257, 4099), (20003, 700, 131)]
 
