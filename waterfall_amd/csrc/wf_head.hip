@@ -1253,8 +1253,15 @@ __global__ void __launch_bounds__(1024) total_kernel(const float* loss, int64_t 
 // and the splitting of fp32 operands 6.5 (rows brought to LDS in whole 256-byte pieces first: 18 us there, 22.4 against 20.9 at
 // 296 x 5001, D 257; 64 outputs a workgroup at that size: 23).  Where one workgroup sees all outputs of its rows it ends them
 // itself: the whole call is this one launch.
+// Workgroup's part of `all` pieces of work: the chip's 8 dies take workgroups in turn, and each gets a run of neighbours, which share
+// what they read in its L2.  -1: none.  The launch has a multiple of 8.
+__device__ inline int dealt(int all) {
+    const int per = (all + 7) / 8, id = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+    return (int)(blockIdx.x >> 3) < per && id < all ? id : -1;
+}
 struct SmallArgs {
     const void *x, *w;
+    int32_t vtiles, ntiles;
     int64_t ldx, ldw, N;
     int32_t D;
     Logits l;
@@ -1305,8 +1312,10 @@ template <class X, int MV, bool DZ> __global__ void __launch_bounds__(256) small
     __shared__ __align__(16) float part[4][MV][4][64][4];     // [wave][m][q][lane][e]
     __shared__ float wtop[4][32], wsum[4][32], wall[4][32], wzt[32];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int v0 = blockIdx.x * 32 * MV, kl = (lane >> 5) * 8;
-    const int64_t n0 = (int64_t)blockIdx.y * 32, n = n0 + (lane & 31);
+    const int id = dealt(a.vtiles * a.ntiles), tv = id / a.ntiles;
+    if (id < 0) return;
+    const int v0 = tv * 32 * MV, kl = (lane >> 5) * 8;
+    const int64_t n0 = (int64_t)(id % a.ntiles) * 32, n = n0 + (lane & 31);
     const int live = DZ ? *a.live : 0;
     if (DZ && n0 >= (live + kBK - 1) / kBK * kBK) return;     // rows that no product reads
     const X* xr = (const X*)a.x + (DZ ? (int64_t)(n < live ? a.idx[n] : 0) : min(n, a.N - 1)) * a.ldx;
@@ -1425,7 +1434,7 @@ template <class X, int MV, bool DZ> __global__ void __launch_bounds__(256) small
     float lse = 0.f;
     if (a.top) {
         if (wave == 0 && lane < 32) {
-            const int64_t at = blockIdx.x * a.pitch + n;
+            const int64_t at = tv * a.pitch + n;
             a.top[at] = top;
             a.sum[at] = sum;
             if (a.all) a.all[at] = all;
@@ -1502,6 +1511,7 @@ struct SmallGradArgs {
     uint32_t zld, ldb;       // bytes
     const int32_t *live, *idx;           // idx: ~row where a row takes no part and was not left out
     int32_t V, D;
+    int32_t dtiles, mtiles, splits;
     float *part, *colpart;   // [splits][N or V][D], [splits][V], or NULL: straight to the outputs
     const float* scale;
     void *out, *colout;
@@ -1513,11 +1523,13 @@ template <class X, bool ROWS> __global__ void __launch_bounds__(256, 2) small_gr
     __shared__ __align__(16) float meet[2][4][4][64][4];      // [turn][wave][q][lane][e]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, at = lane & 31;
     const int live = *a.live, M = ROWS ? live : a.V, K = ROWS ? a.V : live;
-    const int64_t m0 = (int64_t)blockIdx.y * 32 * NM;
-    const int d0 = blockIdx.x * 64, d = d0 + at * 2;
+    const int id = dealt(a.dtiles * a.mtiles * a.splits), td = id % a.dtiles, tm = id / a.dtiles % a.mtiles, split = id / a.dtiles / a.mtiles;
+    if (id < 0) return;
+    const int64_t m0 = (int64_t)tm * 32 * NM;
+    const int d0 = td * 64, d = d0 + at * 2;
     if (m0 >= M) return;
-    const bool col = !ROWS && a.colout && blockIdx.x == 0;
-    const int steps = (K + 15) / 16, per = (steps + gridDim.z - 1) / gridDim.z, s1 = min(steps, (int)(blockIdx.z + 1) * per), end = min(K, s1 * 16);
+    const bool col = !ROWS && a.colout && td == 0;
+    const int steps = (K + 15) / 16, per = (steps + a.splits - 1) / a.splits, s1 = min(steps, (split + 1) * per), end = min(K, s1 * 16);
     // (dz has whole 64 outputs in every row: what is behind the last output or row is not used)
     const char* zp = (const char*)a.dz + (ROWS ? min(m0 + at, (int64_t)M - 1) * a.zld : (m0 + at * 2) * (int64_t)sizeof(X));
     const char* bp = (const char*)a.b + (int64_t)min(d, a.D - 1) * sizeof(X);
@@ -1591,7 +1603,7 @@ template <class X, bool ROWS> __global__ void __launch_bounds__(256, 2) small_gr
         }
     };
     using std::integral_constant;
-    int s = (int)blockIdx.z * per + wave;
+    int s = split * per + wave;
     if (d0 + 64 <= a.D) {
         for (; (s + 4) * 16 + 16 <= end; s += 8) group(s, integral_constant<int, 2>(), std::true_type());
         if (s * 16 + 16 <= end) { group(s, integral_constant<int, 1>(), std::true_type()); s += 4; }
@@ -1617,11 +1629,11 @@ template <class X, bool ROWS> __global__ void __launch_bounds__(256, 2) small_gr
         for (int e = 0; e < 4; ++e) {
             const int64_t m = m0 + (wave * 8 + half * 4 + e) * NM + i;
             if (m >= M || left <= 0) continue;
-            if (a.part) store_n<float, 2>(a.part + ((int64_t)blockIdx.z * (ROWS ? a.N : a.V) + m) * a.D + d, Pack<float, 2>{{c0[e], c1[e]}}, left);
+            if (a.part) store_n<float, 2>(a.part + ((int64_t)split * (ROWS ? a.N : a.V) + m) * a.D + d, Pack<float, 2>{{c0[e], c1[e]}}, left);
             else if (a.out) {
-                const int64_t id = ROWS ? ids.v[e] : m;
-                const Pack<X, 2> o = {{id < 0 ? (X)0.f : (X)(c0[e] * scale), id < 0 ? (X)0.f : (X)(c1[e] * scale)}};
-                store_n<X, 2>((X*)a.out + (id < 0 ? ~id : id) * a.D + d, o, left);
+                const int64_t row = ROWS ? ids.v[e] : m;
+                const Pack<X, 2> o = {{row < 0 ? (X)0.f : (X)(c0[e] * scale), row < 0 ? (X)0.f : (X)(c1[e] * scale)}};
+                store_n<X, 2>((X*)a.out + (row < 0 ? ~row : row) * a.D + d, o, left);
             }
         }
         if (col) {
@@ -1630,7 +1642,7 @@ template <class X, bool ROWS> __global__ void __launch_bounds__(256, 2) small_gr
             for (int e = 0; e < 4; ++e) {
                 const int64_t m = m0 + (wave * 8 + half * 4 + e) * NM + i;
                 if (at || m >= M) continue;
-                if (a.part) a.colpart[(int64_t)blockIdx.z * a.V + m] = c[e];
+                if (a.part) a.colpart[(int64_t)split * a.V + m] = c[e];
                 else store_any(a.colout, a.ctype, m, c[e] * scale);
             }
         }
@@ -2131,7 +2143,7 @@ constexpr int kSmallOutputs = 128;
 constexpr double kSmallWork = 0.7e9, kSmallWorkF32 = 1.6e9;      // N V D
 bool is_small(int64_t N, int32_t D, int32_t V, int type, bool bwd) {
     if (bwd && (size_t)N * round_up(V, 64) * (type == WF_F32 ? 4 : 2) > kPieceBytes) return false;
-    if (V <= (bwd && type != WF_F32 ? kSmallOutputs / 2 : kSmallOutputs)) return N <= (1 << 21) - 64;      // (workgroups in a launch's second dimension)
+    if (V <= (bwd && type != WF_F32 ? kSmallOutputs / 2 : kSmallOutputs)) return N <= (1 << 21) - 64;      // (what is tested)
     return N <= 65535 && (double)N * V * D <= (type == WF_F32 ? kSmallWorkF32 : kSmallWork);
 }
 // A product of small_grad_kernel that has fewer than 4 workgroups per CU is split over k while a wave keeps 4 steps.
@@ -2324,7 +2336,8 @@ int run_stats(const LinearPlan& p, const Operand& w, const Operand& x, const voi
 int run_small(const LinearPlan& p, SmallArgs a, hipStream_t st) {
     const int mv = small_mv(p.V), tiles = (int)ceil_div(p.V, 32 * mv);
     a.top = p.top; a.sum = p.sum; a.all = a.smoothing != 0.f ? p.all : nullptr; a.zt = p.zt; a.pitch = p.N;
-    const dim3 grid((unsigned)tiles, (unsigned)ceil_div(p.N, 32));
+    a.vtiles = tiles; a.ntiles = (int)ceil_div(p.N, 32);
+    const unsigned grid = (unsigned)round_up((int64_t)a.vtiles * a.ntiles, 8);
     with_type(p.type, [&](auto t) {
         using X = decltype(t);
         if (mv == 1) small_kernel<X, 1, false><<<grid, 256, 0, st>>>(a);
@@ -2342,7 +2355,9 @@ unsigned fold_grid(int64_t elements, int splits) { return (unsigned)std::max<int
 int run_small_grads(const LinearPlan& p, const void* x, int64_t ldx, const void* w, int64_t ldw, const GradOut& o, hipStream_t st) {
     with_type(p.type, [&](auto t) {
         using X = decltype(t);
-        SmallGradArgs g = {p.dzp, w, p.N, (uint32_t)(p.pitch * sizeof(X)), (uint32_t)(ldw * sizeof(X)), p.rows.live, p.rows.idx, p.V, p.D, p.part_x, nullptr, p.rows.scale, o.dx, nullptr, 0};
+        SmallGradArgs g = {p.dzp, w, p.N, (uint32_t)(p.pitch * sizeof(X)), (uint32_t)(ldw * sizeof(X)), p.rows.live, p.rows.idx, p.V, p.D,
+                           (int)ceil_div(p.D, 64), (int)ceil_div(p.N, 32), p.sx, p.part_x, nullptr, p.rows.scale, o.dx, nullptr, 0};
+        auto grid = [&] { return (unsigned)round_up((int64_t)g.dtiles * g.mtiles * g.splits, 8); };
         if (o.dx) {
             if (p.V <= kSmallOutputs) {
                 const int columns = p.V > 64 && p.type == WF_F32 ? 32 : 64;
@@ -2352,8 +2367,7 @@ int run_small_grads(const LinearPlan& p, const void* x, int64_t ldx, const void*
                 if (p.V <= 64) small_dx_kernel<X, 4><<<grid, 256, 0, st>>>(g);
                 else small_dx_kernel<X, 8><<<grid, 256, 0, st>>>(g);
             } else {
-                const dim3 grid((unsigned)ceil_div(p.D, 64), (unsigned)ceil_div(p.N, 32), (unsigned)p.sx);
-                small_grad_kernel<X, true><<<grid, 256, 0, st>>>(g);
+                small_grad_kernel<X, true><<<grid(), 256, 0, st>>>(g);
             }
             if (p.part_x) {
                 FoldArgs f = {p.part_x, nullptr, p.rows.scale, p.sx, p.D, p.N, p.rows.live, p.rows.idx, o.dx, nullptr, p.type, 0};
@@ -2362,8 +2376,8 @@ int run_small_grads(const LinearPlan& p, const void* x, int64_t ldx, const void*
         }
         if (o.dw || o.db) {
             g.b = x; g.ldb = (uint32_t)(ldx * sizeof(X)); g.part = p.part_w; g.colpart = p.part_c; g.out = o.dw; g.colout = o.db; g.ctype = o.btype;
-            const dim3 grid(o.dw ? (unsigned)ceil_div(p.D, 64) : 1, (unsigned)ceil_div(p.V, 64), (unsigned)p.sw);
-            small_grad_kernel<X, false><<<grid, 256, 0, st>>>(g);
+            g.dtiles = o.dw ? g.dtiles : 1; g.mtiles = (int)ceil_div(p.V, 64); g.splits = p.sw;
+            small_grad_kernel<X, false><<<grid(), 256, 0, st>>>(g);
             if (p.part_w) {
                 const int M = o.dw ? p.D : 0;
                 FoldArgs f = {p.part_w, p.part_c, p.rows.scale, p.sw, M, p.V, nullptr, nullptr, o.dw, o.db, p.type, o.btype};
@@ -2589,7 +2603,8 @@ extern "C" int wf_linear_cross_entropy_backward(const float* grad, int32_t grad_
         s.x = x; s.w = weight; s.ldx = ldx; s.ldw = ldw; s.N = N; s.D = D; s.l = {bias, bias_type, 0, V}; s.smoothing = smoothing;
         s.live = p.rows.live; s.idx = p.rows.idx; s.want = p.rows.target; s.g = p.rows.g; s.glse = p.rows.lse; s.dz = p.dzp; s.zpitch = p.pitch;
         const int mv = small_mv(V);
-        const dim3 grid((unsigned)ceil_div(round_up(V, kBK), 32 * mv), (unsigned)ceil_div(round_up(N, kBK), 32));
+        s.vtiles = (int)ceil_div(round_up(V, kBK), 32 * mv); s.ntiles = (int)ceil_div(round_up(N, kBK), 32);
+        const unsigned grid = (unsigned)round_up((int64_t)s.vtiles * s.ntiles, 8);
         with_type(type, [&](auto t) {
             using X = decltype(t);
             if (mv == 1) small_kernel<X, 1, true><<<grid, 256, 0, st>>>(s);
