@@ -2022,8 +2022,8 @@ template <bool FULL> __global__ void __launch_bounds__(256) grad_rows_kernel(con
     if (lane == 0) peak[n] = m;
 }
 // dz = G - exp(lp) sum(G) of the live rows, packed.  TPR threads a row, which stays in registers between its sum and its result
-// (R pieces of 4 a thread); R = 0: rows that do not fit are read twice.  Bound by HBM: 14000 of 16000 x 5001 to bf16 149 us (4.7
-// TB/s).
+// (R pieces of 4 a thread); R = 0: rows that do not fit are read twice.  A row whose every lp is -inf (all outputs masked) has
+// no gradient, whatever comes in.  Bound by HBM: 14000 of 16000 x 5001 to bf16 149 us (4.7 TB/s).
 struct LogDzArgs {
     const float *G, *lp, *scale;
     int64_t ldg;
@@ -2050,7 +2050,11 @@ template <class X, int TPR, int R> __global__ void __launch_bounds__(256) log_dz
     const float* lp = a.lp + n * a.V;
     const int V = in ? a.V : 0;
     const float inv = all ? 1.f : 1.f / *a.scale;
-    bool some = false;       // (of the thread, then of the row)
+    bool some = false, open = false;     // a gradient, an output that is not masked (of the thread, then of the row)
+    auto look = [&](int v, const Pack<float, 4>& l) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) open |= (v + e < V) & (l.v[e] != -INFINITY);
+    };
     auto add = [&](const Pack<float, 4>& q) {
         some |= (q.v[0] != 0.f) | (q.v[1] != 0.f) | (q.v[2] != 0.f) | (q.v[3] != 0.f);
         return (q.v[0] + q.v[1]) + (q.v[2] + q.v[3]);
@@ -2063,18 +2067,20 @@ template <class X, int TPR, int R> __global__ void __launch_bounds__(256) log_dz
 #pragma unroll
         for (int i = 0; i < R; ++i) lv[i] = load_n<float, 4>(lp + (i * TPR + t) * 4, V - (i * TPR + t) * 4);
 #pragma unroll
-        for (int i = 0; i < R; ++i) s += add(gv[i]);
+        for (int i = 0; i < R; ++i) { s += add(gv[i]); look((i * TPR + t) * 4, lv[i]); }
     } else {
         for (int v = t * 4; v < V; v += TPR * 4) s += add(load_n<float, 4>(g + v, V - v));
+        for (int v = t * 4; v < V && !__any(open); v += TPR * 4) look(v, load_n<float, 4>(lp + v, V - v));     // (mostly once)
     }
     s = wave_sum(s);
-    some = __any(some);
+    int row_has = (__any(some) ? 1 : 0) | (__any(open) ? 2 : 0);
     if constexpr (TPR > 64) {
-        if ((threadIdx.x & 63) == 0) { part[threadIdx.x >> 6] = s; held[threadIdx.x >> 6] = some; }
+        if ((threadIdx.x & 63) == 0) { part[threadIdx.x >> 6] = s; held[threadIdx.x >> 6] = row_has; }
         __syncthreads();
         s = (part[0] + part[1]) + (part[2] + part[3]);
-        some = (held[0] | held[1] | held[2] | held[3]) != 0;
+        row_has = held[0] | held[1] | held[2] | held[3];
     }
+    some = row_has == 3;
     if (all && t == 0) {
         if (in) a.idx_out[c] = some ? (int)c : ~(int)c;
         if (c == 0) { *a.live_out = live; *a.scale_out = 1.f; }
