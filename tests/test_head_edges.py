@@ -1,9 +1,12 @@
-"""The output head's operators at the edges of what they promise.  Bounds as in test_head_linear.py: they count roundings."""
+"""The output head's operators at the edges of what they promise.  Bounds as in test_head_linear.py: they count roundings.
+
+float16 gradients of logits are stored relative to a power of two: what `Case.products` takes as its last argument.  Log-probabilities:
+with B the largest of max |G| and |sum(G)| over the rows, B is 2^13 to 2^14 of it, so it is at most 2^-13 B."""
 import pytest
 import torch
 
 import waterfall_amd as wf
-from tests.test_head_linear import Case, check_grads, DEV, TYPES
+from tests.test_head_linear import Case, check_grads, dz_of_log_softmax, DEV, TYPES
 
 gpu = pytest.mark.gpu
 
@@ -32,3 +35,17 @@ def test_rows_whose_every_output_is_masked_have_no_gradient(N, D, V, dtype):
         dz[:, -1] -= s
         check_grads(got, c.products(dz, (V / 256 + 20) * 2.0 ** -24 * size * torch.nn.functional.one_hot(torch.tensor(V - 1, device=DEV), V) + 3 * 2.0 ** -24 * dz.abs(),
                                     2 * size.max().item()), (N, D, V))
+
+
+@gpu
+@pytest.mark.parametrize("N,D", [(4, 64), (300, 64)])
+def test_half_precision_gradients_of_a_confident_row_and_a_gradient_that_sums_up(N, D):
+    V = 262144
+    c = Case(N, D, V, torch.float16)
+    with torch.no_grad():
+        c.b[7] = 40.0
+    a = [v.detach().requires_grad_() for v in (c.x, c.w, c.b)]
+    G = torch.full((N, V), 1.0 / V, device=DEV)
+    got = torch.autograd.grad(wf.linear_log_softmax(*a), a, G)
+    with torch.no_grad():
+        check_grads(got, c.products(*dz_of_log_softmax(c, G), 2.0 ** -13), (N, D, V))

@@ -917,15 +917,15 @@ struct PrepArgs {
     const void* targets;     // cross entropy: row n is live iff targets[n] != ignore
     int target_wide;
     int64_t ignore;
-    const float* peak;       // log-softmax backward: row n is live iff peak[n] (largest |gradient|) is not 0
+    const float* peak;       // log-softmax backward: row n is live iff peak[n] (of grad_rows_kernel) is not 0
     float *loss, *lse;       // cross entropy forward: dead rows' outputs (0)
     const float* gout;       // backward: incoming gradient, one for all rows or per row
     int gout_rows, mean;
     const float* lse_in;
-    int narrow;              // log-softmax backward in fp16: the gradients are scaled by peak's largest
+    int narrow;              // log-softmax backward in fp16: the gradients are scaled by peak's largest bound
     float hit;               // backward: 1 - smoothing, or 1 where that is 0
     int row_blocks, tail_blocks;         // workgroups over the rows, over the rows behind the last live one, then over W
-    int32_t* count;          // per kCountRows rows: how many are live, and the largest |gradient|; NULL: every workgroup looks itself
+    int32_t* count;          // per kCountRows rows: how many are live, and the largest row_peak; NULL: every workgroup looks itself
     float* most;
 };
 __device__ inline int64_t target_of(const PrepArgs& a, int64_t n) {
@@ -977,8 +977,9 @@ template <class T> __global__ void __launch_bounds__(256) prep_kernel(PrepArgs a
     }
     // What a 16-bit gradient of a logit is relative to.  Cross entropy: the largest incoming gradient, times the target's own
     // share 1 - smoothing: where all rows weigh the same, the entry of a target is then -1 + p / (1 - smoothing) and not some
-    // number whose rounding is the same in every row and adds up over them.  Log-probabilities: a power of two near the largest
-    // incoming gradient.  fp16 needs either to stay inside its range: what then falls below its 2^-24 is below that of a row's.
+    // number whose rounding is the same in every row and adds up over them.  Log-probabilities in fp16: a power of two that brings
+    // the largest bound of grad_rows_kernel to 2^13 .. 2^14, so that no gradient of a logit passes 2^15 and all of fp16's range below
+    // is there for the smaller ones.
     float scale = 0.f;
     if (a.gout && !a.gout_rows) {
         scale = fabsf(a.gout[0]);
@@ -997,7 +998,7 @@ template <class T> __global__ void __launch_bounds__(256) prep_kernel(PrepArgs a
     else if (a.narrow) {
         int e = 0;
         (void)frexpf(scale, &e);
-        scale = ldexpf(1.f, max(-100, min(100, e)));
+        scale = ldexpf(1.f, max(-100, e) - 14);
     }
     int c = 0;
     int64_t seen = 0;                      // rows whose count is known
@@ -1999,19 +2000,20 @@ __global__ void __launch_bounds__(256) fold_kernel(FoldArgs a) {
 }
 
 // ---- the gradient that comes into log-probabilities -----------------------------------------------------------------
-// Which rows of G hold anything: peak[n] = 0 where all of it is zero.  FULL: the largest magnitude (infinite where something is
-// no number); else some value that is not 0, and a row is read up to its first one.  A wave a row.  16000 x 5001, an eighth of the
-// rows zero: 25 us, the reading of those.
+// Which rows of G hold anything: peak[n] = 0 where all of it is zero.  FULL: a bound of |G - p sum(G)| that is at most twice too
+// small, the larger of the largest magnitude and |sum(G)| (infinite where something is no number); else some value that is not 0, and a
+// row is read up to its first one.  A wave a row.  16000 x 5001, an eighth of the rows zero: 25 us, the reading of those.
 template <bool FULL> __global__ void __launch_bounds__(256) grad_rows_kernel(const float* G, int64_t ldg, int64_t N, int V, float* peak) {
     const int lane = threadIdx.x & 63;
     const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (n >= N) return;
     const float* g = G + n * ldg;
-    float m = 0.f;
+    float m = 0.f, s = 0.f;
     auto look = [&](int v) {
         const auto q = load_n<float, 4>(g + v + lane * 4, V - v - lane * 4);
 #pragma unroll
         for (int e = 0; e < 4; ++e) m = fmaxf(m, q.v[e] != q.v[e] ? INFINITY : fabsf(q.v[e]));
+        if (FULL) s += (q.v[0] + q.v[1]) + (q.v[2] + q.v[3]);
     };
     look(0);
     for (int v = 256; v < V && (FULL || !__any(m != 0.f)); v += 2048)
@@ -2019,6 +2021,7 @@ template <bool FULL> __global__ void __launch_bounds__(256) grad_rows_kernel(con
         for (int u = 0; u < 8; ++u)
             if (v + u * 256 < V) look(v + u * 256);
     m = wave_max(m);
+    if (FULL) m = fmaxf(m, fabsf(wave_sum(s)));               // (a sum that is no number: m is infinite)
     if (lane == 0) peak[n] = m;
 }
 // dz = G - exp(lp) sum(G) of the live rows, packed.  TPR threads a row, which stays in registers between its sum and its result
