@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import waterfall_amd as wf
-from tests.test_head_linear import Case, check_grads, dz_of_log_softmax, DEV, TYPES
+from tests.test_head_linear import Case, check_grads, dz_of_entropy, dz_of_log_softmax, DEV, TYPES
 
 gpu = pytest.mark.gpu
 
@@ -49,3 +49,18 @@ def test_half_precision_gradients_of_a_confident_row_and_a_gradient_that_sums_up
     got = torch.autograd.grad(wf.linear_log_softmax(*a), a, G)
     with torch.no_grad():
         check_grads(got, c.products(*dz_of_log_softmax(c, G), 2.0 ** -13), (N, D, V))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,D,V", [(40, 64, 59), (40, 64, 700), (300, 1031, 6007)])
+@pytest.mark.parametrize("eps", [0.5, 0.9, 0.996, 0.999, 0.99999, 1 - 2.0 ** -24])
+def test_label_smoothing_just_under_one(N, D, V, eps, dtype):
+    c = Case(N, D, V, dtype)
+    with torch.no_grad():
+        c.b[3] = 30.0                                       # probabilities near 1
+    a = [v.detach().requires_grad_() for v in (c.x, c.w, c.b)]
+    up = torch.randn(N, generator=c.g).to(DEV)
+    got = torch.autograd.grad(wf.linear_cross_entropy(a[0], a[1], c.t, a[2], label_smoothing=eps, reduction="none"), a, up)
+    with torch.no_grad():
+        check_grads(got, c.products(*dz_of_entropy(c, up, eps), 2 * up.abs().max().item()), (N, D, V, eps))

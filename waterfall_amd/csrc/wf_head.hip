@@ -923,11 +923,14 @@ struct PrepArgs {
     int gout_rows, mean;
     const float* lse_in;
     int narrow;              // log-softmax backward in fp16: the gradients are scaled by peak's largest bound
-    float hit;               // backward: 1 - smoothing, or 1 where that is 0
+    float unit;              // backward: unit_of(smoothing)
     int row_blocks, tail_blocks;         // workgroups over the rows, over the rows behind the last live one, then over W
     int32_t* count;          // per kCountRows rows: how many are live, and the largest row_peak; NULL: every workgroup looks itself
     float* most;
 };
+// The unit of cross entropy's logit gradients: the target's share, while the others' stay below 256 times of it (fp16 ends at 65504);
+// beyond, the target's is one small number among others.
+inline float unit_of(float smoothing) { return 1.f - smoothing >= 1.f / 256 ? 1.f - smoothing : 1.f; }
 __device__ inline int64_t target_of(const PrepArgs& a, int64_t n) {
     return a.target_wide ? ((const int64_t*)a.targets)[n] : (int64_t)((const int32_t*)a.targets)[n];
 }
@@ -976,7 +979,7 @@ template <class T> __global__ void __launch_bounds__(256) prep_kernel(PrepArgs a
         return;
     }
     // What a 16-bit gradient of a logit is relative to.  Cross entropy: the largest incoming gradient, times the target's own
-    // share 1 - smoothing: where all rows weigh the same, the entry of a target is then -1 + p / (1 - smoothing) and not some
+    // share 1 - smoothing (unit_of): where all rows weigh the same, the entry of a target is then -1 + p / (1 - smoothing) and not some
     // number whose rounding is the same in every row and adds up over them.  Log-probabilities in fp16: a power of two that brings
     // the largest bound of grad_rows_kernel to 2^13 .. 2^14, so that no gradient of a logit passes 2^15 and all of fp16's range below
     // is there for the smaller ones.
@@ -1016,7 +1019,7 @@ template <class T> __global__ void __launch_bounds__(256) prep_kernel(PrepArgs a
         b -= a.row_blocks;
         if (b == 0 && t == 0) {
             *a.r.live = base;
-            *a.r.scale = (a.mean && base > 0 ? scale / (float)base : scale) * a.hit;
+            *a.r.scale = (a.mean && base > 0 ? scale / (float)base : scale) * a.unit;
         }
         for (int i = wave; i < kPrepRows; i += 4) {
             const int at = base + b * kPrepRows + i;
@@ -1272,7 +1275,7 @@ struct SmallArgs {
     const void* targets;     // cross entropy
     int32_t target_wide;
     int64_t ignore;
-    float smoothing;
+    float smoothing, unit;
     float *zt, *lse, *loss;
     // gradients of the logits instead: of the packed rows, see dz_kernel
     const int32_t *live, *idx, *want;
@@ -1371,7 +1374,7 @@ template <class X, int MV, bool DZ> __global__ void __launch_bounds__(256) small
     __syncthreads();
     // wave q ends quarter q of every 32 outputs: v0 + 32 m + 8 q + 4 (lane / 32) .. + 3 of row lane % 32
     if constexpr (DZ) {
-        const float share = a.smoothing < 1.f ? 1.f / (1.f - a.smoothing) : 1.f, hit = a.smoothing < 1.f ? 1.f : 0.f;
+        const float share = 1.f / a.unit, hit = (1.f - a.smoothing) / a.unit;
         const float g = n < live ? a.g[n] : 0.f, lse = n < live ? a.glse[n] : 0.f, ref = lse == -INFINITY ? 0.f : lse;
         const int target = n < live ? a.want[n] : -1;
         const bool none = g == 0.f || lse == -INFINITY;
@@ -1778,7 +1781,7 @@ struct DzArgs {
     Logits l;
     const int32_t* target;
     const float *g, *lse;
-    float smoothing;
+    float smoothing, unit;
     int32_t outputs;         // all of them, not the piece's
     uint16_t* dz;            // [Npad][planes][pitch]
     int64_t pitch;
@@ -1828,8 +1831,7 @@ template <class X, bool BIG> __global__ void __launch_bounds__(Shape<BIG>::kThre
         stage_bias(a.l, t.tm * S::BM, S::BM, bias);
         t.run(a.p, lds, bias);
         // relative to g_max (1 - e): (p - e / V) / (1 - e) - [v = target]
-        const float even = a.smoothing / (float)a.outputs, share = a.smoothing < 1.f ? 1.f / (1.f - a.smoothing) : 1.f;
-        const float hit = a.smoothing < 1.f ? 1.f : 0.f;
+        const float even = a.smoothing / (float)a.outputs, share = 1.f / a.unit, hit = (1.f - a.smoothing) / a.unit;
         const int first = t.m(0, 0) - 4 * (t.lane >> 5);
         const bool whole = a.l.v0 + first + S::BM / S::WM <= a.l.V;
         __syncthreads();                                             // the tiles are read: their LDS takes the results
@@ -2536,7 +2538,7 @@ extern "C" int wf_linear_log_softmax_backward(const float* log_probs, const floa
         if (type == WF_F16) grad_rows_kernel<true><<<blocks, 256, 0, st>>>(grad, ldg, N, V, p.gpeak);
         else grad_rows_kernel<false><<<blocks, 256, 0, st>>>(grad, ldg, N, V, p.gpeak);
         PrepArgs r = {};
-        r.xp = p.xp; r.dx = dx; r.peak = p.gpeak; r.hit = 1.f; r.narrow = type == WF_F16;
+        r.xp = p.xp; r.dx = dx; r.peak = p.gpeak; r.unit = 1.f; r.narrow = type == WF_F16;
         if ((rc = run_prep(p, r, x, ldx, weight, ldw, st, &w))) return rc;
     }
     with_type(type, [&](auto t) {
@@ -2575,7 +2577,7 @@ extern "C" int wf_linear_cross_entropy(const void* x, int64_t ldx, int64_t N, in
     }
     Operand w;
     PrepArgs r = {};
-    r.xp = p.xp; r.targets = targets; r.target_wide = targets_wide; r.ignore = ignore_index; r.loss = loss; r.lse = lse; r.hit = 1.f;
+    r.xp = p.xp; r.targets = targets; r.target_wide = targets_wide; r.ignore = ignore_index; r.loss = loss; r.lse = lse; r.unit = 1.f;
     if ((rc = run_prep(p, r, x, ldx, weight, ldw, st, &w))) return rc;
     if ((rc = run_stats(p, w, packed_x(p), bias, bias_type, p.rows.live, p.rows.target, smoothing != 0.f, st))) return rc;
     JoinArgs j = {};
@@ -2605,11 +2607,11 @@ extern "C" int wf_linear_cross_entropy_backward(const float* grad, int32_t grad_
     Operand w;
     PrepArgs r = {};
     r.xp = p.xp; r.dx = dx; r.targets = targets; r.target_wide = targets_wide; r.ignore = ignore_index;
-    r.gout = grad; r.gout_rows = grad_rows; r.mean = mean; r.lse_in = lse; r.hit = smoothing < 1.f ? 1.f - smoothing : 1.f;
+    r.gout = grad; r.gout_rows = grad_rows; r.mean = mean; r.lse_in = lse; r.unit = unit_of(smoothing);
     if ((rc = run_prep(p, r, x, ldx, weight, ldw, st, &w))) return rc;
     if (p.small) {
         SmallArgs s = {};
-        s.x = x; s.w = weight; s.ldx = ldx; s.ldw = ldw; s.N = N; s.D = D; s.l = {bias, bias_type, 0, V}; s.smoothing = smoothing;
+        s.x = x; s.w = weight; s.ldx = ldx; s.ldw = ldw; s.N = N; s.D = D; s.l = {bias, bias_type, 0, V}; s.smoothing = smoothing; s.unit = unit_of(smoothing);
         s.live = p.rows.live; s.idx = p.rows.idx; s.want = p.rows.target; s.g = p.rows.g; s.glse = p.rows.lse; s.dz = p.dzp; s.zpitch = p.pitch;
         const int mv = small_mv(V);
         s.vtiles = (int)ceil_div(round_up(V, kBK), 32 * mv); s.ntiles = (int)ceil_div(round_up(N, kBK), 32);
@@ -2630,7 +2632,7 @@ extern "C" int wf_linear_cross_entropy_backward(const float* grad, int32_t grad_
         z.p = {wv, packed_x(p), (int32_t)ceil_div(width, p.dz.big ? 256 : 128), p.dz.nt, p.Dp / kBK, 1, {}, {}, p.rows.live, 0, 1};
         set_parts(&z.p, type, p.Dp, p.Dp);
         z.l = {bias, bias_type, (int32_t)v0, (int32_t)(v0 + width)};
-        z.target = p.rows.target; z.g = p.rows.g; z.lse = p.rows.lse; z.smoothing = smoothing; z.outputs = V; z.dz = p.dzp; z.pitch = p.pitch;
+        z.target = p.rows.target; z.g = p.rows.g; z.lse = p.rows.lse; z.smoothing = smoothing; z.unit = unit_of(smoothing); z.outputs = V; z.dz = p.dzp; z.pitch = p.pitch;
         with_type(type, [&](auto t) {
             with_big(p.dz.big, [&](auto b) {
                 rc = launch_tiles<Shape<decltype(b)::value>, dz_kernel<decltype(t), decltype(b)::value>>(z, st, kCUs / 2);
