@@ -467,8 +467,9 @@ int wf_dropout(const void* x, int64_t n, int32_t type, double p, uint64_t seed, 
  * wf_linear_cross_entropy_backward: grad: device, [N] (grad_rows) or one value for every row; `mean` as in the forward call.
  *   The gradients of the logits exist for pieces of the outputs, 256 MB at a time.
  * Both backward calls: dx [N][D], dweight [V][D] of `type`, dbias [V] of `bias_type`, each may be NULL.  16-bit types: the
- * gradient of a logit is rounded to `type` before the products (fp16: relative to the largest incoming gradient).  Sums run
- * in a fixed order: the same inputs give the same bits.                                                                  */
+ * gradient of a logit is rounded to `type` before the products (fp16: scaled so that the largest that can come lies at the
+ * upper end of the type's range: bits are lost below 2^-26 of it).  Sums run in a fixed order: the same inputs give the same
+ * bits.                                                                                                                  */
 int wf_linear_workspace_bytes(int32_t what, int64_t N, int32_t D, int32_t V, int32_t type, size_t* bytes);
 int wf_linear_log_softmax(const void* x, int64_t ldx, int64_t N, int32_t D, const void* weight, int64_t ldw, int32_t V, int32_t type,
                           const void* bias, int32_t bias_type, float* log_probs, void* workspace, size_t workspace_bytes,

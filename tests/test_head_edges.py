@@ -1,7 +1,8 @@
 """The output head's operators at the edges of what they promise.  Bounds as in test_head_linear.py: they count roundings.
 
 float16 gradients of logits are stored relative to a power of two: what `Case.products` takes as its last argument.  Log-probabilities:
-with B the largest of max |G| and |sum(G)| over the rows, B is 2^13 to 2^14 of it, so it is at most 2^-13 B."""
+with B the largest of max |G| and |sum(G)| over the rows, B is 2^13 to 2^14 of it, so it is at most 2^-13 B.  Cross entropy without
+label smoothing: the largest incoming gradient is 2^14 of it."""
 import pytest
 import torch
 
@@ -64,3 +65,19 @@ def test_label_smoothing_just_under_one(N, D, V, eps, dtype):
     got = torch.autograd.grad(wf.linear_cross_entropy(a[0], a[1], c.t, a[2], label_smoothing=eps, reduction="none"), a, up)
     with torch.no_grad():
         check_grads(got, c.products(*dz_of_entropy(c, up, eps), 2 * up.abs().max().item()), (N, D, V, eps))
+
+
+@gpu
+@pytest.mark.parametrize("N,D,V", [(40, 64, 59), (40, 64, 700), (300, 1031, 6007), (700, 640, 5001)])
+def test_half_precision_rows_of_unlike_weight(N, D, V):
+    c = Case(N, D, V, torch.float16)
+    up = (10.0 ** -(torch.arange(N) % 7).float()).to(DEV)
+    a = [v.detach().requires_grad_() for v in (c.x, c.w, c.b)]
+    got = torch.autograd.grad(wf.linear_cross_entropy(a[0], a[1], c.t, a[2], reduction="none"), a, up)
+    with torch.no_grad():
+        check_grads(got, c.products(*dz_of_entropy(c, up, 0.0), 2.0 ** -14), (N, D, V))
+        G = torch.randn(N, V, generator=c.g).to(DEV) * up[:, None]
+        most = torch.maximum(G.abs().amax(1), G.sum(1).abs()).max().item()
+    got = torch.autograd.grad(wf.linear_log_softmax(*a), a, G)
+    with torch.no_grad():
+        check_grads(got, c.products(*dz_of_log_softmax(c, G), most * 2.0 ** -13), (N, D, V))

@@ -903,7 +903,7 @@ struct Rows {                // in the workspace
     float* scale;            // [1] what the gradients of logits are relative to when they are rounded to 16 bits
     int32_t* idx;            // [Npad] row of packed row c
     int32_t* target;         // [Npad] its target, -1: none that is in range
-    float* g;                // [Npad] its incoming gradient relative to the largest
+    float* g;                // [Npad] its incoming gradient relative to the largest, times PrepArgs::lift
     float* lse;              // [Npad]
 };
 struct PrepArgs {
@@ -923,7 +923,7 @@ struct PrepArgs {
     int gout_rows, mean;
     const float* lse_in;
     int narrow;              // log-softmax backward in fp16: the gradients are scaled by peak's largest bound
-    float unit;              // backward: unit_of(smoothing)
+    float unit, lift;        // backward of cross entropy: unit_of(smoothing), lift_of(type, unit)
     int row_blocks, tail_blocks;         // workgroups over the rows, over the rows behind the last live one, then over W
     int32_t* count;          // per kCountRows rows: how many are live, and the largest row_peak; NULL: every workgroup looks itself
     float* most;
@@ -931,6 +931,9 @@ struct PrepArgs {
 // The unit of cross entropy's logit gradients: the target's share, while the others' stay below 256 times of it (fp16 ends at 65504);
 // beyond, the target's is one small number among others.
 inline float unit_of(float smoothing) { return 1.f - smoothing >= 1.f / 256 ? 1.f - smoothing : 1.f; }
+// fp16: in this unit the gradients of the row of the largest weight are at most 1 / unit; they are held 2^k times as large, up to 2^14
+// (a factor of 4 below the type's end), so that rows of 1e-5 of its weight keep their bits too.
+inline float lift_of(int type, float unit) { return type == WF_F16 ? ldexpf(1.f, 14 + ilogbf(unit)) : 1.f; }
 __device__ inline int64_t target_of(const PrepArgs& a, int64_t n) {
     return a.target_wide ? ((const int64_t*)a.targets)[n] : (int64_t)((const int32_t*)a.targets)[n];
 }
@@ -1019,7 +1022,7 @@ template <class T> __global__ void __launch_bounds__(256) prep_kernel(PrepArgs a
         b -= a.row_blocks;
         if (b == 0 && t == 0) {
             *a.r.live = base;
-            *a.r.scale = (a.mean && base > 0 ? scale / (float)base : scale) * a.unit;
+            *a.r.scale = (a.mean && base > 0 ? scale / (float)base : scale) * a.unit / a.lift;
         }
         for (int i = wave; i < kPrepRows; i += 4) {
             const int at = base + b * kPrepRows + i;
@@ -1044,7 +1047,7 @@ template <class T> __global__ void __launch_bounds__(256) prep_kernel(PrepArgs a
                 a.r.target[at] = want;
             }
             if (a.gout) {
-                a.r.g[at] = want < 0 ? 0.f : a.gout[a.gout_rows ? n : 0] / scale;
+                a.r.g[at] = want < 0 ? 0.f : a.gout[a.gout_rows ? n : 0] / scale * a.lift;
                 a.r.lse[at] = a.lse_in[n];
             }
         } else if (in) {
@@ -1830,7 +1833,7 @@ template <class X, bool BIG> __global__ void __launch_bounds__(Shape<BIG>::kThre
         using Tl = std::remove_reference_t<decltype(t)>;
         stage_bias(a.l, t.tm * S::BM, S::BM, bias);
         t.run(a.p, lds, bias);
-        // relative to g_max (1 - e): (p - e / V) / (1 - e) - [v = target]
+        // relative to g_max unit: (p - e / V) / unit - [v = target] (1 - e) / unit
         const float even = a.smoothing / (float)a.outputs, share = 1.f / a.unit, hit = (1.f - a.smoothing) / a.unit;
         const int first = t.m(0, 0) - 4 * (t.lane >> 5);
         const bool whole = a.l.v0 + first + S::BM / S::WM <= a.l.V;
@@ -2538,7 +2541,7 @@ extern "C" int wf_linear_log_softmax_backward(const float* log_probs, const floa
         if (type == WF_F16) grad_rows_kernel<true><<<blocks, 256, 0, st>>>(grad, ldg, N, V, p.gpeak);
         else grad_rows_kernel<false><<<blocks, 256, 0, st>>>(grad, ldg, N, V, p.gpeak);
         PrepArgs r = {};
-        r.xp = p.xp; r.dx = dx; r.peak = p.gpeak; r.unit = 1.f; r.narrow = type == WF_F16;
+        r.xp = p.xp; r.dx = dx; r.peak = p.gpeak; r.unit = r.lift = 1.f; r.narrow = type == WF_F16;
         if ((rc = run_prep(p, r, x, ldx, weight, ldw, st, &w))) return rc;
     }
     with_type(type, [&](auto t) {
@@ -2577,7 +2580,7 @@ extern "C" int wf_linear_cross_entropy(const void* x, int64_t ldx, int64_t N, in
     }
     Operand w;
     PrepArgs r = {};
-    r.xp = p.xp; r.targets = targets; r.target_wide = targets_wide; r.ignore = ignore_index; r.loss = loss; r.lse = lse; r.unit = 1.f;
+    r.xp = p.xp; r.targets = targets; r.target_wide = targets_wide; r.ignore = ignore_index; r.loss = loss; r.lse = lse; r.unit = r.lift = 1.f;
     if ((rc = run_prep(p, r, x, ldx, weight, ldw, st, &w))) return rc;
     if ((rc = run_stats(p, w, packed_x(p), bias, bias_type, p.rows.live, p.rows.target, smoothing != 0.f, st))) return rc;
     JoinArgs j = {};
@@ -2607,7 +2610,7 @@ extern "C" int wf_linear_cross_entropy_backward(const float* grad, int32_t grad_
     Operand w;
     PrepArgs r = {};
     r.xp = p.xp; r.dx = dx; r.targets = targets; r.target_wide = targets_wide; r.ignore = ignore_index;
-    r.gout = grad; r.gout_rows = grad_rows; r.mean = mean; r.lse_in = lse; r.unit = unit_of(smoothing);
+    r.gout = grad; r.gout_rows = grad_rows; r.mean = mean; r.lse_in = lse; r.unit = unit_of(smoothing); r.lift = lift_of(type, r.unit);
     if ((rc = run_prep(p, r, x, ldx, weight, ldw, st, &w))) return rc;
     if (p.small) {
         SmallArgs s = {};

@@ -128,7 +128,7 @@ def linear_log_softmax(x, weight, bias=None):
     computed to float32's accuracy (no reduced-precision product).  A bias of -inf masks an output; a row whose every output
     is masked is all -inf and has no gradient.  In the backward pass rows whose incoming gradient is all zero (frames behind an
     utterance's end) are left out whatever they hold; 16-bit types round the gradient of a logit to x's type before it enters
-    the products."""
+    the products (float16: scaled to the upper end of the type's range, bits are lost below 2^-26 of the largest)."""
     _check_linear("linear_log_softmax", x, weight, bias)
     return _run("linear_log_softmax", x, x, weight, None if bias is None else bias.contiguous())
 
