@@ -81,3 +81,25 @@ def test_half_precision_rows_of_unlike_weight(N, D, V):
     got = torch.autograd.grad(wf.linear_log_softmax(*a), a, G)
     with torch.no_grad():
         check_grads(got, c.products(*dz_of_log_softmax(c, G), most * 2.0 ** -13), (N, D, V))
+
+
+@gpu
+@pytest.mark.parametrize("N,D,V", [(40, 64, 59), (40, 64, 700), (3000, 257, 4099)])
+def test_half_precision_rows_beside_one_whose_gradient_is_not_finite(N, D, V):
+    c = Case(N, D, V, torch.float16)
+    up = torch.full((N,), 1e-6, device=DEV)
+    up[2] = float("inf")
+    up[5] = float("nan")
+    rows = torch.ones(N, dtype=torch.bool, device=DEV)
+    rows[[2, 5]] = False
+    a = [v.detach().requires_grad_() for v in (c.x, c.w, c.b)]
+    few = Case(N, D, V, torch.float16)
+    few.x, few.t = c.x[rows], c.t[rows]
+    dx, = torch.autograd.grad(wf.linear_cross_entropy(a[0], a[1], c.t, a[2], reduction="none"), a[:1], up)
+    with torch.no_grad():
+        check_grads((dx[rows],), few.products(*dz_of_entropy(few, up[rows], 0.0), 1e-6 * 2.0 ** -14), (N, D, V))
+        G = torch.randn(N, V, generator=c.g).to(DEV) * up[:, None]
+        most = torch.maximum(G[rows].abs().amax(1), G[rows].sum(1).abs()).max().item()
+    dx, = torch.autograd.grad(wf.linear_log_softmax(*a), a[:1], G)
+    with torch.no_grad():
+        check_grads((dx[rows],), few.products(*dz_of_log_softmax(few, G[rows]), most * 2.0 ** -13), (N, D, V))

@@ -938,7 +938,11 @@ __device__ inline int64_t target_of(const PrepArgs& a, int64_t n) {
     return a.target_wide ? ((const int64_t*)a.targets)[n] : (int64_t)((const int32_t*)a.targets)[n];
 }
 __device__ inline bool row_alive(const PrepArgs& a, int64_t n) { return a.targets ? target_of(a, n) != a.ignore : a.peak[n] != 0.f; }
-__device__ inline float row_peak(const PrepArgs& a, int64_t n) { return a.narrow ? a.peak[n] : row_alive(a, n) ? fabsf(a.gout[n]) : 0.f; }
+// (what is not finite stays in its row: it says nothing about the others' scale)
+__device__ inline float row_peak(const PrepArgs& a, int64_t n) {
+    const float v = a.narrow ? a.peak[n] : row_alive(a, n) ? fabsf(a.gout[n]) : 0.f;
+    return v < INFINITY ? v : 0.f;
+}
 
 // Everything before the products in one launch.  A workgroup of rows counts the live rows before its own by itself (no hand-over
 // between workgroups), gives its live rows their places by a wave's vote and packs them; others do the same for the up to 255
