@@ -103,3 +103,51 @@ def test_half_precision_rows_beside_one_whose_gradient_is_not_finite(N, D, V):
     dx, = torch.autograd.grad(wf.linear_log_softmax(*a), a[:1], G)
     with torch.no_grad():
         check_grads((dx[rows],), few.products(*dz_of_log_softmax(few, G[rows]), most * 2.0 ** -13), (N, D, V))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [63, 512, 1500, 3000, 5000, 8200, 20000])
+def test_layer_norm_rows_without_a_gradient_may_hold_anything(D, dtype):
+    g = torch.Generator().manual_seed(D)
+    x, dy = torch.randn(37, D, generator=g).to(dtype).to(DEV), torch.randn(37, D, generator=g).to(dtype).to(DEV)
+    w, b = torch.randn(D, generator=g).to(DEV), torch.randn(D, generator=g).to(DEV)
+    dead = [0, 5, 6, 7, 20, 36]
+    y = x.clone()
+    y[dead] = float("nan")
+    y[5] = float("inf")
+    y[20] = x[20]
+    y[20, D // 2] = float("-inf")
+    dy[dead] = 0
+    got = [torch.autograd.grad(wf.layer_norm(*a), a, dy) for a in ([t.detach().requires_grad_() for t in (v, w, b)] for v in (y, x))]
+    for p, q, what in zip(*got, ("dx", "dweight", "dbias")):
+        assert torch.equal(p, q), what                      # as if those rows were ordinary ones
+    assert not got[0][0][dead].any()
+    # one element of such a row that has a gradient: the row takes part, and nothing about it is hidden
+    dy[5, D - 1] = 1
+    a = [t.detach().requires_grad_() for t in (y, w, b)]
+    dx, dw, _ = torch.autograd.grad(wf.layer_norm(*a), a, dy)
+    assert torch.isnan(dx[5]).all() and torch.isnan(dw[D - 1])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_frames_behind_the_end_may_hold_anything_on_the_way_through_the_head(dtype):
+    torch.manual_seed(4)
+    head = wf.OutputHead(96, 58, dropout=0.2, device=DEV)
+    x = torch.randn(4, 30, 96, device=DEV).to(dtype)
+    length = torch.tensor([30, 21, 17, 5], device=DEV)
+    there = torch.arange(30, device=DEV) < length[:, None]
+    t = torch.where(there, torch.randint(0, 58, (4, 30), device=DEV), -1)
+    G = torch.randn(4, 30, 58, device=DEV) * there[..., None]
+    params = list(head.parameters())
+    got = []
+    for v in (x, torch.where(there[..., None], x, float("nan"))):
+        leaf = v.clone().requires_grad_()
+        torch.manual_seed(9)
+        lp = head(leaf)
+        a = torch.autograd.grad(lp, [leaf] + params, G)
+        torch.manual_seed(9)
+        got.append(a + torch.autograd.grad(head.cross_entropy(leaf, t), [leaf] + params))
+    for p, q in zip(*got):
+        assert torch.equal(p, q)

@@ -105,7 +105,8 @@ __device__ inline void store_any(void* p, int type, int64_t i, float v) {
 // a workgroup of max(4, WAVES) waves.  Backward in one pass as well: with xh = (x - mean) rstd and g = dy w,
 //   dx = rstd (g - mean(g) - xh mean(g xh)),   dw = sum_n dy xh,   db = sum_n dy;
 // every thread keeps the dw / db sums of its own columns in registers over the rows its workgroup walks, one partial row
-// per workgroup goes to the workspace and a second kernel adds the partial rows in a fixed order (no atomics).
+// per workgroup goes to the workspace and a second kernel adds the partial rows in a fixed order (no atomics).  A row whose every dy
+// is 0 has dx = 0 and no share in the sums, whatever it holds.
 //
 // Bound by HBM: 48000 x 1024 fp32 forward 75 us (5.2 TB/s, what a large copy reaches), backward 120 (4.9) + 5 for the fold;
 // 16000 x 512 bf16 9.7 + 12.5 + 3.9 us; one row of 512 2.4 us, a launch.
@@ -205,13 +206,25 @@ layer_norm_backward_kernel(LnArgs a) {
         const bool live = r < a.N;
         const T* x = (const T*)a.x + (live ? r : 0) * a.ldx;
         const T* dy = (const T*)a.dy + (live ? r : 0) * a.lddy;
-        const float mean = live ? a.stats[2 * r] : 0.f, rstd = live ? a.stats[2 * r + 1] : 0.f;
+        float mean = live ? a.stats[2 * r] : 0.f, rstd = live ? a.stats[2 * r + 1] : 0.f;
+        // a row that is not finite takes no part where it has no gradient (0 times NaN otherwise): each of its waves looks for one
+        bool held = live;
+        if (live && !(fabsf(mean) < INFINITY && rstd < INFINITY)) {
+            bool some = false;
+            for (int d = (threadIdx.x & 63) * VEC; d < a.D && !__any(some); d += 64 * VEC) {
+                const auto q = load_n<T, VEC>(dy + d, a.D - d);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) some |= to_f(q.v[i]) != 0.f;
+            }
+            held = __any(some);
+            if (!held) mean = rstd = 0.f;
+        }
         float xh[C][VEC], g[C][VEC];
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int d = (c * TPR + tr) * VEC;
-            const int n = live ? a.D - d : 0;
+            const int n = held ? a.D - d : 0;
             const auto p = load_n<T, VEC>(x + d, n);
             const auto q = load_n<T, VEC>(dy + d, n);
 #pragma unroll

@@ -68,7 +68,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension of ``x`` (at most 32768 elements).
 
     x: float32, bfloat16 or float16, any leading dimensions.  weight, bias: [D] or None, both of one of these types (fp32
-    weights beside bfloat16 activations are fine).  The result is contiguous and of x's type; statistics are fp32."""
+    weights beside bfloat16 activations are fine).  The result is contiguous and of x's type; statistics are fp32.  In the
+    backward pass rows whose incoming gradient is all zero take no part, whatever they hold."""
     _check(x, "x")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("layer_norm: x needs a last dimension of at least one element")
