@@ -151,3 +151,36 @@ def test_frames_behind_the_end_may_hold_anything_on_the_way_through_the_head(dty
         got.append(a + torch.autograd.grad(head.cross_entropy(leaf, t), [leaf] + params))
     for p, q in zip(*got):
         assert torch.equal(p, q)
+
+
+@gpu
+def test_saved_tensors_that_come_back_in_another_shape():
+    """As many elements in other rows: an error on the host before anything is launched, whichever saved tensor it is."""
+    x, w, b = torch.randn(2, 4, 64, device=DEV, requires_grad=True), torch.randn(50, 64, device=DEV, requires_grad=True), torch.randn(50, device=DEV, requires_grad=True)
+    t, g = torch.randint(0, 50, (2, 4), device=DEV), torch.ones(64, device=DEV, requires_grad=True)
+    calls = ((3, lambda: wf.layer_norm(x, g)), (4, lambda: wf.linear_log_softmax(x, w, b)), (5, lambda: wf.linear_cross_entropy(x, w, t, b)),
+             (5, lambda: wf.linear_cross_entropy(x, w, t, b, reduction="none")))
+    shapes = (lambda v: v.reshape(-1), lambda v: v.reshape(-1, 1), lambda v: v.transpose(0, -1), lambda v: v.reshape(2, -1), lambda v: v.reshape((-1,) + v.shape[2:]),
+              lambda v: v[None])
+    for saved, call in calls:
+        for k in range(saved):
+            for other in shapes:
+                seen = []
+
+                def unpack(v):
+                    seen.append(v)
+                    return other(v) if len(seen) == k + 1 else v
+
+                with torch.autograd.graph.saved_tensors_hooks(lambda v: v, unpack):
+                    y = call()
+                changed = False
+                try:
+                    y.sum().backward()
+                except RuntimeError as e:
+                    assert "came back" in str(e), e
+                    changed = True
+                assert len(seen) == saved and changed == (other(seen[k]).shape != seen[k].shape), (saved, k)
+    seed = torch.tensor([3], device=DEV)
+    with torch.autograd.graph.saved_tensors_hooks(lambda v: v, lambda v: v.reshape(())):       # one element in any shape
+        y = wf.dropout(x, 0.5, seed)
+    assert torch.equal(torch.autograd.grad(y.sum(), x)[0], wf.dropout(torch.ones_like(x), 0.5, 3))

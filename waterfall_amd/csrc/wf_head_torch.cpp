@@ -64,13 +64,16 @@ variable_list once(variable_list grads) {
         if (g.defined()) g = out[k++];
     return grads;
 }
-// A saved tensor as hooks hand it back: it has to be where the gradient is, of the type and size it had.
-const Tensor& back(const Tensor& t, const Tensor& grad, int64_t type, int64_t n) {
-    TORCH_CHECK(!t.defined() || (t.device() == grad.device() && (int64_t)t.scalar_type() == type && t.numel() == n),
-                "waterfall_amd.head: a saved tensor came back on another device, of another type or with another size");
+// A saved tensor as hooks hand it back: it has to be where the gradient is, of the type and shape it had (the entry points take their
+// sizes from it); strides and address may be others.
+const Tensor& back(const Tensor& t, const Tensor& grad, int64_t type, at::IntArrayRef shape) {
+    TORCH_CHECK(!t.defined() || (t.device() == grad.device() && (int64_t)t.scalar_type() == type && t.sizes() == shape),
+                "waterfall_amd.head: a saved tensor came back on another device, of another type or in another shape");
     return t;
 }
-Tensor back_whole(const Tensor& t, const Tensor& grad, int64_t type, int64_t n) { return back(t, grad, type, n).defined() ? t.contiguous() : t; }
+Tensor back_whole(const Tensor& t, const Tensor& grad, int64_t type, at::IntArrayRef shape) {
+    return back(t, grad, type, shape).defined() ? t.contiguous() : t;
+}
 int64_t of(const Tensor& t) { return t.defined() ? (int64_t)t.scalar_type() : 0; }
 constexpr int64_t kF32 = (int64_t)at::kFloat;
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
@@ -96,8 +99,8 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         const auto a = ctx->saved_data["a"].toIntVector();
-        const Rows v(back(saved[0], grads[0], a[4], a[5] * a[6])), g(grads[0]);
-        const Tensor weight = back_whole(saved[1], grads[0], a[2], a[6]), stats = back_whole(saved[2], grads[0], kF32, a[5] * 2);
+        const Rows v(back(saved[0], grads[0], a[4], grads[0].sizes())), g(grads[0]);
+        const Tensor weight = back_whole(saved[1], grads[0], a[2], {a[6]}), stats = back_whole(saved[2], grads[0], kF32, {a[5], 2});
         Tensor dx = at::empty(v.t.sizes(), v.t.options()), dw, db, ws;
         const auto par = v.t.options().dtype((at::ScalarType)a[2]);
         size_t n = 0;
@@ -129,7 +132,9 @@ struct Dropout : torch::autograd::Function<Dropout> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto a = ctx->saved_data["a"].toIntVector();
-        const Tensor dx = drop(grads[0], ctx->saved_data["p"].toDouble(), (uint64_t)a[0], back(ctx->get_saved_variables()[0], grads[0], (int64_t)at::kLong, 1), a[1]);
+        const Tensor seed = ctx->get_saved_variables()[0];
+        if (seed.defined()) back(seed.reshape({-1}), grads[0], (int64_t)at::kLong, {1});
+        const Tensor dx = drop(grads[0], ctx->saved_data["p"].toDouble(), (uint64_t)a[0], seed, a[1]);
         return once({dx, Tensor(), Tensor(), Tensor(), Tensor()});
     }
 };
@@ -170,8 +175,8 @@ struct LogSoftmax : torch::autograd::Function<LogSoftmax> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         const auto a = ctx->saved_data["a"].toIntVector();
-        const Rows v(back(saved[0], grads[0], a[4], a[6] * a[7])), w(back(saved[1], grads[0], a[4], a[8] * a[7])), g(grads[0]);
-        const Tensor bias = back(saved[2], grads[0], a[5], a[8]), lp = back_whole(saved[3], grads[0], kF32, a[6] * a[8]);
+        const Rows v(back(saved[0], grads[0], a[4], rows_of(grads[0], a[7]))), w(back(saved[1], grads[0], a[4], {a[8], a[7]})), g(grads[0]);
+        const Tensor bias = back(saved[2], grads[0], a[5], {a[8]}), lp = back_whole(saved[3], grads[0], kF32, grads[0].sizes());
         const Grads o(a, v, w, bias);
         const size_t n = linear_bytes(kLogBwd, v, w);
         const Tensor ws = workspace(n, v.t);
@@ -200,15 +205,18 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
         ctx->save_for_backward({v.t, w.t, targets, bias, lse});
         ctx->saved_data["a"] = std::vector<int64_t>{wants(x), wants(weight), wants(bias), stream, ignore, reduction, of(x), of(bias),
                                                     of(targets), v.n, v.d, w.n};
+        ctx->saved_data["x"] = x.sizes().vec();
         ctx->saved_data["s"] = smoothing;
         return total.defined() ? total : loss;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         const auto a = ctx->saved_data["a"].toIntVector();
-        const Rows v(back(saved[0], grads[0], a[6], a[9] * a[10])), w(back(saved[1], grads[0], a[6], a[11] * a[10]));
-        const Tensor targets = back_whole(saved[2], grads[0], a[8], a[9]), bias = back_whole(saved[3], grads[0], a[7], a[11]);
-        const Tensor lse = back_whole(saved[4], grads[0], kF32, a[9]), g = grads[0].contiguous();
+        const auto shape = ctx->saved_data["x"].toIntVector();
+        const Rows v(back(saved[0], grads[0], a[6], shape)), w(back(saved[1], grads[0], a[6], {a[11], a[10]}));
+        const Tensor targets = back_whole(saved[2], grads[0], a[8], at::IntArrayRef(shape).slice(0, shape.size() - 1));
+        const Tensor bias = back_whole(saved[3], grads[0], a[7], {a[11]}), lse = back_whole(saved[4], grads[0], kF32, {a[9]});
+        const Tensor g = grads[0].contiguous();
         const Grads o(a, v, w, bias);
         const size_t n = linear_bytes(kCeBwd, v, w);
         const Tensor ws = workspace(n, v.t);
