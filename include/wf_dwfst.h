@@ -457,7 +457,8 @@ int wf_dropout(const void* x, int64_t n, int32_t type, double p, uint64_t seed, 
  * (and no gradient), as an infeasible utterance has.  What is not finite in a row of x stays in that row's results.
  *
  * wf_linear_workspace_bytes: what = 0 wf_linear_log_softmax, 1 its backward, 2 wf_linear_cross_entropy, 3 its backward.
- *   Sizes beyond N 2^30, D 2^20, V 2^21: WF_EUNSUPPORTED; so are row strides of x or W of 2^30 elements and more.
+ *   Sizes beyond N 63 * 2^22, D 2^20, V 2^21: WF_EUNSUPPORTED; so are a product of more tiles than one launch takes (of the
+ *   order of N V = 2^39, N D = 2^39) and row strides of x or W of 2^30 elements and more.
  * wf_linear_log_softmax: log_probs fp32 [N][V] = z - logsumexp(z): what wf_fb_logsum takes.
  * wf_linear_log_softmax_backward: grad fp32 [N][V], `ldg` elements between rows.  Rows whose gradient is all zero (the frames
  *   behind an utterance's end) take no part: their x may hold anything.

@@ -3,10 +3,13 @@
 float16 gradients of logits are stored relative to a power of two: what `Case.products` takes as its last argument.  Log-probabilities:
 with B the largest of max |G| and |sum(G)| over the rows, B is 2^13 to 2^14 of it, so it is at most 2^-13 B.  Cross entropy without
 label smoothing: the largest incoming gradient is 2^14 of it."""
+import ctypes as C
+
 import pytest
 import torch
 
 import waterfall_amd as wf
+from waterfall_amd import _lib
 from tests.test_head_linear import Case, check_grads, dz_of_entropy, dz_of_log_softmax, DEV, TYPES
 
 gpu = pytest.mark.gpu
@@ -184,3 +187,27 @@ def test_saved_tensors_that_come_back_in_another_shape():
     with torch.autograd.graph.saved_tensors_hooks(lambda v: v, lambda v: v.reshape(())):       # one element in any shape
         y = wf.dropout(x, 0.5, seed)
     assert torch.equal(torch.autograd.grad(y.sum(), x)[0], wf.dropout(torch.ones_like(x), 0.5, 3))
+
+
+def test_sizes_that_no_launch_takes_are_refused():
+    lib, n = _lib.lib(), C.c_size_t(0)
+    for what, N, D, V, t, rc in ((1, 63 << 22, 8, 3, 1, 0), (1, (63 << 22) + 1, 8, 3, 1, -5), (0, 1 << 28, 8, 3, 0, -5), (2, 1 << 20, 64, 1 << 17, 1, 0),
+                                 (2, 1 << 22, 64, 1 << 20, 1, -5), (3, 1 << 22, 64, 1 << 20, 1, 0), (3, 1 << 27, 1 << 20, 300, 1, -5)):
+        assert lib.wf_linear_workspace_bytes(what, N, D, V, t, C.byref(n)) == rc, (what, N, D, V, t)
+
+
+@gpu
+def test_gradients_of_more_rows_than_one_launch_takes():
+    N, D, V = (1 << 26) + 70, 2, 3                          # a wave a row: more than 2^32 threads
+    if torch.cuda.mem_get_info(0)[0] < 100 << 30:
+        pytest.skip("needs 70 GB")
+    c = Case(2, D, V, torch.bfloat16)
+    c.N = N
+    g = torch.Generator(device=DEV).manual_seed(3)
+    c.x = torch.randn(N, D, generator=g, device=DEV).bfloat16()
+    G = torch.randn(N, V, generator=g, device=DEV)
+    G[torch.rand(N, generator=g, device=DEV) < 0.3] = 0
+    a = [v.detach().requires_grad_() for v in (c.x, c.w, c.b)]
+    got = torch.autograd.grad(wf.linear_log_softmax(*a), a, G)
+    with torch.no_grad():
+        check_grads(got, c.products(*dz_of_log_softmax(c, G)), (N, D, V))

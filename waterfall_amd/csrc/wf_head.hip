@@ -2025,9 +2025,9 @@ __global__ void __launch_bounds__(256) fold_kernel(FoldArgs a) {
 // Which rows of G hold anything: peak[n] = 0 where all of it is zero.  FULL: a bound of |G - p sum(G)| that is at most twice too
 // small, the larger of the largest magnitude and |sum(G)| (infinite where something is no number); else some value that is not 0, and a
 // row is read up to its first one.  A wave a row.  16000 x 5001, an eighth of the rows zero: 25 us, the reading of those.
-template <bool FULL> __global__ void __launch_bounds__(256) grad_rows_kernel(const float* G, int64_t ldg, int64_t N, int V, float* peak) {
+template <bool FULL> __global__ void __launch_bounds__(256) grad_rows_kernel(const float* G, int64_t ldg, int64_t first, int64_t N, int V, float* peak) {
     const int lane = threadIdx.x & 63;
-    const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t n = first + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (n >= N) return;
     const float* g = G + n * ldg;
     float m = 0.f, s = 0.f;
@@ -2059,12 +2059,13 @@ struct LogDzArgs {
     float* scale_out;
     uint16_t* dz;
     int64_t pitch;
+    int64_t first;           // packed row that this launch starts at
 };
 template <class X, int TPR, int R> __global__ void __launch_bounds__(256) log_dz_kernel(LogDzArgs a) {
     __shared__ float part[4];
     __shared__ int held[4];
     const int t = threadIdx.x % TPR;
-    const int64_t c = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    const int64_t c = a.first + (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
     const bool all = a.idx_out != nullptr;
     const int live = all ? (int)a.N : *a.live;
     if (c >= (int64_t)(live + kRowPad - 1) / kRowPad * kRowPad) return;      // (256 rows, whole workgroups)
@@ -2128,6 +2129,9 @@ template <class X, int TPR, int R> __global__ void __launch_bounds__(256) log_dz
 
 // ---- host side --------------------------------------------------------------------------------------------------------
 namespace {
+// A launch has fewer than 2^32 threads.  Kernels with a workgroup or a wave a row go over this many rows (a multiple of kRowPad) at a
+// time; those with 16 threads a row set the most rows of a call (and leave room for W's).
+constexpr int64_t kLaunchRows = (int64_t)1 << 22, kMaxRows = 63 * kLaunchRows;
 constexpr size_t kPieceBytes = (size_t)256 << 20;      // gradients of logits in hand at a time: what the last-level cache holds
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -2203,7 +2207,7 @@ int make_linear_plan(int what, int64_t N, int32_t D, int32_t V, int32_t type, vo
     if (!known_type(type)) return wf_fail(WF_EINVAL, "wf_linear: unknown element type");
     if (N < 0 || D < 1 || V < 1) return wf_fail(WF_EINVAL, "wf_linear: bad size (N %lld, D %d, V %d)", (long long)N, D, V);
     // (a tile's offsets are 32 bits: 256 rows of at most 2^22 x 2 bytes x 3 parts of an operand)
-    if (N > (1 << 30) || D > (1 << 20) || V > (1 << 21) || ceil_div(N, 128) * ceil_div(V, 128) > (1 << 29))
+    if (N > kMaxRows || D > (1 << 20) || V > (1 << 21) || ceil_div(N, 128) * ceil_div(V, 128) > (1 << 29))
         return wf_fail(WF_EUNSUPPORTED, "wf_linear: N %lld, D %d, V %d is beyond what one call takes", (long long)N, D, V);
     LinearPlan p = {};
     p.what = what; p.N = N; p.D = D; p.V = V; p.type = type;
@@ -2250,9 +2254,13 @@ int make_linear_plan(int what, int64_t N, int32_t D, int32_t V, int32_t type, vo
     p.xp = a.take<uint16_t>((size_t)p.Npad * p.parts * p.Dp);
     p.wp = a.take<uint16_t>((size_t)V * p.parts * p.Dp);
     const int64_t dits = (int64_t)products * p.Dp / kBK;
+    // (tiles of 256 threads per 128 x 128 or 512 per 256 x 256, and the spare ones of with_tile)
+    auto fits = [](const Grid& g) { return ((int64_t)g.mt * g.nt * g.splits + kCUs) * (g.big ? 512 : 256) < (int64_t)1 << 32; };
+    bool ok = true;
     if (!bwd) {
         p.fwd = plan_grid(V, N, dits, false);
         p.logp = plan_grid(N, V, dits, false);
+        ok = fits(p.fwd) && (what == kCeFwd || fits(p.logp));
         const size_t q = (size_t)p.fwd.mt * 2 * p.Npad;
         p.top = a.take<float>(q);
         p.sum = a.take<float>(q);
@@ -2268,11 +2276,13 @@ int make_linear_plan(int what, int64_t N, int32_t D, int32_t V, int32_t type, vo
         p.dz = plan_grid(p.width, N, dits, false);
         p.dx = plan_grid(D, N, products * p.pitch / kBK, true);
         p.dw = plan_grid(D, p.width, products * ceil_div(N, kBK), true);
+        ok = fits(p.dz) && fits(p.dx) && fits(p.dw);
         if (p.dx.splits > 1 || p.pieces > 1) p.part_x = a.take<float>((size_t)p.dx.splits * N * D);
         if (p.dw.splits > 1) p.part_w = a.take<float>((size_t)p.dw.splits * p.width * D);
         p.part_c = a.take<float>((size_t)p.dw.splits * p.width);
         if (what == kLogBwd) p.gpeak = a.take<float>(N);
     }
+    if (!ok) return wf_fail(WF_EUNSUPPORTED, "wf_linear: N %lld, D %d, V %d has more tiles than one launch takes", (long long)N, D, V);
     p.bytes = a.used + 256;
     *out = p;
     return WF_OK;
@@ -2545,29 +2555,34 @@ extern "C" int wf_linear_log_softmax_backward(const float* log_probs, const floa
     hipStream_t st = (hipStream_t)stream;
     if (N == 0) return (rc = zero_fill(dweight, (int64_t)V * D, type, st)) ? rc : zero_fill(dbias, V, bias_type, st);
     if (!log_probs || !grad || ldg < 0) return wf_fail(WF_EINVAL, "wf_linear_log_softmax_backward: null pointer");
-    const unsigned blocks = (unsigned)ceil_div(N, 4);
     // All rows in their places, those without a gradient masked, or (fp16: its scale comes first) counted and left out.  us, in place /
     // left out, V 59, D 512, an eighth of the rows without a gradient: fp32 2000: 25 / 33, 16000: 50 / 62, 100000: 183 / 216; bf16 2000:
     // 22 / 28, 16000: 43 / 44, 100000: 152 / 140; with nine tenths: fp32 16000 48 / 41, bf16 43 / 35.
     const bool in_place = p.small && (type == WF_F32 || (type == WF_BF16 && N <= 32768));
     Operand w;
-    LogDzArgs z = {grad, log_probs, p.rows.scale, ldg, p.rows.live, p.rows.idx, V, p.small, N, nullptr, nullptr, nullptr, p.dzp, p.pitch};
+    LogDzArgs z = {grad, log_probs, p.rows.scale, ldg, p.rows.live, p.rows.idx, V, p.small, N, nullptr, nullptr, nullptr, p.dzp, p.pitch, 0};
     if (in_place) {
         z.live_out = p.rows.live; z.idx_out = p.rows.idx; z.scale_out = p.rows.scale;
     } else {
-        if (type == WF_F16) grad_rows_kernel<true><<<blocks, 256, 0, st>>>(grad, ldg, N, V, p.gpeak);
-        else grad_rows_kernel<false><<<blocks, 256, 0, st>>>(grad, ldg, N, V, p.gpeak);
+        for (int64_t n = 0; n < N; n += kLaunchRows) {
+            const unsigned blocks = (unsigned)ceil_div(std::min(kLaunchRows, N - n), 4);
+            if (type == WF_F16) grad_rows_kernel<true><<<blocks, 256, 0, st>>>(grad, ldg, n, N, V, p.gpeak);
+            else grad_rows_kernel<false><<<blocks, 256, 0, st>>>(grad, ldg, n, N, V, p.gpeak);
+        }
         PrepArgs r = {};
         r.xp = p.xp; r.dx = dx; r.peak = p.gpeak; r.unit = r.lift = 1.f; r.narrow = type == WF_F16;
         if ((rc = run_prep(p, r, x, ldx, weight, ldw, st, &w))) return rc;
     }
     with_type(type, [&](auto t) {
         using X = decltype(t);
-        if (p.pitch <= 256) log_dz_kernel<X, 64, 1><<<(unsigned)(p.Npad / 4), 256, 0, st>>>(z);
-        else if (p.pitch <= 1024) log_dz_kernel<X, 64, 4><<<(unsigned)(p.Npad / 4), 256, 0, st>>>(z);
-        else if (p.pitch <= 6144) log_dz_kernel<X, 256, 6><<<(unsigned)p.Npad, 256, 0, st>>>(z);
-        else if (p.pitch <= 16384) log_dz_kernel<X, 256, 16><<<(unsigned)p.Npad, 256, 0, st>>>(z);
-        else log_dz_kernel<X, 256, 0><<<(unsigned)p.Npad, 256, 0, st>>>(z);
+        for (; z.first < p.Npad; z.first += kLaunchRows) {
+            const unsigned rows = (unsigned)std::min(kLaunchRows, p.Npad - z.first);
+            if (p.pitch <= 256) log_dz_kernel<X, 64, 1><<<rows / 4, 256, 0, st>>>(z);
+            else if (p.pitch <= 1024) log_dz_kernel<X, 64, 4><<<rows / 4, 256, 0, st>>>(z);
+            else if (p.pitch <= 6144) log_dz_kernel<X, 256, 6><<<rows, 256, 0, st>>>(z);
+            else if (p.pitch <= 16384) log_dz_kernel<X, 256, 16><<<rows, 256, 0, st>>>(z);
+            else log_dz_kernel<X, 256, 0><<<rows, 256, 0, st>>>(z);
+        }
     });
     HIP_TRY(hipGetLastError());
     if (p.small) return run_small_grads(p, x, ldx, weight, ldw, {dx, dweight, dbias, bias_type}, st);
