@@ -211,3 +211,37 @@ def test_gradients_of_more_rows_than_one_launch_takes():
     got = torch.autograd.grad(wf.linear_log_softmax(*a), a, G)
     with torch.no_grad():
         check_grads(got, c.products(*dz_of_log_softmax(c, G)), (N, D, V))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_capture_while_an_eager_graph_of_the_same_leaves_is_alive_is_refused(dtype):
+    head = wf.OutputHead(64, 200, device=DEV)
+    x, t = torch.randn(40, 64, device=DEV).to(dtype), torch.randint(0, 200, (40,), device=DEV)
+    params = list(head.parameters())
+
+    def step():
+        return torch.autograd.grad(head.cross_entropy(x, t), params)
+
+    def capture():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        return graph, out
+
+    alive = head.cross_entropy(x, t)                        # made on the default stream, as the leaves' accumulators are
+    with pytest.raises(RuntimeError, match="eager graph of the same leaves"):
+        capture()
+    want = torch.autograd.grad(alive, params)               # everything else goes on
+    del alive
+    graph, out = capture()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for p, q, r in zip(out, want, step()):
+            assert torch.equal(p, q) and torch.equal(p, r)

@@ -397,6 +397,12 @@ int ln_check(const char* who, const void* x, int64_t ldx, int64_t N, int32_t D, 
 }
 }  // namespace
 
+// 1 while work on `stream` is being captured (never the default stream's), for the autograd nodes
+extern "C" int wf_stream_captures(void* stream) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    return stream && hipStreamIsCapturing((hipStream_t)stream, &status) == hipSuccess && status == hipStreamCaptureStatusActive;
+}
+
 extern "C" int wf_layer_norm(const void* x, int64_t ldx, int64_t N, int32_t D, int32_t type, const void* weight, const void* bias,
                              int32_t param_type, float eps, void* y, float* stats, void* stream) {
     int rc = ln_check("wf_layer_norm", x, ldx, N, D, type, param_type);

@@ -4,9 +4,15 @@
 // of 8 x 16 x 64, forward and backward: 131 us with Python nodes).
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <ATen/TensorUtils.h>
+#include <c10/core/StreamGuard.h>
+
+#include <unordered_set>
 
 #include "../../include/wf_dwfst.h"
+
+extern "C" int wf_stream_captures(void* stream);                 // wf_head.hip: 1 while a graph is captured from it
 
 namespace {
 using at::Tensor;
@@ -79,6 +85,45 @@ constexpr int64_t kF32 = (int64_t)at::kFloat;
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 void* as_stream(int64_t s) { return (void*)(uintptr_t)s; }
 
+// the device's own handle of a stream (asked for under capture alone)
+void* handle_of(const c10::Stream& s) {
+    const c10::StreamGuard guard(s);
+    const pybind11::gil_scoped_acquire gil;
+    return as_stream(pybind11::module_::import("torch._C").attr("_cuda_getCurrentRawStream")((int)s.device_index()).cast<int64_t>());
+}
+// A backward pass that is being captured hands its gradients to the nodes behind it, on the streams where those were made.  The
+// accumulator of a leaf that an eager graph uses too is that graph's: the engine would draw the default stream into the capture, or
+// another one that nothing joins again, and the process ends when the capture does.  Said here, before it happens.
+void no_eager_leaves(int64_t stream) {
+    if (!wf_stream_captures(as_stream(stream))) return;
+    using torch::autograd::Node;
+    const auto* runs = torch::autograd::get_current_graph_task_exec_info();      // empty: everything runs
+    std::unordered_set<Node*> seen;
+    std::vector<Node*> next{torch::autograd::get_current_node().get()};
+    while (!next.empty()) {
+        Node* at = next.back();
+        next.pop_back();
+        if (!at) continue;
+        for (const auto& e : at->next_edges()) {
+            Node* to = e.function.get();
+            if (!to || !seen.insert(to).second) continue;
+            bool taken = false;                                  // its gradient is asked for, and it is not run itself
+            if (runs && !runs->empty()) {
+                const auto it = runs->find(to);
+                if (it == runs->end() || !it->second.should_execute()) continue;
+                taken = !it->second.needed_;
+            }
+            if (const auto own = to->stream()) {
+                void* s = handle_of(*own);
+                TORCH_CHECK(s == as_stream(stream) || (s && !taken) || wf_stream_captures(s),
+                            "waterfall_amd.head: a backward pass cannot be captured while an eager graph of the same leaves is alive (", to->name(),
+                            " belongs to another stream): delete its outputs first");
+            }
+            if (!taken) next.push_back(to);
+        }
+    }
+}
+
 // (the engine runs backward with the forward's device and stream current: the stream is kept as it came)
 struct LayerNorm : torch::autograd::Function<LayerNorm> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Maybe& weight_, const Maybe& bias_, double eps, int64_t stream) {
@@ -99,6 +144,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         const auto a = ctx->saved_data["a"].toIntVector();
+        no_eager_leaves(a[3]);
         const Rows v(back(saved[0], grads[0], a[4], grads[0].sizes())), g(grads[0]);
         const Tensor weight = back_whole(saved[1], grads[0], a[2], {a[6]}), stats = back_whole(saved[2], grads[0], kF32, {a[5], 2});
         Tensor dx = at::empty(v.t.sizes(), v.t.options()), dw, db, ws;
@@ -132,6 +178,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto a = ctx->saved_data["a"].toIntVector();
+        no_eager_leaves(a[1]);
         const Tensor seed = ctx->get_saved_variables()[0];
         if (seed.defined()) back(seed.reshape({-1}), grads[0], (int64_t)at::kLong, {1});
         const Tensor dx = drop(grads[0], ctx->saved_data["p"].toDouble(), (uint64_t)a[0], seed, a[1]);
@@ -175,6 +222,7 @@ struct LogSoftmax : torch::autograd::Function<LogSoftmax> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         const auto a = ctx->saved_data["a"].toIntVector();
+        no_eager_leaves(a[3]);
         const Rows v(back(saved[0], grads[0], a[4], rows_of(grads[0], a[7]))), w(back(saved[1], grads[0], a[4], {a[8], a[7]})), g(grads[0]);
         const Tensor bias = back(saved[2], grads[0], a[5], {a[8]}), lp = back_whole(saved[3], grads[0], kF32, grads[0].sizes());
         const Grads o(a, v, w, bias);
@@ -212,6 +260,7 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         const auto a = ctx->saved_data["a"].toIntVector();
+        no_eager_leaves(a[3]);
         const auto shape = ctx->saved_data["x"].toIntVector();
         const Rows v(back(saved[0], grads[0], a[6], shape)), w(back(saved[1], grads[0], a[6], {a[11], a[10]}));
         const Tensor targets = back_whole(saved[2], grads[0], a[8], at::IntArrayRef(shape).slice(0, shape.size() - 1));

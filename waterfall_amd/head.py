@@ -7,7 +7,9 @@ entropy on the same projection, is a kernel of the library with its own gradient
     lp = linear_log_softmax(x, weight, bias)      fp32 log-probabilities, what DenseFsaVec takes
     ce = linear_cross_entropy(x, weight, targets, bias)   the logits are never kept
 
-``OutputHead`` is the module over them.  All run on the current stream of the tensors' device and can be captured in a graph.
+``OutputHead`` is the module over them.  All run on the current stream of the tensors' device and can be captured in a graph; a
+backward pass only while no eager graph of the same leaves is alive (a loss that was kept, say): it raises, since torch's engine would
+draw that graph's stream into the capture.
 """
 import torch
 from torch import nn
