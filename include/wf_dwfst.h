@@ -437,7 +437,7 @@ int wf_timing_read(float* ms);
  *   D <= 32768 (WF_EUNSUPPORTED beyond).
  * wf_layer_norm_backward: dx [N][D] of `type`; dweight / dbias [D] of `param_type`, either may be NULL (then no workspace is
  *   needed when both are).  Sums over the rows run in a fixed order: the same inputs give the same bits.  A row whose every
- *   dy is 0 may hold anything: dx 0, no share in the sums.                                                               */
+ *   dy is 0 may hold anything: dx 0, no share in the sums.  dx overlaps neither dy nor x.                                */
 int wf_layer_norm(const void* x, int64_t ldx, int64_t N, int32_t D, int32_t type, const void* weight, const void* bias,
                   int32_t param_type, float eps, void* y, float* stats, void* stream);
 int wf_layer_norm_backward_workspace_bytes(int64_t N, int32_t D, int32_t type, size_t* bytes);

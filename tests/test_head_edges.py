@@ -11,6 +11,7 @@ import torch
 import waterfall_amd as wf
 from waterfall_amd import _lib
 from tests.test_head_linear import Case, check_grads, dz_of_entropy, dz_of_log_softmax, DEV, TYPES
+from tests.test_head_rows import norm64, U, within
 
 gpu = pytest.mark.gpu
 
@@ -245,3 +246,26 @@ def test_a_capture_while_an_eager_graph_of_the_same_leaves_is_alive_is_refused(d
         torch.cuda.synchronize()
         for p, q, r in zip(out, want, step()):
             assert torch.equal(p, q) and torch.equal(p, r)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(3, 1025), (37, 1280), (300, 1536), (2, 2047), (9, 2048), (1, 4099), (270, 6001), (3, 8191), (5, 12007), (2, 30001)])
+def test_layer_norm_of_wide_rows(shape, dtype):
+    """Every way of sharing a row that test_head_rows.py has no length of: the last piece whole, of one element, of all but one."""
+    g = torch.Generator().manual_seed(shape[1])
+    D = shape[-1]
+    x = (torch.randn(shape, generator=g) * 1.5 + 0.7).to(dtype)
+    w, b = (torch.randn(D, generator=g) + 1).to(dtype), torch.randn(D, generator=g).to(dtype)
+    dy = torch.randn(shape, generator=g).to(dtype)
+    leaves = [v.to(DEV).requires_grad_() for v in (x, w, b)]
+    y = wf.layer_norm(*leaves)
+    got = torch.autograd.grad(y, leaves, dy.to(DEV))
+    want, dx, dw, db, adw, adb, r, gw, h = norm64(x, w, b, 1e-5, dy)
+    u, f = U[dtype], 32 * U[torch.float32]                  # (bounds of test_head_rows.py: sums of 32 elements a lane are as deep)
+    big = x.double().abs().amax(-1, keepdim=True)
+    within(y.detach(), want, u * want.abs() + f * ((big * r + h.abs()) * w.double().abs() + want.abs()) + 1e-30, "y")
+    size = r * (gw.abs() + gw.abs().mean(-1, keepdim=True) + (h.abs() + big * r) * (1 + (gw * h).abs().mean(-1, keepdim=True) + gw.abs().amax(-1, keepdim=True)))
+    within(got[0], dx, u * dx.abs() + f * size, "dx")
+    within(got[1], dw, u * dw.abs() + f * (1 + shape[0] / 4096) * (adw + (dy.double().abs() * big * r).sum(0)), "dweight")
+    within(got[2], db, u * db.abs() + f * (1 + shape[0] / 4096) * adb, "dbias")

@@ -102,14 +102,17 @@ __device__ inline void store_any(void* p, int type, int64_t i, float v) {
 //
 // y = (x - mean) rstd w + b over a row of D.  One pass over HBM: the row stays in registers between the mean, the variance
 // about that mean (two sums, no E[x^2] - mean^2 cancellation) and the result.  WAVES waves share a row (1, 4 or 16 by D);
-// a workgroup of max(4, WAVES) waves.  Backward in one pass as well: with xh = (x - mean) rstd and g = dy w,
+// a workgroup of max(4, WAVES) waves.  Backward in one pass over HBM as well (lanes of 32 elements, 16-bit rows of 1025 - 2048 and
+// above 4096 and fp32 rows above 16384, read theirs a second time from the cache): with xh = (x - mean) rstd and g = dy w,
 //   dx = rstd (g - mean(g) - xh mean(g xh)),   dw = sum_n dy xh,   db = sum_n dy;
 // every thread keeps the dw / db sums of its own columns in registers over the rows its workgroup walks, one partial row
 // per workgroup goes to the workspace and a second kernel adds the partial rows in a fixed order (no atomics).  A row whose every dy
 // is 0 has dx = 0 and no share in the sums, whatever it holds.
 //
 // Bound by HBM: 48000 x 1024 fp32 forward 75 us (5.2 TB/s, what a large copy reaches), backward 120 (4.9) + 5 for the fold;
-// 16000 x 512 bf16 9.7 + 12.5 + 3.9 us; one row of 512 2.4 us, a launch.
+// 16000 x 512 bf16 9.7 + 12.5 + 3.9 us; one row of 512 2.4 us, a launch.  Backward of 2^25 elements of bf16 with the fold, D 1024, 1280,
+// 2048, 8192, 32768: 40, 55, 67, 66, 110 us (with such rows held in fp32, in scratch memory for the most part: 346 at 1280, 240 at 2048).
+// The forward pass of 16-bit rows above 8192 keeps 92 registers there: 2796 x 12000 69 us, 1.9 TB/s.
 
 constexpr int kLnVecs = 4;                 // 16-byte pieces of a row that a lane holds at most
 template <class T> constexpr int vec_of() { return 16 / (int)sizeof(T); }
@@ -187,63 +190,106 @@ layer_norm_kernel(LnArgs a) {
     }
 }
 
+// Whether anything of a row is not 0, by one wave.
+template <class T> __device__ inline bool has_any(const T* p, int n) {
+    constexpr int VEC = vec_of<T>();
+    bool some = false;
+    for (int d = (threadIdx.x & 63) * VEC; d < n && !__any(some); d += 64 * VEC) {
+        const auto q = load_n<T, VEC>(p + d, n - d);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) some |= to_f(q.v[i]) != 0.f;
+    }
+    return __any(some);
+}
 template <class T, int WAVES, int C> __global__ void __launch_bounds__(1024)
 layer_norm_backward_kernel(LnArgs a) {
     constexpr int VEC = vec_of<T>(), TPR = WAVES * 64, RPB = 16 / WAVES;   // rows a workgroup of 16 waves has in hand
+    // A lane of up to 16 elements holds (x - mean) rstd, dy w and w of them.  One of 32 has registers for its sums alone (AGAIN): it goes
+    // over x, dy and w piece by piece, twice (the second time from the cache).  Its pieces are whole, without a branch: the row's last
+    // one starts early and leaves its first `skip` elements to the lane before it.
+    constexpr bool AGAIN = C * VEC > 16;
+    constexpr int H = AGAIN ? 1 : C;
     __shared__ float red[WAVES > 1 ? 2 * 16 : 1];
     __shared__ float fold[WAVES == 16 ? 1 : 16 * 64 * VEC];
-    const int tr = threadIdx.x % TPR, slot = threadIdx.x / TPR;
-    float dw[C][VEC] = {}, db[C][VEC] = {}, w[C][VEC];
+    int tr = threadIdx.x % TPR;
+    const int slot = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);    // (a wave has one row)
+    float dw[C][VEC] = {}, db[C][VEC] = {}, w[H][VEC];
+    if constexpr (!AGAIN)
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-        const int d = (c * TPR + tr) * VEC;
-        load_params<VEC>(a.w, a.ptype, d, a.D - d, 1.f, w[c]);
-    }
+        for (int c = 0; c < C; ++c) {
+            const int d = (c * TPR + tr) * VEC;
+            load_params<VEC>(a.w, a.ptype, d, a.D - d, 1.f, w[c]);
+        }
+    auto start = [&](int c) { return min((c * TPR + tr) * VEC, a.D - VEC); };       // (AGAIN)
     const float inv = 1.f / (float)a.D;
-    // rounds of gridDim * RPB rows; the trip count is the same for all waves of a workgroup (barriers inside)
-    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.N; r0 += (int64_t)gridDim.x * RPB) {
+    // rounds of gridDim * RPB rows; the trip count is the same for all waves of a workgroup (barriers inside).  A row's statistics are
+    // read a round ahead: where its x is read depends on them.
+    const int64_t first = (int64_t)blockIdx.x * RPB, step = (int64_t)gridDim.x * RPB;
+    auto stat = [&](int64_t r, int k) { return r < a.N ? a.stats[2 * r + k] : 0.f; };
+    float mean1 = stat(first + slot, 0), rstd1 = stat(first + slot, 1);
+    for (int64_t r0 = first; r0 < a.N; r0 += step) {
+        asm volatile("" : "+v"(tr));       // (offsets are computed for every row: kept over the loop, they take the registers a row needs)
         const int64_t r = r0 + slot;
         const bool live = r < a.N;
         const T* x = (const T*)a.x + (live ? r : 0) * a.ldx;
         const T* dy = (const T*)a.dy + (live ? r : 0) * a.lddy;
-        float mean = live ? a.stats[2 * r] : 0.f, rstd = live ? a.stats[2 * r + 1] : 0.f;
-        // a row that is not finite takes no part where it has no gradient (0 times NaN otherwise): each of its waves looks for one
-        bool held = live;
-        if (live && !(fabsf(mean) < INFINITY && rstd < INFINITY)) {
-            bool some = false;
-            for (int d = (threadIdx.x & 63) * VEC; d < a.D && !__any(some); d += 64 * VEC) {
-                const auto q = load_n<T, VEC>(dy + d, a.D - d);
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) some |= to_f(q.v[i]) != 0.f;
-            }
-            held = __any(some);
-            if (!held) mean = rstd = 0.f;
+        float mean = mean1, rstd = rstd1;
+        // a row that is not finite takes no part where it has no gradient (0 times NaN otherwise): its zeros stand in for x
+        if (live && !(fabsf(mean) < INFINITY && rstd < INFINITY) && !has_any<T>(dy, a.D)) {
+            x = dy;
+            mean = rstd = 0.f;
         }
-        float xh[C][VEC], g[C][VEC];
+        mean1 = stat(r + step, 0);
+        rstd1 = stat(r + step, 1);
+        float xh[H][VEC], g[H][VEC];
         float s1 = 0.f, s2 = 0.f;
+        auto again = [&](int c, auto&& f) {
+            Pack<T, VEC> p, q;
+            __builtin_memcpy(&p, x + start(c), sizeof(p));
+            __builtin_memcpy(&q, dy + start(c), sizeof(q));
+            load_params<VEC>(a.w, a.ptype, start(c), VEC, 1.f, w[0]);
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int d = (c * TPR + tr) * VEC;
-            const int n = held ? a.D - d : 0;
-            const auto p = load_n<T, VEC>(x + d, n);
-            const auto q = load_n<T, VEC>(dy + d, n);
+            for (int i = 0; i < VEC; ++i) f(i, (to_f(p.v[i]) - mean) * rstd, to_f(q.v[i]), w[0][i]);
+        };
+        if constexpr (AGAIN) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const float xi = i < n ? (to_f(p.v[i]) - mean) * rstd : 0.f, gi = to_f(q.v[i]);
-                dw[c][i] += gi * xi;
-                db[c][i] += gi;
-                xh[c][i] = xi;
-                g[c][i] = gi * w[c][i];
-                s1 += g[c][i];
-                s2 += g[c][i] * xi;
+            for (int c = 0; c < C; ++c) {
+                const int skip = live ? (c * TPR + tr) * VEC - start(c) : VEC;
+                again(c, [&](int i, float xi, float gi, float wi) {
+                    xi = i < skip ? 0.f : xi;
+                    gi = i < skip ? 0.f : gi;
+                    dw[c][i] += gi * xi;
+                    db[c][i] += gi;
+                    s1 += gi * wi;
+                    s2 += gi * wi * xi;
+                });
+                // (piece by piece: put off to the end, a piece's sums would hold its values until then)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) asm volatile("" : "+v"(dw[c][i]), "+v"(db[c][i]));
+                asm volatile("" : "+v"(s1), "+v"(s2) :: "memory");
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const int d = (c * TPR + tr) * VEC;
+                const int n = live ? a.D - d : 0;
+                const auto p = load_n<T, VEC>(x + d, n);
+                const auto q = load_n<T, VEC>(dy + d, n);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const float xi = i < n ? (to_f(p.v[i]) - mean) * rstd : 0.f, gi = to_f(q.v[i]);
+                    dw[c][i] += gi * xi;
+                    db[c][i] += gi;
+                    xh[c][i] = xi;
+                    g[c][i] = gi * w[c][i];
+                    s1 += g[c][i];
+                    s2 += g[c][i] * xi;
+                }
             }
         }
-        if constexpr (WAVES == 1) {
-            s1 = wave_sum(s1);
-            s2 = wave_sum(s2);
-        } else {                           // the waves of one row meet in LDS
-            s1 = wave_sum(s1);
-            s2 = wave_sum(s2);
+        s1 = wave_sum(s1);
+        s2 = wave_sum(s2);
+        if constexpr (WAVES > 1) {         // the waves of one row meet in LDS
             const int wv = threadIdx.x >> 6;
             __syncthreads();
             if ((threadIdx.x & 63) == 0) { red[wv] = s1; red[16 + wv] = s2; }
@@ -256,14 +302,20 @@ layer_norm_backward_kernel(LnArgs a) {
         s2 *= inv;
         if (live) {
             T* dx = (T*)a.y + r * (int64_t)a.D;
+            if constexpr (AGAIN) asm volatile("" : "+v"(tr));
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 const int d = (c * TPR + tr) * VEC;
                 if (d >= a.D) break;
-                Pack<T, VEC> p;
+                Pack<T, VEC> o;
+                if constexpr (AGAIN) {     // (a shared element is the same from both lanes)
+                    again(c, [&](int i, float xi, float gi, float wi) { o.v[i] = (T)(rstd * (gi * wi - s1 - xi * s2)); });
+                    __builtin_memcpy(dx + start(c), &o, sizeof(o));
+                } else {
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) p.v[i] = (T)(rstd * (g[c][i] - s1 - xh[c][i] * s2));
-                store_n<T, VEC>(dx + d, p, a.D - d);
+                    for (int i = 0; i < VEC; ++i) o.v[i] = (T)(rstd * (g[c][i] - s1 - xh[c][i] * s2));
+                    store_n<T, VEC>(dx + d, o, a.D - d);
+                }
             }
         }
     }
@@ -275,15 +327,17 @@ layer_norm_backward_kernel(LnArgs a) {
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             float(&v)[C][VEC] = k ? db : dw;
+            const int skip = AGAIN ? (c * TPR + tr) * VEC - start(c) : 0;
             if constexpr (WAVES == 16) {
-                const int d = (c * TPR + tr) * VEC;
+                const int d = (c * TPR + tr) * VEC - skip;
 #pragma unroll
                 for (int i = 0; i < VEC; ++i)
-                    if (d + i < a.D) part[(size_t)k * a.D + d + i] = v[c][i];
+                    if (i >= skip && d + i < a.D) part[(size_t)k * a.D + d + i] = v[c][i];
             } else {
                 __syncthreads();
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) fold[(slot * TPR + tr) * VEC + i] = v[c][i];
+                for (int i = 0; i < VEC; ++i)
+                    if (i >= skip) fold[(slot * TPR + tr) * VEC + i - skip] = v[c][i];
                 __syncthreads();
                 for (int j = threadIdx.x; j < TPR * VEC; j += 1024) {
                     float s = 0.f;
@@ -379,8 +433,8 @@ template <class T, class F> void with_ln_shape(int D, F&& f) {
     else if (in(1, 4)) f(integral_constant<int, 1>(), integral_constant<int, 4>());
     else if (in(4, 2)) f(integral_constant<int, 4>(), integral_constant<int, 2>());
     else if (in(4, 4)) f(integral_constant<int, 4>(), integral_constant<int, 4>());
-    else if (in(16, 4)) f(integral_constant<int, 16>(), integral_constant<int, 4>());
-    else f(integral_constant<int, 16>(), integral_constant<int, 8>());      // fp32 rows above 16384
+    else if (VEC == 8 || in(16, 4)) f(integral_constant<int, 16>(), integral_constant<int, 4>());
+    else if constexpr (VEC == 4) f(integral_constant<int, 16>(), integral_constant<int, 8>());      // fp32 rows above 16384
 }
 template <class F> void with_type(int type, F&& f) {
     if (type == WF_F32) f(float());
