@@ -452,9 +452,11 @@ int wf_layer_norm_backward(const void* dy, int64_t lddy, const void* x, int64_t 
 int wf_dropout(const void* x, int64_t n, int32_t type, double p, uint64_t seed, const uint64_t* seed_dev, void* y, void* stream);
 
 /* The projection z = x W^T + b (x [N][D], W [V][D], both of `type`; bias [V] of `bias_type` or NULL) and what ends it.  fp32
- * operands are multiplied in three exact bf16 parts (errors of fp32's own size), 16-bit ones as they are, sums in fp32.
+ * operands are multiplied in three exact bf16 parts (a product is off by less than 2^-21 of itself, 2^-24.5 on average), 16-bit
+ * ones as they are, sums in fp32.
  * An output whose bias is -inf is masked: probability 0.  A row whose every output is masked has log-probabilities of -inf
- * (and no gradient), as an infeasible utterance has.  What is not finite in a row of x stays in that row's results.
+ * (and no gradient), as an infeasible utterance has.  What is not finite in a row of x stays in that row's results
+ * (and in the sums over the rows, where it has a gradient).
  *
  * wf_linear_workspace_bytes: what = 0 wf_linear_log_softmax, 1 its backward, 2 wf_linear_cross_entropy, 3 its backward.
  *   Sizes beyond N 63 * 2^22, D 2^20, V 2^21: WF_EUNSUPPORTED; so are a product of more tiles than one launch takes (of the

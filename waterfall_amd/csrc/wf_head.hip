@@ -535,9 +535,11 @@ extern "C" int wf_dropout(const void* x, int64_t n, int32_t type, double p, uint
 //
 // Forward of both losses, and every product of their gradients, is one tiled matrix product on the matrix cores with its own
 // epilogue.  Operands are 16-bit.  fp32 operands are split exactly into three bf16 parts by truncation (8 + 8 + 8 bits of the
-// 24) and the six products of parts down to 2^-16 of the leading one are summed in the same fp32 accumulators: the three
-// that are left out are below 2^-23 of |a||b|, the size of fp32's own rounding.  (At 1/6 of the 16-bit rate that is still 2.6
-// times what the fp32 matrix instructions could give.)
+// 24) and the six products of parts down to 2^-16 of the leading one are summed in the same fp32 accumulators.  What the three
+// that are left out come to has the sign of a b and is below 2^-21 of it (the second part is below 2^-7 of the value, the third
+// below 2^-15), 2^-24.5 on average over normal values: one rounding of fp32.  (Parts rounded to nearest would halve each, for one
+// more instruction a part and element in kernels that the splitting bounds.)  At 1/6 of the 16-bit rate that is still 2.6 times
+// what the fp32 matrix instructions could give.
 //
 // A tile is staged by direct global -> LDS loads, double buffered, one barrier per 64 of K.  An operand is stored either
 // with K contiguous (rows of 64 K values are staged, fragments are plain 16-byte LDS reads) or with K as its row index (64
@@ -2197,7 +2199,8 @@ constexpr size_t kPieceBytes = (size_t)256 << 20;      // gradients of logits in
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 
-// Tile shape and K splits of a product of m x n over `its` K tiles.  256 x 256 tiles run one per CU at 1.15 times the rate of
+// Tile shape and K splits of a product of m x n over `its` K tiles.  (Every round of the chip is priced as a full one, also where with_tile
+// halves the last: near the border 128 x 128 tiles may be taken where 256 x 256 with halves would do as well.)  256 x 256 tiles run one per CU at 1.15 times the rate of
 // 128 x 128 tiles, which run two per CU (measured at 5120 x 16384 x 512: 926 against 837 TFLOP/s; 4096^3: 1172 / 983); the
 // cheaper of both by rounds of the chip is taken.  A product that does not fill the chip is split over K while a split
 // keeps 8 K tiles.  A tile's prologue and epilogue cost about 6 K tiles, 12 where it writes partial sums (gradients of cross entropy,
@@ -2234,6 +2237,8 @@ struct Arena {               // carves the workspace; with base == NULL it only 
 //   gradients of cross entropy: fp32 8: 36 / 75, 256: 72 / 104, 512: 109 / 122; bf16 8: 24 / 38, 128: 35 / 43, 256: 45 / 46, 512:
 //     65 / 55; of V 15001, D 1024: fp32 64: 104 / 169, 256: 267 / 246, bf16 64: 67 / 62; of V 59: 16000: fp32 67 / 115, bf16 48 / 57,
 //     100000: 279 / 580, 174 / 212; of V 128: 16000: 99 / 123, 66 / 59
+// One limit for both directions, between the gradients' crossings: log-probabilities alone cross later where W is large (bf16, 64 rows
+// of V 15001, D 1024, and fp32, 1024 rows of V 5001, take the tiles).
 constexpr int kSmallOutputs = 128;
 constexpr double kSmallWork = 0.7e9, kSmallWorkF32 = 1.6e9;      // N V D
 bool is_small(int64_t N, int32_t D, int32_t V, int type, bool bwd) {

@@ -127,10 +127,10 @@ def _check_linear(who, x, weight, bias):
 def linear_log_softmax(x, weight, bias=None):
     """log_softmax(x weight^T + bias) as float32 [..., V]: the log-probabilities that ``DenseFsaVec`` takes.
 
-    x [..., D], weight [V, D]: float32, bfloat16 or float16, both of one type; bias [V] or None, any of the three.  float32 is
-    computed to float32's accuracy (no reduced-precision product).  A bias of -inf masks an output; a row whose every output
-    is masked is all -inf and has no gradient.  In the backward pass rows whose incoming gradient is all zero (frames behind an
-    utterance's end) are left out whatever they hold; 16-bit types round the gradient of a logit to x's type before it enters
+    x [..., D], weight [V, D]: float32, bfloat16 or float16, both of one type; bias [V] or None, any of the three.  float32
+    products are off by less than 2^-21 of themselves, 2^-24.5 on average (about one rounding of float32).  A bias of -inf masks
+    an output; a row whose every output is masked is all -inf and has no gradient.  In the backward pass rows whose incoming
+    gradient is all zero (frames behind an utterance's end) are left out whatever they hold; 16-bit types round the gradient of a logit to x's type before it enters
     the products (float16: scaled to the upper end of the type's range, bits are lost below 2^-26 of the largest)."""
     _check_linear("linear_log_softmax", x, weight, bias)
     return _run("linear_log_softmax", x, x, weight, None if bias is None else bias.contiguous())
@@ -169,9 +169,16 @@ class OutputHead(nn.Module):
 
         head = wf.OutputHead(encoder_dim, lang.num_nn_output, dropout=0.1)
         loss = wf.graphloss(decoding_graph=graphs, dense_fsa_vec=wf.DenseFsaVec(head(enc), segments), ...)
-        loss = loss + 0.1 * head.cross_entropy(enc, frame_targets)         # on the same projection
 
-    Parameters may be float32 beside 16-bit activations: the projection's are cast to the activations' type.  Dropout takes
+    ``cross_entropy`` takes the same path to a loss of its own.  Each of the two calls norms and draws a dropout mask; both losses
+    of one step share them like this:
+
+        x, w = head.features(enc), head.weight.to(enc.dtype)
+        loss = wf.graphloss(dense_fsa_vec=wf.DenseFsaVec(wf.linear_log_softmax(x, w, head.bias), segments), ...)
+        loss = loss + 0.1 * wf.linear_cross_entropy(x, w, frame_targets, head.bias)
+
+    Parameters may be float32 beside 16-bit activations: the projection's weight is cast to the activations' type (and its
+    gradient comes back in it).  Frames without a target, or whose incoming gradient is zero, may hold anything.  Dropout takes
     its seed from torch's generator of the device (``torch.manual_seed``), on the device: it can be captured in a graph."""
 
     def __init__(self, idim, num_outputs, dropout=0.0, norm=True, bias=True, eps=1e-5, device=None, dtype=None):
