@@ -10,6 +10,7 @@ import torch
 
 import waterfall_amd as wf
 from waterfall_amd import _lib
+from tests import util
 from tests.test_head_linear import Case, check_grads, dz_of_entropy, dz_of_log_softmax, DEV, TYPES
 from tests.test_head_rows import norm64, U, within
 
@@ -269,3 +270,59 @@ def test_layer_norm_of_wide_rows(shape, dtype):
     within(got[0], dx, u * dx.abs() + f * size, "dx")
     within(got[1], dw, u * dw.abs() + f * (1 + shape[0] / 4096) * (adw + (dy.double().abs() * big * r).sum(0)), "dweight")
     within(got[2], db, u * db.abs() + f * (1 + shape[0] / 4096) * adb, "dbias")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_graph_loss_through_the_head_on_a_batch_padded_with_anything(dtype):
+    c = util.random_case(77, "ctc", B=4, T=30, L=5, P=58)
+    B, T, V = c["lp"].shape
+    torch.manual_seed(3)
+    head = wf.OutputHead(96, V, dropout=0.2, device=DEV)
+    segs = torch.from_numpy(c["segs"])
+    there = torch.arange(T, device=DEV)[None, :] < segs[:, 2].to(DEV)[:, None]
+    assert not there.all()
+    enc = torch.randn(B, T, 96, device=DEV).to(dtype)
+    got = []
+    for v in (enc, torch.where(there[..., None], enc, float("nan"))):
+        x = v.clone().requires_grad_()
+        torch.manual_seed(5)
+        loss = wf.graphloss(c["fsa"], wf.DenseFsaVec(head(x), segs), reduction="sum")
+        got.append((loss.detach(),) + torch.autograd.grad(loss, [x] + list(head.parameters())))
+    for p, q in zip(*got):
+        assert torch.equal(p, q) and torch.isfinite(p).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_one_row_without_leading_dimensions(dtype):
+    x, w = torch.randn(64, device=DEV).to(dtype).requires_grad_(), torch.randn(40, 64, device=DEV).to(dtype).requires_grad_()
+    b, t = torch.randn(40, device=DEV, requires_grad=True), torch.tensor(7, device=DEV)
+    for reduction in ("mean", "sum", "none"):
+        loss = wf.linear_cross_entropy(x, w, t, b, reduction=reduction)
+        assert loss.shape == ()
+        rows = wf.linear_cross_entropy(x[None], w, t[None], b, reduction=reduction).sum()
+        for p, q in zip(torch.autograd.grad(loss, (x, w, b)), torch.autograd.grad(rows, (x, w, b))):
+            assert torch.equal(p, q)
+    lp = wf.linear_log_softmax(x, w, b)
+    assert lp.shape == (40,) and torch.equal(lp, wf.linear_log_softmax(x[None], w, b)[0])
+    assert torch.equal(wf.layer_norm(x), wf.layer_norm(x[None])[0])
+    assert torch.autograd.grad(wf.layer_norm(x).sum() + lp.sum() + wf.dropout(x, 0.5, 3).sum(), x)[0].shape == (64,)
+
+
+@gpu
+def test_the_head_under_checkpointing_and_in_inference_mode():
+    from torch.utils.checkpoint import checkpoint
+    head = wf.OutputHead(64, 40, dropout=0.3, device=DEV)
+    x = torch.randn(4, 64, device=DEV, requires_grad=True)
+    torch.manual_seed(1)
+    want = torch.autograd.grad(head(x).square().sum(), x)[0]
+    for reentrant in (False, True):
+        torch.manual_seed(1)
+        checkpoint(head, x, use_reentrant=reentrant).square().sum().backward()
+        assert torch.equal(x.grad, want)
+        x.grad = None
+    head.eval()
+    lp = head(x).detach()
+    with torch.inference_mode():
+        assert torch.equal(head(x), lp)

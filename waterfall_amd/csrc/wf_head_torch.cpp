@@ -251,9 +251,9 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
                                       (float)smoothing, (float*)loss.data_ptr(), (float*)lse.data_ptr(), (float*)ptr(total),
                                       reduction == kMean, ws.data_ptr(), n, as_stream(stream)));
         ctx->save_for_backward({v.t, w.t, targets, bias, lse});
-        ctx->saved_data["a"] = std::vector<int64_t>{wants(x), wants(weight), wants(bias), stream, ignore, reduction, of(x), of(bias),
-                                                    of(targets), v.n, v.d, w.n};
-        ctx->saved_data["x"] = x.sizes().vec();
+        std::vector<int64_t> a{wants(x), wants(weight), wants(bias), stream, ignore, reduction, of(x), of(bias), of(targets), v.n, v.d, w.n};
+        a.insert(a.end(), x.sizes().begin(), x.sizes().end());
+        ctx->saved_data["a"] = std::move(a);
         ctx->saved_data["s"] = smoothing;
         return total.defined() ? total : loss;
     }
@@ -261,9 +261,9 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
         const auto saved = ctx->get_saved_variables();
         const auto a = ctx->saved_data["a"].toIntVector();
         no_eager_leaves(a[3]);
-        const auto shape = ctx->saved_data["x"].toIntVector();
+        const auto shape = at::IntArrayRef(a).slice(12);
         const Rows v(back(saved[0], grads[0], a[6], shape)), w(back(saved[1], grads[0], a[6], {a[11], a[10]}));
-        const Tensor targets = back_whole(saved[2], grads[0], a[8], at::IntArrayRef(shape).slice(0, shape.size() - 1));
+        const Tensor targets = back_whole(saved[2], grads[0], a[8], shape.slice(0, shape.size() - 1));
         const Tensor bias = back_whole(saved[3], grads[0], a[7], {a[11]}), lse = back_whole(saved[4], grads[0], kF32, {a[9]});
         const Tensor g = grads[0].contiguous();
         const Grads o(a, v, w, bias);
