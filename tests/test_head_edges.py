@@ -326,3 +326,29 @@ def test_the_head_under_checkpointing_and_in_inference_mode():
     lp = head(x).detach()
     with torch.inference_mode():
         assert torch.equal(head(x), lp)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,D,V", [(40, 64, 59), (300, 257, 700), (2100, 641, 5003), (5000, 64, 131)])
+def test_leaves_of_which_only_one_wants_a_gradient(N, D, V, dtype):
+    c = Case(N, D, V, dtype)
+    c.t[::5] = -1
+    G = torch.randn(N, V, generator=c.g).to(DEV)
+    G[3::7] = 0
+    calls = (lambda x, w, b: torch.autograd.grad(wf.linear_log_softmax(x, w, b), [v for v in (x, w, b) if v.requires_grad], G),
+             lambda x, w, b: torch.autograd.grad(wf.linear_cross_entropy(x, w, c.t, b, label_smoothing=0.1), [v for v in (x, w, b) if v.requires_grad]))
+    for call in calls:
+        whole = call(*[v.detach().requires_grad_() for v in (c.x, c.w, c.b)])
+        for wants in ((0,), (1,), (2,), (0, 1), (0, 2), (1, 2)):
+            got = call(*[v.detach().requires_grad_(k in wants) for k, v in enumerate((c.x, c.w, c.b))])
+            for k, g in zip(wants, got):
+                assert torch.equal(g, whole[k]), (wants, k)
+    # the row operators: one of x, weight, bias
+    y = [torch.randn(37, 300, generator=c.g).to(dtype).to(DEV), torch.randn(300, device=DEV), torch.randn(300, device=DEV)]
+    dy = torch.randn(37, 300, generator=c.g).to(dtype).to(DEV)
+    a = [v.clone().requires_grad_() for v in y]
+    whole = torch.autograd.grad(wf.layer_norm(*a), a, dy)
+    for k in range(3):
+        a = [v.clone().requires_grad_(i == k) for i, v in enumerate(y)]
+        assert torch.equal(torch.autograd.grad(wf.layer_norm(*a), a[k], dy)[0], whole[k]), k
