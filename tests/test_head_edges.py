@@ -352,3 +352,21 @@ def test_leaves_of_which_only_one_wants_a_gradient(N, D, V, dtype):
     for k in range(3):
         a = [v.clone().requires_grad_(i == k) for i, v in enumerate(y)]
         assert torch.equal(torch.autograd.grad(wf.layer_norm(*a), a[k], dy)[0], whole[k]), k
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 1500, 3000, 9000])
+def test_layer_norm_rows_without_a_gradient_at_the_ends_of_the_type(D, dtype):
+    g = torch.Generator().manual_seed(D)
+    x, dy = torch.randn(9, D, generator=g).to(dtype).to(DEV), torch.randn(9, D, generator=g).to(dtype).to(DEV)
+    w, b = torch.randn(D, generator=g).to(DEV), torch.randn(D, generator=g).to(DEV)
+    dead = [1, 4]
+    dy[dead] = 0
+    y = x.clone()
+    most = torch.finfo(dtype).max                           # the mean is finite, and the first element's distance from it is not
+    y[dead] = 0
+    y[dead[0], :3] = y[dead[1], :3] = torch.tensor([-most, most, 0.99 * most], device=DEV).to(dtype)
+    got = [torch.autograd.grad(wf.layer_norm(*a), a, dy) for a in ([t.detach().requires_grad_() for t in (v, w, b)] for v in (y, x))]
+    for p, q in zip(*got):
+        assert torch.equal(p, q)

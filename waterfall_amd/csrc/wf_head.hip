@@ -234,8 +234,9 @@ layer_norm_backward_kernel(LnArgs a) {
         const T* x = (const T*)a.x + (live ? r : 0) * a.ldx;
         const T* dy = (const T*)a.dy + (live ? r : 0) * a.lddy;
         float mean = mean1, rstd = rstd1;
-        // a row that is not finite takes no part where it has no gradient (0 times NaN otherwise): its zeros stand in for x
-        if (live && !(fabsf(mean) < INFINITY && rstd < INFINITY) && !has_any<T>(dy, a.D)) {
+        // a row that is not finite, or whose variance is not, takes no part where it has no gradient (0 times NaN otherwise): its zeros
+        // stand in for x
+        if (live && !(fabsf(mean) < INFINITY && rstd > 0.f && rstd < INFINITY) && !has_any<T>(dy, a.D)) {
             x = dy;
             mean = rstd = 0.f;
         }
