@@ -468,7 +468,8 @@ int wf_dropout(const void* x, int64_t n, int32_t type, double p, uint64_t seed, 
  *   (targets_wide 0) or int64.  Rows whose target is `ignore_index` take no part: loss 0, their x may hold anything.  Any
  *   other target outside [0, V): loss NaN, no gradient.  lse [N] is what the backward call takes.  total (may be NULL): the
  *   sum of the losses, divided by the number of rows that take part where `mean` (0 rows: 0).  The logits are not kept.
- * wf_linear_cross_entropy_backward: grad: device, [N] (grad_rows) or one value for every row; `mean` as in the forward call.
+ * wf_linear_cross_entropy_backward: grad: device, [N] (grad_rows: rows where it is 0 take no part) or one value for every
+ *   row; `mean` as in the forward call.
  *   The gradients of the logits exist for pieces of the outputs, 256 MB at a time.
  * Both backward calls: dx [N][D], dweight [V][D] of `type`, dbias [V] of `bias_type`, each may be NULL.  16-bit types: the
  * gradient of a logit is rounded to `type` before the products (fp16: scaled so that the largest that can come lies at the

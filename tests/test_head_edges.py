@@ -370,3 +370,24 @@ def test_layer_norm_rows_without_a_gradient_at_the_ends_of_the_type(D, dtype):
     got = [torch.autograd.grad(wf.layer_norm(*a), a, dy) for a in ([t.detach().requires_grad_() for t in (v, w, b)] for v in (y, x))]
     for p, q in zip(*got):
         assert torch.equal(p, q)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,D,V", [(40, 64, 59), (300, 257, 700), (2100, 641, 5003)])
+def test_rows_of_cross_entropy_without_an_incoming_gradient_may_hold_anything(N, D, V, dtype):
+    c = Case(N, D, V, dtype)
+    c.t[1::6] = -1
+    c.t[3] = V + 5                                          # no output: a loss of NaN, no gradient
+    up = torch.randn(N, generator=c.g).to(DEV)
+    dead = torch.zeros(N, dtype=torch.bool, device=DEV)
+    dead[2::5] = True
+    dead[3] = True
+    up[dead] = 0
+    x = c.x.clone()
+    x[dead] = float("nan")
+    a = [v.detach().requires_grad_() for v in (x, c.w, c.b)]
+    got = torch.autograd.grad(wf.linear_cross_entropy(a[0], a[1], c.t, a[2], label_smoothing=0.1, reduction="none"), a, up)
+    assert not got[0][dead].any()
+    with torch.no_grad():
+        check_grads(got, c.products(*dz_of_entropy(c, up, 0.1), 2 * up.abs().max().item()), (N, D, V))

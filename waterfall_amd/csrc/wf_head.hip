@@ -990,7 +990,7 @@ struct PrepArgs {
     uint16_t *xp, *wp;       // packed operands, or NULL where they are used as they lie
     int all;                 // every row is live and stays where it is (log-softmax forward): x and W are packed, no more
     void* dx;                // backward: the gradient of x; its dead rows become 0
-    const void* targets;     // cross entropy: row n is live iff targets[n] != ignore
+    const void* targets;     // cross entropy: row n is live iff targets[n] != ignore (and, with a gradient per row, it is not 0)
     int target_wide;
     int64_t ignore;
     const float* peak;       // log-softmax backward: row n is live iff peak[n] (of grad_rows_kernel) is not 0
@@ -1013,7 +1013,9 @@ inline float lift_of(int type, float unit) { return type == WF_F16 ? ldexpf(1.f,
 __device__ inline int64_t target_of(const PrepArgs& a, int64_t n) {
     return a.target_wide ? ((const int64_t*)a.targets)[n] : (int64_t)((const int32_t*)a.targets)[n];
 }
-__device__ inline bool row_alive(const PrepArgs& a, int64_t n) { return a.targets ? target_of(a, n) != a.ignore : a.peak[n] != 0.f; }
+__device__ inline bool row_alive(const PrepArgs& a, int64_t n) {
+    return a.targets ? target_of(a, n) != a.ignore && !(a.gout_rows && a.gout[n] == 0.f) : a.peak[n] != 0.f;
+}
 // (what is not finite stays in its row: it says nothing about the others' scale)
 __device__ inline float row_peak(const PrepArgs& a, int64_t n) {
     const float v = a.narrow ? a.peak[n] : row_alive(a, n) ? fabsf(a.gout[n]) : 0.f;

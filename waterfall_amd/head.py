@@ -146,8 +146,10 @@ def linear_cross_entropy(x, weight, targets, bias=None, ignore_index=-1, label_s
     x [..., D], weight [V, D], bias as for ``linear_log_softmax``; targets [...]: int32 or int64.  Rows whose target is
     ``ignore_index`` (by default -1, the label of the arcs that take no frame) have no loss, no gradient and may hold anything.
     A target that is neither it nor an output makes its row's loss NaN (nothing is read out of range) and has no gradient.
+    ``label_smoothing`` spreads its share over all outputs, those masked by a bias of -inf too: the loss is then infinite.
 
-    reduction: 'none' (float32 [...]), 'sum', or 'mean' over the rows that take part (0 where there are none)."""
+    reduction: 'none' (float32 [...]; rows whose incoming gradient is zero are left out of the backward pass whatever they
+    hold), 'sum', or 'mean' over the rows that take part (0 where there are none)."""
     _check_linear("linear_cross_entropy", x, weight, bias)
     if not isinstance(targets, torch.Tensor) or targets.dtype not in (torch.int32, torch.int64):
         raise TypeError("linear_cross_entropy: targets must be an int32 or int64 tensor")
